@@ -1,0 +1,420 @@
+"""The operators that train shared appearance codes, as cases to be timed and compared: the lookup of codebook rows and its
+gradient by sorted indices (`efgs.embedding`), and the AdamW step over many tensors with states in 32 or in 8 bits, clipped by
+the norm of all gradients or not (`efgs.AdamW`).
+
+`run` computes them from elementary torch operations where `own` is false, and through the framework's entry points where it
+is true. `listed` gives the standing cases, `draw` more of the same ranges, `exact` the same results in 64 bits.
+"""
+import math
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+DTYPES = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
+BETAS, EPS, WEIGHT_DECAY, STEPS_BEFORE, MAX_NORM = (0.9, 0.999), 1e-15, 1e-2, 40, 1.0
+# floats per Gaussian of each appearance model's residual parameters
+RESIDUAL = {'sh': 45, 'sv': 56, 'neural': 8}
+
+
+def _efgs():
+    package = str(Path(__file__).resolve().parent.parent / 'efficient-gaussian-appearance_amd')
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import efgs
+    return efgs
+
+
+def scene(bits, n, model, dtype='f32', clip=False):
+    return dict(kind='adamw', layout='scene', bits=bits, n=n, model=model, dtype=dtype, clip=clip)
+
+
+def many(bits, tensors, size, dtype='bf16', clip=False):
+    return dict(kind='adamw', layout='many', bits=bits, tensors=tensors, size=size, dtype=dtype, clip=clip)
+
+
+def embed(kind, n, rows, columns, dtype='f32', skew=2.0, invalid=0.0, scale=1.0):
+    return dict(kind=kind, n=n, rows=rows, columns=columns, dtype=dtype, skew=skew, invalid=invalid, scale=scale)
+
+
+def listed():
+    return [
+        # a small object's optimiser step, clipped: launches and host time count
+        dict(scene(32, 10_000, 'sh', clip=True), name='adamw32_sh_10k_clip'),
+        # every parameter of a full HD benchmark scene with its largest per-primitive rows
+        dict(scene(32, 1_000_000, 'sh'), name='adamw32_sh_1m'),
+        # the same with a learning rate per column of the residual parameters, clipped by the norm of all gradients
+        dict(scene(32, 1_000_000, 'sv', clip=True), name='adamw32_sv_1m_clip'),
+        # many objects (or layers) trained at once: 240 small 16-bit tensors of odd sizes in one flat buffer, clipped
+        dict(many(32, 240, 9_001, clip=True), name='adamw32_240_tensors'),
+        # 8-bit states: an odd-sized scene whose residual parameters have a learning rate per column
+        dict(scene(8, 50_001, 'sv'), name='adamw8_sv_50k_odd'),
+        # 8-bit states of the benchmark scene with the neural appearance
+        dict(scene(8, 1_000_000, 'neural'), name='adamw8_neural_1m'),
+        # 8-bit states of a network's 16-bit layers
+        dict(many(8, 20, 700_001), name='adamw8_20_layers_bf16'),
+        # training: one codebook row of 8 features for each of a million primitives
+        dict(embed('train', 1_000_000, 4096, 8), name='embed_train_1m_codes'),
+        # training: a step's tokens into a large 16-bit table, scaled by the root of its width, padding among them
+        dict(embed('train', 16_383, 49_999, 1024, 'bf16', 3.0, 0.05, 32.0), name='embed_train_16k_tokens'),
+        # training: few rows, each met by thousands of primitives, rows of an odd width
+        dict(embed('train', 200_001, 257, 45, 'f32', 2.0, 0.01), name='embed_train_hot_rows'),
+        # viewing: the codebook rows of a scene's primitives, without a gradient
+        dict(embed('lookup', 1_000_000, 4096, 8), name='embed_lookup_1m_codes'),
+        # answering: a few tokens' rows
+        dict(embed('lookup', 4, 49_999, 4096, 'bf16', 1.0, 0.0, 64.0), name='embed_lookup_4_tokens'),
+    ]
+
+
+def _log_uniform(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    kind = rng.choice(('scene', 'scene', 'many', 'train', 'train', 'train', 'lookup'))
+    if kind == 'scene':
+        bits = rng.choice((32, 8))
+        return scene(bits, _log_uniform(rng, 2_000, 800_000), rng.choice(tuple(RESIDUAL)), rng.choice(('f32', 'f32', 'bf16')),
+                     bits == 32 and rng.random() < 0.5)
+    if kind == 'many':
+        bits = rng.choice((32, 8))
+        tensors = _log_uniform(rng, 2, 300) if bits == 32 else rng.randint(2, 20)
+        return many(bits, tensors, _log_uniform(rng, 50, 20_000_000 // tensors), rng.choice(tuple(DTYPES)), bits == 32 and rng.random() < 0.5)
+    dtype, columns = rng.choice((('f32', rng.choice((3, 8, 16, 45, 48, 64))), ('bf16', _log_uniform(rng, 32, 4096)), ('f16', _log_uniform(rng, 8, 1024))))
+    rows = _log_uniform(rng, 16, min(200_000, 100_000_000 // columns))
+    if kind == 'lookup':
+        return embed(kind, _log_uniform(rng, 1, min(1_000_000, 60_000_000 // columns)), rows, columns, dtype, 1.0, 0.0, round(math.sqrt(columns), 3))
+    n = _log_uniform(rng, 100, min(1_000_000, 60_000_000 // columns))
+    # (the commonest row is met at most about 30,000 times: a plain sum in 32 bits of many more says little)
+    skew = rng.choice((1.0, 2.0, 3.0))
+    while n * rows ** (-1.0 / skew) > 30_000:
+        n //= 2
+    return embed(kind, n, rows, columns, dtype, skew, rng.choice((0.0, 0.02)), round(rng.uniform(0.5, 8.0), 3))
+
+
+# ---- inputs ----------------------------------------------------------------------------------------------------------
+
+def _shapes(case):
+    """(shape, learning rate or rates by column) of every tensor."""
+    if case['layout'] == 'many':
+        # sizes from a fifth to nine fifths of the mean, most of them odd
+        return [((max(1, int(case['size'] * (0.2 + 1.6 * (k * 0.618034 % 1.0)))),), 1e-3) for k in range(case['tensors'])]
+    n, r = case['n'], RESIDUAL[case['model']]
+    residual = {'sh': ((n, 15, 3), 2.5e-3), 'sv': ((n, 8, 7), [2.5e-3] * 3 + [1e-2] + [1.25e-3] * 3), 'neural': ((n, r), 2.5e-3)}[case['model']]
+    mlp = [((6144,), 1e-3)] if case['model'] == 'neural' else []
+    return [((n, 3), 1.6e-3), ((n, 3), 5e-3), ((n, 4), 1e-3), ((n, 1), 2.5e-2), ((n, 3), 2.5e-3), residual] + mlp
+
+
+def _elements(case):
+    return sum(math.prod(s) for s, _ in _shapes(case))
+
+
+def _flat_views(flat, shapes):
+    at, views = 0, []
+    for shape, _ in shapes:
+        size = math.prod(shape)
+        views.append(flat[at:at + size].view(shape))
+        at += size
+    return views
+
+
+def _gradients(case, generator):
+    """Gradients whose size varies over rows (primitives near and far); nearly a third of the rows are out of view: zeros."""
+    shapes, total, dtype = _shapes(case), _elements(case), DTYPES[case['dtype']]
+    size = torch.exp(torch.randn(total // 8 + 1, generator=generator, device='cuda') * 1.5 - 9.0)
+    size = size * (torch.rand(total // 8 + 1, generator=generator, device='cuda') > 0.3)
+    size = size.repeat_interleave(8)[:total]
+    flat = (torch.randn(total, generator=generator, device='cuda') * size).to(dtype)
+    return shapes, flat, size, dtype
+
+
+def _optimiser_inputs(case, seed):
+    """Parameters, gradients and the states of an optimiser that has taken STEPS_BEFORE steps."""
+    generator = torch.Generator('cuda').manual_seed(int(seed) & 0x7fffffff)
+    shapes, g, size, dtype = _gradients(case, generator)
+    total = g.numel()
+    flat = dict(p=torch.randn(total, generator=generator, device='cuda').to(dtype), g=g)
+    root = (size * (0.05 + 0.3 * torch.rand(total, generator=generator, device='cuda')) + 1e-9)
+    ratio = torch.randn(total, generator=generator, device='cuda') * 0.4
+    views = {k: _flat_views(v, shapes) for k, v in flat.items()}
+    if case['bits'] == 32:
+        flat.update(m=ratio * root, v=root * root)
+        views.update(m=_flat_views(flat['m'], shapes), v=_flat_views(flat['v'], shapes))
+    else:
+        coded = [_code_states(u.reshape(-1), r.reshape(-1)) for u, r in zip(_flat_views(ratio, shapes), _flat_views(root, shapes))]
+        views.update(ratio=[c[0].view(s) for c, (s, _) in zip(coded, shapes)], root=[c[1].view(s) for c, (s, _) in zip(coded, shapes)],
+                     scale=[c[2] for c in coded])
+    return flat, views, shapes
+
+
+def _embedding_inputs(case, seed):
+    generator = torch.Generator('cuda').manual_seed(int(seed) & 0x7fffffff)
+    n, rows, dtype = case['n'], case['rows'], DTYPES[case['dtype']]
+    table = (torch.randn((rows, case['columns']), generator=generator, device='cuda') * 0.1).to(dtype)
+    u = torch.rand(n, generator=generator, device='cuda', dtype=torch.float64)
+    indices = (rows * u ** case['skew']).long().clamp(max=rows - 1)
+    if case['invalid']:  # primitives without a code
+        indices[torch.rand(n, generator=generator, device='cuda') < case['invalid']] = -1
+    grad = torch.randn((n, case['columns']), generator=generator, device='cuda').to(dtype) if case['kind'] == 'train' else None
+    return table, indices, grad
+
+
+def prepare(case, seed):
+    if case['kind'] in ('train', 'lookup'):
+        table, indices, grad = _embedding_inputs(case, seed)
+        state = dict(case=case, table=table.requires_grad_(grad is not None), indices=indices, grad=grad, padding=min(1, case['rows'] - 1))
+    else:
+        flat, views, shapes = _optimiser_inputs(case, seed)
+        state = dict(case=case, flat=flat, views=views, shapes=shapes, step=STEPS_BEFORE)
+        if own:
+            groups = []
+            for p, g, (_, lr) in zip(views['p'], views['g'], shapes):
+                p.requires_grad_()
+                p.grad = g
+                if groups and groups[-1]['lr'] == lr:
+                    groups[-1]['params'].append(p)
+                else:
+                    groups.append({'params': [p], 'lr': lr})
+            state['optimizer'] = _efgs().AdamW(groups, betas=BETAS, eps=EPS, weight_decay=WEIGHT_DECAY, state_bits=case['bits'],
+                                               max_grad_norm=MAX_NORM if case['clip'] else None, seed=7)
+            for k, p in enumerate(views['p']):
+                if case['bits'] == 32:
+                    state['optimizer'].state[p] = dict(step=STEPS_BEFORE, exp_avg=views['m'][k], exp_avg_sq=views['v'][k])
+                else:
+                    state['optimizer'].state[p] = dict(step=STEPS_BEFORE, exp_avg_ratio=views['ratio'][k], exp_avg_sq_root=views['root'][k],
+                                                       root_scale=views['scale'][k])
+    if own:
+        _efgs()
+    return state
+
+
+# ---- the operators in plain form -------------------------------------------------------------------------------------
+# 8-bit states: a value y >= 0 is held as the top bits (4 of the mantissa) of the float y + c, counted from those of c; the
+# root r of the second moment with c = 2^-16 against its block's scale (256 elements), the ratio u = m / r with c = 2^-8
+# against its bound, and a sign. Rounded by a dither of 16 bits.
+BLOCK = 256
+ROOT_C, ROOT_BASE, ROOT_TOP = 2.0 ** -16, 111 * 16, 31 / 32 - 2.0 ** -16
+RATIO_C, RATIO_BASE, RATIO_TOP = 2.0 ** -8, 119 * 16, 31 / 32 - 2.0 ** -8
+LEAST_SCALE = 2.0 ** -100
+RATIO_BOUND = (1 - BETAS[0]) / math.sqrt((1 - BETAS[1]) * (1 - BETAS[0] ** 2 / BETAS[1]))
+
+
+def _mix(x):
+    """A hash of 32 bits, of whole numbers or of int64 tensors."""
+    x = x & 0xffffffff
+    x = ((x ^ (x >> 16)) * 0x6C8E9CF5) & 0xffffffff
+    x = ((x ^ (x >> 15)) * 0x3A2F4D1B) & 0xffffffff
+    return x ^ (x >> 16)
+
+
+def _dither(n, step, seed):
+    key = _mix(_mix(seed) + step)
+    h = _mix(torch.arange(n, device='cuda') * 0x9E3779B1 + key)
+    return (h & 0xffff).int(), (h >> 16).int()
+
+
+def _decode(code, base, c):
+    return ((code.int() + base) << 19).view(torch.float32) - c
+
+
+def _encode(y, dither, base, c, top):
+    return ((((y + c).view(torch.int32) + (dither << 3)) >> 19) - base).clamp(max=top)
+
+
+def _blocks(x):
+    n = x.numel()
+    return torch.nn.functional.pad(x, (0, -n % BLOCK)).view(-1, BLOCK)
+
+
+def _scales(root):
+    scale = _blocks(root).amax(1) * torch.tensor(1 / ROOT_TOP, dtype=torch.float32, device=root.device)
+    scale = torch.where(scale < LEAST_SCALE, torch.zeros_like(scale), scale)
+    return scale, torch.where(scale > 0, 1.0 / scale, torch.zeros_like(scale))
+
+
+def _code_states(u, r):
+    half = torch.full_like(u, 1 << 15, dtype=torch.int32)
+    scale, inverse = _scales(r)
+    root = _encode((_blocks(r) * inverse[:, None]).view(-1)[:r.numel()], half, ROOT_BASE, ROOT_C, 255)
+    ratio = _encode((u.abs() * (RATIO_TOP / RATIO_BOUND)).clamp(max=RATIO_TOP), half, RATIO_BASE, RATIO_C, 127)
+    return (ratio + 128 * (u < 0)).to(torch.uint8), root.to(torch.uint8), scale
+
+
+def _decode_states(ratio, root, scale):
+    ratio, root = ratio.view(-1), root.view(-1)
+    r = (_blocks(_decode(root, ROOT_BASE, ROOT_C)) * scale[:, None]).view(-1)[:root.numel()]
+    u = _decode(ratio & 127, RATIO_BASE, RATIO_C) * (RATIO_BOUND / RATIO_TOP)
+    return torch.where(ratio >= 128, -u, u), r
+
+
+def _norm(grads):
+    return torch.stack([g.float().square().sum() for g in grads]).sum().sqrt()
+
+
+def _updated(p, lr, m, root, step):
+    """The parameters after the step; a list holds a learning rate per column."""
+    columns, bias = 1, 1 / (1 - BETAS[0] ** step)
+    if isinstance(lr, float):
+        decay, rate = 1 - lr * WEIGHT_DECAY, lr * bias
+    else:
+        columns, rates = len(lr), torch.tensor(lr, dtype=torch.float64)
+        decay, rate = (1 - rates * WEIGHT_DECAY).to(p.device, torch.float32), (rates * bias).to(p.device, torch.float32)
+    update = m / (root * (1 / math.sqrt(1 - BETAS[1] ** step)) + EPS)
+    return (p.float().view(-1, columns) * decay - rate * update.view(-1, columns)).view(p.shape).to(p.dtype)
+
+
+def _plain_step(state):
+    case, views, step = state['case'], state['views'], state['step'] + 1
+    state['step'] = step
+    norm = _norm(views['g']) if case['clip'] else None
+    coefficient = (MAX_NORM / (norm + 1e-6)).clamp(max=1.0) if case['clip'] else None
+    b1, b2 = BETAS
+    moments = []
+    for k, (p, g, (_, lr)) in enumerate(zip(views['p'], views['g'], state['shapes'])):
+        g = g.float().view(-1)
+        g = g * coefficient if case['clip'] else g
+        if case['bits'] == 32:
+            m, v = views['m'][k].view(-1), views['v'][k].view(-1)
+            m.copy_(b1 * m + (1 - b1) * g)
+            v.copy_(b2 * v + (1 - b2) * (g * g))
+            p.copy_(_updated(p, lr, m, v.sqrt(), step))
+            continue
+        ratio, root, scale = views['ratio'][k].view(-1), views['root'][k].view(-1), views['scale'][k]
+        u, r = _decode_states(ratio, root, scale)
+        m = b1 * (u * r) + (1 - b1) * g
+        r = (b2 * (r * r) + (1 - b2) * (g * g)).sqrt()
+        p.copy_(_updated(p, lr, m, r, step))
+        r = torch.where(r.isfinite(), r, torch.zeros_like(r))
+        low, high = _dither(r.numel(), step, 7)
+        new_scale, inverse = _scales(r)
+        root.copy_(_encode((_blocks(r) * inverse[:, None]).view(-1)[:r.numel()], low, ROOT_BASE, ROOT_C, 255))
+        y = torch.where(r > 0, m / r, torch.zeros_like(r)).abs() * (RATIO_TOP / RATIO_BOUND)
+        ratio.copy_(_encode(y.clamp(max=RATIO_TOP), high, RATIO_BASE, RATIO_C, 127) + 128 * (m < 0))
+        scale.copy_(new_scale)
+        u, r = _decode_states(ratio, root, scale)
+        moments.append(((u * r).view(p.shape), (r * r).view(p.shape)))
+    return moments, norm
+
+
+def _plain_embedding(state):
+    case, table, indices, grad = state['case'], state['table'].detach(), state['indices'], state['grad']
+    valid = (indices >= 0) & (indices < case['rows'])
+    out = (table[indices.clamp(0, case['rows'] - 1)].float() * case['scale'] * valid[:, None]).to(table.dtype)
+    if grad is None:
+        return dict(out=out)
+    counted = valid & (indices != state['padding'])
+    sums = torch.zeros(table.shape, device='cuda').index_add_(0, indices.clamp(0, case['rows'] - 1), grad.float() * counted[:, None])
+    return dict(out=out, grad=(sums * case['scale']).to(table.dtype))
+
+
+def run(state):
+    case = state['case']
+    if case['kind'] != 'adamw':
+        if not own:
+            return _plain_embedding(state)
+        out = _efgs().embedding(state['indices'], state['table'], scale=case['scale'], padding_idx=state['padding'])
+        if state['grad'] is None:
+            return dict(out=out)
+        return dict(out=out, grad=torch.autograd.grad(out, state['table'], state['grad'])[0])
+    if own:
+        state['optimizer'].step()
+        moments = state['optimizer'].moments(state['views']['p']) if case['bits'] == 8 else None
+        norm = state['optimizer'].grad_norm
+    else:
+        with torch.no_grad():
+            moments, norm = _plain_step(state)
+    if case['bits'] == 8:
+        return dict(p=[p.detach() for p in state['views']['p']], m=[a for a, _ in moments], v=[b for _, b in moments])
+    out = dict(p=state['flat']['p'], m=state['flat']['m'], v=state['flat']['v'])
+    return dict(out, norm=norm) if case['clip'] else out
+
+
+# ---- what a pass cannot do without -------------------------------------------------------------------------------------
+
+def work(case):
+    size = DTYPES[case['dtype']].itemsize
+    if case['kind'] == 'adamw':
+        # 8 bits: the states in and out, and the values that they stand for
+        states = 16 if case['bits'] == 32 else 4 + 8 / BLOCK + 8
+        return dict(bytes=_elements(case) * (3 * size + states), flops=16 * _elements(case))
+    row, n = size * case['columns'], case['n']
+    met = _rows_met(case)
+    if case['kind'] == 'lookup':
+        return dict(bytes=8 * n + row * (met + n), flops=n * case['columns'])
+    return dict(bytes=8 * n + row * (met + 2 * n + case['rows']), flops=2 * n * case['columns'])
+
+
+def _rows_met(case):
+    """How many different rows n indices meet, in the mean."""
+    edges = (torch.arange(min(case['rows'], 200_001), dtype=torch.float64) / case['rows']) ** (1 / case['skew'])
+    p = torch.diff(torch.cat([edges, torch.ones(1, dtype=torch.float64)]))
+    return float((1 - (1 - p) ** (case['n'] * (1 - case['invalid']))).sum())
+
+
+# ---- the same in 64 bits -------------------------------------------------------------------------------------------------
+
+def _exact_decode(code, mantissa_c, first_exponent):
+    """Value of a code: 16 steps to an octave from c on, less c."""
+    code = code.long()
+    return (1 + (code % 16).double() / 16) * torch.pow(2.0, (code // 16 + first_exponent).double()) - mantissa_c
+
+
+def _exact_encode(y, c, first_exponent, dither, top):
+    fraction, exponent = torch.frexp(y + c)
+    position = (exponent.double() - 1 - first_exponent + 2 * fraction - 1) * 16
+    return torch.floor(position + dither.double() / 65536).clamp(max=top)
+
+
+def _exact_adamw(case, seed):
+    flat, views, shapes = _optimiser_inputs(case, seed)
+    t, (b1, b2) = STEPS_BEFORE + 1, BETAS
+    out = dict(p=[], m=[], v=[])
+    norm = math.sqrt(float(flat['g'].double().square().sum()))
+    factor = min(1.0, MAX_NORM / (norm + 1e-6)) if case['clip'] else 1.0
+    bound = (1 - b1) / math.sqrt((1 - b2) * (1 - b1 * b1 / b2))
+    for k, (shape, lr) in enumerate(shapes):
+        g = views['g'][k].double().reshape(-1) * factor
+        if case['bits'] == 32:
+            m, v = views['m'][k].double().reshape(-1), views['v'][k].double().reshape(-1)
+        else:
+            group = torch.arange(g.numel(), device=g.device) // 256
+            code = views['ratio'][k].reshape(-1).long()
+            r = _exact_decode(views['root'][k].reshape(-1), 2.0 ** -16, -16) * views['scale'][k].double()[group]
+            u = _exact_decode(code % 128, 2.0 ** -8, -8) * bound / (31 / 32 - 2.0 ** -8) * (1 - 2 * (code // 128).double())
+            m, v = u * r, r * r
+        m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g ** 2
+        rate = torch.tensor(lr, dtype=torch.float64, device=g.device).reshape(-1).repeat(g.numel() // (len(lr) if isinstance(lr, list) else 1))
+        p = views['p'][k].double().reshape(-1)
+        p = p - rate * WEIGHT_DECAY * p - rate * (m / (1 - b1 ** t)) / (torch.sqrt(v / (1 - b2 ** t)) + EPS)
+        if case['bits'] == 8:
+            r = v.sqrt()
+            y = torch.where(r > 0, m / r, 0.0).abs() / bound * (31 / 32 - 2.0 ** -8)
+            top = torch.zeros(int(group[-1]) + 1, dtype=torch.float64, device=g.device).scatter_reduce(0, group, r, 'amax')
+            scale = top / (31 / 32 - 2.0 ** -16)
+            scale = torch.where(scale < LEAST_SCALE, 0.0, scale)[group]
+            low, high = _dither(g.numel(), t, 7)
+            root = _exact_decode(_exact_encode(torch.where(scale > 0, r / scale, 0.0), 2.0 ** -16, -16, low, 255), 2.0 ** -16, -16) * scale
+            ratio = _exact_decode(_exact_encode(y, 2.0 ** -8, -8, high, 127), 2.0 ** -8, -8) * bound / (31 / 32 - 2.0 ** -8)
+            m, v = torch.where(m < 0, -ratio, ratio) * root, root * root
+        for name, x in (('p', p), ('m', m), ('v', v)):
+            out[name].append(x.view(shape))
+    if case['bits'] == 8:
+        return out
+    out = {k: torch.cat([x.reshape(-1) for x in v]) for k, v in out.items()}
+    return dict(out, norm=torch.tensor(norm, dtype=torch.float64)) if case['clip'] else out
+
+
+def exact(case, seed):
+    if case['kind'] == 'adamw':
+        return _exact_adamw(case, seed)
+    table, indices, grad = _embedding_inputs(case, seed)
+    inside = (indices >= 0) & (indices < case['rows'])
+    out = torch.zeros((case['n'], case['columns']), dtype=torch.float64, device='cuda')
+    out[inside] = table.double()[indices[inside]] * case['scale']
+    if grad is None:
+        return dict(out=out)
+    inside &= indices != min(1, case['rows'] - 1)
+    sums = torch.zeros((case['rows'], case['columns']), dtype=torch.float64, device='cuda')
+    return dict(out=out, grad=sums.index_add_(0, indices[inside], grad[inside].double()) * case['scale'])
