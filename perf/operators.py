@@ -184,7 +184,7 @@ def prepare(case, seed):
                     state['optimizer'].state[p] = dict(step=STEPS_BEFORE, exp_avg=views['m'][k], exp_avg_sq=views['v'][k])
                 else:
                     state['optimizer'].state[p] = dict(step=STEPS_BEFORE, exp_avg_ratio=views['ratio'][k], exp_avg_sq_root=views['root'][k],
-                                                       root_scale=views['scale'][k])
+                                                       root_scale=views['scale'][k], ratio_bound=RATIO_BOUND)
     if own:
         _efgs()
     return state
