@@ -21,11 +21,14 @@ NATIVE = os.path.join(HERE, 'efgs', '_native.so')
 # Adam follow the exact operation sequence of their definitions.
 SOURCES = [
     ('api.cpp', []),
+    ('training_api.cpp', []),
     ('rtc.cpp', []),
     ('scan.hip', []),
     ('raster.hip', ['-ffp-contract=off']),
     ('blend.hip', ['-ffp-contract=off']),
     ('adam.hip', ['-ffp-contract=off']),
+    ('adamw.hip', ['-ffp-contract=off']),
+    ('embedding.hip', []),
     ('densification.hip', ['-ffp-contract=off']),
     ('ngsplat.hip', ['-ffp-contract=off']),
 ]
@@ -49,24 +52,28 @@ def _run(what: str, cmd: list[str]) -> None:
         raise RuntimeError(f'{what} failed:\n{" ".join(cmd)}\n{r.stdout}\n{r.stderr}')
 
 
-def _compile_binding() -> str:
-    """csrc/torch_binding.cpp against the installed torch (host code only)."""
+# sources of the Python extension (host code only)
+BINDING_SOURCES = ('torch_binding.cpp', 'torch_training.cpp')
+
+
+def _compile_binding(src: str) -> str:
+    """A source of the Python extension against the installed torch."""
     import torch
     inc = os.path.join(os.path.dirname(torch.__file__), 'include')
-    obj = os.path.join(BUILD, 'torch_binding.cpp.o')
-    _run('compiling torch_binding.cpp',
+    obj = os.path.join(BUILD, src + '.o')
+    _run(f'compiling {src}',
          ['g++', '-O2', '-std=c++17', '-fPIC', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1', '-DTORCH_EXTENSION_NAME=_native',
           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', '-I', inc, '-I', os.path.join(inc, 'torch', 'csrc', 'api', 'include'),
           '-I', os.path.join(os.environ.get('ROCM_PATH', '/opt/rocm'), 'include'), '-I', sysconfig.get_paths()['include'],
-          '-c', os.path.join(CSRC, 'torch_binding.cpp'), '-o', obj])
+          '-c', os.path.join(CSRC, src), '-o', obj])
     return obj
 
 
-def _link_binding(obj: str) -> None:
+def _link_binding(objs: list[str]) -> None:
     import torch
     libs = os.path.join(os.path.dirname(torch.__file__), 'lib')
     tmp = NATIVE + '.tmp'
-    _run('linking _native.so', ['g++', '-shared', '-fPIC', '-o', tmp, obj, '-L', libs, '-ltorch_python', '-ltorch', '-ltorch_cpu', '-lc10', '-lc10_hip',
+    _run('linking _native.so', ['g++', '-shared', '-fPIC', '-o', tmp, *objs, '-L', libs, '-ltorch_python', '-ltorch', '-ltorch_cpu', '-lc10', '-lc10_hip',
                                 '-L', os.path.dirname(LIB), '-l:libefgs_hip.so', '-Wl,-rpath,$ORIGIN'])
     os.replace(tmp, NATIVE)
 
@@ -74,13 +81,13 @@ def _link_binding(obj: str) -> None:
 def build(arch: str = 'gfx950', jobs: int = 8, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        binding = ex.submit(_compile_binding)
+        binding = [ex.submit(_compile_binding, s) for s in BINDING_SOURCES]
         objs = list(ex.map(lambda s: _compile(s[0], s[1], arch), SOURCES))
-        binding_obj = binding.result()
+        binding_objs = [b.result() for b in binding]
     tmp = LIB + '.tmp'
     _run('linking', ['hipcc', f'--offload-arch={arch}', '-shared', '-fPIC', '-Wl,-soname,libefgs_hip.so', '-o', tmp, *objs, '-lhiprtc'])
     os.replace(tmp, LIB)
-    _link_binding(binding_obj)
+    _link_binding(binding_objs)
     if verbose:
         print(f'built {LIB} and {NATIVE}')
     return LIB

@@ -1,0 +1,621 @@
+// Rows of a table by index, scaled, and the table's gradient.
+//
+//   out[i, :] = scale table[idx[i], :]                  an index outside [0, rows) gives a zero row
+//   gradient[v, :] = scale sum over idx[i] = v of g[i, :]  in 32 bits; not for such indices, nor for the padding row
+//
+// The gradient sorts the indices (stable, least significant digit first), so that a row's sum is over a contiguous run of
+// the sorted list, in an order that the data alone gives: results are the same from call to call, without atomics on
+// floats. Runs are uneven (a common code is met by a large part of all primitives, most rows of a large table by none) and
+// the zero rows have to be written too, so the work is cut by the merged list of both: entry e of row k stands at
+// position e + k, behind e entries and the ends of k rows, and the end of a row is an item of its own, which writes
+// it. Every group of lanes takes the same number of items whatever the runs are; a sum that crosses groups is carried by a
+// segmented scan within the block, and a row that crosses blocks is put together by a second kernel from the blocks' first
+// and last pieces, in their order.
+#include "internal.h"
+
+namespace efgs {
+
+namespace {
+
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 half8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 bfloat8u __attribute__((ext_vector_type(8), aligned(2)));
+
+// 16 bytes of a row
+template <typename T> struct Lane16;
+template <> struct Lane16<float> { using type = float4u; static constexpr int values = 4; };
+template <> struct Lane16<_Float16> { using type = half8u; static constexpr int values = 8; };
+template <> struct Lane16<__bf16> { using type = bfloat8u; static constexpr int values = 8; };
+
+// v = the lane's values at p; past `count` zeros
+template <typename T>
+__device__ __forceinline__ typename Lane16<T>::type load16(const T* p, int count) {
+    using V = typename Lane16<T>::type;
+    if (count >= Lane16<T>::values) return *reinterpret_cast<const V*>(p);
+    V v;
+#pragma unroll
+    for (int k = 0; k < Lane16<T>::values; k++) v[k] = k < count ? p[k] : static_cast<T>(0.0f);
+    return v;
+}
+
+// a float32 product, then rounded to T: the compiler would make one instruction of both for float16 (v_fma_mixlo_f16), whose
+// one rounding now and then gives another value than the multiplication and the cast of a tensor
+template <typename T>
+__device__ __forceinline__ T scaled(float x, float scale) {
+    float y = x * scale;
+    asm("" : "+v"(y));
+    return static_cast<T>(y);
+}
+
+template <typename T>
+__device__ __forceinline__ void store16(T* p, int count, const float* x, float scale) {
+    if (count >= Lane16<T>::values) {
+        typename Lane16<T>::type v;
+#pragma unroll
+        for (int k = 0; k < Lane16<T>::values; k++) v[k] = scaled<T>(x[k], scale);
+        *reinterpret_cast<typename Lane16<T>::type*>(p) = v;
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < Lane16<T>::values; k++)
+        if (k < count) p[k] = scaled<T>(x[k], scale);
+}
+
+constexpr uint32_t max_blocks = 1u << 23;  // of a launch of 256 threads (32 bits of threads)
+
+// row of an index, or `rows` for none
+__device__ __forceinline__ uint32_t row_of(int64_t index, uint32_t rows) {
+    return static_cast<uint64_t>(index) < rows ? static_cast<uint32_t>(index) : rows;
+}
+
+// ---- lookup ----------------------------------------------------------------------------------------------------------
+
+constexpr uint32_t lookup_block = 256, lookup_items = 4, lookup_tile = lookup_block * lookup_items;
+
+struct LookupArgs {
+    const void* indices;
+    const void* table;
+    void* out;
+    uint64_t row_stride;      // of the table
+    uint32_t first, n, rows, columns;  // this launch: indices from `first` on
+    uint32_t lanes;           // 16-byte lanes of a row in this tile of columns (<= lookup_tile)
+    uint32_t lanes_rcp;       // 2^20 / lanes + 1: t / lanes = t * lanes_rcp >> 20 for t < 1024
+    uint32_t rows_per_block;
+    float scale;
+};
+
+// A block takes whole rows (or, past 1,024 lanes of 16 bytes, 1,024 lanes of one row), consecutive lanes of it a row's
+// consecutive 16 bytes, four of them to a thread, all loaded before the first is stored.
+template <typename T, typename I>
+__global__ __launch_bounds__(lookup_block) void embedding_lookup_kernel(LookupArgs a) {
+    constexpr int values = Lane16<T>::values;
+    const uint32_t first_lane = blockIdx.y * lookup_tile;
+    const uint32_t items = a.rows_per_block * a.lanes;
+    typename Lane16<T>::type v[lookup_items];
+    uint64_t at[lookup_items];
+    int count[lookup_items];
+#pragma unroll
+    for (uint32_t k = 0; k < lookup_items; k++) {
+        const uint32_t t = k * lookup_block + threadIdx.x;
+        const uint32_t q = (t * a.lanes_rcp) >> 20, lane = first_lane + t - q * a.lanes;
+        const uint64_t i = a.first + static_cast<uint64_t>(blockIdx.x) * a.rows_per_block + q;
+        count[k] = 0;
+        if (t >= items || i >= a.n || lane * values >= a.columns) continue;
+        const uint32_t column = lane * values;
+        count[k] = static_cast<int>(min(a.columns - column, static_cast<uint32_t>(values)));
+        at[k] = i * a.columns + column;
+        const uint32_t row = row_of(static_cast<const I*>(a.indices)[i], a.rows);
+        v[k] = load16(static_cast<const T*>(a.table) + row * a.row_stride + column, row < a.rows ? count[k] : 0);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < lookup_items; k++) {
+        if (count[k] == 0) continue;
+        float x[values];
+#pragma unroll
+        for (int j = 0; j < values; j++) x[j] = static_cast<float>(v[k][j]);
+        store16(static_cast<T*>(a.out) + at[k], count[k], x, a.scale);
+    }
+}
+
+// ---- sort --------------------------------------------------------------------------------------------------------------
+// Keys are rows (or `rows` for an index that counts nowhere), values the positions of their indices. A pass orders by up
+// to 8 bits: blocks count their segments' digits into a table, then every block sums the table itself (its digits'
+// places behind all smaller digits and behind the same digits of earlier blocks) and writes its keys there, each at its
+// rank among the equal digits before it in its wave.
+
+constexpr uint32_t sort_block = 256, sort_waves = sort_block / 64, sort_steps = 16, sort_tile = sort_block * sort_steps;
+constexpr uint32_t sort_max_blocks = 256, sort_digits = 256;
+
+struct SortPass {
+    const void* indices;       // first pass: int32 or int64
+    const uint32_t* keys_in;   // later ones
+    const uint32_t* values_in;
+    uint32_t* keys_out;
+    uint32_t* values_out;
+    uint32_t* table;           // blocks x 256
+    uint32_t n, rows, padding; // padding: a row that counts nowhere (>= rows: none)
+    uint32_t shift, digit_mask;
+    uint32_t tiles_per_block;
+};
+
+template <typename I>
+__device__ __forceinline__ uint32_t key_at(const SortPass& a, uint32_t i) {
+    if constexpr (sizeof(I) == 1) return a.keys_in[i];
+    else {
+        const uint32_t row = row_of(static_cast<const I*>(a.indices)[i], a.rows);
+        return row == a.padding ? a.rows : row;
+    }
+}
+
+template <typename I>
+__global__ __launch_bounds__(sort_block) void sort_count_kernel(SortPass a) {
+    __shared__ uint32_t counts[sort_digits];
+    counts[threadIdx.x] = 0;
+    __syncthreads();
+    const uint64_t first = static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block * sort_tile;
+    const uint64_t last = min(first + static_cast<uint64_t>(a.tiles_per_block) * sort_tile, static_cast<uint64_t>(a.n));
+    for (uint64_t i = first + threadIdx.x; i < last; i += sort_block)
+        atomicAdd(&counts[(key_at<I>(a, static_cast<uint32_t>(i)) >> a.shift) & a.digit_mask], 1u);
+    __syncthreads();
+    a.table[blockIdx.x * sort_digits + threadIdx.x] = counts[threadIdx.x];
+}
+
+// exclusive prefix over the block's 256 threads
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* wave_totals) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t inclusive = v;
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const uint32_t t = __shfl_up(inclusive, o);
+        if (lane >= o) inclusive += t;
+    }
+    if (lane == 63) wave_totals[wave] = inclusive;
+    __syncthreads();
+    uint32_t before = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < sort_waves; w++)
+        if (w < wave) before += wave_totals[w];
+    return before + inclusive - v;
+}
+
+template <typename I>
+__global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
+    __shared__ uint32_t counts[sort_waves][sort_digits];
+    __shared__ uint32_t wave_totals[sort_waves];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t before = 0, total = 0;
+    for (uint32_t b = 0; b < gridDim.x; b++) {
+        const uint32_t c = a.table[b * sort_digits + threadIdx.x];
+        total += c;
+        if (b < blockIdx.x) before += c;
+    }
+    uint32_t place = block_exclusive(total, wave_totals) + before;  // of the thread's digit
+    for (uint32_t tile = 0; tile < a.tiles_per_block; tile++) {
+        const uint64_t first = (static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block + tile) * sort_tile;
+        if (first >= a.n) break;
+        for (uint32_t w = 0; w < sort_waves; w++) counts[w][threadIdx.x] = 0;
+        __syncthreads();
+        uint32_t key[sort_steps], value[sort_steps], rank[sort_steps];
+        const uint64_t wave_first = first + wave * 64u * sort_steps + lane;
+#pragma unroll
+        for (uint32_t s = 0; s < sort_steps; s++) {
+            const uint64_t i = wave_first + s * 64u;
+            key[s] = i < a.n ? key_at<I>(a, static_cast<uint32_t>(i)) : 0u;
+            if constexpr (sizeof(I) == 1) value[s] = i < a.n ? a.values_in[i] : 0u;
+            else value[s] = static_cast<uint32_t>(i);
+        }
+        volatile uint32_t* const mine = counts[wave];
+#pragma unroll
+        for (uint32_t s = 0; s < sort_steps; s++) {
+            const uint32_t digit = (key[s] >> a.shift) & a.digit_mask;
+            const bool valid = wave_first + s * 64u < a.n;
+            uint64_t same = __ballot(valid);
+#pragma unroll
+            for (uint32_t b = 0; b < 8; b++) {
+                const bool bit = (digit >> b) & 1u;
+                const uint64_t with = __ballot(bit);
+                same &= bit ? with : ~with;
+            }
+            const uint32_t earlier = static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1ull)));
+            const uint32_t so_far = mine[digit];
+            rank[s] = so_far + earlier;
+            __builtin_amdgcn_wave_barrier();
+            if (valid && earlier == 0) mine[digit] = so_far + static_cast<uint32_t>(__popcll(same));
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < sort_waves; w++) {
+            const uint32_t c = counts[w][threadIdx.x];
+            counts[w][threadIdx.x] = place;
+            place += c;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t s = 0; s < sort_steps; s++) {
+            if (wave_first + s * 64u < a.n) {
+                const uint32_t to = counts[wave][(key[s] >> a.shift) & a.digit_mask] + rank[s];
+                a.keys_out[to] = key[s];
+                a.values_out[to] = value[s];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- sums ----------------------------------------------------------------------------------------------------------------
+
+constexpr uint32_t sum_block = 256, sum_items = 8;  // items of a group of lanes
+
+struct SumArgs {
+    const uint32_t* keys;      // sorted
+    const uint32_t* values;
+    const void* grad_out;
+    void* gradient;
+    float* heads;              // per block: its first row's piece up to that row's end
+    float* tails;              // per block: the sum of the row that is open at its end
+    uint32_t* closed;          // per block: 1 where a row ends in it
+    uint32_t* first_row;       // per block: the row that is open at its start
+    uint32_t n, rows, columns, padded_columns;
+    uint32_t blocks;
+    float scale;
+};
+
+// entries among the first `position` items of the merged list, over the wave
+__device__ __forceinline__ uint32_t entries_before(const SumArgs& a, uint32_t position) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t lo = position > a.rows ? position - a.rows : 0u, hi = min(position, a.n);
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + 63u) / 64u, at = lo + lane * step;
+        const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(at < hi && at + a.keys[min(at, hi - 1)] < position)));
+        if (before == 0) break;
+        hi = min(hi, lo + before * step);
+        lo = lo + (before - 1) * step + 1;
+    }
+    return lo;
+}
+
+// G lanes to a row (of a tile of columns), 16 bytes each.
+template <typename T, int G>
+__global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
+    constexpr int values = Lane16<T>::values;
+    constexpr uint32_t groups = sum_block / G, items = groups * sum_items;
+    __shared__ uint32_t s_keys[items], s_values[items], s_start[groups + 1], s_bounds[2];
+    __shared__ float s_tail[sum_block / 64][G * values];
+    __shared__ uint32_t s_closed[sum_block / 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t total = a.n + a.rows, first = blockIdx.x * items, last = min(first + items, total);
+    if (wave < 2) {
+        const uint32_t e = entries_before(a, wave == 0 ? first : last);
+        if (lane == 0) s_bounds[wave] = e;
+    }
+    __syncthreads();
+    const uint32_t e0 = s_bounds[0], entries = s_bounds[1] - e0;
+    for (uint32_t k = threadIdx.x; k < entries; k += sum_block) {
+        s_keys[k] = a.keys[e0 + k];
+        s_values[k] = a.values[e0 + k];
+    }
+    __syncthreads();
+    for (uint32_t g = threadIdx.x; g <= groups; g += sum_block) {
+        const uint32_t position = min(first + g * sum_items, last);
+        uint32_t lo = 0, hi = entries;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (e0 + mid + s_keys[mid] < position) lo = mid + 1;
+            else hi = mid;
+        }
+        s_start[g] = lo;
+    }
+    __syncthreads();
+
+    const uint32_t group = threadIdx.x / G, column = (blockIdx.y * G + threadIdx.x % G) * values;
+    const int count = column < a.columns ? static_cast<int>(min(a.columns - column, static_cast<uint32_t>(values))) : 0;
+    const uint32_t start = s_start[group], end = s_start[group + 1];
+    const uint32_t position = min(first + group * sum_items, last), position_end = min(position + sum_items, last);
+    const uint32_t row_start = position - (e0 + start), row_end = position_end - (e0 + end);
+
+    typename Lane16<T>::type data[sum_items];
+#pragma unroll
+    for (uint32_t k = 0; k < sum_items; k++) {
+        const bool is_entry = start + k < end && s_keys[min(start + k, items - 1)] < a.rows;
+        data[k] = load16(static_cast<const T*>(a.grad_out) + static_cast<uint64_t>(is_entry ? s_values[start + k] : 0u) * a.columns + column,
+                         is_entry ? count : 0);
+    }
+
+    T* const gradient = static_cast<T*>(a.gradient);
+    float sum[values] = {}, head[values] = {};
+    bool any_closed = false;
+    uint32_t row = row_start;
+    auto close = [&]() {
+        if (!any_closed) {
+#pragma unroll
+            for (int j = 0; j < values; j++) head[j] = sum[j];
+            any_closed = true;
+        } else {
+            store16(gradient + static_cast<uint64_t>(row) * a.columns + column, count, sum, a.scale);
+        }
+#pragma unroll
+        for (int j = 0; j < values; j++) sum[j] = 0.0f;
+        row++;
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < sum_items; k++) {
+        if (start + k < end) {
+            const uint32_t key = s_keys[start + k];
+            while (row < key && row < row_end) close();
+#pragma unroll
+            for (int j = 0; j < values; j++) sum[j] += static_cast<float>(data[k][j]);
+        }
+    }
+    while (row < row_end) close();
+
+    // what is open at the start of each group: a segmented scan of the groups' open sums, first over the wave, then over the block
+    float scanned[values];
+    uint32_t flag = any_closed ? 1u : 0u;
+#pragma unroll
+    for (int j = 0; j < values; j++) scanned[j] = sum[j];
+#pragma unroll
+    for (uint32_t o = G; o < 64; o <<= 1) {
+        const uint32_t other_flag = __shfl_up(flag, o);
+#pragma unroll
+        for (int j = 0; j < values; j++) {
+            const float other = __shfl_up(scanned[j], o);
+            if (lane >= o && !flag) scanned[j] += other;
+        }
+        if (lane >= o) flag |= other_flag;
+    }
+    if (lane >= 64 - G) {
+#pragma unroll
+        for (int j = 0; j < values; j++) s_tail[wave][(lane % G) * values + j] = scanned[j];
+        if (lane == 63) s_closed[wave] = flag;
+    }
+    __syncthreads();
+    uint32_t before_flag = 0, block_flag = 0;
+    float before[values] = {}, block_tail[values] = {};
+#pragma unroll
+    for (uint32_t w = 0; w < sum_block / 64; w++) {
+        if (w == wave) {
+            before_flag = block_flag;
+#pragma unroll
+            for (int j = 0; j < values; j++) before[j] = block_tail[j];
+        }
+        const bool closed = s_closed[w] != 0;
+#pragma unroll
+        for (int j = 0; j < values; j++) block_tail[j] = s_tail[w][(lane % G) * values + j] + (closed ? 0.0f : block_tail[j]);
+        block_flag |= closed ? 1u : 0u;
+    }
+    if constexpr (G < 64) {
+        const uint32_t wave_flag = __shfl_up(flag, G);
+#pragma unroll
+        for (int j = 0; j < values; j++) {
+            const float other = __shfl_up(scanned[j], G);
+            if (lane >= G) before[j] = other + (wave_flag ? 0.0f : before[j]);
+        }
+        if (lane >= G) before_flag |= wave_flag;
+    }
+    const uint64_t piece = static_cast<uint64_t>(blockIdx.x) * a.padded_columns + column;
+    if (any_closed) {
+#pragma unroll
+        for (int j = 0; j < values; j++) head[j] += before[j];
+        if (before_flag) {
+            store16(gradient + static_cast<uint64_t>(row_start) * a.columns + column, count, head, a.scale);
+        } else {
+#pragma unroll
+            for (int j = 0; j < values; j++) a.heads[piece + j] = head[j];
+        }
+    }
+    if (threadIdx.x < G) {
+#pragma unroll
+        for (int j = 0; j < values; j++) a.tails[piece + j] = block_tail[j];
+    }
+    if (threadIdx.x == 0 && blockIdx.y == 0) {
+        a.closed[blockIdx.x] = block_flag;
+        a.first_row[blockIdx.x] = first - e0;
+    }
+}
+
+// One wave per block of the sums and tile of columns: the row that was open at the block's start, if it ends there, from
+// the open sums of the blocks before it since the last end of a row, and the block's own first piece.
+template <typename T, int G>
+__global__ __launch_bounds__(64) void embedding_join_kernel(SumArgs a) {
+    constexpr int values = Lane16<T>::values;
+    constexpr uint32_t slots = 64 / G;
+    const uint32_t lane = threadIdx.x, slot = lane / G, b = blockIdx.x;
+    if (!a.closed[b]) return;
+    const uint32_t column = (blockIdx.y * G + lane % G) * values;
+    const int count = column < a.columns ? static_cast<int>(min(a.columns - column, static_cast<uint32_t>(values))) : 0;
+    uint32_t from = b;
+    while (from > 0) {  // back to the last block before b in which a row ends
+        const bool in = lane < from;
+        const uint64_t ends = __ballot(in && a.closed[in ? from - 1 - lane : 0] != 0);
+        if (ends) {
+            from -= static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(ends)));
+            break;
+        }
+        from = from > 64 ? from - 64 : 0;
+    }
+    float sum[values] = {};
+    for (uint32_t k = from + slot; k < b; k += slots) {
+#pragma unroll
+        for (int j = 0; j < values; j++) sum[j] += a.tails[static_cast<uint64_t>(k) * a.padded_columns + column + j];
+    }
+#pragma unroll
+    for (uint32_t o = G; o < 64; o <<= 1) {
+#pragma unroll
+        for (int j = 0; j < values; j++) sum[j] += __shfl_xor(sum[j], o);
+    }
+    if (slot == 0) {
+#pragma unroll
+        for (int j = 0; j < values; j++) sum[j] += a.heads[static_cast<uint64_t>(b) * a.padded_columns + column + j];
+        store16(static_cast<T*>(a.gradient) + static_cast<uint64_t>(a.first_row[b]) * a.columns + column, count, sum, a.scale);
+    }
+}
+
+uint32_t bit_width(uint32_t x) { return x == 0 ? 0u : 32u - static_cast<uint32_t>(__builtin_clz(x)); }
+
+template <typename F>
+void with_type(int type, F&& f) {
+    if (type == type_float) f(float{});
+    else if (type == type_bfloat16) f(__bf16{});
+    else f(_Float16{});
+}
+
+uint32_t lanes_of_row(const EmbeddingArgs& a) { return div_up(a.columns, a.type == type_float ? 4 : 8); }
+
+// lanes of a group: the power of two that holds a row, or a wave
+uint32_t group_lanes(const EmbeddingArgs& a) {
+    uint32_t g = 1;
+    while (g < 64 && g < lanes_of_row(a)) g *= 2;
+    return g;
+}
+
+uint32_t sum_blocks(const EmbeddingArgs& a) { return div_up(static_cast<uint64_t>(a.n) + a.rows, sum_block / group_lanes(a) * sum_items); }
+
+uint32_t sort_tiles_per_block(uint32_t n) { return div_up(div_up(n, sort_tile), sort_max_blocks); }
+
+struct GradientLayout {
+    uint32_t* keys[2];
+    uint32_t* values[2];
+    uint32_t* table;
+    float* heads;
+    float* tails;
+    uint32_t* closed;
+    uint32_t* first_row;
+    uint32_t padded_columns;
+    size_t bytes;
+
+    static GradientLayout carve(char* base, const EmbeddingArgs& a) {
+        GradientLayout l;
+        size_t used = 0;
+        auto take = [&](size_t bytes) {
+            char* p = base + used;
+            used += (bytes + 255) / 256 * 256;
+            return p;
+        };
+        const uint32_t lanes = group_lanes(a), per_lane = a.type == type_float ? 4 : 8;
+        l.padded_columns = div_up(lanes_of_row(a), lanes) * lanes * per_lane;
+        const size_t blocks = sum_blocks(a);
+        for (int k = 0; k < 2; k++) l.keys[k] = reinterpret_cast<uint32_t*>(take(size_t{a.n} * 4));
+        for (int k = 0; k < 2; k++) l.values[k] = reinterpret_cast<uint32_t*>(take(size_t{a.n} * 4));
+        l.table = reinterpret_cast<uint32_t*>(take(size_t{sort_max_blocks} * sort_digits * 4));
+        l.heads = reinterpret_cast<float*>(take(blocks * l.padded_columns * 4));
+        l.tails = reinterpret_cast<float*>(take(blocks * l.padded_columns * 4));
+        l.closed = reinterpret_cast<uint32_t*>(take(blocks * 4));
+        l.first_row = reinterpret_cast<uint32_t*>(take(blocks * 4));
+        l.bytes = used;
+        return l;
+    }
+};
+
+template <typename T, int G>
+void launch_sums(const SumArgs& a, uint32_t lanes, hipStream_t s) {
+    const uint32_t tiles = div_up(lanes, G);
+    embedding_sum_kernel<T, G><<<dim3(a.blocks, tiles), sum_block, 0, s>>>(a);
+    embedding_join_kernel<T, G><<<dim3(a.blocks, tiles), 64, 0, s>>>(a);
+}
+
+}  // namespace
+
+bool launch_embedding_lookup(const EmbeddingArgs& a, const void* table, uint64_t row_stride, void* out, hipStream_t s) {
+    if (a.n == 0 || a.columns == 0) return true;
+    LookupArgs l;
+    l.indices = a.indices;
+    l.table = table;
+    l.out = out;
+    l.row_stride = row_stride;
+    l.n = a.n;
+    l.rows = a.rows;
+    l.columns = a.columns;
+    const uint32_t lanes = lanes_of_row(a);
+    l.lanes = lanes < lookup_tile ? lanes : lookup_tile;
+    l.lanes_rcp = (1u << 20) / l.lanes + 1;
+    l.rows_per_block = lookup_tile / l.lanes;
+    l.scale = a.scale;
+    const uint64_t blocks = div_up(a.n, l.rows_per_block);
+    for (uint64_t b = 0; b < blocks; b += max_blocks) {
+        l.first = static_cast<uint32_t>(b * l.rows_per_block);
+        const dim3 grid(static_cast<uint32_t>(blocks - b < max_blocks ? blocks - b : max_blocks), div_up(lanes, lookup_tile));
+        with_type(a.type, [&](auto t) {
+            using T = decltype(t);
+            if (a.index_bytes == 4) embedding_lookup_kernel<T, int32_t><<<grid, lookup_block, 0, s>>>(l);
+            else embedding_lookup_kernel<T, int64_t><<<grid, lookup_block, 0, s>>>(l);
+        });
+        EFGS_HIP_CHECK(hipGetLastError());
+    }
+    return true;
+}
+
+bool embedding_gradient_fits(const EmbeddingArgs& a) {
+    return static_cast<uint64_t>(a.n) + a.rows <= 0xffff0000ull && sum_blocks(a) <= max_blocks;
+}
+
+size_t embedding_gradient_bytes(const EmbeddingArgs& a) { return GradientLayout::carve(nullptr, a).bytes; }
+
+bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uint32_t padding, void* gradient, void* workspace, hipStream_t s) {
+    if (a.rows == 0 || a.columns == 0) return true;
+    const GradientLayout l = GradientLayout::carve(static_cast<char*>(workspace), a);
+    uint32_t current = 0;
+    if (a.n > 0) {
+        SortPass p;
+        p.indices = a.indices;
+        p.table = l.table;
+        p.n = a.n;
+        p.rows = a.rows;
+        p.padding = padding;
+        p.tiles_per_block = sort_tiles_per_block(a.n);
+        const uint32_t blocks = div_up(a.n, static_cast<uint64_t>(sort_tile) * p.tiles_per_block);
+        const uint32_t bits = bit_width(a.rows), passes = bits > 8 ? div_up(bits, 8) : 1u, digit_bits = div_up(bits, passes);
+        p.digit_mask = (1u << digit_bits) - 1u;
+        for (uint32_t k = 0; k < passes; k++) {
+            p.shift = k * digit_bits;
+            p.keys_in = l.keys[current];
+            p.values_in = l.values[current];
+            if (k > 0) current ^= 1u;
+            p.keys_out = l.keys[current];
+            p.values_out = l.values[current];
+            if (k > 0) {
+                sort_count_kernel<uint8_t><<<blocks, sort_block, 0, s>>>(p);
+                sort_scatter_kernel<uint8_t><<<blocks, sort_block, 0, s>>>(p);
+            } else if (a.index_bytes == 4) {
+                sort_count_kernel<int32_t><<<blocks, sort_block, 0, s>>>(p);
+                sort_scatter_kernel<int32_t><<<blocks, sort_block, 0, s>>>(p);
+            } else {
+                sort_count_kernel<int64_t><<<blocks, sort_block, 0, s>>>(p);
+                sort_scatter_kernel<int64_t><<<blocks, sort_block, 0, s>>>(p);
+            }
+            EFGS_HIP_CHECK(hipGetLastError());
+        }
+    }
+    SumArgs u;
+    u.keys = l.keys[current];
+    u.values = l.values[current];
+    u.grad_out = grad_out;
+    u.gradient = gradient;
+    u.heads = l.heads;
+    u.tails = l.tails;
+    u.closed = l.closed;
+    u.first_row = l.first_row;
+    u.n = a.n;
+    u.rows = a.rows;
+    u.columns = a.columns;
+    u.padded_columns = l.padded_columns;
+    u.blocks = sum_blocks(a);
+    u.scale = a.scale;
+    const uint32_t lanes = lanes_of_row(a);
+    with_type(a.type, [&](auto t) {
+        using T = decltype(t);
+        switch (group_lanes(a)) {
+            case 1: launch_sums<T, 1>(u, lanes, s); break;
+            case 2: launch_sums<T, 2>(u, lanes, s); break;
+            case 4: launch_sums<T, 4>(u, lanes, s); break;
+            case 8: launch_sums<T, 8>(u, lanes, s); break;
+            case 16: launch_sums<T, 16>(u, lanes, s); break;
+            case 32: launch_sums<T, 32>(u, lanes, s); break;
+            default: launch_sums<T, 64>(u, lanes, s); break;
+        }
+    });
+    EFGS_HIP_CHECK(hipGetLastError());
+    return true;
+}
+
+}  // namespace efgs

@@ -209,6 +209,73 @@ struct AdamGroupDevice {
 };
 bool launch_adam(const AdamGroupDevice* groups, int n_groups, hipStream_t s);
 
+// ---- AdamW over many tensors ------------------------------------------------------------------------------------
+enum ElementType { type_float = 0, type_bfloat16 = 1, type_half = 2 };
+constexpr uint32_t adamw_max_tensors = 40, adamw_max_groups = 8;  // per launch (4 KB of kernel arguments)
+constexpr uint32_t moments_max_tensors = 64, norm_max_tensors = 64;
+constexpr uint32_t adamw_max_blocks = 1u << 23;  // per launch, unless a tensor alone has more
+constexpr int64_t adamw_max_elements = 1ll << 33;  // of a tensor
+struct AdamWTensorDevice {  // no empty tensors
+    void* param;
+    const void* grad;
+    void* m;                // 32-bit states: float; 8-bit: codes of u = m / r
+    void* v;                // 32-bit states: float; 8-bit: codes of r = sqrt(v)
+    float* scale;           // 8-bit: per 256 elements
+    uint64_t n;
+    float step_factor;      // 1 / (1 - beta1^t)
+    float root_factor;      // 1 / sqrt(1 - beta2^t)
+    float ratio_decode;     // 8-bit: bound of u when it was coded over its top code's value
+    uint32_t key;           // 8-bit: dither key of the step
+    uint32_t group;
+    uint16_t param_type, grad_type;
+};
+struct AdamWGroupDevice {
+    float lrs[adam_max_lrs], decays[adam_max_lrs];  // lr, 1 - lr wd
+    float beta1, beta1_rest, beta2, beta2_rest, eps;
+    float ratio_encode;     // 8-bit: the top code's value over the bound of u
+    uint32_t n_lrs;
+};
+struct AdamWMomentsDevice {
+    const uint8_t* ratios;
+    const uint8_t* roots;
+    const float* scale;
+    float* m;
+    float* v;
+    uint64_t n;
+    float ratio_decode;
+};
+struct NormTensorDevice {
+    const void* data;
+    uint64_t n_and_type;    // elements << 2 | ElementType
+};
+constexpr double adamw_ratio_top = 0.96484375;  // value of the top code of |u| (31/32 - 2^-8)
+// hash of 32 bits: two rounds of a shifted xor and an odd factor
+__host__ __device__ inline uint32_t adamw_mix(uint32_t x) {
+    x = (x ^ (x >> 16)) * 0x6C8E9CF5u;
+    x = (x ^ (x >> 15)) * 0x3A2F4D1Bu;
+    return x ^ (x >> 16);
+}
+bool launch_adamw(const AdamWTensorDevice* tensors, uint64_t n_tensors, const AdamWGroupDevice* groups, int bits, const float* grad_norm,
+                  float max_grad_norm, hipStream_t s);
+bool launch_adamw_moments(const AdamWMomentsDevice* tensors, uint64_t n_tensors, hipStream_t s);
+uint64_t norm_partials_of(uint64_t n);  // doubles that a tensor of n elements takes of `partials`
+bool launch_grad_norm(const NormTensorDevice* tensors, uint64_t n_tensors, double* partials, float* norm, hipStream_t s);
+
+// ---- rows of a table by index -----------------------------------------------------------------------------------
+struct EmbeddingArgs {
+    const void* indices;
+    int index_bytes;        // 4 or 8 (signed)
+    int type;               // ElementType of the table, the output and the gradients
+    uint32_t n, rows, columns;
+    float scale;
+};
+constexpr int64_t embedding_max = (1ll << 31) - 1;  // indices, rows, columns
+bool launch_embedding_lookup(const EmbeddingArgs& a, const void* table, uint64_t row_stride, void* out, hipStream_t s);
+bool embedding_gradient_fits(const EmbeddingArgs& a);     // whether the launches can count its items
+size_t embedding_gradient_bytes(const EmbeddingArgs& a);  // of `workspace`
+// every row of `gradient` is written; `padding`: a row that gets no gradient (>= rows: none)
+bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uint32_t padding, void* gradient, void* workspace, hipStream_t s);
+
 // ---- MCMC densification ---------------------------------------------------------------------------------------
 constexpr uint32_t mcmc_max_samples = 50;  // samples per relocated Gaussian (larger counts are clamped)
 bool launch_add_noise(const float* raw_scales, const float* raw_rotations, const float* raw_opacities, float* means, uint32_t n, float lr,

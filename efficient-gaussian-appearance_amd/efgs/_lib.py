@@ -50,6 +50,26 @@ class AdamGroup(ctypes.Structure):
                 ('beta1', ctypes.c_double), ('beta2', ctypes.c_double), ('eps', ctypes.c_double)]
 
 
+class AdamWGroup(ctypes.Structure):
+    _fields_ = [('lrs', ctypes.c_double * 7), ('beta1', ctypes.c_double), ('beta2', ctypes.c_double), ('eps', ctypes.c_double),
+                ('weight_decay', ctypes.c_double), ('n_lrs', ctypes.c_int32), ('state_bits', ctypes.c_int32)]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [('param', ctypes.c_void_p), ('grad', ctypes.c_void_p), ('exp_avg', ctypes.c_void_p), ('exp_avg_sq', ctypes.c_void_p),
+                ('root_scale', ctypes.c_void_p), ('ratio_bound', ctypes.c_double), ('n_elements', ctypes.c_int64), ('step', ctypes.c_int64),
+                ('group', ctypes.c_int32), ('param_type', ctypes.c_int32), ('grad_type', ctypes.c_int32), ('pad_', ctypes.c_int32)]
+
+
+class AdamWState(ctypes.Structure):
+    _fields_ = [('ratios', ctypes.c_void_p), ('roots', ctypes.c_void_p), ('root_scale', ctypes.c_void_p), ('exp_avg', ctypes.c_void_p),
+                ('exp_avg_sq', ctypes.c_void_p), ('ratio_bound', ctypes.c_double), ('n_elements', ctypes.c_int64)]
+
+
+class NormTensor(ctypes.Structure):
+    _fields_ = [('data', ctypes.c_void_p), ('n_elements', ctypes.c_int64), ('type', ctypes.c_int32), ('pad_', ctypes.c_int32)]
+
+
 class Workspace(ctypes.Structure):
     _fields_ = [('base', ctypes.c_void_p), ('capacity', ctypes.c_size_t), ('used', ctypes.c_size_t), ('requested', ctypes.c_size_t),
                 ('fallback', ctypes.c_void_p), ('fallback_ctx', ctypes.c_void_p)]
@@ -81,7 +101,8 @@ EXPORTED = ('efgs_last_error', 'efgs_set_rtc_dirs', 'efgs_rasterizer_create', 'e
             'efgs_set_residual_mlp', 'efgs_mlp_param_count', 'efgs_forward', 'efgs_forward_no_backward', 'efgs_backward', 'efgs_adam_step',
             'efgs_get_frame_views', 'efgs_get_frame_tile_views', 'efgs_precompile', 'efgs_set_stage_timing', 'efgs_get_stage_times', 'efgs_workspace_alloc',
             'efgs_neural_decode_forward', 'efgs_neural_decode_backward', 'efgs_neural_decode_backward_no_alloc', 'efgs_add_noise', 'efgs_relocation_adjustment', 'efgs_render', 'efgs_update_pruning_scores',
-            'efgs_ngsplat_layout', 'efgs_ngsplat_pack')
+            'efgs_ngsplat_layout', 'efgs_ngsplat_pack', 'efgs_adamw_step', 'efgs_adamw_moments', 'efgs_adamw_ratio_bound', 'efgs_grad_norm',
+            'efgs_embedding_forward', 'efgs_embedding_backward')
 
 # stage ids of efgs_get_stage_times, in order (include/efgs.h)
 STAGES = ('preprocess_forward', 'compact', 'counter_read', 'create_instances', 'tile_offsets', 'tile_buckets', 'tile_sort',
@@ -124,6 +145,18 @@ lib.efgs_add_noise.argtypes = [ctypes.c_int64] + [ctypes.c_void_p] * 4 + [ctypes
 lib.efgs_relocation_adjustment.argtypes = [ctypes.c_int64] + [ctypes.c_void_p] * 5 + [ctypes.c_void_p]
 lib.efgs_ngsplat_layout.argtypes = [ctypes.POINTER(NgsplatInput), ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]
 lib.efgs_ngsplat_pack.argtypes = [ctypes.POINTER(NgsplatInput), ctypes.POINTER(NgsplatOutput), ALLOC_FN, ctypes.c_void_p, ctypes.c_void_p]
+
+lib.efgs_adamw_step.argtypes = [ctypes.POINTER(AdamWTensor), ctypes.c_int64, ctypes.POINTER(AdamWGroup), ctypes.c_int, ctypes.c_void_p,
+                                ctypes.c_double, ctypes.c_uint32, ctypes.c_void_p]
+lib.efgs_adamw_moments.argtypes = [ctypes.POINTER(AdamWState), ctypes.c_int64, ctypes.c_void_p]
+lib.efgs_adamw_ratio_bound.restype = ctypes.c_double
+lib.efgs_adamw_ratio_bound.argtypes = [ctypes.c_double, ctypes.c_double]
+lib.efgs_grad_norm.argtypes = [ctypes.POINTER(NormTensor), ctypes.c_int64, ctypes.c_void_p, ALLOC_FN, ctypes.c_void_p, ctypes.c_void_p]
+lib.efgs_embedding_forward.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                       ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]
+lib.efgs_embedding_backward.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                        ctypes.c_int, ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, ALLOC_FN, ctypes.c_void_p,
+                                        ctypes.c_void_p]
 
 
 def check(rc: int) -> None:

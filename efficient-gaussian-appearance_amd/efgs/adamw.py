@@ -1,0 +1,115 @@
+"""AdamW over many tensors at once, with states in 32 or in 8 bits, clipped by the norm of all gradients without a wait of
+the host. No counterpart in the reference, whose optimizer is `FusedAdam` (one float32 tensor per group, no weight decay).
+"""
+from __future__ import annotations
+
+import copy
+from typing import Any, Callable, Iterable, Sequence
+
+import torch
+
+from . import _native
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay): per element, c the clipping coefficient and t the parameter's step,
+
+        g = c grad, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+    in 32 bits, p rounded once to its type. Parameters and gradients are contiguous float32, bfloat16 or float16 GPU tensors
+    (a gradient that is not contiguous is copied); a launch takes 40 tensors, whatever groups they are in.
+
+    lr, betas, eps, weight_decay, state_bits: defaults that a group may override. `lr` is a float or a list of up to 7 rates
+    cycled over the last dimension's columns, as `FusedAdam` has them.
+
+    state_bits 32: states `exp_avg` and `exp_avg_sq` (float32), as torch.optim.AdamW names them. 8: m / sqrt(v) and sqrt(v) as
+    bytes `exp_avg_ratio` and `exp_avg_sq_root` with one float per 256 elements (`root_scale`; the codes are described in
+    efgs.h), rounded by a dither from (element, step, seed) so that they are right in the mean; 16 bytes of traffic an
+    element and step for float32 parameters in place of 28. They need beta1^2 < beta2. `moments` reads either as float32.
+
+    max_grad_norm: if set, gradients count times min(1, max_grad_norm / (norm + 1e-6)), norm over all gradients of the step (they
+    themselves stay as they are); where the norm is not finite, parameters and moments stay as they are. The
+    norm is read on the device and left in `grad_norm` (a tensor of no dimensions; None before the first such step).
+
+    The step count is the host's, so a step cannot be captured into a graph.
+    """
+
+    def __init__(self, params: Iterable, lr: float | Sequence[float] = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, max_grad_norm: float | None = None, seed: int = 0) -> None:
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f'efgs: max_grad_norm must be positive, got {max_grad_norm}')
+        self.max_grad_norm = max_grad_norm
+        self.seed = int(seed)
+        self.grad_norm: torch.Tensor | None = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, param_group: dict[str, Any]) -> None:
+        super().add_param_group(param_group)
+        try:
+            _native_group(self.param_groups[-1])
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    @torch.no_grad()
+    def step(self, closure: Callable[[], Any] | None = None) -> Any:
+        """One step of every parameter that has a gradient; returns what `closure` (re-evaluated first, if given) returns."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('efgs: AdamW counts its steps on the host and cannot be captured into a graph')
+        self.grad_norm = _native.adamw_step([_native_group(g) for g in self.param_groups], self.state, self.max_grad_norm, self.seed & 0xffffffff)
+        return loss
+
+    def moments(self, params: torch.Tensor | Sequence[torch.Tensor]) -> Any:
+        """(exp_avg, exp_avg_sq) in float32 of a parameter, or a list of them for a sequence of parameters: 32-bit states
+        themselves, new tensors for 8-bit ones."""
+        if isinstance(params, torch.Tensor):
+            return _native.adamw_moments([params], self.state)[0]
+        return _native.adamw_moments(list(params), self.state)
+
+    def load_state_dict(self, state_dict: dict[str, Any]) -> None:
+        super().load_state_dict(state_dict)
+        # (the base class casts every floating state to its parameter's type, and bytes too)
+        saved_ids = [i for g in state_dict['param_groups'] for i in g['params']]
+        params = [p for g in self.param_groups for p in g['params']]
+        for i, p in zip(saved_ids, params):
+            if i not in state_dict['state']:
+                continue
+            own = {}
+            for key, value in state_dict['state'][i].items():
+                if key == 'step':
+                    own[key] = int(value)
+                elif isinstance(value, torch.Tensor):
+                    own[key] = value.detach().to(p.device).clone()
+                else:
+                    own[key] = copy.deepcopy(value)
+            self.state[p] = own
+
+
+def _native_group(group: dict[str, Any]) -> tuple:
+    lr = group['lr']
+    lrs = [float(x) for x in lr] if isinstance(lr, (list, tuple)) else [float(lr)]
+    if not 1 <= len(lrs) <= 7:
+        raise ValueError('efgs: between 1 and 7 learning rates are supported')
+    beta1, beta2 = (float(b) for b in group['betas'])
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError(f'efgs: betas must lie in [0, 1), got {(beta1, beta2)}')
+    eps = float(group['eps'])
+    if not eps >= 0.0:
+        raise ValueError(f'efgs: eps must not be negative, got {eps}')
+    bits = group['state_bits']
+    if bits not in (8, 32):
+        raise ValueError(f'efgs: state_bits must be 32 or 8, got {bits}')
+    if bits == 8 and not beta1 * beta1 < beta2:
+        raise ValueError(f'efgs: 8-bit states need beta1^2 < beta2, got {(beta1, beta2)}')
+    return group['params'], lrs, beta1, beta2, eps, float(group['weight_decay']), int(bits)
+
+
+def grad_norm(tensors: torch.Tensor | Iterable[torch.Tensor]) -> torch.Tensor:
+    """The 2-norm over all elements of `tensors` (float32, bfloat16 or float16 on one GPU device) as a float32 tensor of no
+    dimensions: summed in 64 bits in a fixed order, without a wait of the host."""
+    return _native.grad_norm([tensors] if isinstance(tensors, torch.Tensor) else list(tensors))

@@ -277,6 +277,81 @@ int efgs_ngsplat_layout(const efgs_ngsplat_input* in, int* n_textures, int* texe
  * (pack_sh_quantized) and :624-765 (SV / NASG / NASGabor payloads). */
 int efgs_ngsplat_pack(const efgs_ngsplat_input* in, efgs_ngsplat_output* out, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
 
+/* ---- training operators beside the rasterizer (no counterparts in the reference) ---- */
+
+/* element types of the operators below */
+enum { EFGS_FLOAT = 0, EFGS_BFLOAT16 = 1, EFGS_HALF = 2 };
+
+/* One AdamW step (decoupled weight decay) over many tensors, 40 to a launch. Per element, t the tensor's step from 1:
+ *   g = c grad, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * with lr cycled by element index over the group's n_lrs rates, in 32 bits, p rounded once to its type.
+ * Clipping: with grad_norm (device, one float: efgs_grad_norm of all gradients) c = min(1, max_grad_norm / (*grad_norm + 1e-6)),
+ * read on the device; where *grad_norm is not finite the step changes nothing. Without it c = 1.
+ * States of 32 bits are m and v. States of 8 bits are codes of u = m / sqrt(v) (exp_avg) and of r = sqrt(v)
+ * (exp_avg_sq), one byte each, and one float per 256 elements (root_scale): zeros to begin with. r of element i is
+ * (f((code + 1776) << 19) - 2^-16) root_scale[i / 256] and |u| (f(((code & 127) + 1904) << 19) - 2^-8) ratio_bound / 0.96484375, f the float
+ * of these bits, u's sign the code's top bit. ratio_bound is efgs_adamw_ratio_bound of the betas with which the
+ * state was written (the step writes it for its group's betas), and needs beta1^2 < beta2. Codes are rounded by a dither from (element, step,
+ * seed), unbiased; results do not depend on the tensors that share a call. An element whose new v is not finite has a zero state.
+ * Tensors are contiguous, of any alignment of their type. Stream-ordered; nothing is kept of the arguments. */
+typedef struct efgs_adamw_group {
+    double lrs[7];
+    double beta1, beta2, eps, weight_decay;
+    int32_t n_lrs;
+    int32_t state_bits;      /* 32 or 8 */
+} efgs_adamw_group;
+typedef struct efgs_adamw_tensor {
+    void* param;             /* param_type, updated */
+    const void* grad;        /* grad_type */
+    void* exp_avg;           /* float, or 8-bit codes of u; updated */
+    void* exp_avg_sq;        /* float, or 8-bit codes of r; updated */
+    float* root_scale;       /* 8 bits: ceil(n / 256) floats, updated */
+    double ratio_bound;      /* 8 bits: of the state as it is */
+    int64_t n_elements;      /* up to 2^33 */
+    int64_t step;
+    int32_t group;
+    int32_t param_type, grad_type;
+    int32_t pad_;
+} efgs_adamw_tensor;
+int efgs_adamw_step(const efgs_adamw_tensor* tensors, int64_t n_tensors, const efgs_adamw_group* groups, int n_groups, const float* grad_norm,
+                    double max_grad_norm, uint32_t seed, void* stream);
+
+/* Bound of |m| / sqrt(v) for these betas: (1 - beta1) / sqrt((1 - beta2) (1 - beta1^2 / beta2)). */
+double efgs_adamw_ratio_bound(double beta1, double beta2);
+
+/* The moments m and v (float) that 8-bit states stand for. */
+typedef struct efgs_adamw_state {
+    const uint8_t* ratios;   /* codes of u */
+    const uint8_t* roots;    /* codes of r */
+    const float* root_scale;
+    float* exp_avg;          /* written */
+    float* exp_avg_sq;       /* written */
+    double ratio_bound;
+    int64_t n_elements;
+} efgs_adamw_state;
+int efgs_adamw_moments(const efgs_adamw_state* states, int64_t n_states, void* stream);
+
+/* norm (device, one float) = sqrt of the sum of the squares of all tensors' elements, summed in 64 bits in a fixed order.
+ * Its partial sums come from `alloc` (8 bytes per 4,096 elements). Stream-ordered. */
+typedef struct efgs_norm_tensor {
+    const void* data;
+    int64_t n_elements;
+    int32_t type;
+    int32_t pad_;
+} efgs_norm_tensor;
+int efgs_grad_norm(const efgs_norm_tensor* tensors, int64_t n_tensors, float* norm, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
+
+/* out (n x columns) = scale table[indices] in 32 bits, rounded once to `type`; an index outside [0, rows) gives a zero row.
+ * indices: n int32 or int64 (index_bytes 4 or 8); table: rows of `columns` elements, row_stride elements apart. */
+int efgs_embedding_forward(const void* indices, int index_bytes, int64_t n, const void* table, int64_t rows, int64_t columns, int64_t row_stride,
+                           int type, float scale, void* out, void* stream);
+/* grad_table (rows x columns, every row written) = per row scale times the sum of grad_out's rows (n x columns) whose index it is, in
+ * 32 bits in an order that the indices give (the same results every time); rows that no index meets are zero, and so is
+ * padding_row (outside [0, rows): none). Scratch from `alloc`. Stream-ordered, no host synchronisation. */
+int efgs_embedding_backward(const void* indices, int index_bytes, int64_t n, const void* grad_out, int64_t rows, int64_t columns, int type,
+                            float scale, int64_t padding_row, void* grad_table, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
+
 /* Standalone neural decode: the configured residual MLP (efgs_set_residual_mlp, model 5) on n primitives'
  * features (n x n_features, the learned latents), base colours (n x 3, read with base input only) and unit
  * view directions (n x 3; not read, and may be NULL, when the encoding has no SH degree), encoded as in the
