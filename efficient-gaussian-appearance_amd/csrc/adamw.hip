@@ -1,5 +1,5 @@
 // AdamW over many tensors at once, with states in 32 or in 8 bits, the decoding of 8-bit states, and the gradient norm
-// over many tensors that clips a step. A launch takes the descriptors of up to 40 tensors as kernel arguments (nothing is
+// over many tensors that clips a step. A launch takes the descriptors of 60 to 72 tensors as kernel arguments (nothing is
 // copied to the device and nothing has to outlive the call); a block finds its tensor from the first blocks of all.
 //
 // Per element, t the step, c the clipping coefficient min(1, max_norm / (norm + 1e-6)):
@@ -21,6 +21,8 @@
 // An element whose new r is not finite (a gradient that is not, or whose square overflows) gets the update that the formula
 // gives and a zero state, and does not count in its block's maximum: its neighbours keep theirs. Contraction is off for
 // this file: every operation of the 8-bit state is rounded by itself, so that the codes follow from the formulas above.
+#include <type_traits>
+
 #include "internal.h"
 
 namespace efgs {
@@ -39,10 +41,11 @@ template <> struct Vector4<float> { using type = float4u; };
 template <> struct Vector4<_Float16> { using type = half4u; };
 template <> struct Vector4<__bf16> { using type = bfloat4u; };
 
-// x[0..3] = p[0..3] in 32 bits; past `count` zeros
-template <typename T>
+// x[0..3] = p[0..3] in 32 bits; past `count` zeros. WHOLE: the block lies within its tensor (known for all its threads, so that its
+// loads stand in no branch).
+template <bool WHOLE, typename T>
 __device__ __forceinline__ void load4(const T* p, uint32_t count, float* x) {
-    if (count >= 4) {
+    if (WHOLE || count >= 4) {
         const typename Vector4<T>::type v = *reinterpret_cast<const typename Vector4<T>::type*>(p);
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = static_cast<float>(v[k]);
@@ -53,9 +56,9 @@ __device__ __forceinline__ void load4(const T* p, uint32_t count, float* x) {
 }
 
 // rounded to nearest even, what a cast of a tensor does
-template <typename T>
+template <bool WHOLE, typename T>
 __device__ __forceinline__ void store4(T* p, uint32_t count, const float* x) {
-    if (count >= 4) {
+    if (WHOLE || count >= 4) {
         typename Vector4<T>::type v;
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = static_cast<T>(x[k]);
@@ -67,8 +70,9 @@ __device__ __forceinline__ void store4(T* p, uint32_t count, const float* x) {
     }
 }
 
+template <bool WHOLE>
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, uint32_t count) {
-    if (count >= 4) return *reinterpret_cast<const uint32u*>(p);
+    if (WHOLE || count >= 4) return *reinterpret_cast<const uint32u*>(p);
     uint32_t v = 0;
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++)
@@ -76,8 +80,9 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, uint32_t count)
     return v;
 }
 
+template <bool WHOLE>
 __device__ __forceinline__ void store_codes(uint8_t* p, uint32_t count, uint32_t v) {
-    if (count >= 4) {
+    if (WHOLE || count >= 4) {
         *reinterpret_cast<uint32u*>(p) = v;
         return;
     }
@@ -98,68 +103,91 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return max(static_cast<uint32_t>(b[0]), static_cast<uint32_t>(b[1]));
 }
 
-// the last of the n (<= 64) tensors whose first block is at most `block`
+// the last of the n tensors whose first block is at most `block`
+template <uint32_t MAX>
 __device__ __forceinline__ uint32_t tensor_of_block(const uint32_t* first_block, uint32_t n, uint32_t block) {
     const uint32_t lane = threadIdx.x & 63u;
-    const bool at_most = lane < n && first_block[lane] <= block;
-    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(__popcll(__ballot(at_most)))) - 1u;
+    uint32_t count = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < MAX; k += 64) {
+        if (k > 0 && k >= n) break;
+        count += static_cast<uint32_t>(__popcll(__ballot(k + lane < n && first_block[min(k + lane, MAX - 1)] <= block)));
+    }
+    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(count))) - 1u;
 }
 
+template <int BITS>
 struct AdamWLaunch {
-    uint32_t first_block[adamw_max_tensors];
-    AdamWTensorDevice tensors[adamw_max_tensors];
+    static constexpr uint32_t max_tensors = BITS == 32 ? 72 : 60;
+    using Tensor = std::conditional_t<BITS == 32, AdamWTensor, AdamWTensor8>;
+    uint32_t first_block[max_tensors];
+    Tensor tensors[max_tensors];
     AdamWGroupDevice groups[adamw_max_groups];
     const float* grad_norm;  // null: gradients as they are
     float max_grad_norm;
     uint32_t n_tensors;
 };
-static_assert(sizeof(AdamWLaunch) <= 4096, "kernel arguments");
+static_assert(sizeof(AdamWLaunch<32>) <= 4096 && sizeof(AdamWLaunch<8>) <= 4096, "kernel arguments");
 
 // the clipping coefficient; false where the norm is not finite (the step is left out)
-__device__ __forceinline__ bool clipping(const AdamWLaunch& L, float& coefficient) {
+__device__ __forceinline__ bool clipping(const float* grad_norm, float max_grad_norm, float& coefficient) {
     coefficient = 1.0f;
-    if (!L.grad_norm) return true;
-    const float norm = *L.grad_norm;
-    coefficient = fminf(L.max_grad_norm / (norm + 1e-6f), 1.0f);
+    if (!grad_norm) return true;
+    const float norm = *grad_norm;
+    coefficient = fminf(max_grad_norm / (norm + 1e-6f), 1.0f);
     return norm < INFINITY;
 }
 
-// learning rate and decay of element i, whose position in the cycle of learning rates is `column`
-__device__ __forceinline__ float updated(const AdamWGroupDevice& G, const AdamWTensorDevice& T, float p, float m, float root, uint32_t column) {
-    const float update = m / (root * T.root_factor + G.eps);
-    return p * G.decays[column] - G.lrs[column] * T.step_factor * update;
+// The parameter after the step. The reciprocal is the hardware's (1 ulp): the division's last bit would be
+// 6e-8 of the update, for about ten operations an element. root is 0 or at least 3e-23, a float's least square root, so that
+// the sum is no denormal unless eps alone is one.
+__device__ __forceinline__ float updated(const AdamWGroupDevice& G, float p, float m, float root, float rate, float decay) {
+    const float update = m * __builtin_amdgcn_rcpf(root * G.root_factor + G.eps);
+    return p * decay - rate * update;
 }
 
-// position in the cycle of learning rates of the thread's first element
-__device__ __forceinline__ uint32_t first_column(const AdamWGroupDevice& G, uint64_t block_base, uint32_t offset) {
-    if (G.n_lrs == 1) return 0;
-    return (static_cast<uint32_t>(block_base % G.n_lrs) + offset) % G.n_lrs;
+// Learning rates of four consecutive elements: the group's one, or from the table of its cycle (in LDS, rate and decay).
+struct Rates {
+    float2 of[4];
+};
+template <bool CYCLE>
+__device__ __forceinline__ Rates rates_of(const AdamWGroupDevice& G, const float2* cycle, uint32_t first_column) {
+    Rates r;
+    uint32_t column = first_column;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (CYCLE) {
+            r.of[k] = cycle[column];
+            column = column + 1 == G.n_lrs ? 0 : column + 1;
+        } else {
+            r.of[k] = make_float2(G.rates[0], G.decays[0]);
+        }
+    }
+    return r;
 }
 
-__device__ __forceinline__ uint32_t next_column(const AdamWGroupDevice& G, uint32_t column) { return column + 1 == G.n_lrs ? 0 : column + 1; }
-
-template <typename P, typename D>
-__device__ __forceinline__ void step32(const AdamWTensorDevice& T, const AdamWGroupDevice& G, uint32_t block, float coefficient) {
-    const uint64_t base = static_cast<uint64_t>(block) * adamw_block * 4, i = base + threadIdx.x * 4u;
-    if (i >= T.n) return;
-    const uint32_t count = T.n - i >= 4 ? 4u : static_cast<uint32_t>(T.n - i);
+template <bool WHOLE, bool CYCLE, typename P, typename D>
+__device__ __forceinline__ void step_block(const AdamWTensor& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
+                                           float coefficient) {
+    const uint64_t i = base + threadIdx.x * 4u;
+    if (!WHOLE && i >= n) return;
+    const uint32_t count = WHOLE || n - i >= 4 ? 4u : static_cast<uint32_t>(n - i);
     float p[4], g[4], m[4], v[4];
-    load4(static_cast<const D*>(T.grad) + i, count, g);
-    load4(static_cast<const float*>(T.m) + i, count, m);
-    load4(static_cast<const float*>(T.v) + i, count, v);
-    load4(static_cast<const P*>(T.param) + i, count, p);
-    uint32_t column = first_column(G, base, threadIdx.x * 4u);
+    load4<WHOLE>(static_cast<const D*>(T.grad) + i, count, g);
+    load4<WHOLE>(static_cast<const float*>(T.m) + i, count, m);
+    load4<WHOLE>(static_cast<const float*>(T.v) + i, count, v);
+    load4<WHOLE>(static_cast<const P*>(T.param) + i, count, p);
+    const Rates rates = rates_of<CYCLE>(G, cycle, column);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const float gk = g[k] * coefficient;
         m[k] = G.beta1 * m[k] + G.beta1_rest * gk;
         v[k] = G.beta2 * v[k] + G.beta2_rest * (gk * gk);
-        p[k] = updated(G, T, p[k], m[k], sqrtf(v[k]), column);
-        column = next_column(G, column);
+        p[k] = updated(G, p[k], m[k], sqrtf(v[k]), rates.of[k].x, rates.of[k].y);
     }
-    store4(static_cast<float*>(T.m) + i, count, m);
-    store4(static_cast<float*>(T.v) + i, count, v);
-    store4(static_cast<P*>(T.param) + i, count, p);
+    store4<WHOLE>(static_cast<float*>(T.m) + i, count, m);
+    store4<WHOLE>(static_cast<float*>(T.v) + i, count, v);
+    store4<WHOLE>(static_cast<P*>(T.param) + i, count, p);
 }
 
 // ---- 8-bit codes -----------------------------------------------------------------------------------------------------
@@ -180,76 +208,122 @@ __device__ __forceinline__ uint32_t encode(float y, float c, uint32_t dither, ui
 
 __device__ __forceinline__ uint32_t dither_of(uint32_t element, uint32_t key) { return adamw_mix(element * 0x9E3779B1u + key); }
 
-// One wave per block of 256 elements, four to a lane.
-template <typename P, typename D>
-__device__ __forceinline__ void step8(const AdamWTensorDevice& T, const AdamWGroupDevice& G, uint32_t block, float coefficient) {
+// sqrt(x) and its reciprocal's approximation for x = 0 or x >= 2^-100, rounded to nearest: one step from the hardware's reciprocal
+// square root (s = x y, s + (x - s^2) y / 2, the residual exact by the fused operation).
+__device__ __forceinline__ float rounded_sqrt(float x, float& reciprocal) {
+    reciprocal = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-100f));
+    const float s = x * reciprocal;
+    return __builtin_fmaf(__builtin_fmaf(-s, s, x), 0.5f * reciprocal, s);
+}
+
+// a / b rounded to nearest from an approximation of 1 / b (the quotient's residual exact by the fused operation)
+__device__ __forceinline__ float rounded_quotient(float a, float b, float reciprocal) {
+    const float q = a * reciprocal;
+    return __builtin_fmaf(__builtin_fmaf(-q, b, a), reciprocal, q);
+}
+
+// One wave per block of 256 elements, four to a lane. What bounds it is the vector units, not memory: about 85 operations an
+// element, of which a square root and a quotient with the library's full range would be 30 more. So they are done in five
+// and three where every element's v is zero, or at least 2^-100 and finite (a gradient of 1e-13 after one step), and by the
+// library where the wave holds another one; both round to nearest.
+template <bool WHOLE, bool CYCLE, typename P, typename D>
+__device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
+                                           float coefficient) {
     const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t group = static_cast<uint64_t>(block) * (adamw_block / 64) + (threadIdx.x >> 6), base = group * 256;
-    if (base >= T.n) return;
-    const uint64_t i = base + lane * 4u;
-    const uint32_t count = i >= T.n ? 0u : T.n - i >= 4 ? 4u : static_cast<uint32_t>(T.n - i);
+    const uint64_t i = base + threadIdx.x * 4u, first = i - lane * 4u;
+    if (!WHOLE && first >= n) return;
+    const uint32_t count = !WHOLE && i >= n ? 0u : WHOLE || n - i >= 4 ? 4u : static_cast<uint32_t>(n - i);
     uint8_t* const ratios = static_cast<uint8_t*>(T.m) + i;
     uint8_t* const roots = static_cast<uint8_t*>(T.v) + i;
-    float p[4], g[4], r[4], u[4];
-    load4(static_cast<const D*>(T.grad) + i, count, g);
-    const uint32_t ratio_codes = load_codes(ratios, count), root_codes = load_codes(roots, count);
-    load4(static_cast<const P*>(T.param) + i, count, p);
-    const float scale = T.scale[group];
-    uint32_t column = first_column(G, base, lane * 4u);
-    uint32_t top = 0;
+    float p[4], g[4], m[4], v[4], r[4], u[4];
+    load4<WHOLE>(static_cast<const D*>(T.grad) + i, count, g);
+    const uint32_t ratio_codes = load_codes<WHOLE>(ratios, count), root_codes = load_codes<WHOLE>(roots, count);
+    load4<WHOLE>(static_cast<const P*>(T.param) + i, count, p);
+    const float scale = T.scale[first / 256];
+    const Rates rates = rates_of<CYCLE>(G, cycle, column);
+    bool plain = true;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const float gk = g[k] * coefficient;
         const float old = decode_root((root_codes >> (8 * k)) & 255u, scale);
-        const float m = G.beta1 * (decode_ratio((ratio_codes >> (8 * k)) & 255u, T.ratio_decode) * old) + G.beta1_rest * gk;
-        r[k] = sqrtf(G.beta2 * (old * old) + G.beta2_rest * (gk * gk));
-        p[k] = updated(G, T, p[k], m, r[k], column);
-        column = next_column(G, column);
-        r[k] = r[k] < INFINITY && static_cast<uint32_t>(k) < count ? r[k] : 0.0f;
-        u[k] = r[k] > 0.0f ? m / r[k] : 0.0f;
-        top = max(top, __float_as_uint(r[k]));
+        m[k] = G.beta1 * (decode_ratio((ratio_codes >> (8 * k)) & 255u, G.ratio_decode) * old) + G.beta1_rest * gk;
+        v[k] = G.beta2 * (old * old) + G.beta2_rest * (gk * gk);
+        // (past the tensor's end: code 0 and gradient 0 make 0)
+        plain = plain && ((v[k] >= 0x1p-100f && v[k] < INFINITY) || v[k] == 0.0f);
     }
+    if (__ballot(!plain) == 0) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float reciprocal;
+            r[k] = rounded_sqrt(v[k], reciprocal);
+            u[k] = v[k] > 0.0f ? rounded_quotient(m[k], r[k], reciprocal) : 0.0f;
+            p[k] = updated(G, p[k], m[k], r[k], rates.of[k].x, rates.of[k].y);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            r[k] = sqrtf(v[k]);
+            p[k] = updated(G, p[k], m[k], r[k], rates.of[k].x, rates.of[k].y);
+            r[k] = r[k] < INFINITY ? r[k] : 0.0f;
+            u[k] = r[k] > 0.0f ? m[k] / r[k] : 0.0f;
+        }
+    }
+    const uint32_t top = max(max(__float_as_uint(r[0]), __float_as_uint(r[1])), max(__float_as_uint(r[2]), __float_as_uint(r[3])));
     float new_scale = __uint_as_float(wave_max(top)) * (1.0f / root_top);
     if (new_scale < least_scale) new_scale = 0.0f;
-    const float inverse = new_scale > 0.0f ? 1.0f / new_scale : 0.0f;
+    const float inverse = new_scale > 0.0f ? rounded_quotient(1.0f, new_scale, __builtin_amdgcn_rcpf(new_scale)) : 0.0f;
     uint32_t new_ratios = 0, new_roots = 0;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const uint32_t h = dither_of(static_cast<uint32_t>(i) + k, T.key);
+        const uint32_t h = dither_of(static_cast<uint32_t>(i) + k, G.key);
         new_roots |= encode(r[k] * inverse, root_c, h & 0xffffu, root_base, 255u) << (8 * k);
         const float y = fminf(fabsf(u[k]) * G.ratio_encode, ratio_top);
-        new_ratios |= (encode(y, ratio_c, h >> 16, ratio_base, 127u) | (u[k] < 0.0f ? 128u : 0u)) << (8 * k);
+        new_ratios |= (encode(y, ratio_c, h >> 16, ratio_base, 127u) | ((__float_as_uint(u[k]) >> 24) & 128u)) << (8 * k);
     }
-    store4(static_cast<P*>(T.param) + i, count, p);
-    store_codes(ratios, count, new_ratios);
-    store_codes(roots, count, new_roots);
-    if (lane == 0) T.scale[group] = new_scale;
+    store4<WHOLE>(static_cast<P*>(T.param) + i, count, p);
+    store_codes<WHOLE>(ratios, count, new_ratios);
+    store_codes<WHOLE>(roots, count, new_roots);
+    if (lane == 0) T.scale[first / 256] = new_scale;
 }
 
-template <int BITS, typename P, typename D>
-__device__ __forceinline__ void step_block(const AdamWTensorDevice& T, const AdamWGroupDevice& G, uint32_t block, float coefficient) {
-    if constexpr (BITS == 32) step32<P, D>(T, G, block, coefficient);
-    else step8<P, D>(T, G, block, coefficient);
+template <bool WHOLE, bool CYCLE, typename P, typename T>
+__device__ __forceinline__ void step_gradient(const T& tensor, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
+                                              float coefficient) {
+    const uint32_t type = tensor.grad_type();
+    if (type == type_float) step_block<WHOLE, CYCLE, P, float>(tensor, G, cycle, base, n, column, coefficient);
+    else if (type == type_bfloat16) step_block<WHOLE, CYCLE, P, __bf16>(tensor, G, cycle, base, n, column, coefficient);
+    else step_block<WHOLE, CYCLE, P, _Float16>(tensor, G, cycle, base, n, column, coefficient);
 }
 
-template <int BITS, typename P>
-__device__ __forceinline__ void step_gradient(const AdamWTensorDevice& T, const AdamWGroupDevice& G, uint32_t block, float coefficient) {
-    if (T.grad_type == type_float) step_block<BITS, P, float>(T, G, block, coefficient);
-    else if (T.grad_type == type_bfloat16) step_block<BITS, P, __bf16>(T, G, block, coefficient);
-    else step_block<BITS, P, _Float16>(T, G, block, coefficient);
+template <bool WHOLE, bool CYCLE, typename T>
+__device__ __forceinline__ void step_tensor(const T& tensor, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
+                                            float coefficient) {
+    const uint32_t type = tensor.param_type();
+    if (type == type_float) step_gradient<WHOLE, CYCLE, float>(tensor, G, cycle, base, n, column, coefficient);
+    else if (type == type_bfloat16) step_gradient<WHOLE, CYCLE, __bf16>(tensor, G, cycle, base, n, column, coefficient);
+    else step_gradient<WHOLE, CYCLE, _Float16>(tensor, G, cycle, base, n, column, coefficient);
 }
 
 template <int BITS>
-__global__ __launch_bounds__(adamw_block) void adamw_kernel(AdamWLaunch L) {
+__global__ __launch_bounds__(adamw_block) void adamw_kernel(AdamWLaunch<BITS> L) {
+    __shared__ float2 cycle[adam_max_lrs];
     float coefficient;
-    if (!clipping(L, coefficient)) return;
-    const uint32_t k = tensor_of_block(L.first_block, L.n_tensors, blockIdx.x);
-    const AdamWTensorDevice& T = L.tensors[k];
-    const AdamWGroupDevice& G = L.groups[T.group];
-    const uint32_t block = blockIdx.x - L.first_block[k];
-    if (T.param_type == type_float) step_gradient<BITS, float>(T, G, block, coefficient);
-    else if (T.param_type == type_bfloat16) step_gradient<BITS, __bf16>(T, G, block, coefficient);
-    else step_gradient<BITS, _Float16>(T, G, block, coefficient);
+    if (!clipping(L.grad_norm, L.max_grad_norm, coefficient)) return;
+    const uint32_t k = tensor_of_block<AdamWLaunch<BITS>::max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
+    const auto T = L.tensors[k];
+    const AdamWGroupDevice G = L.groups[T.group()];
+    const uint64_t base = static_cast<uint64_t>(blockIdx.x - L.first_block[k]) * adamw_block * 4, n = T.n();
+    const bool whole = base + adamw_block * 4 <= n;
+    if (G.n_lrs == 1) {
+        if (whole) step_tensor<true, false>(T, G, cycle, base, n, 0u, coefficient);
+        else step_tensor<false, false>(T, G, cycle, base, n, 0u, coefficient);
+        return;
+    }
+    if (threadIdx.x < G.n_lrs) cycle[threadIdx.x] = make_float2(L.groups[T.group()].rates[threadIdx.x], L.groups[T.group()].decays[threadIdx.x]);
+    __syncthreads();
+    const uint32_t column = (static_cast<uint32_t>(base % G.n_lrs) + threadIdx.x * 4u) % G.n_lrs;
+    if (whole) step_tensor<true, true>(T, G, cycle, base, n, column, coefficient);
+    else step_tensor<false, true>(T, G, cycle, base, n, column, coefficient);
 }
 
 // ---- decoding ----------------------------------------------------------------------------------------------------------
@@ -262,12 +336,12 @@ struct MomentsLaunch {
 static_assert(sizeof(MomentsLaunch) <= 4096, "kernel arguments");
 
 __global__ __launch_bounds__(adamw_block) void adamw_moments_kernel(MomentsLaunch L) {
-    const uint32_t k = tensor_of_block(L.first_block, L.n_tensors, blockIdx.x);
+    const uint32_t k = tensor_of_block<moments_max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
     const AdamWMomentsDevice& T = L.tensors[k];
     const uint64_t i = static_cast<uint64_t>(blockIdx.x - L.first_block[k]) * adamw_block * 4 + threadIdx.x * 4u;
     if (i >= T.n) return;
     const uint32_t count = T.n - i >= 4 ? 4u : static_cast<uint32_t>(T.n - i);
-    const uint32_t ratio_codes = load_codes(T.ratios + i, count), root_codes = load_codes(T.roots + i, count);
+    const uint32_t ratio_codes = load_codes<false>(T.ratios + i, count), root_codes = load_codes<false>(T.roots + i, count);
     const float scale = T.scale[i / 256];
     float m[4], v[4];
 #pragma unroll
@@ -276,21 +350,26 @@ __global__ __launch_bounds__(adamw_block) void adamw_moments_kernel(MomentsLaunc
         m[j] = decode_ratio((ratio_codes >> (8 * j)) & 255u, T.ratio_decode) * r;
         v[j] = r * r;
     }
-    store4(T.m + i, count, m);
-    store4(T.v + i, count, v);
+    store4<false>(T.m + i, count, m);
+    store4<false>(T.v + i, count, v);
 }
 
 // ---- gradient norm -----------------------------------------------------------------------------------------------------
 
-constexpr uint32_t norm_chunk = adamw_block * 16;
+constexpr uint32_t norm_loads = 8, norm_step = adamw_block * 4 * norm_loads;  // loads of a thread at once, and a block's elements
 
 struct NormLaunch {
     uint32_t first_block[norm_max_tensors];
     NormTensorDevice tensors[norm_max_tensors];
     double* partials;
     uint32_t n_tensors;
+    uint32_t steps;  // of a block
 };
 static_assert(sizeof(NormLaunch) <= 4096, "kernel arguments");
+
+__host__ __device__ inline uint32_t norm_blocks(uint64_t n, uint32_t steps) {
+    return static_cast<uint32_t>((n + static_cast<uint64_t>(norm_step) * steps - 1) / (static_cast<uint64_t>(norm_step) * steps));
+}
 
 // sum over the block's threads in a fixed order (thread 0's result counts)
 template <uint32_t BLOCK>
@@ -306,30 +385,43 @@ __device__ __forceinline__ double block_sum(double x) {
     return sum;
 }
 
-template <typename T>
-__device__ __forceinline__ double squares(const T* data, uint64_t n, uint64_t base) {
-    double sum = 0.0;
+// eight loads `stride` elements apart
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void add_squares(const T* data, uint64_t n, uint64_t base, uint64_t stride, double* sum) {
+    float x[norm_loads][4];
 #pragma unroll
-    for (uint32_t j = 0; j < 4; j++) {
-        const uint64_t i = base + j * adamw_block * 4 + threadIdx.x * 4u;
-        float x[4];
-        load4(data + i, i >= n ? 0u : n - i >= 4 ? 4u : static_cast<uint32_t>(n - i), x);
-#pragma unroll
-        for (int k = 0; k < 4; k++) sum = __builtin_fma(static_cast<double>(x[k]), static_cast<double>(x[k]), sum);
+    for (uint32_t j = 0; j < norm_loads; j++) {
+        const uint64_t i = base + j * stride + threadIdx.x * 4u;
+        load4<WHOLE>(data + i, WHOLE ? 4u : i >= n ? 0u : n - i >= 4 ? 4u : static_cast<uint32_t>(n - i), x[j]);
     }
-    return sum;
+#pragma unroll
+    for (uint32_t j = 0; j < norm_loads; j++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) sum[k] = __builtin_fma(static_cast<double>(x[j][k]), static_cast<double>(x[j][k]), sum[k]);
+}
+
+// A tensor's blocks take its 1,024-element pieces in turn, so that at any time they read one stretch of memory: with a stretch
+// of its own for each block (32 to 128 KB apart) they met on few memory channels, and 280 MB took 98 us.
+template <typename T>
+__device__ __forceinline__ double squares(const T* data, uint64_t n, uint32_t block, uint32_t blocks) {
+    double sum[4] = {};
+    const uint64_t stride = static_cast<uint64_t>(blocks) * adamw_block * 4;
+    for (uint64_t base = static_cast<uint64_t>(block) * adamw_block * 4; base < n; base += norm_loads * stride) {
+        if (base + (norm_loads - 1) * stride + adamw_block * 4 <= n) add_squares<true>(data, n, base, stride, sum);
+        else add_squares<false>(data, n, base, stride, sum);
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 __global__ __launch_bounds__(adamw_block) void norm_partials_kernel(NormLaunch L) {
-    const uint32_t k = tensor_of_block(L.first_block, L.n_tensors, blockIdx.x);
-    const NormTensorDevice& T = L.tensors[k];
-    const uint64_t base = static_cast<uint64_t>(blockIdx.x - L.first_block[k]) * norm_chunk;
+    const uint32_t k = tensor_of_block<norm_max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
+    const NormTensorDevice T = L.tensors[k];
     const uint64_t n = T.n_and_type >> 2;
-    const uint32_t type = static_cast<uint32_t>(T.n_and_type & 3u);
+    const uint32_t type = static_cast<uint32_t>(T.n_and_type & 3u), block = blockIdx.x - L.first_block[k], blocks = norm_blocks(n, L.steps);
     double sum;
-    if (type == type_float) sum = squares(static_cast<const float*>(T.data), n, base);
-    else if (type == type_bfloat16) sum = squares(static_cast<const __bf16*>(T.data), n, base);
-    else sum = squares(static_cast<const _Float16*>(T.data), n, base);
+    if (type == type_float) sum = squares(static_cast<const float*>(T.data), n, block, blocks);
+    else if (type == type_bfloat16) sum = squares(static_cast<const __bf16*>(T.data), n, block, blocks);
+    else sum = squares(static_cast<const _Float16*>(T.data), n, block, blocks);
     sum = block_sum<adamw_block>(sum);
     if (threadIdx.x == 0) L.partials[blockIdx.x] = sum;
 }
@@ -343,36 +435,46 @@ __global__ __launch_bounds__(1024) void norm_kernel(const double* __restrict__ p
 
 }  // namespace
 
-bool launch_adamw(const AdamWTensorDevice* tensors, uint64_t n_tensors, const AdamWGroupDevice* groups, int bits, const float* grad_norm,
+template <int BITS, typename T>
+bool launch_steps(const T* tensors, const uint32_t* of_tensor, uint64_t n_tensors, const AdamWGroupDevice* groups, const float* grad_norm,
                   float max_grad_norm, hipStream_t s) {
-    AdamWLaunch L;
+    AdamWLaunch<BITS> L;
     L.grad_norm = grad_norm;
     L.max_grad_norm = max_grad_norm;
     uint64_t at = 0;
     while (at < n_tensors) {
         uint32_t blocks = 0, n_groups = 0;
-        uint32_t of_group[adamw_max_groups];
+        uint32_t group_of[adamw_max_groups];
         L.n_tensors = 0;
-        for (; at < n_tensors && L.n_tensors < adamw_max_tensors; at++) {
-            const uint32_t more = div_up(tensors[at].n, adamw_block * 4);
+        for (; at < n_tensors && L.n_tensors < AdamWLaunch<BITS>::max_tensors; at++) {
+            const uint32_t more = div_up(tensors[at].n(), adamw_block * 4);
             if (blocks + more > adamw_max_blocks && L.n_tensors > 0) break;
             uint32_t g = 0;
-            while (g < n_groups && of_group[g] != tensors[at].group) g++;
+            while (g < n_groups && group_of[g] != of_tensor[at]) g++;
             if (g == n_groups) {
                 if (n_groups == adamw_max_groups) break;
-                of_group[n_groups++] = tensors[at].group;
-                L.groups[g] = groups[tensors[at].group];
+                group_of[n_groups++] = of_tensor[at];
+                L.groups[g] = groups[of_tensor[at]];
             }
             L.tensors[L.n_tensors] = tensors[at];
-            L.tensors[L.n_tensors].group = g;
+            L.tensors[L.n_tensors].set_group(g);
             L.first_block[L.n_tensors++] = blocks;
             blocks += more;
         }
-        if (bits == 32) adamw_kernel<32><<<blocks, adamw_block, 0, s>>>(L);
-        else adamw_kernel<8><<<blocks, adamw_block, 0, s>>>(L);
+        adamw_kernel<BITS><<<blocks, adamw_block, 0, s>>>(L);
         EFGS_HIP_CHECK(hipGetLastError());
     }
     return true;
+}
+
+bool launch_adamw(const AdamWTensor* tensors, const uint32_t* of_tensor, uint64_t n_tensors, const AdamWGroupDevice* groups, const float* grad_norm,
+                  float max_grad_norm, hipStream_t s) {
+    return launch_steps<32>(tensors, of_tensor, n_tensors, groups, grad_norm, max_grad_norm, s);
+}
+
+bool launch_adamw8(const AdamWTensor8* tensors, const uint32_t* of_tensor, uint64_t n_tensors, const AdamWGroupDevice* groups, const float* grad_norm,
+                   float max_grad_norm, hipStream_t s) {
+    return launch_steps<8>(tensors, of_tensor, n_tensors, groups, grad_norm, max_grad_norm, s);
 }
 
 bool launch_adamw_moments(const AdamWMomentsDevice* tensors, uint64_t n_tensors, hipStream_t s) {
@@ -394,10 +496,24 @@ bool launch_adamw_moments(const AdamWMomentsDevice* tensors, uint64_t n_tensors,
     return true;
 }
 
-uint64_t norm_partials_of(uint64_t n) { return (n + norm_chunk - 1) / norm_chunk; }
+// Steps of a block: one, until that makes as many blocks as the GPU holds (2,048), then more, which keeps the partial sums few.
+static uint32_t norm_steps(const NormTensorDevice* tensors, uint64_t n_tensors) {
+    uint64_t total = 0;
+    for (uint64_t k = 0; k < n_tensors; k++) total += tensors[k].n_and_type >> 2;
+    const uint64_t steps = total / (2048ull * norm_step);
+    return static_cast<uint32_t>(steps < 1 ? 1 : steps > 4096 ? 4096 : steps);
+}
+
+uint64_t norm_partials(const NormTensorDevice* tensors, uint64_t n_tensors) {
+    const uint32_t steps = norm_steps(tensors, n_tensors);
+    uint64_t partials = 0;
+    for (uint64_t k = 0; k < n_tensors; k++) partials += norm_blocks(tensors[k].n_and_type >> 2, steps);
+    return partials;
+}
 
 bool launch_grad_norm(const NormTensorDevice* tensors, uint64_t n_tensors, double* partials, float* norm, hipStream_t s) {
     NormLaunch L;
+    L.steps = norm_steps(tensors, n_tensors);
     uint64_t at = 0;
     uint32_t done = 0;
     while (at < n_tensors) {
@@ -405,7 +521,7 @@ bool launch_grad_norm(const NormTensorDevice* tensors, uint64_t n_tensors, doubl
         L.n_tensors = 0;
         L.partials = partials + done;
         for (; at < n_tensors && L.n_tensors < norm_max_tensors; at++) {
-            const uint32_t more = static_cast<uint32_t>(norm_partials_of(tensors[at].n_and_type >> 2));
+            const uint32_t more = norm_blocks(tensors[at].n_and_type >> 2, L.steps);
             if (blocks + more > adamw_max_blocks && L.n_tensors > 0) break;
             L.tensors[L.n_tensors] = tensors[at];
             L.first_block[L.n_tensors++] = blocks;

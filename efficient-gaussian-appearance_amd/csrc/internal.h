@@ -211,28 +211,34 @@ bool launch_adam(const AdamGroupDevice* groups, int n_groups, hipStream_t s);
 
 // ---- AdamW over many tensors ------------------------------------------------------------------------------------
 enum ElementType { type_float = 0, type_bfloat16 = 1, type_half = 2 };
-constexpr uint32_t adamw_max_tensors = 40, adamw_max_groups = 8;  // per launch (4 KB of kernel arguments)
-constexpr uint32_t moments_max_tensors = 64, norm_max_tensors = 64;
-constexpr uint32_t adamw_max_blocks = 1u << 23;  // per launch, unless a tensor alone has more
+constexpr uint32_t adamw_max_groups = 8;         // of a launch (4 KB of kernel arguments)
+constexpr uint32_t moments_max_tensors = 64, norm_max_tensors = 200;
+constexpr uint32_t adamw_max_blocks = 1u << 23;  // of a launch, unless a tensor alone has more
 constexpr int64_t adamw_max_elements = 1ll << 33;  // of a tensor
-struct AdamWTensorDevice {  // no empty tensors
+struct AdamWTensor {        // no empty tensors
     void* param;
     const void* grad;
-    void* m;                // 32-bit states: float; 8-bit: codes of u = m / r
-    void* v;                // 32-bit states: float; 8-bit: codes of r = sqrt(v)
-    float* scale;           // 8-bit: per 256 elements
-    uint64_t n;
-    float step_factor;      // 1 / (1 - beta1^t)
-    float root_factor;      // 1 / sqrt(1 - beta2^t)
-    float ratio_decode;     // 8-bit: bound of u when it was coded over its top code's value
-    uint32_t key;           // 8-bit: dither key of the step
-    uint32_t group;
-    uint16_t param_type, grad_type;
+    void* m;                // float; 8-bit: codes of u = m / r
+    void* v;                // float; 8-bit: codes of r = sqrt(v)
+    uint64_t packed;        // elements << 16 | group << 8 | gradient's type << 4 | parameter's type
+    __host__ __device__ uint64_t n() const { return packed >> 16; }
+    __host__ __device__ uint32_t group() const { return static_cast<uint32_t>(packed >> 8) & 255u; }
+    __host__ __device__ uint32_t grad_type() const { return static_cast<uint32_t>(packed >> 4) & 15u; }
+    __host__ __device__ uint32_t param_type() const { return static_cast<uint32_t>(packed) & 15u; }
+    void set(uint64_t n, uint32_t param_type, uint32_t grad_type) { packed = n << 16 | grad_type << 4 | param_type; }
+    void set_group(uint32_t g) { packed = (packed & ~0xff00ull) | g << 8; }
 };
+struct AdamWTensor8 : AdamWTensor {
+    float* scale;           // per 256 elements
+};
+// what the tensors of one group that have taken the same number of steps share
 struct AdamWGroupDevice {
-    float lrs[adam_max_lrs], decays[adam_max_lrs];  // lr, 1 - lr wd
+    float rates[adam_max_lrs], decays[adam_max_lrs];  // lr / (1 - beta1^t), 1 - lr wd
     float beta1, beta1_rest, beta2, beta2_rest, eps;
+    float root_factor;      // 1 / sqrt(1 - beta2^t)
     float ratio_encode;     // 8-bit: the top code's value over the bound of u
+    float ratio_decode;     // 8-bit: bound of u when the state was coded over its top code's value
+    uint32_t key;           // 8-bit: dither key of the step
     uint32_t n_lrs;
 };
 struct AdamWMomentsDevice {
@@ -255,10 +261,13 @@ __host__ __device__ inline uint32_t adamw_mix(uint32_t x) {
     x = (x ^ (x >> 15)) * 0x3A2F4D1Bu;
     return x ^ (x >> 16);
 }
-bool launch_adamw(const AdamWTensorDevice* tensors, uint64_t n_tensors, const AdamWGroupDevice* groups, int bits, const float* grad_norm,
+// of_tensor: each tensor's group
+bool launch_adamw(const AdamWTensor* tensors, const uint32_t* of_tensor, uint64_t n_tensors, const AdamWGroupDevice* groups, const float* grad_norm,
                   float max_grad_norm, hipStream_t s);
+bool launch_adamw8(const AdamWTensor8* tensors, const uint32_t* of_tensor, uint64_t n_tensors, const AdamWGroupDevice* groups, const float* grad_norm,
+                   float max_grad_norm, hipStream_t s);
 bool launch_adamw_moments(const AdamWMomentsDevice* tensors, uint64_t n_tensors, hipStream_t s);
-uint64_t norm_partials_of(uint64_t n);  // doubles that a tensor of n elements takes of `partials`
+uint64_t norm_partials(const NormTensorDevice* tensors, uint64_t n_tensors);  // doubles of `partials`
 bool launch_grad_norm(const NormTensorDevice* tensors, uint64_t n_tensors, double* partials, float* norm, hipStream_t s);
 
 // ---- rows of a table by index -----------------------------------------------------------------------------------

@@ -43,10 +43,11 @@ const char* group_fault(const efgs_adamw_group& g) {
     return nullptr;
 }
 
-AdamWGroupDevice device_group(const efgs_adamw_group& g) {
+AdamWGroupDevice device_group(const efgs_adamw_group& g, int64_t step, double ratio_bound, uint32_t seed) {
     AdamWGroupDevice d{};
+    const double step_factor = 1.0 / (1.0 - std::pow(g.beta1, static_cast<double>(step)));
     for (int k = 0; k < g.n_lrs; k++) {
-        d.lrs[k] = static_cast<float>(g.lrs[k]);
+        d.rates[k] = static_cast<float>(g.lrs[k] * step_factor);
         d.decays[k] = static_cast<float>(1.0 - g.lrs[k] * g.weight_decay);
     }
     d.n_lrs = static_cast<uint32_t>(g.n_lrs);
@@ -55,9 +56,46 @@ AdamWGroupDevice device_group(const efgs_adamw_group& g) {
     d.beta2 = static_cast<float>(g.beta2);
     d.beta2_rest = static_cast<float>(1.0 - g.beta2);
     d.eps = static_cast<float>(g.eps);
-    if (g.state_bits == 8) d.ratio_encode = static_cast<float>(adamw_ratio_top / efgs_adamw_ratio_bound(g.beta1, g.beta2));
+    d.root_factor = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(g.beta2, static_cast<double>(step))));
+    if (g.state_bits == 8) {
+        d.ratio_encode = static_cast<float>(adamw_ratio_top / efgs_adamw_ratio_bound(g.beta1, g.beta2));
+        d.ratio_decode = static_cast<float>(ratio_bound / adamw_ratio_top);
+        d.key = adamw_mix(adamw_mix(seed) + static_cast<uint32_t>(step));
+    }
     return d;
 }
+
+// The groups that tensors of one step and, with 8 bits, one ratio bound share; most programs have one for each of theirs.
+class SharedGroups {
+  public:
+    SharedGroups(const efgs_adamw_group* groups, int n_groups, uint32_t seed) : groups_(groups), seed_(seed), last_(static_cast<size_t>(n_groups), none) {}
+    uint32_t of(int32_t group, int64_t step, double ratio_bound) {
+        if (groups_[group].state_bits != 8) ratio_bound = 0.0;
+        const uint32_t last = last_[static_cast<size_t>(group)];
+        if (last != none && keys_[last].step == step && keys_[last].ratio_bound == ratio_bound) return last;
+        uint32_t k = 0;
+        while (k < keys_.size() && !(keys_[k].group == group && keys_[k].step == step && keys_[k].ratio_bound == ratio_bound)) k++;
+        if (k == keys_.size()) {
+            keys_.push_back({group, step, ratio_bound});
+            device_.push_back(device_group(groups_[group], step, ratio_bound, seed_));
+        }
+        return last_[static_cast<size_t>(group)] = k;
+    }
+    const AdamWGroupDevice* data() const { return device_.data(); }
+
+  private:
+    static constexpr uint32_t none = 0xffffffffu;
+    struct Key {
+        int32_t group;
+        int64_t step;
+        double ratio_bound;
+    };
+    const efgs_adamw_group* groups_;
+    uint32_t seed_;
+    std::vector<uint32_t> last_;
+    std::vector<Key> keys_;
+    std::vector<AdamWGroupDevice> device_;
+};
 
 bool scale_pointer_ok(const void* p) { return p && reinterpret_cast<uintptr_t>(p) % alignof(float) == 0; }
 
@@ -95,12 +133,12 @@ int efgs_adamw_step(const efgs_adamw_tensor* tensors, int64_t n_tensors, const e
         if (n_tensors < 0 || n_groups < 0 || (n_tensors > 0 && !tensors) || (n_groups > 0 && !groups))
             return fail(EFGS_ERR_INVALID_ARGUMENT, "invalid adamw tensors or groups");
         if (grad_norm && !(max_grad_norm > 0.0)) return fail(EFGS_ERR_INVALID_ARGUMENT, "the largest gradient norm must be positive");
-        std::vector<AdamWGroupDevice> device_groups;
-        for (int g = 0; g < n_groups; g++) {
+        for (int g = 0; g < n_groups; g++)
             if (const char* fault = group_fault(groups[g])) return fail(EFGS_ERR_INVALID_ARGUMENT, fault);
-            device_groups.push_back(device_group(groups[g]));
-        }
-        std::vector<AdamWTensorDevice> in_bits[2];  // 32, 8
+        SharedGroups shared(groups, n_groups, seed);
+        std::vector<AdamWTensor> wide;
+        std::vector<AdamWTensor8> coded;
+        std::vector<uint32_t> wide_groups, coded_groups;
         for (int64_t k = 0; k < n_tensors; k++) {
             const efgs_adamw_tensor& t = tensors[k];
             if (t.group < 0 || t.group >= n_groups) return fail(EFGS_ERR_INVALID_ARGUMENT, "adamw group out of range");
@@ -109,31 +147,27 @@ int efgs_adamw_step(const efgs_adamw_tensor* tensors, int64_t n_tensors, const e
             if (!known_type(t.param_type) || !known_type(t.grad_type)) return fail(EFGS_ERR_INVALID_ARGUMENT, "unknown element type");
             if (t.n_elements == 0) continue;
             if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return fail(EFGS_ERR_INVALID_ARGUMENT, "null adamw tensor");
-            const efgs_adamw_group& g = groups[t.group];
-            AdamWTensorDevice d{};
+            AdamWTensor8 d{};
             d.param = t.param;
             d.grad = t.grad;
             d.m = t.exp_avg;
             d.v = t.exp_avg_sq;
-            d.n = static_cast<uint64_t>(t.n_elements);
-            d.step_factor = static_cast<float>(1.0 / (1.0 - std::pow(g.beta1, static_cast<double>(t.step))));
-            d.root_factor = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(g.beta2, static_cast<double>(t.step))));
-            d.group = static_cast<uint32_t>(t.group);
-            d.param_type = static_cast<uint16_t>(t.param_type);
-            d.grad_type = static_cast<uint16_t>(t.grad_type);
-            if (g.state_bits == 8) {
+            d.set(static_cast<uint64_t>(t.n_elements), static_cast<uint32_t>(t.param_type), static_cast<uint32_t>(t.grad_type));
+            if (groups[t.group].state_bits == 8) {
                 if (!scale_pointer_ok(t.root_scale)) return fail(EFGS_ERR_INVALID_ARGUMENT, "8-bit adamw states need their block scales");
                 if (!(t.ratio_bound > 0.0 && std::isfinite(t.ratio_bound))) return fail(EFGS_ERR_INVALID_ARGUMENT, "8-bit adamw states need their ratio bound");
                 d.scale = t.root_scale;
-                d.ratio_decode = static_cast<float>(t.ratio_bound / adamw_ratio_top);
-                d.key = adamw_mix(adamw_mix(seed) + static_cast<uint32_t>(t.step));
+                coded.push_back(d);
+                coded_groups.push_back(shared.of(t.group, t.step, t.ratio_bound));
+            } else {
+                wide.push_back(d);
+                wide_groups.push_back(shared.of(t.group, t.step, 0.0));
             }
-            in_bits[g.state_bits == 8 ? 1 : 0].push_back(d);
         }
-        for (int k = 0; k < 2; k++)
-            if (!launch_adamw(in_bits[k].data(), in_bits[k].size(), device_groups.data(), k == 0 ? 32 : 8, grad_norm,
-                              static_cast<float>(max_grad_norm), static_cast<hipStream_t>(stream)))
-                return EFGS_ERR_HIP;
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        const float max_norm = static_cast<float>(max_grad_norm);
+        if (!launch_adamw(wide.data(), wide_groups.data(), wide.size(), shared.data(), grad_norm, max_norm, s)) return EFGS_ERR_HIP;
+        if (!launch_adamw8(coded.data(), coded_groups.data(), coded.size(), shared.data(), grad_norm, max_norm, s)) return EFGS_ERR_HIP;
         return EFGS_OK;
     });
 }
@@ -167,7 +201,6 @@ int efgs_grad_norm(const efgs_norm_tensor* tensors, int64_t n_tensors, float* no
     return guarded([&]() -> int {
         if (n_tensors < 0 || (n_tensors > 0 && !tensors) || !norm || !alloc) return fail(EFGS_ERR_INVALID_ARGUMENT, "invalid gradient norm arguments");
         std::vector<NormTensorDevice> device;
-        uint64_t partials = 0;
         for (int64_t k = 0; k < n_tensors; k++) {
             const efgs_norm_tensor& t = tensors[k];
             if (t.n_elements < 0 || t.n_elements > adamw_max_elements) return fail(EFGS_ERR_INVALID_ARGUMENT, "gradient element count out of range");
@@ -175,8 +208,8 @@ int efgs_grad_norm(const efgs_norm_tensor* tensors, int64_t n_tensors, float* no
             if (t.n_elements == 0) continue;
             if (!t.data) return fail(EFGS_ERR_INVALID_ARGUMENT, "null gradient");
             device.push_back({t.data, static_cast<uint64_t>(t.n_elements) << 2 | static_cast<uint64_t>(t.type)});
-            partials += norm_partials_of(static_cast<uint64_t>(t.n_elements));
         }
+        const uint64_t partials = norm_partials(device.data(), device.size());
         if (partials > 0xffffffffull) return fail(EFGS_ERR_INVALID_ARGUMENT, "too many gradients");
         double* buffer = static_cast<double*>(alloc(alloc_ctx, static_cast<size_t>(partials > 0 ? partials : 1) * sizeof(double)));
         if (!buffer) return fail(EFGS_ERR_ALLOC, "allocation of the gradient norm's partial sums failed");

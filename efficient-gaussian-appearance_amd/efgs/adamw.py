@@ -18,7 +18,7 @@ class AdamW(torch.optim.Optimizer):
         p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 
     in 32 bits, p rounded once to its type. Parameters and gradients are contiguous float32, bfloat16 or float16 GPU tensors
-    (a gradient that is not contiguous is copied); a launch takes 40 tensors, whatever groups they are in.
+    (a gradient that is not contiguous is copied); a launch takes 60 to 72 tensors, of up to 8 groups.
 
     lr, betas, eps, weight_decay, state_bits: defaults that a group may override. `lr` is a float or a list of up to 7 rates
     cycled over the last dimension's columns, as `FusedAdam` has them.

@@ -282,7 +282,7 @@ int efgs_ngsplat_pack(const efgs_ngsplat_input* in, efgs_ngsplat_output* out, ef
 /* element types of the operators below */
 enum { EFGS_FLOAT = 0, EFGS_BFLOAT16 = 1, EFGS_HALF = 2 };
 
-/* One AdamW step (decoupled weight decay) over many tensors, 40 to a launch. Per element, t the tensor's step from 1:
+/* One AdamW step (decoupled weight decay) over many tensors, 60 to 72 to a launch. Per element, t the tensor's step from 1:
  *   g = c grad, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
  *   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * with lr cycled by element index over the group's n_lrs rates, in 32 bits, p rounded once to its type.
@@ -333,7 +333,7 @@ typedef struct efgs_adamw_state {
 int efgs_adamw_moments(const efgs_adamw_state* states, int64_t n_states, void* stream);
 
 /* norm (device, one float) = sqrt of the sum of the squares of all tensors' elements, summed in 64 bits in a fixed order.
- * Its partial sums come from `alloc` (8 bytes per 4,096 elements). Stream-ordered. */
+ * Its partial sums come from `alloc` (at most 8 bytes per 8,192 elements and one per tensor). Stream-ordered. */
 typedef struct efgs_norm_tensor {
     const void* data;
     int64_t n_elements;
