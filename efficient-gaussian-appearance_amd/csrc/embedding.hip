@@ -119,12 +119,15 @@ __global__ __launch_bounds__(lookup_block) void embedding_lookup_kernel(LookupAr
 
 // ---- sort --------------------------------------------------------------------------------------------------------------
 // Keys are rows (or `rows` for an index that counts nowhere), values the positions of their indices. A pass orders by up
-// to 8 bits: blocks count their segments' digits into a table, then every block sums the table itself (its digits'
-// places behind all smaller digits and behind the same digits of earlier blocks) and writes its keys there, each at its
-// rank among the equal digits before it in its wave.
+// to 8 bits: every block knows its digits' places (behind all smaller digits, and behind the same digits of earlier blocks)
+// and writes its keys there, each at its rank among the equal digits before it. The counts come from a table that a kernel
+// of the same blocks writes, or, up to 32,768 keys, from the block's own count of the whole list, which spares that launch.
+// Up to 8,192 keys one kernel counts for each key the smaller ones.
 
-constexpr uint32_t sort_block = 256, sort_waves = sort_block / 64, sort_steps = 16, sort_tile = sort_block * sort_steps;
+constexpr uint32_t sort_block = 1024, sort_waves = sort_block / 64, sort_steps = 4, sort_tile = sort_block * sort_steps;
 constexpr uint32_t sort_max_blocks = 256, sort_digits = 256;
+constexpr uint32_t sort_alone = 8 * sort_tile;     // largest list that every block counts by itself
+constexpr uint32_t rank_most = 8192, rank_keys = 64;  // largest list ordered by ranks, and keys of a block
 
 struct SortPass {
     const void* indices;       // first pass: int32 or int64
@@ -150,51 +153,87 @@ __device__ __forceinline__ uint32_t key_at(const SortPass& a, uint32_t i) {
 template <typename I>
 __global__ __launch_bounds__(sort_block) void sort_count_kernel(SortPass a) {
     __shared__ uint32_t counts[sort_digits];
-    counts[threadIdx.x] = 0;
+    if (threadIdx.x < sort_digits) counts[threadIdx.x] = 0;
     __syncthreads();
-    const uint64_t first = static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block * sort_tile;
-    const uint64_t last = min(first + static_cast<uint64_t>(a.tiles_per_block) * sort_tile, static_cast<uint64_t>(a.n));
-    for (uint64_t i = first + threadIdx.x; i < last; i += sort_block)
-        atomicAdd(&counts[(key_at<I>(a, static_cast<uint32_t>(i)) >> a.shift) & a.digit_mask], 1u);
-    __syncthreads();
-    a.table[blockIdx.x * sort_digits + threadIdx.x] = counts[threadIdx.x];
-}
-
-// exclusive prefix over the block's 256 threads
-__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* wave_totals) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint32_t inclusive = v;
-#pragma unroll
-    for (uint32_t o = 1; o < 64; o <<= 1) {
-        const uint32_t t = __shfl_up(inclusive, o);
-        if (lane >= o) inclusive += t;
-    }
-    if (lane == 63) wave_totals[wave] = inclusive;
-    __syncthreads();
-    uint32_t before = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < sort_waves; w++)
-        if (w < wave) before += wave_totals[w];
-    return before + inclusive - v;
-}
-
-template <typename I>
-__global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
-    __shared__ uint32_t counts[sort_waves][sort_digits];
-    __shared__ uint32_t wave_totals[sort_waves];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint32_t before = 0, total = 0;
-    for (uint32_t b = 0; b < gridDim.x; b++) {
-        const uint32_t c = a.table[b * sort_digits + threadIdx.x];
-        total += c;
-        if (b < blockIdx.x) before += c;
-    }
-    uint32_t place = block_exclusive(total, wave_totals) + before;  // of the thread's digit
     for (uint32_t tile = 0; tile < a.tiles_per_block; tile++) {
-        const uint64_t first = (static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block + tile) * sort_tile;
-        if (first >= a.n) break;
-        for (uint32_t w = 0; w < sort_waves; w++) counts[w][threadIdx.x] = 0;
+        const uint64_t first = (static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block + tile) * sort_tile + threadIdx.x;
+        uint32_t key[sort_steps];
+#pragma unroll
+        for (uint32_t s = 0; s < sort_steps; s++) {
+            const uint64_t i = first + s * sort_block;
+            key[s] = i < a.n ? key_at<I>(a, static_cast<uint32_t>(i)) : 0u;
+        }
+#pragma unroll
+        for (uint32_t s = 0; s < sort_steps; s++)
+            if (first + s * sort_block < a.n) atomicAdd(&counts[(key[s] >> a.shift) & a.digit_mask], 1u);
+    }
+    __syncthreads();
+    if (threadIdx.x < sort_digits) a.table[blockIdx.x * sort_digits + threadIdx.x] = counts[threadIdx.x];
+}
+
+// ALONE: the block counts the digits of the whole list
+template <typename I, bool ALONE>
+__global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
+    __shared__ uint32_t counts[sort_waves][sort_digits];  // keys of each digit in a wave's part of the tile, then their first place
+    __shared__ uint32_t parts[2][4][sort_digits], wave_totals[4];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, digit = threadIdx.x & (sort_digits - 1), quarter = threadIdx.x >> 8;
+    const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block * sort_tile;
+    // keys of the digit in all blocks and in those before this one, a quarter of the list or of the table's rows at a time
+    if constexpr (ALONE) {
+        parts[0][quarter][digit] = parts[1][quarter][digit] = 0;
         __syncthreads();
+        for (uint32_t from = threadIdx.x; from < a.n; from += sort_tile) {
+            uint32_t key[sort_steps];
+#pragma unroll
+            for (uint32_t s = 0; s < sort_steps; s++) key[s] = from + s * sort_block < a.n ? key_at<I>(a, from + s * sort_block) : 0u;
+#pragma unroll
+            for (uint32_t s = 0; s < sort_steps; s++) {
+                const uint32_t i = from + s * sort_block;
+                if (i < a.n) atomicAdd(&parts[i < begin ? 1 : 0][quarter][(key[s] >> a.shift) & a.digit_mask], 1u);
+            }
+        }
+        __syncthreads();
+    } else {
+        uint32_t before = 0, total = 0;
+        const uint32_t rows = (gridDim.x + 3) / 4;
+#pragma unroll 16
+        for (uint32_t k = 0; k < rows; k++) {
+            const uint32_t b = quarter * rows + k;
+            const uint32_t c = b < gridDim.x ? a.table[b * sort_digits + digit] : 0u;
+            total += c;
+            before += b < blockIdx.x ? c : 0u;
+        }
+        parts[0][quarter][digit] = total - before;
+        parts[1][quarter][digit] = before;
+        __syncthreads();
+    }
+    uint32_t place = 0, total = 0;  // (threads of the first quarter: their digit's)
+    if (quarter == 0) {
+        uint32_t before = 0;
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++) {
+            before += parts[1][q][digit];
+            total += parts[0][q][digit];
+        }
+        total += before;
+        uint32_t inclusive = total;
+#pragma unroll
+        for (uint32_t o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(inclusive, o);
+            if (lane >= o) inclusive += t;
+        }
+        if (lane == 63) wave_totals[wave] = inclusive;
+        place = inclusive - total + before;
+    }
+    __syncthreads();
+    if (quarter == 0) {
+#pragma unroll
+        for (uint32_t w = 0; w < 4; w++)
+            if (w < wave) place += wave_totals[w];
+    }
+    for (uint32_t tile = 0; tile < a.tiles_per_block; tile++) {
+        const uint64_t first = begin + tile * static_cast<uint64_t>(sort_tile);
+        if (first >= a.n) break;
         uint32_t key[sort_steps], value[sort_steps], rank[sort_steps];
         const uint64_t wave_first = first + wave * 64u * sort_steps + lane;
 #pragma unroll
@@ -204,31 +243,36 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
             if constexpr (sizeof(I) == 1) value[s] = i < a.n ? a.values_in[i] : 0u;
             else value[s] = static_cast<uint32_t>(i);
         }
+#pragma unroll
+        for (uint32_t k = 0; k < sort_digits / 64; k++) counts[wave][k * 64 + lane] = 0;
         volatile uint32_t* const mine = counts[wave];
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++) {
-            const uint32_t digit = (key[s] >> a.shift) & a.digit_mask;
+            const uint32_t d = (key[s] >> a.shift) & a.digit_mask;
             const bool valid = wave_first + s * 64u < a.n;
             uint64_t same = __ballot(valid);
 #pragma unroll
             for (uint32_t b = 0; b < 8; b++) {
-                const bool bit = (digit >> b) & 1u;
+                const bool bit = (d >> b) & 1u;
                 const uint64_t with = __ballot(bit);
                 same &= bit ? with : ~with;
             }
             const uint32_t earlier = static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1ull)));
-            const uint32_t so_far = mine[digit];
+            const uint32_t so_far = mine[d];
             rank[s] = so_far + earlier;
             __builtin_amdgcn_wave_barrier();
-            if (valid && earlier == 0) mine[digit] = so_far + static_cast<uint32_t>(__popcll(same));
+            if (valid && earlier == 0) mine[d] = so_far + static_cast<uint32_t>(__popcll(same));
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
+        if (quarter == 0) {
 #pragma unroll
-        for (uint32_t w = 0; w < sort_waves; w++) {
-            const uint32_t c = counts[w][threadIdx.x];
-            counts[w][threadIdx.x] = place;
-            place += c;
+            for (uint32_t w = 0; w < sort_waves; w++) {
+                const uint32_t c = counts[w][digit];
+                counts[w][digit] = place;
+                place += c;
+            }
         }
         __syncthreads();
 #pragma unroll
@@ -240,6 +284,37 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
             }
         }
         __syncthreads();
+    }
+}
+
+// A key's place is the number of smaller keys, and of equal ones before it: 64 keys to a block, each compared by 16 threads
+// with a 16th of the list.
+template <typename I>
+__global__ __launch_bounds__(sort_block) void sort_rank_kernel(SortPass a) {
+    __shared__ __attribute__((aligned(16))) uint32_t keys[rank_most];
+    __shared__ uint32_t places[sort_waves][rank_keys];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t per = (a.n + sort_waves * 4 - 1) / (sort_waves * 4) * 4;  // of a wave, in fours
+    for (uint32_t i = threadIdx.x; i < per * sort_waves; i += sort_block) keys[i] = i < a.n ? key_at<I>(a, i) : 0xffffffffu;
+    __syncthreads();
+    const uint32_t i = blockIdx.x * rank_keys + lane, mine = keys[min(i, a.n - 1)];
+    uint32_t smaller = 0;
+    const uint4* const part = reinterpret_cast<const uint4*>(keys + wave * per);
+    for (uint32_t k = 0; k < per / 4; k++) {
+        const uint4 other = part[k];
+        const uint32_t at = wave * per + k * 4;
+        // (equal keys count where they stand before: as if they were smaller)
+        smaller += (other.x < mine + (at < i ? 1u : 0u)) + (other.y < mine + (at + 1 < i ? 1u : 0u)) + (other.z < mine + (at + 2 < i ? 1u : 0u)) +
+                   (other.w < mine + (at + 3 < i ? 1u : 0u));
+    }
+    places[wave][lane] = smaller;
+    __syncthreads();
+    if (wave == 0 && i < a.n) {
+        uint32_t to = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < sort_waves; w++) to += places[w][lane];
+        a.keys_out[to] = mine;
+        a.values_out[to] = i;
     }
 }
 
@@ -261,13 +336,14 @@ struct SumArgs {
     float scale;
 };
 
-// entries among the first `position` items of the merged list, over the wave
+// entries among the first `position` items of the merged list, over the wave: 128 places tried a round
 __device__ __forceinline__ uint32_t entries_before(const SumArgs& a, uint32_t position) {
     const uint32_t lane = threadIdx.x & 63u;
     uint32_t lo = position > a.rows ? position - a.rows : 0u, hi = min(position, a.n);
     while (lo < hi) {
-        const uint32_t step = (hi - lo + 63u) / 64u, at = lo + lane * step;
-        const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(at < hi && at + a.keys[min(at, hi - 1)] < position)));
+        const uint32_t step = (hi - lo + 127u) / 128u, at = lo + lane * step, at2 = at + 64u * step;
+        const uint32_t key = a.keys[min(at, hi - 1)], key2 = a.keys[min(at2, hi - 1)];
+        const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(at < hi && at + key < position)) + __popcll(__ballot(at2 < hi && at2 + key2 < position)));
         if (before == 0) break;
         hi = min(hi, lo + before * step);
         lo = lo + (before - 1) * step + 1;
@@ -435,6 +511,7 @@ __global__ __launch_bounds__(64) void embedding_join_kernel(SumArgs a) {
         from = from > 64 ? from - 64 : 0;
     }
     float sum[values] = {};
+#pragma unroll 8
     for (uint32_t k = from + slot; k < b; k += slots) {
 #pragma unroll
         for (int j = 0; j < values; j++) sum[j] += a.tails[static_cast<uint64_t>(k) * a.padded_columns + column + j];
@@ -471,7 +548,16 @@ uint32_t group_lanes(const EmbeddingArgs& a) {
 
 uint32_t sum_blocks(const EmbeddingArgs& a) { return div_up(static_cast<uint64_t>(a.n) + a.rows, sum_block / group_lanes(a) * sum_items); }
 
-uint32_t sort_tiles_per_block(uint32_t n) { return div_up(div_up(n, sort_tile), sort_max_blocks); }
+template <typename I>
+void launch_sort_pass(const SortPass& p, hipStream_t s) {
+    const uint32_t blocks = div_up(p.n, static_cast<uint64_t>(sort_tile) * p.tiles_per_block);
+    if (p.n <= sort_alone) {
+        sort_scatter_kernel<I, true><<<blocks, sort_block, 0, s>>>(p);
+    } else {
+        sort_count_kernel<I><<<blocks, sort_block, 0, s>>>(p);
+        sort_scatter_kernel<I, false><<<blocks, sort_block, 0, s>>>(p);
+    }
+}
 
 struct GradientLayout {
     uint32_t* keys[2];
@@ -558,33 +644,35 @@ bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uin
     if (a.n > 0) {
         SortPass p;
         p.indices = a.indices;
+        p.keys_in = p.values_in = nullptr;
+        p.keys_out = l.keys[0];
+        p.values_out = l.values[0];
         p.table = l.table;
         p.n = a.n;
         p.rows = a.rows;
         p.padding = padding;
-        p.tiles_per_block = sort_tiles_per_block(a.n);
-        const uint32_t blocks = div_up(a.n, static_cast<uint64_t>(sort_tile) * p.tiles_per_block);
-        const uint32_t bits = bit_width(a.rows), passes = bits > 8 ? div_up(bits, 8) : 1u, digit_bits = div_up(bits, passes);
-        p.digit_mask = (1u << digit_bits) - 1u;
-        for (uint32_t k = 0; k < passes; k++) {
-            p.shift = k * digit_bits;
-            p.keys_in = l.keys[current];
-            p.values_in = l.values[current];
-            if (k > 0) current ^= 1u;
-            p.keys_out = l.keys[current];
-            p.values_out = l.values[current];
-            if (k > 0) {
-                sort_count_kernel<uint8_t><<<blocks, sort_block, 0, s>>>(p);
-                sort_scatter_kernel<uint8_t><<<blocks, sort_block, 0, s>>>(p);
-            } else if (a.index_bytes == 4) {
-                sort_count_kernel<int32_t><<<blocks, sort_block, 0, s>>>(p);
-                sort_scatter_kernel<int32_t><<<blocks, sort_block, 0, s>>>(p);
-            } else {
-                sort_count_kernel<int64_t><<<blocks, sort_block, 0, s>>>(p);
-                sort_scatter_kernel<int64_t><<<blocks, sort_block, 0, s>>>(p);
+        p.shift = 0;
+        p.tiles_per_block = div_up(div_up(a.n, sort_tile), sort_max_blocks);
+        if (a.n <= rank_most) {
+            const uint32_t blocks = div_up(a.n, rank_keys);
+            if (a.index_bytes == 4) sort_rank_kernel<int32_t><<<blocks, sort_block, 0, s>>>(p);
+            else sort_rank_kernel<int64_t><<<blocks, sort_block, 0, s>>>(p);
+        } else {
+            const uint32_t bits = bit_width(a.rows), passes = bits > 8 ? div_up(bits, 8) : 1u, digit_bits = div_up(bits, passes);
+            p.digit_mask = (1u << digit_bits) - 1u;
+            if (a.index_bytes == 4) launch_sort_pass<int32_t>(p, s);
+            else launch_sort_pass<int64_t>(p, s);
+            for (uint32_t k = 1; k < passes; k++) {
+                p.shift = k * digit_bits;
+                p.keys_in = l.keys[current];
+                p.values_in = l.values[current];
+                current ^= 1u;
+                p.keys_out = l.keys[current];
+                p.values_out = l.values[current];
+                launch_sort_pass<uint8_t>(p, s);
             }
-            EFGS_HIP_CHECK(hipGetLastError());
         }
+        EFGS_HIP_CHECK(hipGetLastError());
     }
     SumArgs u;
     u.keys = l.keys[current];

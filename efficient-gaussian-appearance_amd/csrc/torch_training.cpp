@@ -1,6 +1,7 @@
 // The training operators beside the rasterizer for Python: rows of a table by index as a C++ autograd function, the AdamW
 // step over all tensors of an optimizer (gathered from its groups and states here: a step over many small tensors is bound
 // by the host), the moments of 8-bit states and the gradient norm.
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -206,8 +207,46 @@ PyObject* state_of(PyObject* states, PyObject* key, const Tensor& param, int bit
     return state;
 }
 
-// One step over every parameter that has a gradient. groups: (parameters, learning rates, beta1, beta2, eps, weight decay,
-// state bits) each; states: the optimizer's. Returns the gradients' norm where it clips. Nothing has changed if this throws
+PyObject* group_entry(PyObject* group, PyObject* key) {
+    PyObject* const item = PyDict_GetItemWithError(group, key);
+    TORCH_CHECK_VALUE(item, "efgs: AdamW: a parameter group lacks ", PyUnicode_AsUTF8(key));
+    return item;
+}
+
+double as_double(PyObject* item) {
+    const double x = PyFloat_AsDouble(item);  // (numbers, and whatever turns into a float: a tensor of one value)
+    if (x == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+    return x;
+}
+
+efgs_adamw_group native_group(PyObject* group) {
+    static PyObject* const lr_name = PyUnicode_InternFromString("lr");
+    static PyObject* const betas_name = PyUnicode_InternFromString("betas");
+    static PyObject* const eps_name = PyUnicode_InternFromString("eps");
+    static PyObject* const decay_name = PyUnicode_InternFromString("weight_decay");
+    static PyObject* const bits_name = PyUnicode_InternFromString("state_bits");
+    efgs_adamw_group native{};
+    PyObject* const lr = group_entry(group, lr_name);
+    if (PyList_Check(lr) || PyTuple_Check(lr)) {
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(lr);
+        TORCH_CHECK_VALUE(n >= 1 && n <= 7, "efgs: between 1 and 7 learning rates are supported");
+        for (Py_ssize_t k = 0; k < n; k++) native.lrs[k] = as_double(PySequence_Fast_GET_ITEM(lr, k));
+        native.n_lrs = static_cast<int32_t>(n);
+    } else {
+        native.lrs[0] = as_double(lr);
+        native.n_lrs = 1;
+    }
+    PyObject* const betas = group_entry(group, betas_name);
+    TORCH_CHECK_VALUE((PyTuple_Check(betas) || PyList_Check(betas)) && PySequence_Fast_GET_SIZE(betas) == 2, "efgs: AdamW: betas must be two numbers");
+    native.beta1 = as_double(PySequence_Fast_GET_ITEM(betas, 0));
+    native.beta2 = as_double(PySequence_Fast_GET_ITEM(betas, 1));
+    native.eps = as_double(group_entry(group, eps_name));
+    native.weight_decay = as_double(group_entry(group, decay_name));
+    native.state_bits = static_cast<int32_t>(as_double(group_entry(group, bits_name)));
+    return native;
+}
+
+// One step over every parameter that has a gradient. groups: the optimizer's param_groups; states: its state. Returns the gradients' norm where it clips. Nothing has changed if this throws
 // before the launch (states of zeros may have been made).
 c10::optional<Tensor> adamw_step(const py::list& groups, const py::dict& states, const c10::optional<double>& max_grad_norm, uint32_t seed) {
     at::NoGradGuard no_grad;
@@ -224,22 +263,14 @@ c10::optional<Tensor> adamw_step(const py::list& groups, const py::dict& states,
     std::vector<efgs_adamw_group> native_groups;
     c10::optional<at::Device> device;
     for (const py::handle item : groups) {
-        const py::tuple g = py::cast<py::tuple>(item);
-        efgs_adamw_group native{};
-        const std::vector<double> lrs = py::cast<std::vector<double>>(g[1]);
-        TORCH_CHECK(lrs.size() >= 1 && lrs.size() <= 7, "between 1 and 7 learning rates are supported");
-        for (size_t k = 0; k < lrs.size(); k++) native.lrs[k] = lrs[k];
-        native.n_lrs = static_cast<int32_t>(lrs.size());
-        native.beta1 = py::cast<double>(g[2]);
-        native.beta2 = py::cast<double>(g[3]);
-        native.eps = py::cast<double>(g[4]);
-        native.weight_decay = py::cast<double>(g[5]);
-        native.state_bits = py::cast<int32_t>(g[6]);
+        static PyObject* const params_name = PyUnicode_InternFromString("params");
+        TORCH_CHECK_VALUE(PyDict_Check(item.ptr()), "efgs: AdamW: a parameter group must be a dict");
+        PyObject* const params = group_entry(item.ptr(), params_name);
+        TORCH_CHECK_VALUE(PyList_Check(params), "efgs: AdamW: a group's parameters must be a list");
+        native_groups.push_back(native_group(item.ptr()));
+        const efgs_adamw_group& native = native_groups.back();
         const int bits = native.state_bits;
         const double bound = bits == 8 ? efgs_adamw_ratio_bound(native.beta1, native.beta2) : 0.0;
-        native_groups.push_back(native);
-        PyObject* const params = py::cast<py::object>(g[0]).ptr();
-        TORCH_CHECK_VALUE(PyList_Check(params), "efgs: AdamW: a group's parameters must be a list");
         for (Py_ssize_t k = 0; k < PyList_GET_SIZE(params); k++) {
             PyObject* const key = PyList_GET_ITEM(params, k);
             TORCH_CHECK_VALUE(THPVariable_Check(key), "efgs: AdamW: parameters must be tensors");
@@ -285,6 +316,8 @@ c10::optional<Tensor> adamw_step(const py::list& groups, const py::dict& states,
     }
     if (entries.empty()) return c10::nullopt;
     const c10::DeviceGuard guard(*device);
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                "efgs: AdamW counts its steps on the host and cannot be captured into a graph");
     c10::optional<Tensor> norm;
     if (max_grad_norm) norm = norm_of(norms, *device);
     check_status(efgs_adamw_step(tensors.data(), static_cast<int64_t>(tensors.size()), native_groups.data(), static_cast<int>(native_groups.size()),

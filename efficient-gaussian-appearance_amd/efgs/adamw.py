@@ -47,21 +47,18 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, param_group: dict[str, Any]) -> None:
         super().add_param_group(param_group)
         try:
-            _native_group(self.param_groups[-1])
+            _check_group(self.param_groups[-1])
         except ValueError:
             self.param_groups.pop()
             raise
 
-    @torch.no_grad()
     def step(self, closure: Callable[[], Any] | None = None) -> Any:
         """One step of every parameter that has a gradient; returns what `closure` (re-evaluated first, if given) returns."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError('efgs: AdamW counts its steps on the host and cannot be captured into a graph')
-        self.grad_norm = _native.adamw_step([_native_group(g) for g in self.param_groups], self.state, self.max_grad_norm, self.seed & 0xffffffff)
+        self.grad_norm = _native.adamw_step(self.param_groups, self.state, self.max_grad_norm, self.seed & 0xffffffff)
         return loss
 
     def moments(self, params: torch.Tensor | Sequence[torch.Tensor]) -> Any:
@@ -90,23 +87,19 @@ class AdamW(torch.optim.Optimizer):
             self.state[p] = own
 
 
-def _native_group(group: dict[str, Any]) -> tuple:
+def _check_group(group: dict[str, Any]) -> None:
     lr = group['lr']
-    lrs = [float(x) for x in lr] if isinstance(lr, (list, tuple)) else [float(lr)]
-    if not 1 <= len(lrs) <= 7:
+    if isinstance(lr, (list, tuple)) and not 1 <= len(lr) <= 7:
         raise ValueError('efgs: between 1 and 7 learning rates are supported')
     beta1, beta2 = (float(b) for b in group['betas'])
     if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
         raise ValueError(f'efgs: betas must lie in [0, 1), got {(beta1, beta2)}')
-    eps = float(group['eps'])
-    if not eps >= 0.0:
-        raise ValueError(f'efgs: eps must not be negative, got {eps}')
-    bits = group['state_bits']
-    if bits not in (8, 32):
-        raise ValueError(f'efgs: state_bits must be 32 or 8, got {bits}')
-    if bits == 8 and not beta1 * beta1 < beta2:
+    if not float(group['eps']) >= 0.0:
+        raise ValueError(f'efgs: eps must not be negative, got {group["eps"]}')
+    if group['state_bits'] not in (8, 32):
+        raise ValueError(f'efgs: state_bits must be 32 or 8, got {group["state_bits"]}')
+    if group['state_bits'] == 8 and not beta1 * beta1 < beta2:
         raise ValueError(f'efgs: 8-bit states need beta1^2 < beta2, got {(beta1, beta2)}')
-    return group['params'], lrs, beta1, beta2, eps, float(group['weight_decay']), int(bits)
 
 
 def grad_norm(tensors: torch.Tensor | Iterable[torch.Tensor]) -> torch.Tensor:
