@@ -491,10 +491,11 @@ bool launch_steps(const T* tensors, const uint32_t* of_tensor, uint64_t n_tensor
 bool launch_adamw(const AdamWTensor* tensors, const uint32_t* of_tensor, uint64_t n_tensors, const AdamWGroupDevice* groups, const float* grad_norm,
                   float max_grad_norm, hipStream_t s) {
     // Two pieces a thread from about a million elements on (one, two and four: 590k elements 5.9 and 7.5 us, 1M 6.8, 6.5 and 7.6, 4M 22.0, 21.0
-    // and 21.3, 67M 341, 317 and 316; bfloat16 67M 255, 248 and 244): below, the blocks would not fill the GPU.
+    // and 21.3, 67M 341, 317 and 316; bfloat16 67M 255, 248 and 244): below, the blocks of a launch would not fill the GPU.
     uint64_t total = 0;
     for (uint64_t k = 0; k < n_tensors; k++) total += tensors[k].n();
-    if (total < (1u << 20)) return launch_steps<32, 1>(tensors, of_tensor, n_tensors, groups, grad_norm, max_grad_norm, s);
+    const uint64_t launches = (n_tensors + AdamWLaunch<32>::max_tensors - 1) / AdamWLaunch<32>::max_tensors;
+    if (total < (launches << 20)) return launch_steps<32, 1>(tensors, of_tensor, n_tensors, groups, grad_norm, max_grad_norm, s);
     return launch_steps<32, 2>(tensors, of_tensor, n_tensors, groups, grad_norm, max_grad_norm, s);
 }
 

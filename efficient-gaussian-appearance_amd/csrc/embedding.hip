@@ -11,31 +11,27 @@
 // it. Every group of lanes takes the same number of items whatever the runs are; a sum that crosses groups is carried by a
 // segmented scan within the block, and a row that crosses blocks is put together by a second kernel from the blocks' first
 // and last pieces, in their order.
+#include <type_traits>
+
 #include "internal.h"
 
 namespace efgs {
 
 namespace {
 
-typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef _Float16 half8u __attribute__((ext_vector_type(8), aligned(2)));
-typedef __bf16 bfloat8u __attribute__((ext_vector_type(8), aligned(2)));
+// A lane's part of a row: 16 bytes at any of its type's alignments, or one value where rows are shorter than that. A row's last
+// lane takes its last 16 bytes, whatever of them the lane before it has too (both make the same values), so that no access
+// stands in a branch: a kernel whose loads are in branches waits for each before it sends the next.
+template <typename T, int W> struct Part { typedef T type __attribute__((ext_vector_type(W), aligned(sizeof(T)))); };
+template <typename T> struct Part<T, 1> { using type = T; };
 
-// 16 bytes of a row
-template <typename T> struct Lane16;
-template <> struct Lane16<float> { using type = float4u; static constexpr int values = 4; };
-template <> struct Lane16<_Float16> { using type = half8u; static constexpr int values = 8; };
-template <> struct Lane16<__bf16> { using type = bfloat8u; static constexpr int values = 8; };
+template <typename T, int W>
+__device__ __forceinline__ typename Part<T, W>::type load_part(const T* p) { return *reinterpret_cast<const typename Part<T, W>::type*>(p); }
 
-// v = the lane's values at p; past `count` zeros
-template <typename T>
-__device__ __forceinline__ typename Lane16<T>::type load16(const T* p, int count) {
-    using V = typename Lane16<T>::type;
-    if (count >= Lane16<T>::values) return *reinterpret_cast<const V*>(p);
-    V v;
-#pragma unroll
-    for (int k = 0; k < Lane16<T>::values; k++) v[k] = k < count ? p[k] : static_cast<T>(0.0f);
-    return v;
+template <typename T, int W>
+__device__ __forceinline__ float value_of(const typename Part<T, W>::type& v, int k) {
+    if constexpr (W == 1) return static_cast<float>(v);
+    else return static_cast<float>(v[k]);
 }
 
 // a float32 product, then rounded to T: the compiler would make one instruction of both for float16 (v_fma_mixlo_f16), whose
@@ -47,18 +43,16 @@ __device__ __forceinline__ T scaled(float x, float scale) {
     return static_cast<T>(y);
 }
 
-template <typename T>
-__device__ __forceinline__ void store16(T* p, int count, const float* x, float scale) {
-    if (count >= Lane16<T>::values) {
-        typename Lane16<T>::type v;
+template <typename T, int W>
+__device__ __forceinline__ void store_part(T* p, const float* x, float scale) {
+    if constexpr (W == 1) {
+        *p = scaled<T>(x[0], scale);
+    } else {
+        typename Part<T, W>::type v;
 #pragma unroll
-        for (int k = 0; k < Lane16<T>::values; k++) v[k] = scaled<T>(x[k], scale);
-        *reinterpret_cast<typename Lane16<T>::type*>(p) = v;
-        return;
+        for (int k = 0; k < W; k++) v[k] = scaled<T>(x[k], scale);
+        *reinterpret_cast<typename Part<T, W>::type*>(p) = v;
     }
-#pragma unroll
-    for (int k = 0; k < Lane16<T>::values; k++)
-        if (k < count) p[k] = scaled<T>(x[k], scale);
 }
 
 constexpr uint32_t max_blocks = 1u << 23;  // of a launch of 256 threads (32 bits of threads)
@@ -78,43 +72,50 @@ struct LookupArgs {
     void* out;
     uint64_t row_stride;      // of the table
     uint32_t first, n, rows, columns;  // this launch: indices from `first` on
-    uint32_t lanes;           // 16-byte lanes of a row in this tile of columns (<= lookup_tile)
+    uint32_t row_lanes;       // lanes of a row
+    uint32_t lanes;           // of them in a block's tile of columns (<= lookup_tile)
     uint32_t lanes_rcp;       // 2^20 / lanes + 1: t / lanes = t * lanes_rcp >> 20 for t < 1024
     uint32_t rows_per_block;
     float scale;
 };
 
-// A block takes whole rows (or, past 1,024 lanes of 16 bytes, 1,024 lanes of one row), consecutive lanes of it a row's
-// consecutive 16 bytes, four of them to a thread, all loaded before the first is stored.
-template <typename T, typename I>
+// A block takes whole rows (or, past 1,024 lanes, 1,024 lanes of one row), consecutive lanes of it a row's consecutive parts, four
+// of them to a thread: four indices, then four parts, then the stores.
+template <typename T, int W, typename I>
 __global__ __launch_bounds__(lookup_block) void embedding_lookup_kernel(LookupArgs a) {
-    constexpr int values = Lane16<T>::values;
-    const uint32_t first_lane = blockIdx.y * lookup_tile;
-    const uint32_t items = a.rows_per_block * a.lanes;
-    typename Lane16<T>::type v[lookup_items];
-    uint64_t at[lookup_items];
-    int count[lookup_items];
+    const uint32_t first_lane = blockIdx.y * lookup_tile, items = a.rows_per_block * a.lanes;
+    const uint64_t first_row = a.first + static_cast<uint64_t>(blockIdx.x) * a.rows_per_block;
+    uint64_t i[lookup_items];
+    uint32_t column[lookup_items], row[lookup_items];
+    bool valid[lookup_items];
+    typename Part<T, W>::type v[lookup_items];
 #pragma unroll
     for (uint32_t k = 0; k < lookup_items; k++) {
-        const uint32_t t = k * lookup_block + threadIdx.x;
-        const uint32_t q = (t * a.lanes_rcp) >> 20, lane = first_lane + t - q * a.lanes;
-        const uint64_t i = a.first + static_cast<uint64_t>(blockIdx.x) * a.rows_per_block + q;
-        count[k] = 0;
-        if (t >= items || i >= a.n || lane * values >= a.columns) continue;
-        const uint32_t column = lane * values;
-        count[k] = static_cast<int>(min(a.columns - column, static_cast<uint32_t>(values)));
-        at[k] = i * a.columns + column;
-        const uint32_t row = row_of(static_cast<const I*>(a.indices)[i], a.rows);
-        v[k] = load16(static_cast<const T*>(a.table) + row * a.row_stride + column, row < a.rows ? count[k] : 0);
+        const uint32_t t = k * lookup_block + threadIdx.x, u = min(t, items - 1);
+        const uint32_t q = (u * a.lanes_rcp) >> 20, lane = first_lane + u - q * a.lanes;
+        valid[k] = t < items && first_row + q < a.n && lane < a.row_lanes;
+        i[k] = min(first_row + q, static_cast<uint64_t>(a.n - 1));
+        column[k] = min(lane * W, a.columns - W);
+        row[k] = row_of(static_cast<const I*>(a.indices)[i[k]], a.rows);
     }
+    const uint32_t last_row = a.rows - 1;
+#pragma unroll
+    for (uint32_t k = 0; k < lookup_items; k++)
+        v[k] = load_part<T, W>(static_cast<const T*>(a.table) + min(row[k], last_row) * a.row_stride + column[k]);
 #pragma unroll
     for (uint32_t k = 0; k < lookup_items; k++) {
-        if (count[k] == 0) continue;
-        float x[values];
+        float x[W];
 #pragma unroll
-        for (int j = 0; j < values; j++) x[j] = static_cast<float>(v[k][j]);
-        store16(static_cast<T*>(a.out) + at[k], count[k], x, a.scale);
+        for (int j = 0; j < W; j++) x[j] = row[k] < a.rows ? value_of<T, W>(v[k], j) : 0.0f;
+        if (valid[k]) store_part<T, W>(static_cast<T*>(a.out) + i[k] * a.columns + column[k], x, a.scale);
     }
+}
+
+// a table without rows
+template <typename T>
+__global__ __launch_bounds__(lookup_block) void embedding_zero_kernel(T* out, uint64_t n) {
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * lookup_block + threadIdx.x; i < n; i += static_cast<uint64_t>(gridDim.x) * lookup_block)
+        out[i] = static_cast<T>(0.0f);
 }
 
 // ---- sort --------------------------------------------------------------------------------------------------------------
@@ -127,23 +128,22 @@ __global__ __launch_bounds__(lookup_block) void embedding_lookup_kernel(LookupAr
 constexpr uint32_t sort_block = 1024, sort_waves = sort_block / 64, sort_steps = 4, sort_tile = sort_block * sort_steps;
 constexpr uint32_t sort_max_blocks = 256, sort_digits = 256;
 constexpr uint32_t sort_alone = 8 * sort_tile;     // largest list that every block counts by itself
-constexpr uint32_t rank_most = 8192, rank_keys = 64;  // largest list ordered by ranks, and keys of a block
+constexpr uint32_t rank_most = 8192, rank_keys = 16;  // largest list ordered by ranks, and keys of a block
 
 struct SortPass {
     const void* indices;       // first pass: int32 or int64
-    const uint32_t* keys_in;   // later ones
-    const uint32_t* values_in;
-    uint32_t* keys_out;
-    uint32_t* values_out;
+    const uint2* in;           // later ones: key, value
+    uint2* out;
     uint32_t* table;           // blocks x 256
     uint32_t n, rows, padding; // padding: a row that counts nowhere (>= rows: none)
     uint32_t shift, digit_mask;
     uint32_t tiles_per_block;
 };
 
+// I: the indices' type, or uint2 for a later pass
 template <typename I>
 __device__ __forceinline__ uint32_t key_at(const SortPass& a, uint32_t i) {
-    if constexpr (sizeof(I) == 1) return a.keys_in[i];
+    if constexpr (std::is_same_v<I, uint2>) return a.in[i].x;
     else {
         const uint32_t row = row_of(static_cast<const I*>(a.indices)[i], a.rows);
         return row == a.padding ? a.rows : row;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(sort_block) void sort_count_kernel(SortPass a) {
 #pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++) {
             const uint64_t i = first + s * sort_block;
-            key[s] = i < a.n ? key_at<I>(a, static_cast<uint32_t>(i)) : 0u;
+            key[s] = key_at<I>(a, static_cast<uint32_t>(min(i, static_cast<uint64_t>(a.n - 1))));
         }
 #pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++)
@@ -171,23 +171,53 @@ __global__ __launch_bounds__(sort_block) void sort_count_kernel(SortPass a) {
     if (threadIdx.x < sort_digits) a.table[blockIdx.x * sort_digits + threadIdx.x] = counts[threadIdx.x];
 }
 
-// ALONE: the block counts the digits of the whole list
+template <typename I>
+__device__ __forceinline__ uint2 pair_at(const SortPass& a, uint32_t i) {
+    if constexpr (std::is_same_v<I, uint2>) return a.in[i];
+    else return make_uint2(key_at<I>(a, i), i);
+}
+
+// exclusive prefix over the wave's lanes; the wave's total goes to totals[wave]
+__device__ __forceinline__ uint32_t wave_exclusive(uint32_t v, uint32_t* totals) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t inclusive = v;
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const uint32_t t = __shfl_up(inclusive, o);
+        if (lane >= o) inclusive += t;
+    }
+    if (lane == 63) totals[threadIdx.x >> 6] = inclusive;
+    return inclusive - v;
+}
+
+__device__ __forceinline__ uint32_t totals_before(uint32_t wave, const uint32_t* totals) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; w++)
+        if (w < wave) sum += totals[w];
+    return sum;
+}
+
+// ALONE: the block counts the digits of the whole list. A tile is put in order in LDS and written from there, so that a wave's
+// stores meet few lines (written from the keys' own lanes, a pass over 1M keys took 22 us).
 template <typename I, bool ALONE>
 __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
-    __shared__ uint32_t counts[sort_waves][sort_digits];  // keys of each digit in a wave's part of the tile, then their first place
-    __shared__ uint32_t parts[2][4][sort_digits], wave_totals[4];
+    __shared__ uint32_t counts[sort_waves][sort_digits];  // keys of each digit in a wave's part of the tile, then their first place in it
+    __shared__ uint32_t parts[2][4][sort_digits], wave_totals[4], to_global[sort_digits];
+    __shared__ uint2 ordered[sort_tile];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, digit = threadIdx.x & (sort_digits - 1), quarter = threadIdx.x >> 8;
     const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block * sort_tile;
     // keys of the digit in all blocks and in those before this one, a quarter of the list or of the table's rows at a time
     if constexpr (ALONE) {
         parts[0][quarter][digit] = parts[1][quarter][digit] = 0;
         __syncthreads();
-        for (uint32_t from = threadIdx.x; from < a.n; from += sort_tile) {
-            uint32_t key[sort_steps];
+        constexpr uint32_t at_once = 16;
+        for (uint32_t from = threadIdx.x; from < a.n; from += at_once * sort_block) {
+            uint32_t key[at_once];
 #pragma unroll
-            for (uint32_t s = 0; s < sort_steps; s++) key[s] = from + s * sort_block < a.n ? key_at<I>(a, from + s * sort_block) : 0u;
+            for (uint32_t s = 0; s < at_once; s++) key[s] = key_at<I>(a, min(from + s * sort_block, a.n - 1));
 #pragma unroll
-            for (uint32_t s = 0; s < sort_steps; s++) {
+            for (uint32_t s = 0; s < at_once; s++) {
                 const uint32_t i = from + s * sort_block;
                 if (i < a.n) atomicAdd(&parts[i < begin ? 1 : 0][quarter][(key[s] >> a.shift) & a.digit_mask], 1u);
             }
@@ -199,49 +229,37 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
 #pragma unroll 16
         for (uint32_t k = 0; k < rows; k++) {
             const uint32_t b = quarter * rows + k;
-            const uint32_t c = b < gridDim.x ? a.table[b * sort_digits + digit] : 0u;
-            total += c;
+            const uint32_t c = a.table[min(b, gridDim.x - 1) * sort_digits + digit];
+            total += b < gridDim.x ? c : 0u;
             before += b < blockIdx.x ? c : 0u;
         }
         parts[0][quarter][digit] = total - before;
         parts[1][quarter][digit] = before;
         __syncthreads();
     }
-    uint32_t place = 0, total = 0;  // (threads of the first quarter: their digit's)
+    uint32_t place = 0;  // (threads of the first quarter: of their digit's next key)
     if (quarter == 0) {
-        uint32_t before = 0;
+        uint32_t before = 0, total = 0;
 #pragma unroll
         for (uint32_t q = 0; q < 4; q++) {
             before += parts[1][q][digit];
             total += parts[0][q][digit];
         }
         total += before;
-        uint32_t inclusive = total;
-#pragma unroll
-        for (uint32_t o = 1; o < 64; o <<= 1) {
-            const uint32_t t = __shfl_up(inclusive, o);
-            if (lane >= o) inclusive += t;
-        }
-        if (lane == 63) wave_totals[wave] = inclusive;
-        place = inclusive - total + before;
+        place = before + wave_exclusive(total, wave_totals);
     }
     __syncthreads();
-    if (quarter == 0) {
-#pragma unroll
-        for (uint32_t w = 0; w < 4; w++)
-            if (w < wave) place += wave_totals[w];
-    }
+    if (quarter == 0) place += totals_before(wave, wave_totals);
     for (uint32_t tile = 0; tile < a.tiles_per_block; tile++) {
         const uint64_t first = begin + tile * static_cast<uint64_t>(sort_tile);
         if (first >= a.n) break;
-        uint32_t key[sort_steps], value[sort_steps], rank[sort_steps];
+        uint2 pair[sort_steps];
+        uint32_t rank[sort_steps];
         const uint64_t wave_first = first + wave * 64u * sort_steps + lane;
 #pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++) {
             const uint64_t i = wave_first + s * 64u;
-            key[s] = i < a.n ? key_at<I>(a, static_cast<uint32_t>(i)) : 0u;
-            if constexpr (sizeof(I) == 1) value[s] = i < a.n ? a.values_in[i] : 0u;
-            else value[s] = static_cast<uint32_t>(i);
+            pair[s] = pair_at<I>(a, static_cast<uint32_t>(min(i, static_cast<uint64_t>(a.n - 1))));
         }
 #pragma unroll
         for (uint32_t k = 0; k < sort_digits / 64; k++) counts[wave][k * 64 + lane] = 0;
@@ -249,7 +267,7 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++) {
-            const uint32_t d = (key[s] >> a.shift) & a.digit_mask;
+            const uint32_t d = (pair[s].x >> a.shift) & a.digit_mask;
             const bool valid = wave_first + s * 64u < a.n;
             uint64_t same = __ballot(valid);
 #pragma unroll
@@ -266,55 +284,69 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
+        uint32_t in_tile = 0, local = 0;
         if (quarter == 0) {
+#pragma unroll
+            for (uint32_t w = 0; w < sort_waves; w++) in_tile += counts[w][digit];
+            local = wave_exclusive(in_tile, wave_totals);
+        }
+        __syncthreads();
+        if (quarter == 0) {
+            local += totals_before(wave, wave_totals);
+            to_global[digit] = place - local;
+            place += in_tile;
 #pragma unroll
             for (uint32_t w = 0; w < sort_waves; w++) {
                 const uint32_t c = counts[w][digit];
-                counts[w][digit] = place;
-                place += c;
+                counts[w][digit] = local;
+                local += c;
             }
         }
         __syncthreads();
 #pragma unroll
+        for (uint32_t s = 0; s < sort_steps; s++)
+            if (wave_first + s * 64u < a.n) ordered[counts[wave][(pair[s].x >> a.shift) & a.digit_mask] + rank[s]] = pair[s];
+        __syncthreads();
+        const uint32_t here = static_cast<uint32_t>(min(static_cast<uint64_t>(sort_tile), a.n - first));
+#pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++) {
-            if (wave_first + s * 64u < a.n) {
-                const uint32_t to = counts[wave][(key[s] >> a.shift) & a.digit_mask] + rank[s];
-                a.keys_out[to] = key[s];
-                a.values_out[to] = value[s];
+            const uint32_t k = s * sort_block + threadIdx.x;
+            if (k < here) {
+                const uint2 p = ordered[k];
+                a.out[to_global[(p.x >> a.shift) & a.digit_mask] + k] = p;
             }
         }
         __syncthreads();
     }
 }
 
-// A key's place is the number of smaller keys, and of equal ones before it: 64 keys to a block, each compared by 16 threads
-// with a 16th of the list.
+// A key's place is the number of smaller keys, and of equal ones before it: 16 keys to a block, each compared by 64 threads
+// with a 64th of the list.
 template <typename I>
 __global__ __launch_bounds__(sort_block) void sort_rank_kernel(SortPass a) {
     __shared__ __attribute__((aligned(16))) uint32_t keys[rank_most];
-    __shared__ uint32_t places[sort_waves][rank_keys];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t per = (a.n + sort_waves * 4 - 1) / (sort_waves * 4) * 4;  // of a wave, in fours
-    for (uint32_t i = threadIdx.x; i < per * sort_waves; i += sort_block) keys[i] = i < a.n ? key_at<I>(a, i) : 0xffffffffu;
+    __shared__ uint32_t places[sort_block / rank_keys][rank_keys];
+    constexpr uint32_t parts = sort_block / rank_keys;
+    const uint32_t k = threadIdx.x % rank_keys, part = threadIdx.x / rank_keys;
+    const uint32_t per = (a.n + parts * 4 - 1) / (parts * 4) * 4;  // of a part, in fours
+    for (uint32_t i = threadIdx.x; i < per * parts; i += sort_block) keys[i] = i < a.n ? key_at<I>(a, i) : 0xffffffffu;
     __syncthreads();
-    const uint32_t i = blockIdx.x * rank_keys + lane, mine = keys[min(i, a.n - 1)];
+    const uint32_t i = blockIdx.x * rank_keys + k, mine = keys[min(i, a.n - 1)];
     uint32_t smaller = 0;
-    const uint4* const part = reinterpret_cast<const uint4*>(keys + wave * per);
-    for (uint32_t k = 0; k < per / 4; k++) {
-        const uint4 other = part[k];
-        const uint32_t at = wave * per + k * 4;
+    const uint4* const list = reinterpret_cast<const uint4*>(keys + part * per);
+    for (uint32_t j = 0; j < per / 4; j++) {
+        const uint4 other = list[j];
+        const uint32_t at = part * per + j * 4;
         // (equal keys count where they stand before: as if they were smaller)
         smaller += (other.x < mine + (at < i ? 1u : 0u)) + (other.y < mine + (at + 1 < i ? 1u : 0u)) + (other.z < mine + (at + 2 < i ? 1u : 0u)) +
                    (other.w < mine + (at + 3 < i ? 1u : 0u));
     }
-    places[wave][lane] = smaller;
+    places[part][k] = smaller;
     __syncthreads();
-    if (wave == 0 && i < a.n) {
+    if (threadIdx.x < rank_keys && i < a.n) {
         uint32_t to = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < sort_waves; w++) to += places[w][lane];
-        a.keys_out[to] = mine;
-        a.values_out[to] = i;
+        for (uint32_t p = 0; p < parts; p++) to += places[p][k];
+        a.out[to] = make_uint2(mine, i);
     }
 }
 
@@ -323,15 +355,15 @@ __global__ __launch_bounds__(sort_block) void sort_rank_kernel(SortPass a) {
 constexpr uint32_t sum_block = 256, sum_items = 8;  // items of a group of lanes
 
 struct SumArgs {
-    const uint32_t* keys;      // sorted
-    const uint32_t* values;
+    const uint2* pairs;        // row and position, sorted
     const void* grad_out;
     void* gradient;
     float* heads;              // per block: its first row's piece up to that row's end
     float* tails;              // per block: the sum of the row that is open at its end
     uint32_t* closed;          // per block: 1 where a row ends in it
     uint32_t* first_row;       // per block: the row that is open at its start
-    uint32_t n, rows, columns, padded_columns;
+    uint32_t n, rows, columns;
+    uint32_t row_lanes;        // lanes of a row
     uint32_t blocks;
     float scale;
 };
@@ -342,7 +374,7 @@ __device__ __forceinline__ uint32_t entries_before(const SumArgs& a, uint32_t po
     uint32_t lo = position > a.rows ? position - a.rows : 0u, hi = min(position, a.n);
     while (lo < hi) {
         const uint32_t step = (hi - lo + 127u) / 128u, at = lo + lane * step, at2 = at + 64u * step;
-        const uint32_t key = a.keys[min(at, hi - 1)], key2 = a.keys[min(at2, hi - 1)];
+        const uint32_t key = a.pairs[min(at, hi - 1)].x, key2 = a.pairs[min(at2, hi - 1)].x;
         const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(at < hi && at + key < position)) + __popcll(__ballot(at2 < hi && at2 + key2 < position)));
         if (before == 0) break;
         hi = min(hi, lo + before * step);
@@ -351,13 +383,12 @@ __device__ __forceinline__ uint32_t entries_before(const SumArgs& a, uint32_t po
     return lo;
 }
 
-// G lanes to a row (of a tile of columns), 16 bytes each.
-template <typename T, int G>
+// G lanes to a row (of a tile of columns).
+template <typename T, int W, int G>
 __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
-    constexpr int values = Lane16<T>::values;
     constexpr uint32_t groups = sum_block / G, items = groups * sum_items;
     __shared__ uint32_t s_keys[items], s_values[items], s_start[groups + 1], s_bounds[2];
-    __shared__ float s_tail[sum_block / 64][G * values];
+    __shared__ float s_tail[sum_block / 64][G * W];
     __shared__ uint32_t s_closed[sum_block / 64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t total = a.n + a.rows, first = blockIdx.x * items, last = min(first + items, total);
@@ -368,8 +399,9 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
     __syncthreads();
     const uint32_t e0 = s_bounds[0], entries = s_bounds[1] - e0;
     for (uint32_t k = threadIdx.x; k < entries; k += sum_block) {
-        s_keys[k] = a.keys[e0 + k];
-        s_values[k] = a.values[e0 + k];
+        const uint2 p = a.pairs[e0 + k];
+        s_keys[k] = p.x;
+        s_values[k] = p.y;
     }
     __syncthreads();
     for (uint32_t g = threadIdx.x; g <= groups; g += sum_block) {
@@ -384,34 +416,36 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
     }
     __syncthreads();
 
-    const uint32_t group = threadIdx.x / G, column = (blockIdx.y * G + threadIdx.x % G) * values;
-    const int count = column < a.columns ? static_cast<int>(min(a.columns - column, static_cast<uint32_t>(values))) : 0;
+    const uint32_t group = threadIdx.x / G, slot = blockIdx.y * G + threadIdx.x % G, column = min(slot * W, a.columns - W);
+    const bool valid = slot < a.row_lanes;
     const uint32_t start = s_start[group], end = s_start[group + 1];
     const uint32_t position = min(first + group * sum_items, last), position_end = min(position + sum_items, last);
     const uint32_t row_start = position - (e0 + start), row_end = position_end - (e0 + end);
 
-    typename Lane16<T>::type data[sum_items];
+    // the group's entries (past its last one, and for indices that count nowhere, some row that is there)
+    typename Part<T, W>::type data[sum_items];
+    if (entries > 0) {
 #pragma unroll
-    for (uint32_t k = 0; k < sum_items; k++) {
-        const bool is_entry = start + k < end && s_keys[min(start + k, items - 1)] < a.rows;
-        data[k] = load16(static_cast<const T*>(a.grad_out) + static_cast<uint64_t>(is_entry ? s_values[start + k] : 0u) * a.columns + column,
-                         is_entry ? count : 0);
+        for (uint32_t k = 0; k < sum_items; k++) {
+            const uint32_t e = min(start + k, entries - 1);
+            data[k] = load_part<T, W>(static_cast<const T*>(a.grad_out) + static_cast<uint64_t>(s_values[s_keys[e] < a.rows ? e : 0u]) * a.columns + column);
+        }
     }
 
     T* const gradient = static_cast<T*>(a.gradient);
-    float sum[values] = {}, head[values] = {};
+    float sum[W] = {}, head[W] = {};
     bool any_closed = false;
     uint32_t row = row_start;
     auto close = [&]() {
         if (!any_closed) {
 #pragma unroll
-            for (int j = 0; j < values; j++) head[j] = sum[j];
+            for (int j = 0; j < W; j++) head[j] = sum[j];
             any_closed = true;
-        } else {
-            store16(gradient + static_cast<uint64_t>(row) * a.columns + column, count, sum, a.scale);
+        } else if (valid) {
+            store_part<T, W>(gradient + static_cast<uint64_t>(row) * a.columns + column, sum, a.scale);
         }
 #pragma unroll
-        for (int j = 0; j < values; j++) sum[j] = 0.0f;
+        for (int j = 0; j < W; j++) sum[j] = 0.0f;
         row++;
     };
 #pragma unroll
@@ -419,22 +453,23 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
         if (start + k < end) {
             const uint32_t key = s_keys[start + k];
             while (row < key && row < row_end) close();
+            // (entries of indices that count nowhere stand behind the last row's end: their sums go nowhere)
 #pragma unroll
-            for (int j = 0; j < values; j++) sum[j] += static_cast<float>(data[k][j]);
+            for (int j = 0; j < W; j++) sum[j] += value_of<T, W>(data[k], j);
         }
     }
     while (row < row_end) close();
 
     // what is open at the start of each group: a segmented scan of the groups' open sums, first over the wave, then over the block
-    float scanned[values];
+    float scanned[W];
     uint32_t flag = any_closed ? 1u : 0u;
 #pragma unroll
-    for (int j = 0; j < values; j++) scanned[j] = sum[j];
+    for (int j = 0; j < W; j++) scanned[j] = sum[j];
 #pragma unroll
     for (uint32_t o = G; o < 64; o <<= 1) {
         const uint32_t other_flag = __shfl_up(flag, o);
 #pragma unroll
-        for (int j = 0; j < values; j++) {
+        for (int j = 0; j < W; j++) {
             const float other = __shfl_up(scanned[j], o);
             if (lane >= o && !flag) scanned[j] += other;
         }
@@ -442,47 +477,47 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
     }
     if (lane >= 64 - G) {
 #pragma unroll
-        for (int j = 0; j < values; j++) s_tail[wave][(lane % G) * values + j] = scanned[j];
+        for (int j = 0; j < W; j++) s_tail[wave][(lane % G) * W + j] = scanned[j];
         if (lane == 63) s_closed[wave] = flag;
     }
     __syncthreads();
     uint32_t before_flag = 0, block_flag = 0;
-    float before[values] = {}, block_tail[values] = {};
+    float before[W] = {}, block_tail[W] = {};
 #pragma unroll
     for (uint32_t w = 0; w < sum_block / 64; w++) {
         if (w == wave) {
             before_flag = block_flag;
 #pragma unroll
-            for (int j = 0; j < values; j++) before[j] = block_tail[j];
+            for (int j = 0; j < W; j++) before[j] = block_tail[j];
         }
         const bool closed = s_closed[w] != 0;
 #pragma unroll
-        for (int j = 0; j < values; j++) block_tail[j] = s_tail[w][(lane % G) * values + j] + (closed ? 0.0f : block_tail[j]);
+        for (int j = 0; j < W; j++) block_tail[j] = s_tail[w][(lane % G) * W + j] + (closed ? 0.0f : block_tail[j]);
         block_flag |= closed ? 1u : 0u;
     }
     if constexpr (G < 64) {
         const uint32_t wave_flag = __shfl_up(flag, G);
 #pragma unroll
-        for (int j = 0; j < values; j++) {
+        for (int j = 0; j < W; j++) {
             const float other = __shfl_up(scanned[j], G);
             if (lane >= G) before[j] = other + (wave_flag ? 0.0f : before[j]);
         }
         if (lane >= G) before_flag |= wave_flag;
     }
-    const uint64_t piece = static_cast<uint64_t>(blockIdx.x) * a.padded_columns + column;
+    const uint64_t piece = (static_cast<uint64_t>(blockIdx.x) * gridDim.y * G + slot) * W;
     if (any_closed) {
 #pragma unroll
-        for (int j = 0; j < values; j++) head[j] += before[j];
-        if (before_flag) {
-            store16(gradient + static_cast<uint64_t>(row_start) * a.columns + column, count, head, a.scale);
-        } else {
+        for (int j = 0; j < W; j++) head[j] += before[j];
+        if (!before_flag) {
 #pragma unroll
-            for (int j = 0; j < values; j++) a.heads[piece + j] = head[j];
+            for (int j = 0; j < W; j++) a.heads[piece + j] = head[j];
+        } else if (valid) {
+            store_part<T, W>(gradient + static_cast<uint64_t>(row_start) * a.columns + column, head, a.scale);
         }
     }
     if (threadIdx.x < G) {
 #pragma unroll
-        for (int j = 0; j < values; j++) a.tails[piece + j] = block_tail[j];
+        for (int j = 0; j < W; j++) a.tails[piece + j] = block_tail[j];
     }
     if (threadIdx.x == 0 && blockIdx.y == 0) {
         a.closed[blockIdx.x] = block_flag;
@@ -492,14 +527,12 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
 
 // One wave per block of the sums and tile of columns: the row that was open at the block's start, if it ends there, from
 // the open sums of the blocks before it since the last end of a row, and the block's own first piece.
-template <typename T, int G>
+template <typename T, int W, int G>
 __global__ __launch_bounds__(64) void embedding_join_kernel(SumArgs a) {
-    constexpr int values = Lane16<T>::values;
     constexpr uint32_t slots = 64 / G;
-    const uint32_t lane = threadIdx.x, slot = lane / G, b = blockIdx.x;
+    const uint32_t lane = threadIdx.x, part = lane / G, b = blockIdx.x;
     if (!a.closed[b]) return;
-    const uint32_t column = (blockIdx.y * G + lane % G) * values;
-    const int count = column < a.columns ? static_cast<int>(min(a.columns - column, static_cast<uint32_t>(values))) : 0;
+    const uint32_t slot = blockIdx.y * G + lane % G;
     uint32_t from = b;
     while (from > 0) {  // back to the last block before b in which a row ends
         const bool in = lane < from;
@@ -510,34 +543,47 @@ __global__ __launch_bounds__(64) void embedding_join_kernel(SumArgs a) {
         }
         from = from > 64 ? from - 64 : 0;
     }
-    float sum[values] = {};
+    const uint64_t stride = static_cast<uint64_t>(gridDim.y) * G * W, piece = static_cast<uint64_t>(slot) * W;
+    float sum[W] = {};
 #pragma unroll 8
-    for (uint32_t k = from + slot; k < b; k += slots) {
+    for (uint32_t k = from + part; k < b; k += slots) {
 #pragma unroll
-        for (int j = 0; j < values; j++) sum[j] += a.tails[static_cast<uint64_t>(k) * a.padded_columns + column + j];
+        for (int j = 0; j < W; j++) sum[j] += a.tails[k * stride + piece + j];
     }
 #pragma unroll
     for (uint32_t o = G; o < 64; o <<= 1) {
 #pragma unroll
-        for (int j = 0; j < values; j++) sum[j] += __shfl_xor(sum[j], o);
+        for (int j = 0; j < W; j++) sum[j] += __shfl_xor(sum[j], o);
     }
-    if (slot == 0) {
+    if (part == 0 && slot < a.row_lanes) {
 #pragma unroll
-        for (int j = 0; j < values; j++) sum[j] += a.heads[static_cast<uint64_t>(b) * a.padded_columns + column + j];
-        store16(static_cast<T*>(a.gradient) + static_cast<uint64_t>(a.first_row[b]) * a.columns + column, count, sum, a.scale);
+        for (int j = 0; j < W; j++) sum[j] += a.heads[b * stride + piece + j];
+        store_part<T, W>(static_cast<T*>(a.gradient) + static_cast<uint64_t>(a.first_row[b]) * a.columns + min(slot * W, a.columns - W), sum, a.scale);
     }
 }
 
 uint32_t bit_width(uint32_t x) { return x == 0 ? 0u : 32u - static_cast<uint32_t>(__builtin_clz(x)); }
 
-template <typename F>
-void with_type(int type, F&& f) {
-    if (type == type_float) f(float{});
-    else if (type == type_bfloat16) f(__bf16{});
-    else f(_Float16{});
+int lane_values(const EmbeddingArgs& a) {
+    const uint32_t full = a.type == type_float ? 4 : 8;
+    return a.columns >= full ? static_cast<int>(full) : 1;
 }
 
-uint32_t lanes_of_row(const EmbeddingArgs& a) { return div_up(a.columns, a.type == type_float ? 4 : 8); }
+uint32_t lanes_of_row(const EmbeddingArgs& a) { return div_up(a.columns, static_cast<uint32_t>(lane_values(a))); }
+
+// f(a value of the type, the lane's values as a constant)
+template <typename F>
+void with_type(const EmbeddingArgs& a, F&& f) {
+    const bool one = lane_values(a) == 1;
+    auto widths = [&](auto t) {
+        constexpr int full = 16 / sizeof(t);
+        if (one) f(t, std::integral_constant<int, 1>{});
+        else f(t, std::integral_constant<int, full>{});
+    };
+    if (a.type == type_float) widths(float{});
+    else if (a.type == type_bfloat16) widths(__bf16{});
+    else widths(_Float16{});
+}
 
 // lanes of a group: the power of two that holds a row, or a wave
 uint32_t group_lanes(const EmbeddingArgs& a) {
@@ -560,14 +606,12 @@ void launch_sort_pass(const SortPass& p, hipStream_t s) {
 }
 
 struct GradientLayout {
-    uint32_t* keys[2];
-    uint32_t* values[2];
+    uint2* pairs[2];
     uint32_t* table;
     float* heads;
     float* tails;
     uint32_t* closed;
     uint32_t* first_row;
-    uint32_t padded_columns;
     size_t bytes;
 
     static GradientLayout carve(char* base, const EmbeddingArgs& a) {
@@ -578,14 +622,12 @@ struct GradientLayout {
             used += (bytes + 255) / 256 * 256;
             return p;
         };
-        const uint32_t lanes = group_lanes(a), per_lane = a.type == type_float ? 4 : 8;
-        l.padded_columns = div_up(lanes_of_row(a), lanes) * lanes * per_lane;
-        const size_t blocks = sum_blocks(a);
-        for (int k = 0; k < 2; k++) l.keys[k] = reinterpret_cast<uint32_t*>(take(size_t{a.n} * 4));
-        for (int k = 0; k < 2; k++) l.values[k] = reinterpret_cast<uint32_t*>(take(size_t{a.n} * 4));
+        const size_t lanes = group_lanes(a), blocks = sum_blocks(a);
+        const size_t piece = div_up(lanes_of_row(a), lanes) * lanes * static_cast<size_t>(lane_values(a)) * 4;
+        for (int k = 0; k < 2; k++) l.pairs[k] = reinterpret_cast<uint2*>(take(size_t{a.n} * 8));
         l.table = reinterpret_cast<uint32_t*>(take(size_t{sort_max_blocks} * sort_digits * 4));
-        l.heads = reinterpret_cast<float*>(take(blocks * l.padded_columns * 4));
-        l.tails = reinterpret_cast<float*>(take(blocks * l.padded_columns * 4));
+        l.heads = reinterpret_cast<float*>(take(blocks * piece));
+        l.tails = reinterpret_cast<float*>(take(blocks * piece));
         l.closed = reinterpret_cast<uint32_t*>(take(blocks * 4));
         l.first_row = reinterpret_cast<uint32_t*>(take(blocks * 4));
         l.bytes = used;
@@ -593,17 +635,27 @@ struct GradientLayout {
     }
 };
 
-template <typename T, int G>
-void launch_sums(const SumArgs& a, uint32_t lanes, hipStream_t s) {
-    const uint32_t tiles = div_up(lanes, G);
-    embedding_sum_kernel<T, G><<<dim3(a.blocks, tiles), sum_block, 0, s>>>(a);
-    embedding_join_kernel<T, G><<<dim3(a.blocks, tiles), 64, 0, s>>>(a);
+template <typename T, int W, int G>
+void launch_sums(const SumArgs& a, hipStream_t s) {
+    const uint32_t tiles = div_up(a.row_lanes, G);
+    embedding_sum_kernel<T, W, G><<<dim3(a.blocks, tiles), sum_block, 0, s>>>(a);
+    embedding_join_kernel<T, W, G><<<dim3(a.blocks, tiles), 64, 0, s>>>(a);
 }
 
 }  // namespace
 
 bool launch_embedding_lookup(const EmbeddingArgs& a, const void* table, uint64_t row_stride, void* out, hipStream_t s) {
     if (a.n == 0 || a.columns == 0) return true;
+    if (a.rows == 0) {
+        const uint64_t values = static_cast<uint64_t>(a.n) * a.columns;
+        const uint32_t blocks = values > 2048ull * lookup_block ? 2048u : div_up(values, lookup_block);
+        with_type(a, [&](auto t, auto) {
+            using T = decltype(t);
+            embedding_zero_kernel<T><<<blocks, lookup_block, 0, s>>>(static_cast<T*>(out), values);
+        });
+        EFGS_HIP_CHECK(hipGetLastError());
+        return true;
+    }
     LookupArgs l;
     l.indices = a.indices;
     l.table = table;
@@ -612,19 +664,20 @@ bool launch_embedding_lookup(const EmbeddingArgs& a, const void* table, uint64_t
     l.n = a.n;
     l.rows = a.rows;
     l.columns = a.columns;
-    const uint32_t lanes = lanes_of_row(a);
-    l.lanes = lanes < lookup_tile ? lanes : lookup_tile;
+    l.row_lanes = lanes_of_row(a);
+    l.lanes = l.row_lanes < lookup_tile ? l.row_lanes : lookup_tile;
     l.lanes_rcp = (1u << 20) / l.lanes + 1;
     l.rows_per_block = lookup_tile / l.lanes;
     l.scale = a.scale;
     const uint64_t blocks = div_up(a.n, l.rows_per_block);
     for (uint64_t b = 0; b < blocks; b += max_blocks) {
         l.first = static_cast<uint32_t>(b * l.rows_per_block);
-        const dim3 grid(static_cast<uint32_t>(blocks - b < max_blocks ? blocks - b : max_blocks), div_up(lanes, lookup_tile));
-        with_type(a.type, [&](auto t) {
+        const dim3 grid(static_cast<uint32_t>(blocks - b < max_blocks ? blocks - b : max_blocks), div_up(l.row_lanes, lookup_tile));
+        with_type(a, [&](auto t, auto w) {
             using T = decltype(t);
-            if (a.index_bytes == 4) embedding_lookup_kernel<T, int32_t><<<grid, lookup_block, 0, s>>>(l);
-            else embedding_lookup_kernel<T, int64_t><<<grid, lookup_block, 0, s>>>(l);
+            constexpr int W = decltype(w)::value;
+            if (a.index_bytes == 4) embedding_lookup_kernel<T, W, int32_t><<<grid, lookup_block, 0, s>>>(l);
+            else embedding_lookup_kernel<T, W, int64_t><<<grid, lookup_block, 0, s>>>(l);
         });
         EFGS_HIP_CHECK(hipGetLastError());
     }
@@ -644,9 +697,8 @@ bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uin
     if (a.n > 0) {
         SortPass p;
         p.indices = a.indices;
-        p.keys_in = p.values_in = nullptr;
-        p.keys_out = l.keys[0];
-        p.values_out = l.values[0];
+        p.in = nullptr;
+        p.out = l.pairs[0];
         p.table = l.table;
         p.n = a.n;
         p.rows = a.rows;
@@ -664,19 +716,16 @@ bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uin
             else launch_sort_pass<int64_t>(p, s);
             for (uint32_t k = 1; k < passes; k++) {
                 p.shift = k * digit_bits;
-                p.keys_in = l.keys[current];
-                p.values_in = l.values[current];
+                p.in = l.pairs[current];
                 current ^= 1u;
-                p.keys_out = l.keys[current];
-                p.values_out = l.values[current];
-                launch_sort_pass<uint8_t>(p, s);
+                p.out = l.pairs[current];
+                launch_sort_pass<uint2>(p, s);
             }
         }
         EFGS_HIP_CHECK(hipGetLastError());
     }
     SumArgs u;
-    u.keys = l.keys[current];
-    u.values = l.values[current];
+    u.pairs = l.pairs[current];
     u.grad_out = grad_out;
     u.gradient = gradient;
     u.heads = l.heads;
@@ -686,20 +735,27 @@ bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uin
     u.n = a.n;
     u.rows = a.rows;
     u.columns = a.columns;
-    u.padded_columns = l.padded_columns;
+    u.row_lanes = lanes_of_row(a);
     u.blocks = sum_blocks(a);
     u.scale = a.scale;
-    const uint32_t lanes = lanes_of_row(a);
-    with_type(a.type, [&](auto t) {
+    with_type(a, [&](auto t, auto w) {
         using T = decltype(t);
+        constexpr int W = decltype(w)::value;
         switch (group_lanes(a)) {
-            case 1: launch_sums<T, 1>(u, lanes, s); break;
-            case 2: launch_sums<T, 2>(u, lanes, s); break;
-            case 4: launch_sums<T, 4>(u, lanes, s); break;
-            case 8: launch_sums<T, 8>(u, lanes, s); break;
-            case 16: launch_sums<T, 16>(u, lanes, s); break;
-            case 32: launch_sums<T, 32>(u, lanes, s); break;
-            default: launch_sums<T, 64>(u, lanes, s); break;
+            case 1: launch_sums<T, W, 1>(u, s); break;
+            case 2: launch_sums<T, W, 2>(u, s); break;
+            case 4: launch_sums<T, W, 4>(u, s); break;
+            default:
+                if constexpr (W == 1) {
+                    launch_sums<T, W, 8>(u, s);  // (at most 7 lanes of one value)
+                } else {
+                    switch (group_lanes(a)) {
+                        case 8: launch_sums<T, W, 8>(u, s); break;
+                        case 16: launch_sums<T, W, 16>(u, s); break;
+                        case 32: launch_sums<T, W, 32>(u, s); break;
+                        default: launch_sums<T, W, 64>(u, s); break;
+                    }
+                }
         }
     });
     EFGS_HIP_CHECK(hipGetLastError());
