@@ -11,6 +11,7 @@
 // it. Every group of lanes takes the same number of items whatever the runs are; a sum that crosses groups is carried by a
 // segmented scan within the block, and a row that crosses blocks is put together by a second kernel from the blocks' first
 // and last pieces, in their order.
+#include <algorithm>
 #include <type_traits>
 
 #include "internal.h"
@@ -120,13 +121,13 @@ __global__ __launch_bounds__(lookup_block) void embedding_zero_kernel(T* out, ui
 
 // ---- sort --------------------------------------------------------------------------------------------------------------
 // Keys are rows (or `rows` for an index that counts nowhere), values the positions of their indices. A pass orders by up
-// to 8 bits: every block knows its digits' places (behind all smaller digits, and behind the same digits of earlier blocks)
+// to 9 bits: every block knows its digits' places (behind all smaller digits, and behind the same digits of earlier blocks)
 // and writes its keys there, each at its rank among the equal digits before it. The counts come from a table that a kernel
 // of the same blocks writes, or, up to 32,768 keys, from the block's own count of the whole list, which spares that launch.
 // Up to 8,192 keys one kernel counts for each key the smaller ones.
 
 constexpr uint32_t sort_block = 1024, sort_waves = sort_block / 64, sort_steps = 4, sort_tile = sort_block * sort_steps;
-constexpr uint32_t sort_max_blocks = 256, sort_digits = 256;
+constexpr uint32_t sort_max_blocks = 256, sort_least_bits = 6, sort_most_bits = 9, sort_most_digits = 1u << sort_most_bits;
 constexpr uint32_t sort_alone = 8 * sort_tile;     // largest list that every block counts by itself
 constexpr uint32_t rank_most = 8192, rank_keys = 16;  // largest list ordered by ranks, and keys of a block
 
@@ -134,9 +135,9 @@ struct SortPass {
     const void* indices;       // first pass: int32 or int64
     const uint2* in;           // later ones: key, value
     uint2* out;
-    uint32_t* table;           // blocks x 256
+    uint32_t* table;           // blocks x digits
     uint32_t n, rows, padding; // padding: a row that counts nowhere (>= rows: none)
-    uint32_t shift, digit_mask;
+    uint32_t shift, digit_bits;
     uint32_t tiles_per_block;
 };
 
@@ -150,10 +151,13 @@ __device__ __forceinline__ uint32_t key_at(const SortPass& a, uint32_t i) {
     }
 }
 
+__device__ __forceinline__ uint32_t digit_of(const SortPass& a, uint32_t key) { return (key >> a.shift) & ((1u << a.digit_bits) - 1u); }
+
 template <typename I>
 __global__ __launch_bounds__(sort_block) void sort_count_kernel(SortPass a) {
-    __shared__ uint32_t counts[sort_digits];
-    if (threadIdx.x < sort_digits) counts[threadIdx.x] = 0;
+    __shared__ uint32_t counts[sort_most_digits];
+    const uint32_t digits = 1u << a.digit_bits;
+    if (threadIdx.x < digits) counts[threadIdx.x] = 0;
     __syncthreads();
     for (uint32_t tile = 0; tile < a.tiles_per_block; tile++) {
         const uint64_t first = (static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block + tile) * sort_tile + threadIdx.x;
@@ -165,10 +169,10 @@ __global__ __launch_bounds__(sort_block) void sort_count_kernel(SortPass a) {
         }
 #pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++)
-            if (first + s * sort_block < a.n) atomicAdd(&counts[(key[s] >> a.shift) & a.digit_mask], 1u);
+            if (first + s * sort_block < a.n) atomicAdd(&counts[digit_of(a, key[s])], 1u);
     }
     __syncthreads();
-    if (threadIdx.x < sort_digits) a.table[blockIdx.x * sort_digits + threadIdx.x] = counts[threadIdx.x];
+    if (threadIdx.x < digits) a.table[blockIdx.x * digits + threadIdx.x] = counts[threadIdx.x];
 }
 
 template <typename I>
@@ -193,7 +197,7 @@ __device__ __forceinline__ uint32_t wave_exclusive(uint32_t v, uint32_t* totals)
 __device__ __forceinline__ uint32_t totals_before(uint32_t wave, const uint32_t* totals) {
     uint32_t sum = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < 4; w++)
+    for (uint32_t w = 0; w < sort_most_digits / 64; w++)
         if (w < wave) sum += totals[w];
     return sum;
 }
@@ -202,54 +206,64 @@ __device__ __forceinline__ uint32_t totals_before(uint32_t wave, const uint32_t*
 // stores meet few lines (written from the keys' own lanes, a pass over 1M keys took 22 us).
 template <typename I, bool ALONE>
 __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
-    __shared__ uint32_t counts[sort_waves][sort_digits];  // keys of each digit in a wave's part of the tile, then their first place in it
-    __shared__ uint32_t parts[2][4][sort_digits], wave_totals[4], to_global[sort_digits];
+    __shared__ uint16_t counts[sort_waves][sort_most_digits];  // keys of each digit in a wave's part of the tile, then their first place in it
+    __shared__ uint32_t wave_totals[sort_waves], to_global[sort_most_digits];
     __shared__ uint2 ordered[sort_tile];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, digit = threadIdx.x & (sort_digits - 1), quarter = threadIdx.x >> 8;
+    uint32_t* const all = reinterpret_cast<uint32_t*>(ordered);  // before the tiles: keys of each digit, in parts of the list
+    uint32_t* const earlier_blocks = all + sort_block;           // and those of them in blocks before this one
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t digits = 1u << a.digit_bits, parts = sort_block >> a.digit_bits;
     const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block * sort_tile;
-    // keys of the digit in all blocks and in those before this one, a quarter of the list or of the table's rows at a time
     if constexpr (ALONE) {
-        parts[0][quarter][digit] = parts[1][quarter][digit] = 0;
+        all[threadIdx.x] = earlier_blocks[threadIdx.x] = 0;
         __syncthreads();
         constexpr uint32_t at_once = 16;
+        const uint32_t part = threadIdx.x & ~(digits - 1u);
         for (uint32_t from = threadIdx.x; from < a.n; from += at_once * sort_block) {
             uint32_t key[at_once];
 #pragma unroll
             for (uint32_t s = 0; s < at_once; s++) key[s] = key_at<I>(a, min(from + s * sort_block, a.n - 1));
 #pragma unroll
             for (uint32_t s = 0; s < at_once; s++) {
-                const uint32_t i = from + s * sort_block;
-                if (i < a.n) atomicAdd(&parts[i < begin ? 1 : 0][quarter][(key[s] >> a.shift) & a.digit_mask], 1u);
+                const uint32_t i = from + s * sort_block, at = part + digit_of(a, key[s]);
+                if (i < a.n) {
+                    atomicAdd(&all[at], 1u);
+                    if (i < begin) atomicAdd(&earlier_blocks[at], 1u);
+                }
             }
         }
-        __syncthreads();
     } else {
+        const uint32_t digit = threadIdx.x & (digits - 1u), part = threadIdx.x >> a.digit_bits, rows = (gridDim.x + parts - 1) / parts;
         uint32_t before = 0, total = 0;
-        const uint32_t rows = (gridDim.x + 3) / 4;
-#pragma unroll 16
-        for (uint32_t k = 0; k < rows; k++) {
-            const uint32_t b = quarter * rows + k;
-            const uint32_t c = a.table[min(b, gridDim.x - 1) * sort_digits + digit];
-            total += b < gridDim.x ? c : 0u;
-            before += b < blockIdx.x ? c : 0u;
-        }
-        parts[0][quarter][digit] = total - before;
-        parts[1][quarter][digit] = before;
-        __syncthreads();
-    }
-    uint32_t place = 0;  // (threads of the first quarter: of their digit's next key)
-    if (quarter == 0) {
-        uint32_t before = 0, total = 0;
+        constexpr uint32_t at_once = 16;
+        for (uint32_t k = 0; k < rows; k += at_once) {
+            uint32_t c[at_once];
 #pragma unroll
-        for (uint32_t q = 0; q < 4; q++) {
-            before += parts[1][q][digit];
-            total += parts[0][q][digit];
+            for (uint32_t j = 0; j < at_once; j++) c[j] = a.table[min(part * rows + k + j, gridDim.x - 1) * digits + digit];
+#pragma unroll
+            for (uint32_t j = 0; j < at_once; j++) {
+                const uint32_t b = part * rows + k + j;
+                if (k + j >= rows || b >= gridDim.x) c[j] = 0;
+                total += c[j];
+                before += b < blockIdx.x ? c[j] : 0u;
+            }
         }
-        total += before;
+        all[threadIdx.x] = total;
+        earlier_blocks[threadIdx.x] = before;
+    }
+    __syncthreads();
+    const bool owner = threadIdx.x < digits;  // of a digit (whole waves)
+    uint32_t place = 0;                       // of its next key
+    if (owner) {
+        uint32_t before = 0, total = 0;
+        for (uint32_t p = 0; p < parts; p++) {
+            total += all[(p << a.digit_bits) + threadIdx.x];
+            before += earlier_blocks[(p << a.digit_bits) + threadIdx.x];
+        }
         place = before + wave_exclusive(total, wave_totals);
     }
     __syncthreads();
-    if (quarter == 0) place += totals_before(wave, wave_totals);
+    if (owner) place += totals_before(wave, wave_totals);
     for (uint32_t tile = 0; tile < a.tiles_per_block; tile++) {
         const uint64_t first = begin + tile * static_cast<uint64_t>(sort_tile);
         if (first >= a.n) break;
@@ -261,51 +275,48 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
             const uint64_t i = wave_first + s * 64u;
             pair[s] = pair_at<I>(a, static_cast<uint32_t>(min(i, static_cast<uint64_t>(a.n - 1))));
         }
-#pragma unroll
-        for (uint32_t k = 0; k < sort_digits / 64; k++) counts[wave][k * 64 + lane] = 0;
-        volatile uint32_t* const mine = counts[wave];
+        for (uint32_t k = lane; k < digits; k += 64) counts[wave][k] = 0;
+        volatile uint16_t* const mine = counts[wave];
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++) {
-            const uint32_t d = (pair[s].x >> a.shift) & a.digit_mask;
+            const uint32_t d = digit_of(a, pair[s].x);
             const bool valid = wave_first + s * 64u < a.n;
-            uint64_t same = __ballot(valid);
-#pragma unroll
-            for (uint32_t b = 0; b < 8; b++) {
-                const bool bit = (d >> b) & 1u;
-                const uint64_t with = __ballot(bit);
-                same &= bit ? with : ~with;
+            uint64_t same = __ballot(valid);  // lanes with the same digit: those that agree with it in every bit
+            for (uint32_t b = 0; b < a.digit_bits; b++) {
+                const int64_t bit = static_cast<int32_t>(d << (31u - b)) >> 31;  // 0 or all ones
+                same &= ~(__ballot(bit != 0) ^ static_cast<uint64_t>(bit));
             }
             const uint32_t earlier = static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1ull)));
             const uint32_t so_far = mine[d];
             rank[s] = so_far + earlier;
             __builtin_amdgcn_wave_barrier();
-            if (valid && earlier == 0) mine[d] = so_far + static_cast<uint32_t>(__popcll(same));
+            if (valid && earlier == 0) mine[d] = static_cast<uint16_t>(so_far + static_cast<uint32_t>(__popcll(same)));
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
         uint32_t in_tile = 0, local = 0;
-        if (quarter == 0) {
+        if (owner) {
 #pragma unroll
-            for (uint32_t w = 0; w < sort_waves; w++) in_tile += counts[w][digit];
+            for (uint32_t w = 0; w < sort_waves; w++) in_tile += counts[w][threadIdx.x];
             local = wave_exclusive(in_tile, wave_totals);
         }
         __syncthreads();
-        if (quarter == 0) {
+        if (owner) {
             local += totals_before(wave, wave_totals);
-            to_global[digit] = place - local;
+            to_global[threadIdx.x] = place - local;
             place += in_tile;
 #pragma unroll
             for (uint32_t w = 0; w < sort_waves; w++) {
-                const uint32_t c = counts[w][digit];
-                counts[w][digit] = local;
+                const uint32_t c = counts[w][threadIdx.x];
+                counts[w][threadIdx.x] = static_cast<uint16_t>(local);
                 local += c;
             }
         }
         __syncthreads();
 #pragma unroll
         for (uint32_t s = 0; s < sort_steps; s++)
-            if (wave_first + s * 64u < a.n) ordered[counts[wave][(pair[s].x >> a.shift) & a.digit_mask] + rank[s]] = pair[s];
+            if (wave_first + s * 64u < a.n) ordered[counts[wave][digit_of(a, pair[s].x)] + rank[s]] = pair[s];
         __syncthreads();
         const uint32_t here = static_cast<uint32_t>(min(static_cast<uint64_t>(sort_tile), a.n - first));
 #pragma unroll
@@ -313,7 +324,7 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
             const uint32_t k = s * sort_block + threadIdx.x;
             if (k < here) {
                 const uint2 p = ordered[k];
-                a.out[to_global[(p.x >> a.shift) & a.digit_mask] + k] = p;
+                a.out[to_global[digit_of(a, p.x)] + k] = p;
             }
         }
         __syncthreads();
@@ -625,7 +636,7 @@ struct GradientLayout {
         const size_t lanes = group_lanes(a), blocks = sum_blocks(a);
         const size_t piece = div_up(lanes_of_row(a), lanes) * lanes * static_cast<size_t>(lane_values(a)) * 4;
         for (int k = 0; k < 2; k++) l.pairs[k] = reinterpret_cast<uint2*>(take(size_t{a.n} * 8));
-        l.table = reinterpret_cast<uint32_t*>(take(size_t{sort_max_blocks} * sort_digits * 4));
+        l.table = reinterpret_cast<uint32_t*>(take(size_t{sort_max_blocks} * sort_most_digits * 4));
         l.heads = reinterpret_cast<float*>(take(blocks * piece));
         l.tails = reinterpret_cast<float*>(take(blocks * piece));
         l.closed = reinterpret_cast<uint32_t*>(take(blocks * 4));
@@ -710,8 +721,11 @@ bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uin
             if (a.index_bytes == 4) sort_rank_kernel<int32_t><<<blocks, sort_block, 0, s>>>(p);
             else sort_rank_kernel<int64_t><<<blocks, sort_block, 0, s>>>(p);
         } else {
-            const uint32_t bits = bit_width(a.rows), passes = bits > 8 ? div_up(bits, 8) : 1u, digit_bits = div_up(bits, passes);
-            p.digit_mask = (1u << digit_bits) - 1u;
+            // As few passes as digits of 9 bits make, but a block reads the whole table: of 8 bits past 128 blocks.
+            const uint32_t blocks = div_up(a.n, static_cast<uint64_t>(sort_tile) * p.tiles_per_block);
+            const uint32_t bits = bit_width(a.rows), most = blocks > 128 ? sort_most_bits - 1 : sort_most_bits;
+            const uint32_t passes = bits > most ? div_up(bits, most) : 1u, digit_bits = std::max(div_up(bits, passes), sort_least_bits);
+            p.digit_bits = digit_bits;
             if (a.index_bytes == 4) launch_sort_pass<int32_t>(p, s);
             else launch_sort_pass<int64_t>(p, s);
             for (uint32_t k = 1; k < passes; k++) {
