@@ -123,12 +123,14 @@ __global__ __launch_bounds__(lookup_block) void embedding_zero_kernel(T* out, ui
 // Keys are rows (or `rows` for an index that counts nowhere), values the positions of their indices. A pass orders by up
 // to 9 bits: every block knows its digits' places (behind all smaller digits, and behind the same digits of earlier blocks)
 // and writes its keys there, each at its rank among the equal digits before it. The counts come from a table that a kernel
-// of the same blocks writes, or, up to 32,768 keys, from the block's own count of the whole list, which spares that launch.
-// Up to 8,192 keys one kernel counts for each key the smaller ones.
+// of the same blocks writes, or, up to 16,384 keys, from the block's own count of the whole list, which spares that launch (12k
+// indices into 50,000 rows of 8 floats 26.3 -> 24.7 us; 20k 25.7 with the table and 27.6 without). Up to 8,192 keys one kernel counts for
+// each key the smaller ones (8,000 keys 22, 8,300 in two passes 24).
 
-constexpr uint32_t sort_block = 1024, sort_waves = sort_block / 64, sort_steps = 4, sort_tile = sort_block * sort_steps;
+constexpr uint32_t sort_block = 1024, sort_waves = sort_block / 64;
+constexpr uint32_t sort_steps_most = 4;            // keys of a thread in a tile: these, or one
 constexpr uint32_t sort_max_blocks = 256, sort_least_bits = 6, sort_most_bits = 9, sort_most_digits = 1u << sort_most_bits;
-constexpr uint32_t sort_alone = 8 * sort_tile;     // largest list that every block counts by itself
+constexpr uint32_t sort_alone = 16384;              // largest list that every block counts by itself
 constexpr uint32_t rank_most = 8192, rank_keys = 16;  // largest list ordered by ranks, and keys of a block
 
 struct SortPass {
@@ -139,6 +141,7 @@ struct SortPass {
     uint32_t n, rows, padding; // padding: a row that counts nowhere (>= rows: none)
     uint32_t shift, digit_bits;
     uint32_t tiles_per_block;
+    uint32_t steps;            // keys of a thread in a tile
 };
 
 // I: the indices' type, or uint2 for a later pass
@@ -153,8 +156,9 @@ __device__ __forceinline__ uint32_t key_at(const SortPass& a, uint32_t i) {
 
 __device__ __forceinline__ uint32_t digit_of(const SortPass& a, uint32_t key) { return (key >> a.shift) & ((1u << a.digit_bits) - 1u); }
 
-template <typename I>
+template <typename I, uint32_t sort_steps>
 __global__ __launch_bounds__(sort_block) void sort_count_kernel(SortPass a) {
+    constexpr uint32_t sort_tile = sort_block * sort_steps;
     __shared__ uint32_t counts[sort_most_digits];
     const uint32_t digits = 1u << a.digit_bits;
     if (threadIdx.x < digits) counts[threadIdx.x] = 0;
@@ -204,8 +208,9 @@ __device__ __forceinline__ uint32_t totals_before(uint32_t wave, const uint32_t*
 
 // ALONE: the block counts the digits of the whole list. A tile is put in order in LDS and written from there, so that a wave's
 // stores meet few lines (written from the keys' own lanes, a pass over 1M keys took 22 us).
-template <typename I, bool ALONE>
+template <typename I, bool ALONE, uint32_t sort_steps>
 __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
+    constexpr uint32_t sort_tile = sort_block * sort_steps;
     __shared__ uint16_t counts[sort_waves][sort_most_digits];  // keys of each digit in a wave's part of the tile, then their first place in it
     __shared__ uint32_t wave_totals[sort_waves], to_global[sort_most_digits];
     __shared__ uint2 ordered[sort_tile];
@@ -215,7 +220,7 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
     const uint32_t digits = 1u << a.digit_bits, parts = sort_block >> a.digit_bits;
     const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * a.tiles_per_block * sort_tile;
     if constexpr (ALONE) {
-        all[threadIdx.x] = earlier_blocks[threadIdx.x] = 0;
+        all[threadIdx.x] = 0;
         __syncthreads();
         constexpr uint32_t at_once = 16;
         const uint32_t part = threadIdx.x & ~(digits - 1u);
@@ -226,10 +231,7 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
 #pragma unroll
             for (uint32_t s = 0; s < at_once; s++) {
                 const uint32_t i = from + s * sort_block, at = part + digit_of(a, key[s]);
-                if (i < a.n) {
-                    atomicAdd(&all[at], 1u);
-                    if (i < begin) atomicAdd(&earlier_blocks[at], 1u);
-                }
+                if (i < a.n) atomicAdd(&all[at], i < begin ? 0x10001u : 1u);  // (both counts, 16 bits each)
             }
         }
     } else {
@@ -257,8 +259,9 @@ __global__ __launch_bounds__(sort_block) void sort_scatter_kernel(SortPass a) {
     if (owner) {
         uint32_t before = 0, total = 0;
         for (uint32_t p = 0; p < parts; p++) {
-            total += all[(p << a.digit_bits) + threadIdx.x];
-            before += earlier_blocks[(p << a.digit_bits) + threadIdx.x];
+            const uint32_t at = (p << a.digit_bits) + threadIdx.x;
+            total += ALONE ? all[at] & 0xffffu : all[at];
+            before += ALONE ? all[at] >> 16 : earlier_blocks[at];
         }
         place = before + wave_exclusive(total, wave_totals);
     }
@@ -342,15 +345,22 @@ __global__ __launch_bounds__(sort_block) void sort_rank_kernel(SortPass a) {
     const uint32_t per = (a.n + parts * 4 - 1) / (parts * 4) * 4;  // of a part, in fours
     for (uint32_t i = threadIdx.x; i < per * parts; i += sort_block) keys[i] = i < a.n ? key_at<I>(a, i) : 0xffffffffu;
     __syncthreads();
-    const uint32_t i = blockIdx.x * rank_keys + k, mine = keys[min(i, a.n - 1)];
+    const uint32_t first = blockIdx.x * rank_keys, i = first + k, mine = keys[min(i, a.n - 1)];
+    const uint32_t begin = part * per;
     uint32_t smaller = 0;
-    const uint4* const list = reinterpret_cast<const uint4*>(keys + part * per);
-    for (uint32_t j = 0; j < per / 4; j++) {
-        const uint4 other = list[j];
-        const uint32_t at = part * per + j * 4;
-        // (equal keys count where they stand before: as if they were smaller)
-        smaller += (other.x < mine + (at < i ? 1u : 0u)) + (other.y < mine + (at + 1 < i ? 1u : 0u)) + (other.z < mine + (at + 2 < i ? 1u : 0u)) +
-                   (other.w < mine + (at + 3 < i ? 1u : 0u));
+    const uint4* const list = reinterpret_cast<const uint4*>(keys + begin);
+    if (begin + per <= first || begin >= first + rank_keys) {
+        // (equal keys count in the part of the list before the block's keys: as if they were smaller)
+        const uint32_t limit = mine + (begin < first ? 1u : 0u);
+        for (uint32_t j = 0; j < per / 4; j++) {
+            const uint4 other = list[j];
+            smaller += (other.x < limit) + (other.y < limit) + (other.z < limit) + (other.w < limit);
+        }
+    } else {
+        for (uint32_t j = 0; j < per; j++) {
+            const uint32_t other = keys[begin + j];
+            smaller += other < mine + (begin + j < i ? 1u : 0u);
+        }
     }
     places[part][k] = smaller;
     __syncthreads();
@@ -363,7 +373,11 @@ __global__ __launch_bounds__(sort_block) void sort_rank_kernel(SortPass a) {
 
 // ---- sums ----------------------------------------------------------------------------------------------------------------
 
-constexpr uint32_t sum_block = 256, sum_items = 8;  // items of a group of lanes
+constexpr uint32_t sum_block = 256;
+// Items of a group of G lanes: 16 for a wave's (16k indices into 50k rows of 1,024 bfloat16 63 -> 59 us, 60k into 500 rows of 1,000 51 -> 48
+// against 8), 8 for fewer lanes, whose block has more of them (8k indices into 30k rows of 256 24.0 us, 24.8 with 16; 1M into 4,096 of 8 floats
+// 56.5 and 57.1).
+constexpr uint32_t sum_items_of(uint32_t lanes) { return lanes == 64 ? 16 : 8; }
 
 struct SumArgs {
     const uint2* pairs;        // row and position, sorted
@@ -397,7 +411,7 @@ __device__ __forceinline__ uint32_t entries_before(const SumArgs& a, uint32_t po
 // G lanes to a row (of a tile of columns).
 template <typename T, int W, int G>
 __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
-    constexpr uint32_t groups = sum_block / G, items = groups * sum_items;
+    constexpr uint32_t sum_items = sum_items_of(G), groups = sum_block / G, items = groups * sum_items;
     __shared__ uint32_t s_keys[items], s_values[items], s_start[groups + 1], s_bounds[2];
     __shared__ float s_tail[sum_block / 64][G * W];
     __shared__ uint32_t s_closed[sum_block / 64];
@@ -603,16 +617,33 @@ uint32_t group_lanes(const EmbeddingArgs& a) {
     return g;
 }
 
-uint32_t sum_blocks(const EmbeddingArgs& a) { return div_up(static_cast<uint64_t>(a.n) + a.rows, sum_block / group_lanes(a) * sum_items); }
+uint32_t sum_blocks(const EmbeddingArgs& a) { return div_up(static_cast<uint64_t>(a.n) + a.rows, sum_block / group_lanes(a) * sum_items_of(group_lanes(a))); }
+
+uint32_t sort_blocks(const SortPass& p) { return div_up(p.n, static_cast<uint64_t>(sort_block) * p.steps * p.tiles_per_block); }
+
+// Digits, tiles and steps of a list's passes. A block reads the whole table, blocks x digits, so both are held against it: as few
+// passes as digits of 9 bits make, 8 bits past 128 blocks of four keys a thread; and one key a thread, in four times the blocks, where the
+// table has at most 32,768 entries then (us with four and one: 33k indices into 5,000 rows 31 and 26, 130k 33 and 28, 200k 35 and 32.5; past
+// that 100k into 100,000 rows 36 and 38, 200k into 257 25 and 28).
+void plan_sort(SortPass& p) {
+    p.steps = sort_steps_most;
+    p.tiles_per_block = div_up(div_up(p.n, sort_block * p.steps), sort_max_blocks);
+    const uint32_t bits = bit_width(p.rows), most = sort_blocks(p) > 128 ? sort_most_bits - 1 : sort_most_bits;
+    p.digit_bits = std::max(div_up(bits, div_up(bits, most)), sort_least_bits);
+    if (div_up(p.n, sort_block) << p.digit_bits <= 32768) p.steps = p.tiles_per_block = 1;
+}
 
 template <typename I>
 void launch_sort_pass(const SortPass& p, hipStream_t s) {
-    const uint32_t blocks = div_up(p.n, static_cast<uint64_t>(sort_tile) * p.tiles_per_block);
-    if (p.n <= sort_alone) {
-        sort_scatter_kernel<I, true><<<blocks, sort_block, 0, s>>>(p);
+    const uint32_t blocks = sort_blocks(p);
+    if (p.n <= sort_alone && p.steps == 1) {
+        sort_scatter_kernel<I, true, 1><<<blocks, sort_block, 0, s>>>(p);
+    } else if (p.steps == 1) {
+        sort_count_kernel<I, 1><<<blocks, sort_block, 0, s>>>(p);
+        sort_scatter_kernel<I, false, 1><<<blocks, sort_block, 0, s>>>(p);
     } else {
-        sort_count_kernel<I><<<blocks, sort_block, 0, s>>>(p);
-        sort_scatter_kernel<I, false><<<blocks, sort_block, 0, s>>>(p);
+        sort_count_kernel<I, 4><<<blocks, sort_block, 0, s>>>(p);
+        sort_scatter_kernel<I, false, 4><<<blocks, sort_block, 0, s>>>(p);
     }
 }
 
@@ -715,21 +746,17 @@ bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uin
         p.rows = a.rows;
         p.padding = padding;
         p.shift = 0;
-        p.tiles_per_block = div_up(div_up(a.n, sort_tile), sort_max_blocks);
         if (a.n <= rank_most) {
             const uint32_t blocks = div_up(a.n, rank_keys);
             if (a.index_bytes == 4) sort_rank_kernel<int32_t><<<blocks, sort_block, 0, s>>>(p);
             else sort_rank_kernel<int64_t><<<blocks, sort_block, 0, s>>>(p);
         } else {
-            // As few passes as digits of 9 bits make, but a block reads the whole table: of 8 bits past 128 blocks.
-            const uint32_t blocks = div_up(a.n, static_cast<uint64_t>(sort_tile) * p.tiles_per_block);
-            const uint32_t bits = bit_width(a.rows), most = blocks > 128 ? sort_most_bits - 1 : sort_most_bits;
-            const uint32_t passes = bits > most ? div_up(bits, most) : 1u, digit_bits = std::max(div_up(bits, passes), sort_least_bits);
-            p.digit_bits = digit_bits;
+            plan_sort(p);
+            const uint32_t passes = div_up(bit_width(a.rows), p.digit_bits);
             if (a.index_bytes == 4) launch_sort_pass<int32_t>(p, s);
             else launch_sort_pass<int64_t>(p, s);
             for (uint32_t k = 1; k < passes; k++) {
-                p.shift = k * digit_bits;
+                p.shift = k * p.digit_bits;
                 p.in = l.pairs[current];
                 current ^= 1u;
                 p.out = l.pairs[current];
