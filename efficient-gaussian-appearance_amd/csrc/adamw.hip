@@ -41,29 +41,31 @@ template <> struct Vector4<float> { using type = float4u; };
 template <> struct Vector4<_Float16> { using type = half4u; };
 template <> struct Vector4<__bf16> { using type = bfloat4u; };
 
-// x[0..3] = p[0..3] in 32 bits; past `count` zeros. WHOLE: the block lies within its tensor (known for all its threads, so that its
-// loads stand in no branch).
+// x[0..3] = p[0..3] in 32 bits, and zeros past `count`. WHOLE: the block lies within its tensor, and every count is 4. At a tensor's
+// end each value is loaded by itself, from the last one's place past it: whatever its count, no lane waits for a load before all are
+// sent, as it would with one in a branch. (p + 0 has to be in the tensor: callers clamp it.)
 //
 // The step streams its tensors once each way, with nontemporal loads and stores: 59M float32 elements 325 -> 309 us, 30M bfloat16
 // ones 120 -> 106, 22M with 8-bit states 64 -> 56 (loads or stores alone gain nothing).
-template <bool WHOLE, bool STREAM = true, typename T>
+template <bool WHOLE, typename T>
 __device__ __forceinline__ void load4(const T* p, uint32_t count, float* x) {
-    using V = typename Vector4<T>::type;
-    if (WHOLE || count >= 4) {
-        const V* const at = reinterpret_cast<const V*>(p);
-        const V v = STREAM ? __builtin_nontemporal_load(at) : *at;
+    if constexpr (WHOLE) {
+        const typename Vector4<T>::type v = __builtin_nontemporal_load(reinterpret_cast<const typename Vector4<T>::type*>(p));
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = static_cast<float>(v[k]);
     } else {
+        const uint32_t last = count > 0 ? count - 1 : 0u;
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++) x[k] = k < count ? static_cast<float>(p[k]) : 0.0f;
+        for (uint32_t k = 0; k < 4; k++) x[k] = static_cast<float>(p[min(k, last)]);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) x[k] = k < count ? x[k] : 0.0f;
     }
 }
 
 // rounded to nearest even, what a cast of a tensor does
 template <bool WHOLE, typename T>
 __device__ __forceinline__ void store4(T* p, uint32_t count, const float* x) {
-    if (WHOLE || count >= 4) {
+    if constexpr (WHOLE) {
         typename Vector4<T>::type v;
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = static_cast<T>(x[k]);
@@ -77,23 +79,36 @@ __device__ __forceinline__ void store4(T* p, uint32_t count, const float* x) {
 
 template <bool WHOLE>
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, uint32_t count) {
-    if (WHOLE || count >= 4) return *reinterpret_cast<const uint32u*>(p);
-    uint32_t v = 0;
+    if constexpr (WHOLE) return *reinterpret_cast<const uint32u*>(p);
+    const uint32_t last = count > 0 ? count - 1 : 0u;
+    uint32_t code[4], v = 0;
 #pragma unroll
-    for (uint32_t k = 0; k < 4; k++)
-        if (k < count) v |= static_cast<uint32_t>(p[k]) << (8 * k);
+    for (uint32_t k = 0; k < 4; k++) code[k] = p[min(k, last)];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) v |= k < count ? code[k] << (8 * k) : 0u;
     return v;
 }
 
 template <bool WHOLE>
 __device__ __forceinline__ void store_codes(uint8_t* p, uint32_t count, uint32_t v) {
-    if (WHOLE || count >= 4) {
+    if constexpr (WHOLE) {
         *reinterpret_cast<uint32u*>(p) = v;
         return;
     }
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++)
         if (k < count) p[k] = static_cast<uint8_t>(v >> (8 * k));
+}
+
+// a thread's first element and how many of four from there lie in the tensor; past its end 0 of its last element
+struct Four {
+    uint64_t at;
+    uint32_t count;
+};
+template <bool WHOLE>
+__device__ __forceinline__ Four four_from(uint64_t i, uint64_t n) {
+    if constexpr (WHOLE) return {i, 4u};
+    return {i < n ? i : n - 1, i >= n ? 0u : n - i >= 4 ? 4u : static_cast<uint32_t>(n - i)};
 }
 
 // maximum over the wave's lanes
@@ -108,17 +123,27 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return max(static_cast<uint32_t>(b[0]), static_cast<uint32_t>(b[1]));
 }
 
-// the last of the n tensors whose first block is at most `block`
+// A tensor's first block, and in the top bits the launch's group that it belongs to: the descriptors of both are then loaded
+// at once, where the group's number in the tensor's made a load wait for another (arguments are slow to read the first time).
+__host__ __device__ inline uint32_t pack_first_block(uint32_t block, uint32_t group) { return group << 28 | block; }
+__host__ __device__ inline uint32_t first_block_of(uint32_t packed) { return packed & 0x0fffffffu; }
+__host__ __device__ inline uint32_t first_block_group(uint32_t packed) { return packed >> 28; }
+
+// the last of the n tensors whose first block is at most `block`: its index and packed first block
 template <uint32_t MAX>
-__device__ __forceinline__ uint32_t tensor_of_block(const uint32_t* first_block, uint32_t n, uint32_t block) {
+__device__ __forceinline__ uint2 tensor_of_block(const uint32_t* first_blocks, uint32_t n, uint32_t block) {
     const uint32_t lane = threadIdx.x & 63u;
-    uint32_t count = 0;
+    uint32_t packed[(MAX + 63) / 64];
+#pragma unroll
+    for (uint32_t k = 0; k < MAX; k += 64) packed[k / 64] = first_blocks[min(k + lane, n - 1)];
+    uint32_t count = 0, found = 0;
 #pragma unroll
     for (uint32_t k = 0; k < MAX; k += 64) {
-        if (k > 0 && k >= n) break;
-        count += static_cast<uint32_t>(__popcll(__ballot(k + lane < n && first_block[min(k + lane, MAX - 1)] <= block)));
+        const uint64_t at_most = __ballot(k + lane < n && first_block_of(packed[k / 64]) <= block);
+        if (at_most) found = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(packed[k / 64]), 63 - __clzll(at_most)));
+        count += static_cast<uint32_t>(__popcll(at_most));
     }
-    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(count))) - 1u;
+    return make_uint2(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(count))) - 1u, found);
 }
 
 template <int BITS>
@@ -134,13 +159,9 @@ struct AdamWLaunch {
 };
 static_assert(sizeof(AdamWLaunch<32>) <= 4096 && sizeof(AdamWLaunch<8>) <= 4096, "kernel arguments");
 
-// the clipping coefficient; false where the norm is not finite (the step is left out)
-__device__ __forceinline__ bool clipping(const float* grad_norm, float max_grad_norm, float& coefficient) {
-    coefficient = 1.0f;
-    if (!grad_norm) return true;
-    const float norm = *grad_norm;
-    coefficient = fminf(max_grad_norm / (norm + 1e-6f), 1.0f);
-    return norm < INFINITY;
+// The clipping coefficient; not a number where the norm is not finite (the step then stores nothing).
+__device__ __forceinline__ float clipping(float norm, float max_grad_norm) {
+    return norm < INFINITY ? fminf(max_grad_norm / (norm + 1e-6f), 1.0f) : NAN;
 }
 
 // The parameter after the step. The reciprocal is the hardware's (1 ulp): the division's last bit would be
@@ -154,6 +175,13 @@ __device__ __forceinline__ float updated(const AdamWGroupDevice& G, float p, flo
 // Learning rates of four consecutive elements: the group's one, or from the table of its cycle (in LDS, rate and decay).
 struct Rates {
     float2 of[4];
+};
+
+// What the gradients are multiplied with. The norm was loaded before the tensors, and is waited for with them.
+struct Clip {
+    bool on;
+    float norm, max_grad_norm;
+    __device__ __forceinline__ float coefficient() const { return on ? clipping(norm, max_grad_norm) : 1.0f; }
 };
 template <bool CYCLE>
 __device__ __forceinline__ Rates rates_of(const AdamWGroupDevice& G, const float2* cycle, uint32_t first_column) {
@@ -174,19 +202,19 @@ __device__ __forceinline__ Rates rates_of(const AdamWGroupDevice& G, const float
 // PIECES pieces of four elements a thread, 1,024 apart, all loaded before the first is worked on.
 template <bool WHOLE, bool CYCLE, int PIECES, typename P, typename D>
 __device__ __forceinline__ void step_pieces(const AdamWTensor& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
-                                            float coefficient) {
+                                            Clip clip) {
     float p[PIECES][4], g[PIECES][4], m[PIECES][4], v[PIECES][4];
-    uint64_t at[PIECES];
-    uint32_t count[PIECES];
+    Four four[PIECES];
 #pragma unroll
     for (int q = 0; q < PIECES; q++) {
-        at[q] = base + q * adamw_piece + threadIdx.x * 4u;
-        count[q] = WHOLE ? 4u : at[q] >= n ? 0u : n - at[q] >= 4 ? 4u : static_cast<uint32_t>(n - at[q]);
-        load4<WHOLE>(static_cast<const D*>(T.grad) + at[q], count[q], g[q]);
-        load4<WHOLE>(static_cast<const float*>(T.m) + at[q], count[q], m[q]);
-        load4<WHOLE>(static_cast<const float*>(T.v) + at[q], count[q], v[q]);
-        load4<WHOLE>(static_cast<const P*>(T.param) + at[q], count[q], p[q]);
+        four[q] = four_from<WHOLE>(base + q * adamw_piece + threadIdx.x * 4u, n);
+        load4<WHOLE>(static_cast<const D*>(T.grad) + four[q].at, four[q].count, g[q]);
+        load4<WHOLE>(static_cast<const float*>(T.m) + four[q].at, four[q].count, m[q]);
+        load4<WHOLE>(static_cast<const float*>(T.v) + four[q].at, four[q].count, v[q]);
+        load4<WHOLE>(static_cast<const P*>(T.param) + four[q].at, four[q].count, p[q]);
     }
+    const float coefficient = clip.coefficient();
+    if (coefficient != coefficient) return;
 #pragma unroll
     for (int q = 0; q < PIECES; q++) {
         const Rates rates = rates_of<CYCLE>(G, cycle, column);
@@ -198,16 +226,16 @@ __device__ __forceinline__ void step_pieces(const AdamWTensor& T, const AdamWGro
             v[q][k] = G.beta2 * v[q][k] + G.beta2_rest * (gk * gk);
             p[q][k] = updated(G, p[q][k], m[q][k], sqrtf(v[q][k]), rates.of[k].x, rates.of[k].y);
         }
-        store4<WHOLE>(static_cast<float*>(T.m) + at[q], count[q], m[q]);
-        store4<WHOLE>(static_cast<float*>(T.v) + at[q], count[q], v[q]);
-        store4<WHOLE>(static_cast<P*>(T.param) + at[q], count[q], p[q]);
+        store4<WHOLE>(static_cast<float*>(T.m) + four[q].at, four[q].count, m[q]);
+        store4<WHOLE>(static_cast<float*>(T.v) + four[q].at, four[q].count, v[q]);
+        store4<WHOLE>(static_cast<P*>(T.param) + four[q].at, four[q].count, p[q]);
     }
 }
 
 template <bool WHOLE, bool CYCLE, int PIECES, typename P, typename D>
 __device__ __forceinline__ void step_block(const AdamWTensor& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
-                                           float coefficient) {
-    step_pieces<WHOLE, CYCLE, PIECES, P, D>(T, G, cycle, base, n, column, coefficient);
+                                           Clip clip) {
+    step_pieces<WHOLE, CYCLE, PIECES, P, D>(T, G, cycle, base, n, column, clip);
 }
 
 // ---- 8-bit codes -----------------------------------------------------------------------------------------------------
@@ -248,11 +276,13 @@ __device__ __forceinline__ float rounded_quotient(float a, float b, float recipr
 // library where the wave holds another one; both round to nearest.
 template <bool WHOLE, bool CYCLE, int PIECES, typename P, typename D>
 __device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
-                                           float coefficient) {
+                                           Clip clip) {
     const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t i = base + threadIdx.x * 4u, first = i - lane * 4u;
+    const uint64_t first = base + (threadIdx.x - lane) * 4u;  // of the wave's block
     if (!WHOLE && first >= n) return;
-    const uint32_t count = !WHOLE && i >= n ? 0u : WHOLE || n - i >= 4 ? 4u : static_cast<uint32_t>(n - i);
+    const Four four = four_from<WHOLE>(first + lane * 4u, n);
+    const uint64_t i = four.at;
+    const uint32_t count = four.count;
     uint8_t* const ratios = static_cast<uint8_t*>(T.m) + i;
     uint8_t* const roots = static_cast<uint8_t*>(T.v) + i;
     float p[4], g[4], m[4], v[4], r[4], u[4];
@@ -261,6 +291,8 @@ __device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGro
     load4<WHOLE>(static_cast<const P*>(T.param) + i, count, p);
     const float scale = T.scale[first / 256];
     const Rates rates = rates_of<CYCLE>(G, cycle, column);
+    const float coefficient = clip.coefficient();
+    if (coefficient != coefficient) return;
     bool plain = true;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -295,7 +327,7 @@ __device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGro
     uint32_t new_ratios = 0, new_roots = 0;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const uint32_t h = dither_of(static_cast<uint32_t>(i) + k, G.key);
+        const uint32_t h = dither_of(static_cast<uint32_t>(i) + k, G.key);  // (past the end nothing is stored)
         new_roots |= encode(r[k] * inverse, root_c, h & 0xffffu, root_base, 255u) << (8 * k);
         const float y = fminf(fabsf(u[k]) * G.ratio_encode, ratio_top);
         new_ratios |= (encode(y, ratio_c, h >> 16, ratio_base, 127u) | ((__float_as_uint(u[k]) >> 24) & 128u)) << (8 * k);
@@ -308,43 +340,42 @@ __device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGro
 
 template <bool WHOLE, bool CYCLE, int PIECES, typename P, typename T>
 __device__ __forceinline__ void step_gradient(const T& tensor, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
-                                              float coefficient) {
+                                              Clip clip) {
     const uint32_t type = tensor.grad_type();
-    if (type == type_float) step_block<WHOLE, CYCLE, PIECES, P, float>(tensor, G, cycle, base, n, column, coefficient);
-    else if (type == type_bfloat16) step_block<WHOLE, CYCLE, PIECES, P, __bf16>(tensor, G, cycle, base, n, column, coefficient);
-    else step_block<WHOLE, CYCLE, PIECES, P, _Float16>(tensor, G, cycle, base, n, column, coefficient);
+    if (type == type_float) step_block<WHOLE, CYCLE, PIECES, P, float>(tensor, G, cycle, base, n, column, clip);
+    else if (type == type_bfloat16) step_block<WHOLE, CYCLE, PIECES, P, __bf16>(tensor, G, cycle, base, n, column, clip);
+    else step_block<WHOLE, CYCLE, PIECES, P, _Float16>(tensor, G, cycle, base, n, column, clip);
 }
 
 template <bool WHOLE, bool CYCLE, int PIECES, typename T>
 __device__ __forceinline__ void step_tensor(const T& tensor, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
-                                            float coefficient) {
+                                            Clip clip) {
     const uint32_t type = tensor.param_type();
-    if (type == type_float) step_gradient<WHOLE, CYCLE, PIECES, float>(tensor, G, cycle, base, n, column, coefficient);
-    else if (type == type_bfloat16) step_gradient<WHOLE, CYCLE, PIECES, __bf16>(tensor, G, cycle, base, n, column, coefficient);
-    else step_gradient<WHOLE, CYCLE, PIECES, _Float16>(tensor, G, cycle, base, n, column, coefficient);
+    if (type == type_float) step_gradient<WHOLE, CYCLE, PIECES, float>(tensor, G, cycle, base, n, column, clip);
+    else if (type == type_bfloat16) step_gradient<WHOLE, CYCLE, PIECES, __bf16>(tensor, G, cycle, base, n, column, clip);
+    else step_gradient<WHOLE, CYCLE, PIECES, _Float16>(tensor, G, cycle, base, n, column, clip);
 }
 
 template <int BITS, int PIECES>
 __global__ __launch_bounds__(adamw_block) void adamw_kernel(AdamWLaunch<BITS> L) {
     __shared__ float2 cycle[adam_max_lrs];
-    float coefficient;
-    if (!clipping(L.grad_norm, L.max_grad_norm, coefficient)) return;
-    const uint32_t k = tensor_of_block<AdamWLaunch<BITS>::max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
+    const Clip clip = {L.grad_norm != nullptr, L.grad_norm ? *L.grad_norm : 0.0f, L.max_grad_norm};
+    const uint2 found = tensor_of_block<AdamWLaunch<BITS>::max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
     // (copies: with references the whole argument was copied to scratch memory)
-    const auto T = L.tensors[k];
-    const AdamWGroupDevice G = L.groups[T.group()];
-    const uint64_t base = static_cast<uint64_t>(blockIdx.x - L.first_block[k]) * adamw_piece * PIECES, n = T.n();
+    const auto T = L.tensors[found.x];
+    const AdamWGroupDevice G = L.groups[first_block_group(found.y)];
+    const uint64_t base = static_cast<uint64_t>(blockIdx.x - first_block_of(found.y)) * adamw_piece * PIECES, n = T.n();
     const bool whole = base + adamw_piece * PIECES <= n;
     if (G.n_lrs == 1) {
-        if (whole) step_tensor<true, false, PIECES>(T, G, cycle, base, n, 0u, coefficient);
-        else step_tensor<false, false, PIECES>(T, G, cycle, base, n, 0u, coefficient);
+        if (whole) step_tensor<true, false, PIECES>(T, G, cycle, base, n, 0u, clip);
+        else step_tensor<false, false, PIECES>(T, G, cycle, base, n, 0u, clip);
         return;
     }
-    if (threadIdx.x < G.n_lrs) cycle[threadIdx.x] = make_float2(L.groups[T.group()].rates[threadIdx.x], L.groups[T.group()].decays[threadIdx.x]);
+    if (threadIdx.x < G.n_lrs) cycle[threadIdx.x] = make_float2(L.groups[first_block_group(found.y)].rates[threadIdx.x], L.groups[first_block_group(found.y)].decays[threadIdx.x]);
     __syncthreads();
     const uint32_t column = (static_cast<uint32_t>(base % G.n_lrs) + threadIdx.x * 4u) % G.n_lrs;
-    if (whole) step_tensor<true, true, PIECES>(T, G, cycle, base, n, column, coefficient);
-    else step_tensor<false, true, PIECES>(T, G, cycle, base, n, column, coefficient);
+    if (whole) step_tensor<true, true, PIECES>(T, G, cycle, base, n, column, clip);
+    else step_tensor<false, true, PIECES>(T, G, cycle, base, n, column, clip);
 }
 
 // ---- decoding ----------------------------------------------------------------------------------------------------------
@@ -356,14 +387,11 @@ struct MomentsLaunch {
 };
 static_assert(sizeof(MomentsLaunch) <= 4096, "kernel arguments");
 
-__global__ __launch_bounds__(adamw_block) void adamw_moments_kernel(MomentsLaunch L) {
-    const uint32_t k = tensor_of_block<moments_max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
-    const AdamWMomentsDevice& T = L.tensors[k];
-    const uint64_t i = static_cast<uint64_t>(blockIdx.x - L.first_block[k]) * adamw_block * 4 + threadIdx.x * 4u;
-    if (i >= T.n) return;
-    const uint32_t count = T.n - i >= 4 ? 4u : static_cast<uint32_t>(T.n - i);
-    const uint32_t ratio_codes = load_codes<false>(T.ratios + i, count), root_codes = load_codes<false>(T.roots + i, count);
-    const float scale = T.scale[i / 256];
+template <bool WHOLE>
+__device__ __forceinline__ void decode_block(const AdamWMomentsDevice& T, uint64_t base) {
+    const Four four = four_from<WHOLE>(base + threadIdx.x * 4u, T.n);
+    const uint32_t ratio_codes = load_codes<WHOLE>(T.ratios + four.at, four.count), root_codes = load_codes<WHOLE>(T.roots + four.at, four.count);
+    const float scale = T.scale[four.at / 256];
     float m[4], v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -371,8 +399,16 @@ __global__ __launch_bounds__(adamw_block) void adamw_moments_kernel(MomentsLaunc
         m[j] = decode_ratio((ratio_codes >> (8 * j)) & 255u, T.ratio_decode) * r;
         v[j] = r * r;
     }
-    store4<false>(T.m + i, count, m);
-    store4<false>(T.v + i, count, v);
+    store4<WHOLE>(T.m + four.at, four.count, m);
+    store4<WHOLE>(T.v + four.at, four.count, v);
+}
+
+__global__ __launch_bounds__(adamw_block) void adamw_moments_kernel(MomentsLaunch L) {
+    const uint2 found = tensor_of_block<moments_max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
+    const AdamWMomentsDevice T = L.tensors[found.x];
+    const uint64_t base = static_cast<uint64_t>(blockIdx.x - found.y) * adamw_piece;
+    if (base + adamw_piece <= T.n) decode_block<true>(T, base);
+    else decode_block<false>(T, base);
 }
 
 // ---- gradient norm -----------------------------------------------------------------------------------------------------
@@ -406,19 +442,26 @@ __device__ __forceinline__ double block_sum(double x) {
     return sum;
 }
 
-// eight loads `stride` elements apart
+// Eight loads `stride` elements apart. WHOLE: all of them lie in the tensor; else one that does not takes the tensor's last four
+// elements (there are four) and counts those from its own place on.
 template <bool WHOLE, typename T>
 __device__ __forceinline__ void add_squares(const T* data, uint64_t n, uint64_t base, uint64_t stride, double* sum) {
-    float x[norm_loads][4];
+    typename Vector4<T>::type x[norm_loads];
 #pragma unroll
     for (uint32_t j = 0; j < norm_loads; j++) {
         const uint64_t i = base + j * stride + threadIdx.x * 4u;
-        load4<WHOLE, false>(data + i, WHOLE ? 4u : i >= n ? 0u : n - i >= 4 ? 4u : static_cast<uint32_t>(n - i), x[j]);
+        x[j] = *reinterpret_cast<const typename Vector4<T>::type*>(data + (WHOLE ? i : min(i, n - 4)));
     }
 #pragma unroll
-    for (uint32_t j = 0; j < norm_loads; j++)
+    for (uint32_t j = 0; j < norm_loads; j++) {
+        const uint64_t i = base + j * stride + threadIdx.x * 4u;
+        const uint32_t skipped = WHOLE || i + 4 <= n ? 0u : i >= n ? 4u : static_cast<uint32_t>(i + 4 - n);
 #pragma unroll
-        for (int k = 0; k < 4; k++) sum[k] = __builtin_fma(static_cast<double>(x[j][k]), static_cast<double>(x[j][k]), sum[k]);
+        for (uint32_t k = 0; k < 4; k++) {
+            const double value = k >= skipped ? static_cast<double>(static_cast<float>(x[j][k])) : 0.0;
+            sum[k] = __builtin_fma(value, value, sum[k]);
+        }
+    }
 }
 
 // A tensor's blocks take its 1,024-element pieces in turn, so that at any time they read one stretch of memory: with a stretch
@@ -426,6 +469,10 @@ __device__ __forceinline__ void add_squares(const T* data, uint64_t n, uint64_t 
 template <typename T>
 __device__ __forceinline__ double squares(const T* data, uint64_t n, uint32_t block, uint32_t blocks) {
     double sum[4] = {};
+    if (n < 4) {
+        const double value = threadIdx.x < n ? static_cast<double>(static_cast<float>(data[threadIdx.x])) : 0.0;
+        return value * value;
+    }
     const uint64_t stride = static_cast<uint64_t>(blocks) * adamw_block * 4;
     for (uint64_t base = static_cast<uint64_t>(block) * adamw_block * 4; base < n; base += norm_loads * stride) {
         if (base + (norm_loads - 1) * stride + adamw_block * 4 <= n) add_squares<true>(data, n, base, stride, sum);
@@ -435,10 +482,10 @@ __device__ __forceinline__ double squares(const T* data, uint64_t n, uint32_t bl
 }
 
 __global__ __launch_bounds__(adamw_block) void norm_partials_kernel(NormLaunch L) {
-    const uint32_t k = tensor_of_block<norm_max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
-    const NormTensorDevice T = L.tensors[k];
+    const uint2 found = tensor_of_block<norm_max_tensors>(L.first_block, L.n_tensors, blockIdx.x);
+    const NormTensorDevice T = L.tensors[found.x];
     const uint64_t n = T.n_and_type >> 2;
-    const uint32_t type = static_cast<uint32_t>(T.n_and_type & 3u), block = blockIdx.x - L.first_block[k], blocks = norm_blocks(n, L.steps);
+    const uint32_t type = static_cast<uint32_t>(T.n_and_type & 3u), block = blockIdx.x - found.y, blocks = norm_blocks(n, L.steps);
     double sum;
     if (type == type_float) sum = squares(static_cast<const float*>(T.data), n, block, blocks);
     else if (type == type_bfloat16) sum = squares(static_cast<const __bf16*>(T.data), n, block, blocks);
@@ -478,8 +525,7 @@ bool launch_steps(const T* tensors, const uint32_t* of_tensor, uint64_t n_tensor
                 L.groups[g] = groups[of_tensor[at]];
             }
             L.tensors[L.n_tensors] = tensors[at];
-            L.tensors[L.n_tensors].set_group(g);
-            L.first_block[L.n_tensors++] = blocks;
+            L.first_block[L.n_tensors++] = pack_first_block(blocks, g);
             blocks += more;
         }
         adamw_kernel<BITS, PIECES><<<blocks, adamw_block, 0, s>>>(L);

@@ -220,13 +220,11 @@ struct AdamWTensor {        // no empty tensors
     const void* grad;
     void* m;                // float; 8-bit: codes of u = m / r
     void* v;                // float; 8-bit: codes of r = sqrt(v)
-    uint64_t packed;        // elements << 16 | group << 8 | gradient's type << 4 | parameter's type
+    uint64_t packed;        // elements << 16 | gradient's type << 4 | parameter's type
     __host__ __device__ uint64_t n() const { return packed >> 16; }
-    __host__ __device__ uint32_t group() const { return static_cast<uint32_t>(packed >> 8) & 255u; }
     __host__ __device__ uint32_t grad_type() const { return static_cast<uint32_t>(packed >> 4) & 15u; }
     __host__ __device__ uint32_t param_type() const { return static_cast<uint32_t>(packed) & 15u; }
     void set(uint64_t n, uint32_t param_type, uint32_t grad_type) { packed = n << 16 | grad_type << 4 | param_type; }
-    void set_group(uint32_t g) { packed = (packed & ~0xff00ull) | g << 8; }
 };
 struct AdamWTensor8 : AdamWTensor {
     float* scale;           // per 256 elements
