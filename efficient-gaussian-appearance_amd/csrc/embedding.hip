@@ -44,7 +44,12 @@ __device__ __forceinline__ T scaled(float x, float scale) {
     return static_cast<T>(y);
 }
 
-template <typename T, int W>
+// STREAM: past the caches, for outputs of 96 MB and more. What reads an output next is slower then, more so than the store was
+// faster for smaller ones (lookup and a product of it, us, in the caches and past them: 64 MB 45.9 and 47.8, 128 MB 94.5 and 92.3, 576 MB 365 and 353;
+// table gradient of 102 MB and a product of it 84.4 and 81.1).
+constexpr uint64_t stream_from = 96ull << 20;
+
+template <typename T, int W, bool STREAM>
 __device__ __forceinline__ void store_part(T* p, const float* x, float scale) {
     if constexpr (W == 1) {
         *p = scaled<T>(x[0], scale);
@@ -52,7 +57,8 @@ __device__ __forceinline__ void store_part(T* p, const float* x, float scale) {
         typename Part<T, W>::type v;
 #pragma unroll
         for (int k = 0; k < W; k++) v[k] = scaled<T>(x[k], scale);
-        *reinterpret_cast<typename Part<T, W>::type*>(p) = v;
+        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<typename Part<T, W>::type*>(p));
+        else *reinterpret_cast<typename Part<T, W>::type*>(p) = v;
     }
 }
 
@@ -82,7 +88,7 @@ struct LookupArgs {
 
 // A block takes whole rows (or, past 1,024 lanes, 1,024 lanes of one row), consecutive lanes of it a row's consecutive parts, four
 // of them to a thread: four indices, then four parts, then the stores.
-template <typename T, int W, typename I>
+template <typename T, int W, bool STREAM, typename I>
 __global__ __launch_bounds__(lookup_block) void embedding_lookup_kernel(LookupArgs a) {
     const uint32_t first_lane = blockIdx.y * lookup_tile, items = a.rows_per_block * a.lanes;
     const uint64_t first_row = a.first + static_cast<uint64_t>(blockIdx.x) * a.rows_per_block;
@@ -108,7 +114,7 @@ __global__ __launch_bounds__(lookup_block) void embedding_lookup_kernel(LookupAr
         float x[W];
 #pragma unroll
         for (int j = 0; j < W; j++) x[j] = row[k] < a.rows ? value_of<T, W>(v[k], j) : 0.0f;
-        if (valid[k]) store_part<T, W>(static_cast<T*>(a.out) + i[k] * a.columns + column[k], x, a.scale);
+        if (valid[k]) store_part<T, W, STREAM>(static_cast<T*>(a.out) + i[k] * a.columns + column[k], x, a.scale);
     }
 }
 
@@ -409,7 +415,7 @@ __device__ __forceinline__ uint32_t entries_before(const SumArgs& a, uint32_t po
 }
 
 // G lanes to a row (of a tile of columns).
-template <typename T, int W, int G>
+template <typename T, int W, bool STREAM, int G>
 __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
     constexpr uint32_t sum_items = sum_items_of(G), groups = sum_block / G, items = groups * sum_items;
     __shared__ uint32_t s_keys[items], s_values[items], s_start[groups + 1], s_bounds[2];
@@ -467,7 +473,7 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
             for (int j = 0; j < W; j++) head[j] = sum[j];
             any_closed = true;
         } else if (valid) {
-            store_part<T, W>(gradient + static_cast<uint64_t>(row) * a.columns + column, sum, a.scale);
+            store_part<T, W, STREAM>(gradient + static_cast<uint64_t>(row) * a.columns + column, sum, a.scale);
         }
 #pragma unroll
         for (int j = 0; j < W; j++) sum[j] = 0.0f;
@@ -537,7 +543,7 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
 #pragma unroll
             for (int j = 0; j < W; j++) a.heads[piece + j] = head[j];
         } else if (valid) {
-            store_part<T, W>(gradient + static_cast<uint64_t>(row_start) * a.columns + column, head, a.scale);
+            store_part<T, W, STREAM>(gradient + static_cast<uint64_t>(row_start) * a.columns + column, head, a.scale);
         }
     }
     if (threadIdx.x < G) {
@@ -552,7 +558,7 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
 
 // One wave per block of the sums and tile of columns: the row that was open at the block's start, if it ends there, from
 // the open sums of the blocks before it since the last end of a row, and the block's own first piece.
-template <typename T, int W, int G>
+template <typename T, int W, bool STREAM, int G>
 __global__ __launch_bounds__(64) void embedding_join_kernel(SumArgs a) {
     constexpr uint32_t slots = 64 / G;
     const uint32_t lane = threadIdx.x, part = lane / G, b = blockIdx.x;
@@ -583,7 +589,7 @@ __global__ __launch_bounds__(64) void embedding_join_kernel(SumArgs a) {
     if (part == 0 && slot < a.row_lanes) {
 #pragma unroll
         for (int j = 0; j < W; j++) sum[j] += a.heads[b * stride + piece + j];
-        store_part<T, W>(static_cast<T*>(a.gradient) + static_cast<uint64_t>(a.first_row[b]) * a.columns + min(slot * W, a.columns - W), sum, a.scale);
+        store_part<T, W, STREAM>(static_cast<T*>(a.gradient) + static_cast<uint64_t>(a.first_row[b]) * a.columns + min(slot * W, a.columns - W), sum, a.scale);
     }
 }
 
@@ -596,14 +602,17 @@ int lane_values(const EmbeddingArgs& a) {
 
 uint32_t lanes_of_row(const EmbeddingArgs& a) { return div_up(a.columns, static_cast<uint32_t>(lane_values(a))); }
 
-// f(a value of the type, the lane's values as a constant)
+uint64_t output_bytes(const EmbeddingArgs& a, uint64_t rows) { return rows * a.columns * (a.type == type_float ? 4 : 2); }
+
+// f(a value of the type, the lane's values, whether an output of so many rows is stored past the caches), the latter two as constants
 template <typename F>
-void with_type(const EmbeddingArgs& a, F&& f) {
-    const bool one = lane_values(a) == 1;
+void with_type(const EmbeddingArgs& a, uint64_t output_rows, F&& f) {
+    const bool one = lane_values(a) == 1, stream = output_bytes(a, output_rows) >= stream_from;
     auto widths = [&](auto t) {
         constexpr int full = 16 / sizeof(t);
-        if (one) f(t, std::integral_constant<int, 1>{});
-        else f(t, std::integral_constant<int, full>{});
+        if (one) f(t, std::integral_constant<int, 1>{}, std::false_type{});
+        else if (stream) f(t, std::integral_constant<int, full>{}, std::true_type{});
+        else f(t, std::integral_constant<int, full>{}, std::false_type{});
     };
     if (a.type == type_float) widths(float{});
     else if (a.type == type_bfloat16) widths(__bf16{});
@@ -677,11 +686,11 @@ struct GradientLayout {
     }
 };
 
-template <typename T, int W, int G>
+template <typename T, int W, bool STREAM, int G>
 void launch_sums(const SumArgs& a, hipStream_t s) {
     const uint32_t tiles = div_up(a.row_lanes, G);
-    embedding_sum_kernel<T, W, G><<<dim3(a.blocks, tiles), sum_block, 0, s>>>(a);
-    embedding_join_kernel<T, W, G><<<dim3(a.blocks, tiles), 64, 0, s>>>(a);
+    embedding_sum_kernel<T, W, STREAM, G><<<dim3(a.blocks, tiles), sum_block, 0, s>>>(a);
+    embedding_join_kernel<T, W, STREAM, G><<<dim3(a.blocks, tiles), 64, 0, s>>>(a);
 }
 
 }  // namespace
@@ -691,7 +700,7 @@ bool launch_embedding_lookup(const EmbeddingArgs& a, const void* table, uint64_t
     if (a.rows == 0) {
         const uint64_t values = static_cast<uint64_t>(a.n) * a.columns;
         const uint32_t blocks = values > 2048ull * lookup_block ? 2048u : div_up(values, lookup_block);
-        with_type(a, [&](auto t, auto) {
+        with_type(a, a.n, [&](auto t, auto, auto) {
             using T = decltype(t);
             embedding_zero_kernel<T><<<blocks, lookup_block, 0, s>>>(static_cast<T*>(out), values);
         });
@@ -715,11 +724,12 @@ bool launch_embedding_lookup(const EmbeddingArgs& a, const void* table, uint64_t
     for (uint64_t b = 0; b < blocks; b += max_blocks) {
         l.first = static_cast<uint32_t>(b * l.rows_per_block);
         const dim3 grid(static_cast<uint32_t>(blocks - b < max_blocks ? blocks - b : max_blocks), div_up(l.row_lanes, lookup_tile));
-        with_type(a, [&](auto t, auto w) {
+        with_type(a, a.n, [&](auto t, auto w, auto stream) {
             using T = decltype(t);
             constexpr int W = decltype(w)::value;
-            if (a.index_bytes == 4) embedding_lookup_kernel<T, W, int32_t><<<grid, lookup_block, 0, s>>>(l);
-            else embedding_lookup_kernel<T, W, int64_t><<<grid, lookup_block, 0, s>>>(l);
+            constexpr bool S = decltype(stream)::value;
+            if (a.index_bytes == 4) embedding_lookup_kernel<T, W, S, int32_t><<<grid, lookup_block, 0, s>>>(l);
+            else embedding_lookup_kernel<T, W, S, int64_t><<<grid, lookup_block, 0, s>>>(l);
         });
         EFGS_HIP_CHECK(hipGetLastError());
     }
@@ -779,22 +789,23 @@ bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uin
     u.row_lanes = lanes_of_row(a);
     u.blocks = sum_blocks(a);
     u.scale = a.scale;
-    with_type(a, [&](auto t, auto w) {
+    with_type(a, a.rows, [&](auto t, auto w, auto stream) {
         using T = decltype(t);
         constexpr int W = decltype(w)::value;
+        constexpr bool S = decltype(stream)::value;
         switch (group_lanes(a)) {
-            case 1: launch_sums<T, W, 1>(u, s); break;
-            case 2: launch_sums<T, W, 2>(u, s); break;
-            case 4: launch_sums<T, W, 4>(u, s); break;
+            case 1: launch_sums<T, W, S, 1>(u, s); break;
+            case 2: launch_sums<T, W, S, 2>(u, s); break;
+            case 4: launch_sums<T, W, S, 4>(u, s); break;
             default:
                 if constexpr (W == 1) {
-                    launch_sums<T, W, 8>(u, s);  // (at most 7 lanes of one value)
+                    launch_sums<T, W, S, 8>(u, s);  // (at most 7 lanes of one value)
                 } else {
                     switch (group_lanes(a)) {
-                        case 8: launch_sums<T, W, 8>(u, s); break;
-                        case 16: launch_sums<T, W, 16>(u, s); break;
-                        case 32: launch_sums<T, W, 32>(u, s); break;
-                        default: launch_sums<T, W, 64>(u, s); break;
+                        case 8: launch_sums<T, W, S, 8>(u, s); break;
+                        case 16: launch_sums<T, W, S, 16>(u, s); break;
+                        case 32: launch_sums<T, W, S, 32>(u, s); break;
+                        default: launch_sums<T, W, S, 64>(u, s); break;
                     }
                 }
         }
