@@ -101,6 +101,26 @@ def test_hot_row_between_empty_ones():
     _check_gradient(table.grad, indices, grad, rows, 1.0, 'f32')
 
 
+@pytest.mark.parametrize('rows, columns, dtype', [(60_001, 513, 'f32'), (100_003, 1024, 'bf16'), (13_000_001, 5, 'f16')])
+def test_gradient_of_a_table_that_no_cache_holds(rows, columns, dtype):
+    """Gradients of over 100 MB (stored past the caches), most rows zero; against sums in 64 bits on the GPU."""
+    import efgs
+    print(f'case embedding large table {rows} x {columns} {dtype}', flush=True)
+    kind, rounding, least = TYPES[dtype]
+    table = torch.zeros((rows, columns), dtype=kind, device=DEVICE, requires_grad=True)
+    indices = torch.randint(0, rows, (9001,), device=DEVICE)
+    indices[::3] = rows - 1
+    grad = torch.randn(9001, columns, device=DEVICE).to(kind)
+    got = torch.autograd.grad(efgs.embedding(indices, table, 1.5), table, grad)[0]
+    met, where, entries = torch.unique(indices, return_inverse=True, return_counts=True)
+    want = torch.zeros((len(met), columns), dtype=torch.float64, device=DEVICE).index_add_(0, where, grad.double()) * 1.5
+    size = torch.zeros((len(met), columns), dtype=torch.float64, device=DEVICE).index_add_(0, where, grad.double().abs()) * 1.5
+    bound = (entries[:, None] + 1) * E * size + rounding * want.abs() * (1 + 1e-6) + least
+    assert bool(((got[met].double() - want).abs() <= bound).all())
+    got[met] = 0
+    assert not bool(got.any())
+
+
 def test_more_indices_than_a_pass_of_the_sort_takes_at_once():
     """Over a million indices: several tiles to a block of the sort."""
     _check(2_200_003, 3000, 1, 'f32')
