@@ -251,7 +251,7 @@ __device__ __forceinline__ float decode_ratio(uint32_t code, float factor) {
     return code & 128u ? -u : u;
 }
 __device__ __forceinline__ uint32_t encode(float y, float c, uint32_t dither, uint32_t base, uint32_t top) {
-    return min(((__float_as_uint(y + c) + (dither << 3)) >> 19) - base, top);
+    return min((__float_as_uint(y + c) + (dither << 3) - (base << 19)) >> 19, top);
 }
 
 __device__ __forceinline__ uint32_t dither_of(uint32_t element, uint32_t key) { return adamw_mix(element * 0x9E3779B1u + key); }
@@ -259,7 +259,7 @@ __device__ __forceinline__ uint32_t dither_of(uint32_t element, uint32_t key) { 
 // sqrt(x) and its reciprocal's approximation for x = 0 or x >= 2^-100, rounded to nearest: one step from the hardware's reciprocal
 // square root (s = x y, s + (x - s^2) y / 2, the residual exact by the fused operation).
 __device__ __forceinline__ float rounded_sqrt(float x, float& reciprocal) {
-    reciprocal = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-100f));
+    reciprocal = __builtin_amdgcn_rsqf(__uint_as_float(max(__float_as_uint(x), __float_as_uint(0x1p-100f))));
     const float s = x * reciprocal;
     return __builtin_fmaf(__builtin_fmaf(-s, s, x), 0.5f * reciprocal, s);
 }
@@ -293,7 +293,7 @@ __device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGro
     const Rates rates = rates_of<CYCLE>(G, cycle, column);
     const float coefficient = clip.coefficient();
     if (coefficient != coefficient) return;
-    bool plain = true;
+    uint32_t least = 0xffffffffu, most = 0;  // of v's bits less one (which makes zeros the largest), and of v's bits
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const float gk = g[k] * coefficient;
@@ -301,14 +301,16 @@ __device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGro
         m[k] = G.beta1 * (decode_ratio((ratio_codes >> (8 * k)) & 255u, G.ratio_decode) * old) + G.beta1_rest * gk;
         v[k] = G.beta2 * (old * old) + G.beta2_rest * (gk * gk);
         // (past the tensor's end: code 0 and gradient 0 make 0)
-        plain = plain && ((v[k] >= 0x1p-100f && v[k] < INFINITY) || v[k] == 0.0f);
+        least = min(least, __float_as_uint(v[k]) - 1u);
+        most = max(most, __float_as_uint(v[k]));
     }
+    const bool plain = least >= __float_as_uint(0x1p-100f) - 1u && most < __float_as_uint(INFINITY);
     if (__ballot(!plain) == 0) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             float reciprocal;
             r[k] = rounded_sqrt(v[k], reciprocal);
-            u[k] = v[k] > 0.0f ? rounded_quotient(m[k], r[k], reciprocal) : 0.0f;
+            u[k] = rounded_quotient(m[k], r[k], reciprocal);  // (v = 0: whatever it is, r's code is 0)
             p[k] = updated(G, p[k], m[k], r[k], rates.of[k].x, rates.of[k].y);
         }
     } else {
