@@ -6,7 +6,8 @@
 // The gradient sorts the indices (stable, least significant digit first), so that a row's sum is over a contiguous run of
 // the sorted list, in an order that the data alone gives: results are the same from call to call, without atomics on
 // floats. Runs are uneven (a common code is met by a large part of all primitives, most rows of a large table by none) and
-// the zero rows have to be written too, so the work is cut by the merged list of both: entry e of row k stands at
+// the zero rows have to be written too, so the work is cut by the merged list of both (tables of few rows are summed otherwise, see
+// small tables below): entry e of row k stands at
 // position e + k, behind e entries and the ends of k rows, and the end of a row is an item of its own, which writes
 // it. Every group of lanes takes the same number of items whatever the runs are; a sum that crosses groups is carried by a
 // segmented scan within the block, and a row that crosses blocks is put together by a second kernel from the blocks' first
@@ -593,6 +594,274 @@ __global__ __launch_bounds__(64) void embedding_join_kernel(SumArgs a) {
     }
 }
 
+// W floats (one or fours) of a partial table
+template <int W>
+__device__ __forceinline__ void store_floats(float* p, const float* x) {
+    if constexpr (W == 1) {
+        *p = x[0];
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+    }
+}
+
+template <int W>
+__device__ __forceinline__ void load_floats(const float* p, float* x) {
+    if constexpr (W == 1) {
+        x[0] = *p;
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + j);
+            x[j] = v.x;
+            x[j + 1] = v.y;
+            x[j + 2] = v.z;
+            x[j + 3] = v.w;
+        }
+    }
+}
+
+// ---- small tables ----------------------------------------------------------------------------------------------------------
+// A small table needs no list in order over the GPU: a block sorts a tile of the indices in LDS, sums its runs and writes a partial
+// table of its own (every row, in 32 bits), and a second kernel adds the partial tables up. grad_out is read a tile at a time,
+// where the long list's runs gather rows from all over it, 128-byte lines for 32 bytes; two launches stand for five to seven. What it
+// costs is the partial tables, written and read once, so they decide: at most 32 MB of them, 256 KB each (us by the list and by tiles: 1M
+// indices into 4,096 rows of 8 floats, 32 MB, 56 and 37; 200k into 257 rows of 45 30 and 20, 20k into 500 of 8 18 and 11; past that 100k
+// into 4,096 rows of 64 28 and 46, 200k into 700 rows of 64, 35 MB, 31 and 33, 4,000 into 4,096 rows of 64, 1 MB each, 14 and 23).
+
+constexpr uint32_t tile_rows = 4096, tile_lanes = 16, tile_position_bits = 12;
+constexpr uint32_t tile_most_blocks = 256;
+constexpr uint64_t tile_most_bytes = 32ull << 20, tile_table_bytes = 256ull << 10;
+constexpr uint32_t tables_block = 256, tables_parts = 8, tables_lanes = tables_block / tables_parts;
+
+struct TileSumArgs {
+    SortPass keys;             // indices, n, rows, padding, tiles_per_block; digit_bits of a local pass
+    uint32_t passes;
+    const void* grad_out;
+    float* partials;           // blocks x rows x lanes x lane's values
+    uint32_t columns, row_lanes, index_bytes;
+};
+
+template <typename T, int W, int G, uint32_t STEPS>
+__global__ __launch_bounds__(sort_block) void embedding_tile_sum_kernel(TileSumArgs a) {
+    constexpr uint32_t tile_size = sort_block * STEPS, groups = sort_block / G, batch = 8;
+    struct Sorting {
+        uint16_t counts[sort_waves][sort_most_digits];
+        uint32_t wave_totals[sort_waves];
+    };
+    struct Summing {
+        uint32_t closed[sort_waves];
+        float tail[sort_waves][G * W];
+    };
+    __shared__ uint32_t ordered[tile_size];  // row << 12 | position in the tile, in order of rows
+    __shared__ __attribute__((aligned(16))) unsigned char shared[sizeof(Sorting) > sizeof(Summing) ? sizeof(Sorting) : sizeof(Summing)];
+    Sorting& sorting = *reinterpret_cast<Sorting*>(shared);
+    Summing& summing = *reinterpret_cast<Summing*>(shared);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, rows = a.keys.rows;
+    const uint32_t digits = 1u << a.keys.digit_bits;
+    const uint32_t group = threadIdx.x / G, slot = threadIdx.x % G, column = min(slot * W, a.columns - W);
+    const bool valid = slot < a.row_lanes;
+    float* const table = a.partials + static_cast<uint64_t>(blockIdx.x) * rows * a.row_lanes * W;
+    const float zeros[W] = {};
+    for (uint32_t k = threadIdx.x; k < rows * a.row_lanes; k += sort_block) store_floats<W>(table + static_cast<uint64_t>(k) * W, zeros);
+
+    for (uint32_t tile = 0; tile < a.keys.tiles_per_block; tile++) {
+        const uint64_t first = (static_cast<uint64_t>(blockIdx.x) * a.keys.tiles_per_block + tile) * tile_size;
+        const uint32_t here = first >= a.keys.n ? 0u : static_cast<uint32_t>(min(static_cast<uint64_t>(tile_size), a.keys.n - first));
+        if (tile > 0 && here == 0) break;
+        const uint32_t mine = wave * 64u * STEPS + lane;
+        uint32_t x[STEPS], rank[STEPS];
+        auto load_keys = [&](auto index) {
+            using I = decltype(index);
+#pragma unroll
+            for (uint32_t s = 0; s < STEPS; s++) {
+                const uint32_t k = mine + s * 64u;
+                x[s] = key_at<I>(a.keys, static_cast<uint32_t>(min(first + k, static_cast<uint64_t>(a.keys.n - 1)))) << tile_position_bits | k;
+            }
+        };
+        if (a.index_bytes == 4) load_keys(int32_t{});
+        else load_keys(int64_t{});
+        for (uint32_t pass = 0; pass < a.passes; pass++) {
+            const uint32_t shift = tile_position_bits + pass * a.keys.digit_bits;
+            if (pass > 0) {
+#pragma unroll
+                for (uint32_t s = 0; s < STEPS; s++) x[s] = ordered[mine + s * 64u];
+            }
+            for (uint32_t k = lane; k < digits; k += 64) sorting.counts[wave][k] = 0;
+            volatile uint16_t* const counts = sorting.counts[wave];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (uint32_t s = 0; s < STEPS; s++) {
+                const uint32_t d = (x[s] >> shift) & (digits - 1u);
+                const bool in = mine + s * 64u < here;
+                uint64_t same = __ballot(in);
+                for (uint32_t b = 0; b < a.keys.digit_bits; b++) {
+                    const int64_t bit = static_cast<int32_t>(d << (31u - b)) >> 31;
+                    same &= ~(__ballot(bit != 0) ^ static_cast<uint64_t>(bit));
+                }
+                const uint32_t earlier = static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1ull)));
+                const uint32_t so_far = counts[d];
+                rank[s] = so_far + earlier;
+                __builtin_amdgcn_wave_barrier();
+                if (in && earlier == 0) counts[d] = static_cast<uint16_t>(so_far + static_cast<uint32_t>(__popcll(same)));
+                __builtin_amdgcn_wave_barrier();
+            }
+            __syncthreads();
+            const bool owner = threadIdx.x < digits;
+            uint32_t local = 0;
+            if (owner) {
+                uint32_t in_tile = 0;
+#pragma unroll
+                for (uint32_t w = 0; w < sort_waves; w++) in_tile += sorting.counts[w][threadIdx.x];
+                local = wave_exclusive(in_tile, sorting.wave_totals);
+            }
+            __syncthreads();
+            if (owner) {
+                local += totals_before(wave, sorting.wave_totals);
+#pragma unroll
+                for (uint32_t w = 0; w < sort_waves; w++) {
+                    const uint32_t c = sorting.counts[w][threadIdx.x];
+                    sorting.counts[w][threadIdx.x] = static_cast<uint16_t>(local);
+                    local += c;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (uint32_t s = 0; s < STEPS; s++)
+                if (mine + s * 64u < here) ordered[sorting.counts[wave][(x[s] >> shift) & (digits - 1u)] + rank[s]] = x[s];
+            __syncthreads();
+        }
+
+        // the entries that count, evenly over the groups
+        uint32_t entries = here;
+        for (uint32_t lo = 0; lo < entries;) {
+            const uint32_t mid = (lo + entries) / 2;
+            if (ordered[mid] >> tile_position_bits < rows) lo = mid + 1;
+            else entries = mid;
+        }
+        const uint32_t per_group = (entries + groups - 1) / groups;
+        const uint32_t start = min(group * per_group, entries), end = min(start + per_group, entries);
+        float sum[W] = {}, head[W] = {};
+        bool any_closed = false;
+        uint32_t head_row = 0;
+        auto write = [&](uint32_t row, const float* values) {
+            if (!valid) return;
+            float* const at = table + (static_cast<uint64_t>(row) * a.row_lanes + slot) * W;
+            if (tile == 0) {
+                store_floats<W>(at, values);
+            } else {
+                float old[W];
+                load_floats<W>(at, old);
+#pragma unroll
+                for (int j = 0; j < W; j++) old[j] += values[j];
+                store_floats<W>(at, old);
+            }
+        };
+        for (uint32_t from = start; from < end; from += batch) {
+            typename Part<T, W>::type data[batch];
+            uint32_t key[batch + 1];
+#pragma unroll
+            for (uint32_t k = 0; k <= batch; k++) {
+                const uint32_t entry = ordered[min(from + k, entries - 1)];
+                key[k] = from + k < entries ? entry >> tile_position_bits : rows;
+                if (k == batch) break;
+                const uint64_t i = first + (entry & ((1u << tile_position_bits) - 1u));
+                data[k] = load_part<T, W>(static_cast<const T*>(a.grad_out) + i * a.columns + column);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < batch; k++) {
+                if (from + k < end) {
+#pragma unroll
+                    for (int j = 0; j < W; j++) sum[j] += value_of<T, W>(data[k], j);
+                    if (key[k] != key[k + 1]) {  // the run's last entry
+                        if (any_closed) {
+                            write(key[k], sum);
+                        } else {
+                            any_closed = true;
+                            head_row = key[k];
+#pragma unroll
+                            for (int j = 0; j < W; j++) head[j] = sum[j];
+                        }
+#pragma unroll
+                        for (int j = 0; j < W; j++) sum[j] = 0.0f;
+                    }
+                }
+            }
+        }
+
+        // the run that is open at each group's start: the segmented scan of the groups' open sums
+        float scanned[W];
+        uint32_t flag = any_closed ? 1u : 0u;
+#pragma unroll
+        for (int j = 0; j < W; j++) scanned[j] = sum[j];
+#pragma unroll
+        for (uint32_t o = G; o < 64; o <<= 1) {
+            const uint32_t other_flag = __shfl_up(flag, o);
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                const float other = __shfl_up(scanned[j], o);
+                if (lane >= o && !flag) scanned[j] += other;
+            }
+            if (lane >= o) flag |= other_flag;
+        }
+        if (lane >= 64 - G) {
+#pragma unroll
+            for (int j = 0; j < W; j++) summing.tail[wave][(lane % G) * W + j] = scanned[j];
+            if (lane == 63) summing.closed[wave] = flag;
+        }
+        __syncthreads();
+        float before[W] = {};
+        for (uint32_t w = 0; w < wave; w++) {
+            const bool closed = summing.closed[w] != 0;
+#pragma unroll
+            for (int j = 0; j < W; j++) before[j] = summing.tail[w][(lane % G) * W + j] + (closed ? 0.0f : before[j]);
+        }
+        if constexpr (G < 64) {
+            const uint32_t wave_flag = __shfl_up(flag, G);
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                const float other = __shfl_up(scanned[j], G);
+                if (lane >= G) before[j] = other + (wave_flag ? 0.0f : before[j]);
+            }
+        }
+        if (any_closed) {
+#pragma unroll
+            for (int j = 0; j < W; j++) head[j] += before[j];
+            write(head_row, head);
+        }
+        __syncthreads();  // (before the next tile's sort writes where the sums were read)
+    }
+}
+
+// The partial tables' sum, eight threads to a lane of a row, each every eighth table: a fixed order.
+template <typename T, int W>
+__global__ __launch_bounds__(tables_block) void embedding_tables_kernel(const float* __restrict__ partials, T* __restrict__ gradient, uint32_t tables, uint32_t rows,
+                                                               uint32_t row_lanes, uint32_t columns, float scale) {
+    __shared__ float s_sum[tables_parts][tables_lanes][W];
+    const uint32_t part = threadIdx.x / tables_lanes, k = threadIdx.x % tables_lanes, count = rows * row_lanes;
+    const uint32_t at = blockIdx.x * tables_lanes + k, safe = min(at, count - 1);
+    const float* const from = partials + static_cast<uint64_t>(safe) * W;
+    const uint64_t stride = static_cast<uint64_t>(count) * W;
+    float sum[W] = {};
+#pragma unroll 8
+    for (uint32_t t = part; t < tables; t += tables_parts) {
+        float x[W];
+        load_floats<W>(from + t * stride, x);
+#pragma unroll
+        for (int j = 0; j < W; j++) sum[j] += x[j];
+    }
+#pragma unroll
+    for (int j = 0; j < W; j++) s_sum[part][k][j] = sum[j];
+    __syncthreads();
+    if (part != 0 || at >= count) return;
+#pragma unroll
+    for (uint32_t p = 1; p < tables_parts; p++)
+#pragma unroll
+        for (int j = 0; j < W; j++) sum[j] += s_sum[p][k][j];
+    const uint32_t row = at / row_lanes, slot = at - row * row_lanes;
+    store_part<T, W, false>(gradient + static_cast<uint64_t>(row) * columns + min(slot * W, columns - W), sum, scale);
+}
+
 uint32_t bit_width(uint32_t x) { return x == 0 ? 0u : 32u - static_cast<uint32_t>(__builtin_clz(x)); }
 
 int lane_values(const EmbeddingArgs& a) {
@@ -654,6 +923,67 @@ void launch_sort_pass(const SortPass& p, hipStream_t s) {
         sort_count_kernel<I, 4><<<blocks, sort_block, 0, s>>>(p);
         sort_scatter_kernel<I, false, 4><<<blocks, sort_block, 0, s>>>(p);
     }
+}
+
+// The blocks and tiles of a small table's gradient; no blocks where the table is not small.
+struct TilePlan {
+    uint32_t blocks = 0, steps = 1, tiles_per_block = 1;
+    uint64_t bytes = 0;  // of the partial tables
+};
+
+TilePlan plan_tiles(const EmbeddingArgs& a) {
+    TilePlan p;
+    if (a.n == 0 || a.rows > tile_rows || lanes_of_row(a) > tile_lanes) return p;
+    // (one key a thread up to 262,144 indices, so that there are blocks for the GPU; then two, four, and more tiles to a block)
+    const uint32_t pieces = div_up(a.n, sort_block);
+    p.steps = pieces <= tile_most_blocks ? 1 : pieces <= 2 * tile_most_blocks ? 2 : 4;
+    const uint32_t tiles = div_up(pieces, p.steps);
+    p.tiles_per_block = div_up(tiles, tile_most_blocks);
+    p.blocks = div_up(tiles, p.tiles_per_block);
+    const uint64_t table = static_cast<uint64_t>(a.rows) * lanes_of_row(a) * static_cast<uint64_t>(lane_values(a)) * 4;
+    p.bytes = p.blocks * table;
+    if (table > tile_table_bytes || p.bytes > tile_most_bytes) p.blocks = 0;
+    return p;
+}
+
+template <typename T, int W, int G>
+void launch_tiles(const TileSumArgs& a, const TilePlan& p, hipStream_t s) {
+    if (p.steps == 1) embedding_tile_sum_kernel<T, W, G, 1><<<p.blocks, sort_block, 0, s>>>(a);
+    else if (p.steps == 2) embedding_tile_sum_kernel<T, W, G, 2><<<p.blocks, sort_block, 0, s>>>(a);
+    else embedding_tile_sum_kernel<T, W, G, 4><<<p.blocks, sort_block, 0, s>>>(a);
+}
+
+bool launch_small_table(const EmbeddingArgs& a, const TilePlan& p, const void* grad_out, uint32_t padding, void* gradient, float* partials, hipStream_t s) {
+    TileSumArgs t{};  // (of t.keys the tile kernel reads what is set here)
+    t.keys.indices = a.indices;
+    t.keys.n = a.n;
+    t.keys.rows = a.rows;
+    t.keys.padding = padding;
+    t.keys.tiles_per_block = p.tiles_per_block;
+    const uint32_t bits = bit_width(a.rows);
+    t.passes = bits > sort_most_bits ? 2 : 1;
+    t.keys.digit_bits = std::max(div_up(bits, t.passes), sort_least_bits);
+    t.grad_out = grad_out;
+    t.partials = partials;
+    t.columns = a.columns;
+    t.row_lanes = lanes_of_row(a);
+    t.index_bytes = static_cast<uint32_t>(a.index_bytes);
+    with_type(a, 0, [&](auto v, auto w, auto) {
+        using T = decltype(v);
+        constexpr int W = decltype(w)::value;
+        switch (group_lanes(a)) {
+            case 1: launch_tiles<T, W, 1>(t, p, s); break;
+            case 2: launch_tiles<T, W, 2>(t, p, s); break;
+            case 4: launch_tiles<T, W, 4>(t, p, s); break;
+            case 8: launch_tiles<T, W, 8>(t, p, s); break;
+            default:
+                if constexpr (W > 1) launch_tiles<T, W, 16>(t, p, s);
+        }
+        const uint32_t blocks = div_up(static_cast<uint64_t>(a.rows) * t.row_lanes, tables_lanes);
+        embedding_tables_kernel<T, W><<<blocks, tables_block, 0, s>>>(partials, static_cast<T*>(gradient), p.blocks, a.rows, t.row_lanes, a.columns, a.scale);
+    });
+    EFGS_HIP_CHECK(hipGetLastError());
+    return true;
 }
 
 struct GradientLayout {
@@ -740,10 +1070,15 @@ bool embedding_gradient_fits(const EmbeddingArgs& a) {
     return static_cast<uint64_t>(a.n) + a.rows <= 0xffff0000ull && sum_blocks(a) <= max_blocks;
 }
 
-size_t embedding_gradient_bytes(const EmbeddingArgs& a) { return GradientLayout::carve(nullptr, a).bytes; }
+size_t embedding_gradient_bytes(const EmbeddingArgs& a) {
+    const TilePlan tiles = plan_tiles(a);
+    return tiles.blocks > 0 ? static_cast<size_t>(tiles.bytes) : GradientLayout::carve(nullptr, a).bytes;
+}
 
 bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uint32_t padding, void* gradient, void* workspace, hipStream_t s) {
     if (a.rows == 0 || a.columns == 0) return true;
+    const TilePlan tiles = plan_tiles(a);
+    if (tiles.blocks > 0) return launch_small_table(a, tiles, grad_out, padding, gradient, static_cast<float*>(workspace), s);
     const GradientLayout l = GradientLayout::carve(static_cast<char*>(workspace), a);
     uint32_t current = 0;
     if (a.n > 0) {

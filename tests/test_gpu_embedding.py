@@ -90,6 +90,34 @@ def test_rows_met_by_nearly_every_index(n, rows, columns, dtype):
     _check(n, rows, columns, dtype, skew=1.0, invalid=0.001)
 
 
+@pytest.mark.parametrize('n, rows, columns, dtype', [(262_144, 4096, 8, 'f32'), (262_145, 4096, 8, 'f32'), (300_001, 257, 45, 'f32'), (524_289, 511, 4, 'f32'),
+                                                     (530_000, 512, 3, 'f32'), (1_048_577, 300, 8, 'bf16'), (1_100_000, 4096, 8, 'f32'), (4000, 4096, 8, 'f16'),
+                                                     (4000, 4097, 8, 'f16'), (9000, 1024, 64, 'f32'), (9000, 1025, 64, 'f32'), (1500, 4095, 16, 'f32'),
+                                                     (20_000, 1000, 128, 'bf16'), (70_000, 64, 7, 'bf16'), (5000, 40, 68, 'f32')])
+def test_small_tables_and_their_limits(n, rows, columns, dtype):
+    """Tables summed by tiles, and just past that: one, two and four keys a thread, several tiles to a block, one and two passes of the
+    tile's sort, the largest number of rows, the largest table, the widest rows."""
+    _check(n, rows, columns, dtype, seed=n % 1000, padding=3)
+
+
+@pytest.mark.parametrize('n, rows, columns', [(150_000, 6000, 3), (300_000, 5000, 8), (1_200_000, 4200, 2), (1_060_000, 70_000, 1)])
+def test_long_lists_into_larger_tables(n, rows, columns):
+    """The list in order over the GPU: several tiles to a block of its passes, digits of 7 to 9 bits, hot rows among many."""
+    _check(n, rows, columns, 'f32', skew=3.0)
+
+
+@pytest.mark.parametrize('rows', [4500, 100_000])
+def test_one_row_met_by_nearly_all_of_a_larger_table(rows):
+    import efgs
+    n = 120_000
+    indices = torch.full((n,), rows // 2, device=DEVICE)
+    indices[::500] = torch.randint(0, rows, (n // 500,), device=DEVICE)
+    grad = torch.randn(n, 12, device=DEVICE)
+    table = torch.zeros(rows, 12, device=DEVICE, requires_grad=True)
+    got = torch.autograd.grad(efgs.embedding(indices, table, 0.5), table, grad)[0]
+    _check_gradient(got, indices, grad, rows, 0.5, 'f32')
+
+
 def test_hot_row_between_empty_ones():
     import efgs
     n, rows = 50_000, 9000
@@ -181,12 +209,13 @@ def test_padding_row():
             efgs.embedding(indices, table, 1.0, padding)
 
 
-def test_odd_values_stay_in_their_rows():
+@pytest.mark.parametrize('rows', [50, 5000])
+def test_odd_values_stay_in_their_rows(rows):
     """Infinities and NaN in a row of the table or upstream reach that row alone; those behind an index that counts nowhere reach none."""
     import efgs
-    indices = torch.randint(2, 50, (3000,), device=DEVICE)
+    indices = torch.randint(2, rows, (3000,), device=DEVICE)
     indices[7], indices[8], indices[9] = 0, -3, 1
-    table = torch.randn(50, 8, device=DEVICE)
+    table = torch.randn(rows, 8, device=DEVICE)
     table[0] = float('nan')
     leaf = table.requires_grad_()
     out = efgs.embedding(indices, leaf, 1.0, 1)
@@ -198,9 +227,10 @@ def test_odd_values_stay_in_their_rows():
     assert bool(got[2:].isfinite().all())
 
 
-def test_results_repeat_bit_for_bit():
+@pytest.mark.parametrize('n, rows, columns', [(200_000, 700, 24), (200_000, 7000, 24), (1_100_000, 4000, 8), (7000, 50_000, 8)])
+def test_results_repeat_bit_for_bit(n, rows, columns):
     import efgs
-    indices, table, grad = _inputs(200_000, 700, 24, 'f32')
+    indices, table, grad = _inputs(n, rows, columns, 'f32')
     first = torch.autograd.grad(efgs.embedding(indices, table), table, grad)[0]
     for _ in range(3):
         assert torch.equal(first, torch.autograd.grad(efgs.embedding(indices, table), table, grad)[0])
@@ -259,10 +289,11 @@ def test_on_a_stream_of_its_own():
     assert torch.equal(got, want)
 
 
-def test_graph_replays_match_eager():
+@pytest.mark.parametrize('rows', [500, 9000])
+def test_graph_replays_match_eager(rows):
     """Lookup and gradient captured as one graph; every replay, on new values, equals the eager results."""
     import efgs
-    indices, table, grad = _inputs(60_000, 500, 8, 'f32')
+    indices, table, grad = _inputs(60_000, rows, 8, 'f32')
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -275,7 +306,7 @@ def test_graph_replays_match_eager():
         out = efgs.embedding(indices, table, 2.0)
         got = torch.autograd.grad(out, table, grad)[0]
     for seed in range(4):
-        new = _inputs(60_000, 500, 8, 'f32', seed=seed + 1)
+        new = _inputs(60_000, rows, 8, 'f32', seed=seed + 1)
         with torch.no_grad():
             indices.copy_(new[0])
             table.copy_(new[1])
