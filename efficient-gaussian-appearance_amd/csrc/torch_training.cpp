@@ -193,6 +193,7 @@ PyObject* state_of(PyObject* states, PyObject* key, const Tensor& param, int bit
     }
     TORCH_CHECK_VALUE(PyDict_Check(state), "efgs: AdamW: a parameter's state must be a dict");
     if (PyDict_GET_SIZE(state) > 0) return state;
+    const c10::DeviceGuard guard(param.device());
     const auto options = at::TensorOptions().device(param.device());
     if (bits == 32) {
         set_entry(state, exp_avg_name, THPVariable_Wrap(at::zeros(param.sizes(), options.dtype(at::kFloat))));
@@ -267,6 +268,10 @@ c10::optional<Tensor> adamw_step(const py::list& groups, const py::dict& states,
         TORCH_CHECK_VALUE(PyDict_Check(item.ptr()), "efgs: AdamW: a parameter group must be a dict");
         PyObject* const params = group_entry(item.ptr(), params_name);
         TORCH_CHECK_VALUE(PyList_Check(params), "efgs: AdamW: a group's parameters must be a list");
+        const size_t most = tensors.size() + static_cast<size_t>(PyList_GET_SIZE(params));
+        entries.reserve(most);
+        tensors.reserve(most);
+        norms.reserve(max_grad_norm ? most : 0);
         native_groups.push_back(native_group(item.ptr()));
         const efgs_adamw_group& native = native_groups.back();
         const int bits = native.state_bits;
@@ -285,10 +290,10 @@ c10::optional<Tensor> adamw_step(const py::list& groups, const py::dict& states,
             efgs_adamw_tensor t{};
             t.param_type = element_type("AdamW: a parameter", param.scalar_type());
             t.grad_type = element_type("AdamW: a gradient", given.scalar_type());
-            const c10::DeviceGuard guard(*device);
             if (given.is_contiguous()) {
                 t.grad = given.data_ptr();
             } else {
+                const c10::DeviceGuard guard(*device);
                 kept.push_back(given.contiguous());
                 t.grad = kept.back().data_ptr();
             }
