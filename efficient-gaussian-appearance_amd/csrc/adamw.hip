@@ -160,7 +160,7 @@ struct AdamWLaunch {
 };
 static_assert(sizeof(AdamWLaunch<32>) <= 4096 && sizeof(AdamWLaunch<8>) <= 4096, "kernel arguments");
 
-// The clipping coefficient; not a number where the norm is not finite (the step then stores nothing).
+// The clipping coefficient; not a number where the norm is not finite (the step then leaves parameters and moments).
 __device__ __forceinline__ float clipping(float norm, float max_grad_norm) {
     return norm < INFINITY ? fminf(max_grad_norm / (norm + 1e-6f), 1.0f) : NAN;
 }
@@ -273,6 +273,19 @@ __device__ __forceinline__ float rounded_quotient(float a, float b, float recipr
     return __builtin_fmaf(__builtin_fmaf(-q, b, a), reciprocal, q);
 }
 
+// Codes of u for another bound, where a step that is left out was given other betas: its caller counts the state as one of these.
+// Values past the new bound become the bound, as they do in a step.
+__device__ __forceinline__ uint32_t recoded_ratios(uint32_t codes, const AdamWGroupDevice& G, uint32_t element) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t code = (codes >> (8 * k)) & 255u;
+        const float y = fminf(decode_ratio(code & 127u, G.ratio_decode) * G.ratio_encode, ratio_top);
+        out |= (encode(y, ratio_c, dither_of(element + k, G.key) >> 16, ratio_base, 127u) | (code & 128u)) << (8 * k);
+    }
+    return out;
+}
+
 // One wave per block of 256 elements, four to a lane: the block's maximum is one reduction of the wave, and nothing crosses waves.
 // float32 elements are bound by memory (22M, 353 MB, in 60 us, 5.9 TB/s), bfloat16 ones by the vector units (13.4M, 134 MB, in
 // 35 us, 3.8 TB/s, at about 90 vector operations an element). A square root and a quotient with the library's full range would be 30 more, so they
@@ -297,7 +310,11 @@ __device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGro
     const float scale = T.scale[first / 256];
     const Rates rates = rates_of<CYCLE>(G, cycle, column);
     const float coefficient = clip.coefficient();
-    if (coefficient != coefficient) return;
+    if (coefficient != coefficient) {
+        // (for one bound the factors' product is 1 to two roundings)
+        if (fabsf(G.ratio_decode * G.ratio_encode - 1.0f) > 1e-6f) store_codes<WHOLE>(ratios, count, recoded_ratios(ratio_codes, G, static_cast<uint32_t>(i)));
+        return;
+    }
     uint32_t least = 0xffffffffu, most = 0;  // of v's bits less one (which makes zeros the largest), and of v's bits
 #pragma unroll
     for (int k = 0; k < 4; k++) {

@@ -29,7 +29,8 @@ class AdamW(torch.optim.Optimizer):
     element and step for float32 parameters in place of 28. They need beta1^2 < beta2. `moments` reads either as float32.
 
     max_grad_norm: if set, gradients count times min(1, max_grad_norm / (norm + 1e-6)), norm over all gradients of the step (they
-    themselves stay as they are); where the norm is not finite, parameters and moments stay as they are. The
+    themselves stay as they are); where the norm is not finite, parameters and moments stay as they are (8-bit ones to their codes,
+    where the betas have changed). The
     norm is read on the device and left in `grad_norm` (a tensor of no dimensions; None before the first such step).
 
     The step count is the host's, so a step cannot be captured into a graph.

@@ -287,12 +287,13 @@ enum { EFGS_FLOAT = 0, EFGS_BFLOAT16 = 1, EFGS_HALF = 2 };
  *   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * with lr cycled by element index over the group's n_lrs rates, in 32 bits, p rounded once to its type.
  * Clipping: with grad_norm (device, one float: efgs_grad_norm of all gradients) c = min(1, max_grad_norm / (*grad_norm + 1e-6)),
- * read on the device; where *grad_norm is not finite the step changes nothing. Without it c = 1.
+ * read on the device; where *grad_norm is not finite the step changes nothing (but that 8-bit ratios are coded for the group's
+ * betas, where the state was not). Without it c = 1.
  * States of 32 bits are m and v. States of 8 bits are codes of u = m / sqrt(v) (exp_avg) and of r = sqrt(v)
  * (exp_avg_sq), one byte each, and one float per 256 elements (root_scale): zeros to begin with. r of element i is
  * (f((code + 1776) << 19) - 2^-16) root_scale[i / 256] and |u| (f(((code & 127) + 1904) << 19) - 2^-8) ratio_bound / 0.96484375, f the float
  * of these bits, u's sign the code's top bit. ratio_bound is efgs_adamw_ratio_bound of the betas with which the
- * state was written (the step writes it for its group's betas), and needs beta1^2 < beta2. Codes are rounded by a dither from (element, step,
+ * state was written (the step writes it for its group's betas; ratios past a smaller bound become that bound), and needs beta1^2 < beta2. Codes are rounded by a dither from (element, step,
  * seed), unbiased; results do not depend on the tensors that share a call. An element whose new v is not finite has a zero state.
  * Tensors are contiguous, of any alignment of their type. Stream-ordered; nothing is kept of the arguments. */
 typedef struct efgs_adamw_group {

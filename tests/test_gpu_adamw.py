@@ -454,6 +454,30 @@ def test_changed_betas_keep_the_coded_moments():
     assert opt.state[p]['ratio_bound'] == R.ratio_bound(0.8, 0.95)
 
 
+@pytest.mark.parametrize('betas', [(0.8, 0.95), (0.5, 0.9999)])
+@pytest.mark.parametrize('n', [3, 800, 4099])
+def test_changed_betas_and_a_norm_that_is_not_finite(betas, n):
+    """A step that leaves everything keeps the moments also where its group's betas, and with them the bound of the ratios, are
+    not those of the state: m to one step of its code (at most a 16th of the coded value and its offset), up to the new bound."""
+    import efgs
+    p, g = _make(n, torch.float32, torch.float32, 3)
+    opt = efgs.AdamW([p], state_bits=8, max_grad_norm=1.0, **DEFAULTS)
+    for _ in range(3):
+        opt.step()
+    m, v = (_host(x) for x in opt.moments(p))
+    kept = [p.detach().clone(), opt.state[p]['exp_avg_sq_root'].clone(), opt.state[p]['root_scale'].clone()]
+    g[0] = float('inf')
+    opt.param_groups[0]['betas'] = betas
+    opt.step()
+    assert all(torch.equal(a, b) for a, b in zip([p.detach(), opt.state[p]['exp_avg_sq_root'], opt.state[p]['root_scale']], kept))
+    bound, top, c = R.ratio_bound(*betas), R.TOP - R.RATIO['c'], R.RATIO['c']
+    unit = np.sqrt(v) * bound / top
+    y = np.minimum(np.abs(m) / np.where(unit > 0, unit, 1.0), top)
+    got, got_v = (_host(x) for x in opt.moments(p))
+    assert np.array_equal(got_v, v)
+    assert np.all(np.abs(got - np.sign(m) * y * unit) <= ((y + c) / 16 + 1e-5) * unit)
+
+
 def test_a_step_counts_as_a_change_in_place():
     import efgs
     p, _ = _make(64, torch.float32, torch.float32, 1)
