@@ -397,6 +397,8 @@ struct SumArgs {
     float* tails;              // per block: the sum of the row that is open at its end
     uint32_t* closed;          // per block: 1 where a row ends in it
     uint32_t* first_row;       // per block: the row that is open at its start
+    float* chunk_tails;        // long lists, per 64 blocks: the sum of the row that is open at their end
+    uint32_t* chunk_closed;    // and 1 where a row ends in them; null: short lists
     uint32_t n, rows, columns;
     uint32_t row_lanes;        // lanes of a row
     uint32_t blocks;
@@ -561,37 +563,99 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
     }
 }
 
-// One wave per block of the sums and tile of columns: the row that was open at the block's start, if it ends there, from
-// the open sums of the blocks before it since the last end of a row, and the block's own first piece.
-template <typename T, int W, bool STREAM, int G>
-__global__ __launch_bounds__(64) void embedding_join_kernel(SumArgs a) {
-    constexpr uint32_t slots = 64 / G;
-    const uint32_t lane = threadIdx.x, part = lane / G, b = blockIdx.x;
-    if (!a.closed[b]) return;
-    const uint32_t slot = blockIdx.y * G + lane % G;
-    uint32_t from = b;
-    while (from > 0) {  // back to the last block before b in which a row ends
-        const bool in = lane < from;
-        const uint64_t ends = __ballot(in && a.closed[in ? from - 1 - lane : 0] != 0);
-        if (ends) {
-            from -= static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(ends)));
-            break;
-        }
-        from = from > 64 ? from - 64 : 0;
-    }
-    const uint64_t stride = static_cast<uint64_t>(gridDim.y) * G * W, piece = static_cast<uint64_t>(slot) * W;
-    float sum[W] = {};
-#pragma unroll 8
-    for (uint32_t k = from + part; k < b; k += slots) {
+constexpr uint32_t join_block = 256, chunk = 64;
+// Blocks of the sums from which the chunks have a kernel of their own, which costs 2.5 to 4 us: without and with it, us, 130k indices into 40 rows of
+// 2,048 bfloat16 (2,032 blocks) 157 and 166 over even rows, 198 and 165 where one row has half of them; 200k into 50k of 1,024 (3,907) 136 and 139,
+// 181 and 150, and with one row for all 212 and 143.
+constexpr uint32_t chunks_from = 2048;
+
+// The last of closed[floor, at) that is set, or floor and `found` unset. Every wave looks at 256 at once.
+__device__ __forceinline__ uint32_t last_closed(const uint32_t* closed, uint32_t floor, uint32_t at, bool& found) {
+    const uint32_t lane = threadIdx.x & 63u;
+    while (at > floor) {
+        uint32_t flag[4];
 #pragma unroll
-        for (int j = 0; j < W; j++) sum[j] += a.tails[k * stride + piece + j];
+        for (uint32_t j = 0; j < 4; j++) flag[j] = closed[max(at, floor + 1u + j * 64u + lane) - 1u - j * 64u - lane];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const uint64_t ends = __ballot(j * 64u + lane < at - floor && flag[j] != 0);
+            if (ends) {
+                found = true;
+                return at - j * 64u - static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(ends)));
+            }
+        }
+        at = at - floor > 256 ? at - 256 : floor;
     }
+    return floor;
+}
+
+// adds what this thread's part of the block has of tails[from, to)
+template <int W, int G>
+__device__ __forceinline__ void add_tails(const float* tails, uint64_t stride, uint32_t from, uint32_t to, float* sum) {
+#pragma unroll 8
+    for (uint32_t k = from + threadIdx.x / G; k < to; k += join_block / G) {
+#pragma unroll
+        for (int j = 0; j < W; j++) sum[j] += tails[k * stride + j];
+    }
+}
+
+// the sum over the block's parts, in its first G threads
+template <int W, int G>
+__device__ __forceinline__ void sum_parts(float* sum) {
+    __shared__ float parts[join_block / 64][G * W];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
     for (uint32_t o = G; o < 64; o <<= 1) {
 #pragma unroll
         for (int j = 0; j < W; j++) sum[j] += __shfl_xor(sum[j], o);
     }
-    if (part == 0 && slot < a.row_lanes) {
+    if (lane < G) {
+#pragma unroll
+        for (int j = 0; j < W; j++) parts[wave][lane * W + j] = sum[j];
+    }
+    __syncthreads();
+    if (threadIdx.x >= G) return;
+#pragma unroll
+    for (uint32_t w = 1; w < join_block / 64; w++)
+#pragma unroll
+        for (int j = 0; j < W; j++) sum[j] += parts[w][lane * W + j];
+}
+
+// Long lists: what is open at the end of every 64 blocks.
+template <int W, int G>
+__global__ __launch_bounds__(join_block) void embedding_chunk_kernel(SumArgs a) {
+    const uint32_t lane = threadIdx.x & 63u, first = blockIdx.x * chunk, count = min(chunk, a.blocks - first);
+    const uint64_t ends = __ballot(lane < count && a.closed[first + min(lane, count - 1u)] != 0);
+    const uint32_t from = ends ? first + 63u - static_cast<uint32_t>(__clzll(ends)) : first;
+    const uint32_t slot = blockIdx.y * G + threadIdx.x % G;
+    const uint64_t stride = static_cast<uint64_t>(gridDim.y) * G * W, piece = static_cast<uint64_t>(slot) * W;
+    float sum[W] = {};
+    add_tails<W, G>(a.tails + piece, stride, from, first + count, sum);
+    sum_parts<W, G>(sum);
+    if (threadIdx.x < G) {
+#pragma unroll
+        for (int j = 0; j < W; j++) a.chunk_tails[blockIdx.x * stride + piece + j] = sum[j];
+    }
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.chunk_closed[blockIdx.x] = ends != 0;
+}
+
+// A block per block of the sums and tile of columns: the row that was open at that block's start, if it ends there, from
+// the open sums of the blocks before it since the last end of a row, and the block's own first piece. In long lists the blocks
+// of earlier chunks stand summed, so that a row that most indices name is two short chains. (One wave, one block
+// of the sums after another, took 397 us for 200k indices of one row of 1,024 bfloat16 where even rows took 135; 143 now, 139 even.)
+template <typename T, int W, bool STREAM, int G>
+__global__ __launch_bounds__(join_block) void embedding_join_kernel(SumArgs a) {
+    const uint32_t b = blockIdx.x;
+    if (!a.closed[b]) return;
+    const uint32_t slot = blockIdx.y * G + threadIdx.x % G;
+    const uint64_t stride = static_cast<uint64_t>(gridDim.y) * G * W, piece = static_cast<uint64_t>(slot) * W;
+    float sum[W] = {};
+    bool found = false;
+    const uint32_t from = last_closed(a.closed, a.chunk_closed ? b / chunk * chunk : 0u, b, found);
+    add_tails<W, G>(a.tails + piece, stride, from, b, sum);
+    if (a.chunk_closed && !found) add_tails<W, G>(a.chunk_tails + piece, stride, last_closed(a.chunk_closed, 0u, b / chunk, found), b / chunk, sum);
+    sum_parts<W, G>(sum);
+    if (threadIdx.x < G && slot < a.row_lanes) {
 #pragma unroll
         for (int j = 0; j < W; j++) sum[j] += a.heads[b * stride + piece + j];
         store_part<T, W, STREAM>(static_cast<T*>(a.gradient) + static_cast<uint64_t>(a.first_row[b]) * a.columns + min(slot * W, a.columns - W), sum, a.scale);
@@ -1001,6 +1065,8 @@ struct GradientLayout {
     float* tails;
     uint32_t* closed;
     uint32_t* first_row;
+    float* chunk_tails = nullptr;
+    uint32_t* chunk_closed = nullptr;
     size_t bytes;
 
     static GradientLayout carve(char* base, const EmbeddingArgs& a) {
@@ -1019,6 +1085,10 @@ struct GradientLayout {
         l.tails = reinterpret_cast<float*>(take(blocks * piece));
         l.closed = reinterpret_cast<uint32_t*>(take(blocks * 4));
         l.first_row = reinterpret_cast<uint32_t*>(take(blocks * 4));
+        if (blocks > chunks_from) {
+            l.chunk_tails = reinterpret_cast<float*>(take(div_up(blocks, chunk) * piece));
+            l.chunk_closed = reinterpret_cast<uint32_t*>(take(size_t{div_up(blocks, chunk)} * 4));
+        }
         l.bytes = used;
         return l;
     }
@@ -1028,7 +1098,8 @@ template <typename T, int W, bool STREAM, int G>
 void launch_sums(const SumArgs& a, hipStream_t s) {
     const uint32_t tiles = div_up(a.row_lanes, G);
     embedding_sum_kernel<T, W, STREAM, G><<<dim3(a.blocks, tiles), sum_block, 0, s>>>(a);
-    embedding_join_kernel<T, W, STREAM, G><<<dim3(a.blocks, tiles), 64, 0, s>>>(a);
+    if (a.chunk_closed) embedding_chunk_kernel<W, G><<<dim3(div_up(a.blocks, chunk), tiles), join_block, 0, s>>>(a);
+    embedding_join_kernel<T, W, STREAM, G><<<dim3(a.blocks, tiles), join_block, 0, s>>>(a);
 }
 
 }  // namespace
@@ -1126,6 +1197,8 @@ bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uin
     u.tails = l.tails;
     u.closed = l.closed;
     u.first_row = l.first_row;
+    u.chunk_tails = l.chunk_tails;
+    u.chunk_closed = l.chunk_closed;
     u.n = a.n;
     u.rows = a.rows;
     u.columns = a.columns;

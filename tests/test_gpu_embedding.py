@@ -118,6 +118,25 @@ def test_one_row_met_by_nearly_all_of_a_larger_table(rows):
     _check_gradient(got, indices, grad, rows, 0.5, 'f32')
 
 
+@pytest.mark.parametrize('n, rows, columns, dtype', [(131_002, 70, 130, 'f32'), (131_003, 70, 130, 'f32'), (131_066, 70, 513, 'bf16'), (150_000, 5000, 256, 'f32'), (300_001, 5000, 130, 'f32')])
+@pytest.mark.parametrize('hot, share', [(0, 1.0), (69, 1.0), (17, 0.97), (17, 0.5), (5, 0.1)])
+def test_rows_that_run_over_many_blocks(n, rows, columns, dtype, hot, share):
+    """Small whole numbers, whose sums are exact in any order: a part of a row that is lost or counted twice shows. (The sums are of less
+    than 2^24 in float32; bfloat16 rounds them once.) Lists of 131,072 entries and rows on begin the sum in chunks."""
+    import efgs
+    print(f'case embedding hot n={n} rows={rows} columns={columns} {dtype} hot={hot} share={share}', flush=True)
+    generator = torch.Generator(device=DEVICE).manual_seed(n + hot)
+    indices = torch.randint(-1, rows + 1, (n,), device=DEVICE, generator=generator)
+    indices[torch.rand(n, device=DEVICE, generator=generator) < share] = hot
+    grad = torch.randint(-4, 8, (n, columns), device=DEVICE, generator=generator)
+    table = torch.zeros(rows, columns, dtype=TYPES[dtype][0], device=DEVICE, requires_grad=True)
+    efgs.embedding(indices, table).backward(grad.to(table.dtype))
+    others = (indices >= 0) & (indices < rows) & (indices != hot)
+    want = torch.zeros(rows, columns, dtype=torch.float64, device=DEVICE).index_add_(0, indices[others], grad[others].double())
+    want[hot] = grad[indices == hot].sum(0).double()
+    assert torch.equal(table.grad, want.to(table.dtype))
+
+
 def test_hot_row_between_empty_ones():
     import efgs
     n, rows = 50_000, 9000
