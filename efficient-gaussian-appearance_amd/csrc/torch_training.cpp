@@ -66,11 +66,18 @@ struct Embedding : torch::autograd::Function<Embedding> {
         return first_order_only(std::move(grads), upstream[0]);
     }
 
-    static Tensor gradient(AutogradContext* ctx, const Tensor& indices, const Tensor& upstream) {
-        const at::Device device = indices.device();
-        const c10::DeviceGuard guard(device);
-        const Tensor grad_out = upstream.contiguous();
+    static Tensor gradient(AutogradContext* ctx, const Tensor& saved, const Tensor& upstream) {
         const int64_t rows = ctx->saved_data["rows"].toInt(), columns = ctx->saved_data["columns"].toInt();
+        // (a node called directly is given whatever its caller has, and hooks on saved tensors return what they like)
+        const at::Device device = upstream.device();
+        TORCH_CHECK_VALUE(device.is_cuda() && saved.device() == device && (saved.scalar_type() == at::kInt || saved.scalar_type() == at::kLong),
+                          "efgs: the embedding's indices must be int32 or int64 on the gradient's device, got ", saved.dtype(), " on ", saved.device());
+        std::vector<int64_t> shape = saved.sizes().vec();
+        shape.push_back(columns);
+        TORCH_CHECK_VALUE(upstream.sizes() == at::IntArrayRef(shape), "efgs: the embedding's gradient must have the output's shape ", at::IntArrayRef(shape),
+                          ", got ", upstream.sizes());
+        const c10::DeviceGuard guard(device);
+        const Tensor indices = saved.contiguous(), grad_out = upstream.contiguous();
         const Tensor out = at::empty({rows, columns}, grad_out.options());
         Workspace workspace(Workspace::embedding, device);
         check_status(efgs_embedding_backward(indices.numel() > 0 ? indices.data_ptr() : nullptr, static_cast<int>(indices.element_size()),
