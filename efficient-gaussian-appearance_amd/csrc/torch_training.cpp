@@ -359,6 +359,7 @@ std::vector<std::pair<Tensor, Tensor>> adamw_moments(const py::list& params, con
             out.emplace_back(tensor_entry(state, exp_avg_name, param, at::kFloat, n), tensor_entry(state, exp_avg_sq_name, param, at::kFloat, n));
             continue;
         }
+        TORCH_CHECK_VALUE(param.device().is_cuda(), "efgs: AdamW: 8-bit states are read on a GPU device, got ", param.device());
         TORCH_CHECK_VALUE(!device || param.device() == *device, "efgs: AdamW: all parameters must live on one device");
         device = param.device();
         const auto options = at::TensorOptions().dtype(at::kFloat).device(param.device());
