@@ -89,6 +89,9 @@ class AdamW(torch.optim.Optimizer):
 
 
 def _check_group(group: dict[str, Any]) -> None:
+    # (a launch's blocks update all tensors at once)
+    if len({id(p) for p in group['params']}) != len(group['params']):
+        raise ValueError('efgs: a parameter group holds a parameter more than once')
     lr = group['lr']
     if isinstance(lr, (list, tuple)) and not 1 <= len(lr) <= 7:
         raise ValueError('efgs: between 1 and 7 learning rates are supported')

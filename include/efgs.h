@@ -295,7 +295,8 @@ enum { EFGS_FLOAT = 0, EFGS_BFLOAT16 = 1, EFGS_HALF = 2 };
  * of these bits, u's sign the code's top bit. ratio_bound is efgs_adamw_ratio_bound of the betas with which the
  * state was written (the step writes it for its group's betas; ratios past a smaller bound become that bound), and needs beta1^2 < beta2. Codes are rounded by a dither from (element, step,
  * seed), unbiased; results do not depend on the tensors that share a call. An element whose new v is not finite has a zero state.
- * Tensors are contiguous, of any alignment of their type. Stream-ordered; nothing is kept of the arguments. */
+ * Tensors are contiguous, of any alignment of their type, and none that is written overlaps another: all are updated at once.
+ * Stream-ordered; nothing is kept of the arguments. */
 typedef struct efgs_adamw_group {
     double lrs[7];
     double beta1, beta2, eps, weight_decay;

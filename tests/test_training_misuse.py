@@ -18,3 +18,16 @@ def test_moments_of_coded_states_on_the_host_are_refused():
     for params in (p, [p]):
         with pytest.raises(ValueError, match='GPU'):
             opt.moments(params)
+
+
+def test_a_parameter_twice_in_a_group_is_refused():
+    """Blocks of one launch would update the same elements at once."""
+    import efgs
+    p, q = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    with pytest.raises(ValueError, match='more than once'):
+        efgs.AdamW([p, q, p])
+    opt = efgs.AdamW([p])
+    with pytest.raises(ValueError, match='more than once'):
+        opt.add_param_group({'params': [q, q]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({'params': [q]})
