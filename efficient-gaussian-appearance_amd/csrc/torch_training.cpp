@@ -97,6 +97,8 @@ Tensor embedding(const Tensor& indices, const Tensor& table, double scale, const
     TORCH_CHECK_VALUE(table.device().is_cuda(), "efgs: the table must be on a GPU device, got ", table.device());
     TORCH_CHECK_VALUE(indices.device() == table.device(), "efgs: indices are on ", indices.device(), ", expected ", table.device());
     TORCH_CHECK_VALUE(std::isfinite(scale), "efgs: the embedding scale must be finite");
+    // (a lookup that needs no graph passes the autograd function by, which would refuse: its result would have lost the tangent)
+    TORCH_CHECK_NOT_IMPLEMENTED(!table._fw_grad(/*level=*/0).defined(), "efgs: embedding has no forward-mode derivative");
     Rows r;
     r.type = element_type("the table", table.scalar_type());
     r.rows = table.size(0);

@@ -41,3 +41,17 @@ def test_embedding_node_checks_what_hooks_give_back():
     with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x.t().contiguous().t()):
         out = efgs.embedding(indices, table)
     assert torch.equal(torch.autograd.grad(out, table, upstream)[0], want)
+
+
+@pytest.mark.parametrize('requires_grad', [False, True])
+@pytest.mark.parametrize('grad_mode', [False, True])
+def test_embedding_of_a_dual_number_is_refused(requires_grad, grad_mode):
+    """There is no forward-mode derivative: an error, as the rasterizer's, and no result without a tangent."""
+    import efgs
+    from torch.autograd import forward_ad
+    indices = torch.randint(0, 9, (5,), device=DEVICE)
+    table = torch.randn(9, 4, device=DEVICE, requires_grad=requires_grad)
+    with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            efgs.embedding(indices, forward_ad.make_dual(table, torch.ones_like(table)))
+        assert efgs.embedding(indices, table).shape == (5, 4)
