@@ -166,8 +166,8 @@ __device__ __forceinline__ float clipping(float norm, float max_grad_norm) {
 }
 
 // The parameter after the step. The reciprocal is the hardware's (1 ulp): the division's last bit would be
-// 6e-8 of the update, for about ten operations an element. root is 0 or at least 3e-23, a float's least square root, so that
-// the sum is no denormal unless eps alone is one.
+// 6e-8 of the update, for about ten operations an element. root is 0 or at least 3e-23, a float's least square root, and eps, as
+// the host hands it over, 0 or a normal float, so that the sum is no denormal.
 __device__ __forceinline__ float updated(const AdamWGroupDevice& G, float p, float m, float root, float rate, float decay) {
     const float update = m * __builtin_amdgcn_rcpf(root * G.root_factor + G.eps);
     return p * decay - rate * update;

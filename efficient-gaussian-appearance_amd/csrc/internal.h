@@ -233,7 +233,7 @@ struct AdamWTensor8 : AdamWTensor {
 struct AdamWGroupDevice {
     float rates[adam_max_lrs], decays[adam_max_lrs];  // lr / (1 - beta1^t), 1 - lr wd
     float beta1, beta1_rest, beta2, beta2_rest, eps;
-    float root_factor;      // 1 / sqrt(1 - beta2^t)
+    float root_factor;      // 1 / sqrt(1 - beta2^t); rates, eps and this one times 2^32 where eps is no normal float
     float ratio_encode;     // 8-bit: the top code's value over the bound of u
     float ratio_decode;     // 8-bit: bound of u when the state was coded over its top code's value
     uint32_t key;           // 8-bit: dither key of the step

@@ -45,7 +45,11 @@ const char* group_fault(const efgs_adamw_group& g) {
 
 AdamWGroupDevice device_group(const efgs_adamw_group& g, int64_t step, double ratio_bound, uint32_t seed) {
     AdamWGroupDevice d{};
-    const double step_factor = 1.0 / (1.0 - std::pow(g.beta1, static_cast<double>(step)));
+    // An eps below the normal floats has no reciprocal in the hardware (0 times it would be no number for zero moments): the quotient's
+    // denominator is held times 2^32 then, and at least the least float, and so is the rate.
+    const bool tiny = g.eps > 0.0 && g.eps < 0x1p-126;
+    const double eps = tiny ? std::fmax(g.eps, 0x1p-149) : g.eps, factor = tiny ? 0x1p32 : 1.0;
+    const double step_factor = factor / (1.0 - std::pow(g.beta1, static_cast<double>(step)));
     for (int k = 0; k < g.n_lrs; k++) {
         d.rates[k] = static_cast<float>(g.lrs[k] * step_factor);
         d.decays[k] = static_cast<float>(1.0 - g.lrs[k] * g.weight_decay);
@@ -55,8 +59,8 @@ AdamWGroupDevice device_group(const efgs_adamw_group& g, int64_t step, double ra
     d.beta1_rest = static_cast<float>(1.0 - g.beta1);
     d.beta2 = static_cast<float>(g.beta2);
     d.beta2_rest = static_cast<float>(1.0 - g.beta2);
-    d.eps = static_cast<float>(g.eps);
-    d.root_factor = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(g.beta2, static_cast<double>(step))));
+    d.eps = static_cast<float>(eps * factor);
+    d.root_factor = static_cast<float>(factor / std::sqrt(1.0 - std::pow(g.beta2, static_cast<double>(step))));
     if (g.state_bits == 8) {
         d.ratio_encode = static_cast<float>(adamw_ratio_top / efgs_adamw_ratio_bound(g.beta1, g.beta2));
         d.ratio_decode = static_cast<float>(ratio_bound / adamw_ratio_top);

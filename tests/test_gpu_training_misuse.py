@@ -55,3 +55,30 @@ def test_embedding_of_a_dual_number_is_refused(requires_grad, grad_mode):
         with pytest.raises((RuntimeError, NotImplementedError)):
             efgs.embedding(indices, forward_ad.make_dual(table, torch.ones_like(table)))
         assert efgs.embedding(indices, table).shape == (5, 4)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('eps', [1e-38, 2e-39, 1e-42, 2.0 ** -149, 1e-60])
+def test_eps_below_the_least_reciprocal(bits, eps):
+    """The reciprocal of an eps below 2^-128 is no float, yet the formula is: a parameter whose moments are zero keeps to its decay, one whose
+    m is not zero and whose v underflows moves by lr m / eps (an eps below float32's least number counts as that), and to
+    ordinary gradients the eps is nothing. Bars: e = 2^-24; 4 e of p and of the update for the ordinary ones, 16 e for m / eps."""
+    import efgs
+    e, n, lr, decay = 2.0 ** -24, 700, 1e-3, 0.05
+    kept = {}
+    for value in (eps, 1e-33):
+        p = torch.linspace(-2.0, 2.0, n, device=DEVICE).requires_grad_()
+        p0 = p.detach().clone()
+        generator = torch.Generator(DEVICE).manual_seed(3)
+        p.grad = torch.randn(n, generator=generator, device=DEVICE) * 0.1
+        p.grad[256:512] = 0.0
+        p.grad[520] = 1e-24
+        opt = efgs.AdamW([p], lr=lr, weight_decay=decay, eps=value, state_bits=bits)
+        opt.step()
+        kept[value] = p.detach().double()
+    now, other, p0 = kept[eps], kept[1e-33], p0.double()
+    assert bool(((now - p0 * (1 - lr * decay)).abs() <= 3 * e * p0.abs())[256:512].all())
+    ordinary = torch.arange(n, device=DEVICE) != 520
+    assert bool(((now - other).abs() <= 4 * e * (p0.abs() + lr))[ordinary].all())
+    want = float(p0[520]) * (1 - lr * decay) - lr * float(torch.tensor(1e-24)) / max(eps, 2.0 ** -149)
+    assert float(now[520]) == pytest.approx(want, rel=16 * e)
