@@ -45,6 +45,10 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm: torch.Tensor | None = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
+    def __getstate__(self) -> dict[str, Any]:
+        # (of an optimizer the base class copies and pickles its groups and states alone)
+        return {**super().__getstate__(), 'max_grad_norm': self.max_grad_norm, 'seed': self.seed, 'grad_norm': self.grad_norm}
+
     def add_param_group(self, param_group: dict[str, Any]) -> None:
         super().add_param_group(param_group)
         try:

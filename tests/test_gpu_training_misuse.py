@@ -82,3 +82,22 @@ def test_eps_below_the_least_reciprocal(bits, eps):
     assert bool(((now - other).abs() <= 4 * e * (p0.abs() + lr))[ordinary].all())
     want = float(p0[520]) * (1 - lr * decay) - lr * float(torch.tensor(1e-24)) / max(eps, 2.0 ** -149)
     assert float(now[520]) == pytest.approx(want, rel=16 * e)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_copied_optimizer_goes_on_bit_for_bit(bits):
+    """A model and its optimizer copied together, and pickled together."""
+    import copy
+    import pickle
+    import efgs
+    p = torch.randn(1500, device=DEVICE).requires_grad_()
+    p.grad = torch.randn(1500, device=DEVICE)
+    opt = efgs.AdamW([p], state_bits=bits, max_grad_norm=0.5, seed=3)
+    opt.step()
+    copies = [copy.deepcopy((p, opt)), pickle.loads(pickle.dumps((p, opt)))]
+    opt.step()
+    for q, other in copies:
+        q.grad = p.grad.clone()
+        other.step()
+        assert torch.equal(q, p) and float(other.grad_norm) == float(opt.grad_norm)
+        assert all(torch.equal(x, y) for x, y in zip(other.moments(q), opt.moments(p)))

@@ -31,3 +31,21 @@ def test_a_parameter_twice_in_a_group_is_refused():
         opt.add_param_group({'params': [q, q]})
     assert len(opt.param_groups) == 1
     opt.add_param_group({'params': [q]})
+
+
+def test_copies_and_pickles_of_an_optimizer_keep_its_settings():
+    import copy
+    import io
+    import pickle
+    import efgs
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = efgs.AdamW([p], state_bits=8, max_grad_norm=0.5, seed=11)
+    opt.grad_norm = torch.tensor(2.0)
+    saved = io.BytesIO()
+    torch.save(opt, saved)
+    saved.seek(0)
+    for other in (copy.deepcopy(opt), copy.copy(opt), pickle.loads(pickle.dumps(opt)), torch.load(saved, weights_only=False)):
+        assert other.max_grad_norm == 0.5 and other.seed == 11 and float(other.grad_norm) == 2.0
+        assert other.param_groups[0]['state_bits'] == 8
+        other.step()                # no gradients: nothing to do
+        assert other.grad_norm is None
