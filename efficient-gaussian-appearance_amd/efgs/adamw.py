@@ -38,8 +38,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params: Iterable, lr: float | Sequence[float] = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, max_grad_norm: float | None = None, seed: int = 0) -> None:
-        if max_grad_norm is not None and not max_grad_norm > 0.0:
-            raise ValueError(f'efgs: max_grad_norm must be positive, got {max_grad_norm}')
+        _check_max_norm(max_grad_norm)
         self.max_grad_norm = max_grad_norm
         self.seed = int(seed)
         self.grad_norm: torch.Tensor | None = None
@@ -73,8 +72,16 @@ class AdamW(torch.optim.Optimizer):
             return _native.adamw_moments([params], self.state)[0]
         return _native.adamw_moments(list(params), self.state)
 
+    def state_dict(self) -> dict[str, Any]:
+        """The base class's entries, and `seed` and `max_grad_norm`."""
+        return {**super().state_dict(), 'seed': self.seed, 'max_grad_norm': self.max_grad_norm}
+
     def load_state_dict(self, state_dict: dict[str, Any]) -> None:
+        """Goes on where the saved optimizer stood: with its groups' values, and its `seed` and `max_grad_norm` if they are saved."""
+        _check_max_norm(state_dict.get('max_grad_norm'))
         super().load_state_dict(state_dict)
+        self.seed = int(state_dict.get('seed', self.seed))
+        self.max_grad_norm = state_dict.get('max_grad_norm', self.max_grad_norm)
         # (the base class casts every floating state to its parameter's type, and bytes too)
         saved_ids = [i for g in state_dict['param_groups'] for i in g['params']]
         params = [p for g in self.param_groups for p in g['params']]
@@ -90,6 +97,11 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     own[key] = copy.deepcopy(value)
             self.state[p] = own
+
+
+def _check_max_norm(max_grad_norm: float | None) -> None:
+    if max_grad_norm is not None and not max_grad_norm > 0.0:
+        raise ValueError(f'efgs: max_grad_norm must be positive, got {max_grad_norm}')
 
 
 def _check_group(group: dict[str, Any]) -> None:

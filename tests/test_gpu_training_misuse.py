@@ -101,3 +101,20 @@ def test_a_copied_optimizer_goes_on_bit_for_bit(bits):
         other.step()
         assert torch.equal(q, p) and float(other.grad_norm) == float(opt.grad_norm)
         assert all(torch.equal(x, y) for x, y in zip(other.moments(q), opt.moments(p)))
+
+
+def test_a_resumed_run_of_8_bit_states_is_the_same_run():
+    """The dither of a resumed optimizer is the saved one's, whatever seed it was made with."""
+    import copy
+    import efgs
+    p = torch.randn(1500, device=DEVICE).requires_grad_()
+    p.grad = torch.randn(1500, device=DEVICE)
+    opt = efgs.AdamW([p], state_bits=8, max_grad_norm=0.5, seed=3)
+    opt.step()
+    q = p.detach().clone().requires_grad_()
+    q.grad = p.grad.clone()
+    other = efgs.AdamW([q], state_bits=8)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    opt.step()
+    other.step()
+    assert torch.equal(q, p) and all(torch.equal(x, y) for x, y in zip(other.moments(q), opt.moments(p)))

@@ -49,3 +49,21 @@ def test_copies_and_pickles_of_an_optimizer_keep_its_settings():
         assert other.param_groups[0]['state_bits'] == 8
         other.step()                # no gradients: nothing to do
         assert other.grad_norm is None
+
+
+def test_a_saved_state_holds_the_seed_and_the_clipping_bound():
+    """As a learning rate they are taken from what is loaded; saved states without them leave the optimizer's own."""
+    import efgs
+    p = torch.nn.Parameter(torch.zeros(3))
+    saved = efgs.AdamW([p], max_grad_norm=0.5, seed=11).state_dict()
+    assert saved['seed'] == 11 and saved['max_grad_norm'] == 0.5
+    other = efgs.AdamW([p], max_grad_norm=2.0, seed=12)
+    other.load_state_dict({k: saved[k] for k in ('state', 'param_groups')})
+    assert other.seed == 12 and other.max_grad_norm == 2.0
+    other.load_state_dict(saved)
+    assert other.seed == 11 and other.max_grad_norm == 0.5
+    other.load_state_dict(efgs.AdamW([p]).state_dict())
+    assert other.seed == 0 and other.max_grad_norm is None
+    with pytest.raises(ValueError, match='max_grad_norm'):
+        other.load_state_dict({**saved, 'max_grad_norm': -1.0})
+    assert other.seed == 0 and other.max_grad_norm is None
