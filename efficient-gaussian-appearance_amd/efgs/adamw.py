@@ -77,8 +77,12 @@ class AdamW(torch.optim.Optimizer):
         return {**super().state_dict(), 'seed': self.seed, 'max_grad_norm': self.max_grad_norm}
 
     def load_state_dict(self, state_dict: dict[str, Any]) -> None:
-        """Goes on where the saved optimizer stood: with its groups' values, and its `seed` and `max_grad_norm` if they are saved."""
+        """Goes on where the saved optimizer stood: with its groups' values, and its `seed` and `max_grad_norm` if they are saved.
+        torch.optim.AdamW's saved states are taken too (as 32-bit ones), not with amsgrad or maximize."""
         _check_max_norm(state_dict.get('max_grad_norm'))
+        state_dict = {**state_dict, 'param_groups': [{'state_bits': 32, **g} for g in state_dict['param_groups']]}
+        for group in state_dict['param_groups']:
+            _check_group(group)
         super().load_state_dict(state_dict)
         self.seed = int(state_dict.get('seed', self.seed))
         self.max_grad_norm = state_dict.get('max_grad_norm', self.max_grad_norm)
@@ -108,6 +112,12 @@ def _check_group(group: dict[str, Any]) -> None:
     # (a launch's blocks update all tensors at once)
     if len({id(p) for p in group['params']}) != len(group['params']):
         raise ValueError('efgs: a parameter group holds a parameter more than once')
+    for key in ('lr', 'betas', 'eps', 'weight_decay', 'state_bits'):
+        if key not in group:
+            raise ValueError(f'efgs: a parameter group lacks {key}')
+    # (of saved groups of torch's optimizers)
+    if group.get('amsgrad') or group.get('maximize') or group['weight_decay'] and not group.get('decoupled_weight_decay', True):
+        raise ValueError('efgs: AdamW has no amsgrad, no maximize and no weight decay through the gradient')
     lr = group['lr']
     if isinstance(lr, (list, tuple)) and not 1 <= len(lr) <= 7:
         raise ValueError('efgs: between 1 and 7 learning rates are supported')

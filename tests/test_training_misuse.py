@@ -67,3 +67,31 @@ def test_a_saved_state_holds_the_seed_and_the_clipping_bound():
     with pytest.raises(ValueError, match='max_grad_norm'):
         other.load_state_dict({**saved, 'max_grad_norm': -1.0})
     assert other.seed == 0 and other.max_grad_norm is None
+
+
+def test_saved_states_of_torch_optimizers():
+    """torch.optim.AdamW's are taken as they are, whose groups know no state_bits: 32, which their states have. Those of another formula
+    (amsgrad, maximize, weight decay through the gradient) or without what a group needs are refused, and change nothing."""
+    import efgs
+    p = torch.nn.Parameter(torch.randn(4, 3))
+    theirs = torch.optim.AdamW([p], lr=0.25, betas=(0.8, 0.9), eps=1e-5, weight_decay=0.125)
+    p.grad = torch.randn(4, 3)
+    theirs.step()
+    q = torch.nn.Parameter(torch.zeros(4, 3))
+    for bits in (32, 8):
+        ours = efgs.AdamW([q], state_bits=bits)
+        ours.load_state_dict(theirs.state_dict())
+        group, state = ours.param_groups[0], ours.state[q]
+        assert (group['lr'], tuple(group['betas']), group['eps'], group['weight_decay'], group['state_bits']) == (0.25, (0.8, 0.9), 1e-5, 0.125, 32)
+        assert state['step'] == 1 and isinstance(state['step'], int)
+        assert torch.equal(state['exp_avg'], theirs.state[p]['exp_avg']) and torch.equal(state['exp_avg_sq'], theirs.state[p]['exp_avg_sq'])
+    ours = efgs.AdamW([q], lr=0.5)
+    ours.load_state_dict(torch.optim.Adam([p], weight_decay=0.0).state_dict())
+    ours = efgs.AdamW([q], lr=0.5)
+    for other in (torch.optim.AdamW([p], amsgrad=True), torch.optim.AdamW([p], maximize=True), torch.optim.Adam([p], weight_decay=0.1),
+                  torch.optim.SGD([p], lr=0.1)):
+        with pytest.raises(ValueError, match='efgs'):
+            ours.load_state_dict(other.state_dict())
+        assert ours.param_groups[0]['lr'] == 0.5 and len(ours.state) == 0
+    with pytest.raises(ValueError, match='amsgrad'):
+        efgs.AdamW([{'params': [q], 'amsgrad': True}])
