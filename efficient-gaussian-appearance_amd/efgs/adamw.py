@@ -97,7 +97,7 @@ class AdamW(torch.optim.Optimizer):
                 if key == 'step':
                     own[key] = int(value)
                 elif isinstance(value, torch.Tensor):
-                    own[key] = value.detach().to(p.device).clone()
+                    own[key] = value.detach().to(p.device).clone(memory_format=torch.contiguous_format)
                 else:
                     own[key] = copy.deepcopy(value)
             self.state[p] = own

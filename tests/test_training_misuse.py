@@ -95,3 +95,16 @@ def test_saved_states_of_torch_optimizers():
         assert ours.param_groups[0]['lr'] == 0.5 and len(ours.state) == 0
     with pytest.raises(ValueError, match='amsgrad'):
         efgs.AdamW([{'params': [q], 'amsgrad': True}])
+
+
+def test_saved_states_of_other_strides_are_laid_out_anew():
+    import efgs
+    p = torch.nn.Parameter(torch.zeros(4, 3))
+    saved = efgs.AdamW([p]).state_dict()
+    moments = torch.arange(12.0).view(3, 4).t()
+    saved['state'] = {0: dict(step=torch.tensor(5.0), exp_avg=moments, exp_avg_sq=moments + 1)}
+    opt = efgs.AdamW([p])
+    opt.load_state_dict(saved)
+    for key, want in (('exp_avg', moments), ('exp_avg_sq', moments + 1)):
+        assert opt.state[p][key].is_contiguous() and torch.equal(opt.state[p][key], want)
+    assert opt.state[p]['step'] == 5
