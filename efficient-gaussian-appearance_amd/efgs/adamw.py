@@ -79,21 +79,34 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict[str, Any]) -> None:
         """Goes on where the saved optimizer stood: with its groups' values, and its `seed` and `max_grad_norm` if they are saved.
         torch.optim.AdamW's saved states are taken too (as 32-bit ones), not with amsgrad or maximize."""
-        _check_max_norm(state_dict.get('max_grad_norm'))
-        state_dict = {**state_dict, 'param_groups': [{'state_bits': 32, **g} for g in state_dict['param_groups']]}
-        for group in state_dict['param_groups']:
-            _check_group(group)
-        super().load_state_dict(state_dict)
-        self.seed = int(state_dict.get('seed', self.seed))
-        self.max_grad_norm = state_dict.get('max_grad_norm', self.max_grad_norm)
+        loaded: dict[str, Any] = {}
+
+        def take(_: AdamW, given: dict[str, Any]) -> dict[str, Any]:
+            _check_max_norm(given.get('max_grad_norm'))
+            loaded.update(given, param_groups=[{'state_bits': 32, **g} for g in given['param_groups']])
+            for group in loaded['param_groups']:
+                _check_group(group)
+            return loaded
+
+        # behind the hooks that a program has registered, and before those that it has for the end
+        hooks = [self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(lambda _: self._take_states(loaded), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_states(self, loaded: dict[str, Any]) -> None:
         # (the base class casts every floating state to its parameter's type, and bytes too)
-        saved_ids = [i for g in state_dict['param_groups'] for i in g['params']]
+        self.seed = int(loaded.get('seed', self.seed))
+        self.max_grad_norm = loaded.get('max_grad_norm', self.max_grad_norm)
+        saved_ids = [i for g in loaded['param_groups'] for i in g['params']]
         params = [p for g in self.param_groups for p in g['params']]
         for i, p in zip(saved_ids, params):
-            if i not in state_dict['state']:
+            if i not in loaded['state']:
                 continue
             own = {}
-            for key, value in state_dict['state'][i].items():
+            for key, value in loaded['state'][i].items():
                 if key == 'step':
                     own[key] = int(value)
                 elif isinstance(value, torch.Tensor):

@@ -108,3 +108,24 @@ def test_saved_states_of_other_strides_are_laid_out_anew():
     for key, want in (('exp_avg', moments), ('exp_avg_sq', moments + 1)):
         assert opt.state[p][key].is_contiguous() and torch.equal(opt.state[p][key], want)
     assert opt.state[p]['step'] == 5
+
+
+def test_hooks_on_loading_see_and_give_what_is_loaded():
+    """A hook before loading may give another saved state; one behind it sees the states as they stay."""
+    import efgs
+    p = torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16))
+    saved = efgs.AdamW([p], seed=4).state_dict()
+    saved['state'] = {0: dict(step=2, exp_avg=torch.ones(4), exp_avg_sq=torch.ones(4))}
+    opt, seen = efgs.AdamW([p]), []
+    before = opt.register_load_state_dict_pre_hook(
+        lambda _, given: {**given, 'seed': 9, 'state': {0: dict(given['state'][0], step=7, exp_avg=torch.full((4,), 3.0))}})
+    behind = opt.register_load_state_dict_post_hook(lambda o: seen.append((o.state[p]['exp_avg'].dtype, o.state[p]['step'])))
+    opt.load_state_dict(saved)
+    assert opt.state[p]['step'] == 7 and torch.equal(opt.state[p]['exp_avg'], torch.full((4,), 3.0)) and opt.seed == 9
+    assert seen == [(torch.float32, 7)]
+    before.remove()
+    opt.load_state_dict(saved)
+    assert opt.state[p]['step'] == 2 and opt.seed == 4 and len(seen) == 2
+    behind.remove()
+    opt.load_state_dict(saved)
+    assert len(seen) == 2
