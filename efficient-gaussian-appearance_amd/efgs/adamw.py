@@ -4,6 +4,7 @@ the host. No counterpart in the reference, whose optimizer is `FusedAdam` (one f
 from __future__ import annotations
 
 import copy
+import math
 from typing import Any, Callable, Iterable, Sequence
 
 import torch
@@ -121,6 +122,15 @@ def _check_max_norm(max_grad_norm: float | None) -> None:
         raise ValueError(f'efgs: max_grad_norm must be positive, got {max_grad_norm}')
 
 
+def _number(name: str, value: Any) -> float:
+    try:
+        if not isinstance(value, str):  # (which the step does not take)
+            return float(value)
+    except (TypeError, ValueError, RuntimeError):
+        pass
+    raise ValueError(f'efgs: {name} must be a number, got {value!r}')
+
+
 def _check_group(group: dict[str, Any]) -> None:
     # (a launch's blocks update all tensors at once)
     if len({id(p) for p in group['params']}) != len(group['params']):
@@ -131,14 +141,21 @@ def _check_group(group: dict[str, Any]) -> None:
     # (of saved groups of torch's optimizers)
     if group.get('amsgrad') or group.get('maximize') or group['weight_decay'] and not group.get('decoupled_weight_decay', True):
         raise ValueError('efgs: AdamW has no amsgrad, no maximize and no weight decay through the gradient')
-    lr = group['lr']
-    if isinstance(lr, (list, tuple)) and not 1 <= len(lr) <= 7:
+    lr, betas = group['lr'], group['betas']
+    rates = lr if isinstance(lr, (list, tuple)) else [lr]
+    if not 1 <= len(rates) <= 7:
         raise ValueError('efgs: between 1 and 7 learning rates are supported')
-    beta1, beta2 = (float(b) for b in group['betas'])
+    if not all(math.isfinite(_number('lr', rate)) for rate in rates):
+        raise ValueError(f'efgs: learning rates must be finite, got {lr}')
+    if not isinstance(betas, (list, tuple)) or len(betas) != 2:
+        raise ValueError(f'efgs: betas must be two numbers, got {betas}')
+    beta1, beta2 = (_number('betas', b) for b in betas)
     if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
         raise ValueError(f'efgs: betas must lie in [0, 1), got {(beta1, beta2)}')
-    if not float(group['eps']) >= 0.0:
-        raise ValueError(f'efgs: eps must not be negative, got {group["eps"]}')
+    if not 0.0 <= _number('eps', group['eps']) < math.inf:
+        raise ValueError(f'efgs: eps must be finite and not negative, got {group["eps"]}')
+    if not math.isfinite(_number('weight_decay', group['weight_decay'])):
+        raise ValueError(f'efgs: weight_decay must be finite, got {group["weight_decay"]}')
     if group['state_bits'] not in (8, 32):
         raise ValueError(f'efgs: state_bits must be 32 or 8, got {group["state_bits"]}')
     if group['state_bits'] == 8 and not beta1 * beta1 < beta2:

@@ -129,3 +129,26 @@ def test_hooks_on_loading_see_and_give_what_is_loaded():
     behind.remove()
     opt.load_state_dict(saved)
     assert len(seen) == 2
+
+
+@pytest.mark.parametrize('bad', [dict(lr=float('nan')), dict(lr=float('inf')), dict(lr=[1e-3, float('nan')]), dict(lr=torch.tensor([1e-3, 1e-3])), dict(lr='0.1'),
+                                 dict(lr=None), dict(weight_decay=float('nan')), dict(weight_decay=float('-inf')), dict(eps=float('inf')), dict(eps=None),
+                                 dict(betas=(0.9,)), dict(betas=0.9), dict(state_bits='8')])
+def test_values_that_no_step_could_take_are_refused_at_once(bad):
+    import efgs
+    p = torch.nn.Parameter(torch.zeros(3))
+    with pytest.raises(ValueError):
+        efgs.AdamW([p], **bad)
+    with pytest.raises(ValueError):
+        efgs.AdamW([{'params': [p], **bad}])
+    opt = efgs.AdamW([torch.nn.Parameter(torch.zeros(2))])
+    with pytest.raises(ValueError):
+        opt.add_param_group({'params': [p], **bad})
+    assert len(opt.param_groups) == 1
+
+
+def test_values_that_turn_into_numbers_are_taken():
+    import efgs
+    opt = efgs.AdamW([torch.nn.Parameter(torch.zeros(3))], lr=torch.tensor(0.5), betas=[0.5, 0.75], eps=0, weight_decay=1)
+    assert float(opt.param_groups[0]['lr']) == 0.5
+    efgs.AdamW([torch.nn.Parameter(torch.zeros(3))], lr=(1, 2.0, torch.tensor(3.0)))
