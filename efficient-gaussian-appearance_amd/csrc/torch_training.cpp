@@ -273,16 +273,21 @@ c10::optional<Tensor> adamw_step(const py::list& groups, const py::dict& states,
     std::vector<efgs_adamw_group> native_groups;
     c10::optional<at::Device> device;
     for (const py::handle item : groups) {
-        static PyObject* const params_name = PyUnicode_InternFromString("params");
         TORCH_CHECK_VALUE(PyDict_Check(item.ptr()), "efgs: AdamW: a parameter group must be a dict");
+        native_groups.push_back(native_group(item.ptr()));
+    }
+    // (a step over no tensors: the groups' values are checked before states are made by them)
+    check_status(efgs_adamw_step(nullptr, 0, native_groups.data(), static_cast<int>(native_groups.size()), nullptr, 0.0, seed, nullptr));
+    int32_t group = -1;
+    for (const py::handle item : groups) {
+        static PyObject* const params_name = PyUnicode_InternFromString("params");
         PyObject* const params = group_entry(item.ptr(), params_name);
         TORCH_CHECK_VALUE(PyList_Check(params), "efgs: AdamW: a group's parameters must be a list");
         const size_t most = tensors.size() + static_cast<size_t>(PyList_GET_SIZE(params));
         entries.reserve(most);
         tensors.reserve(most);
         norms.reserve(max_grad_norm ? most : 0);
-        native_groups.push_back(native_group(item.ptr()));
-        const efgs_adamw_group& native = native_groups.back();
+        const efgs_adamw_group& native = native_groups[static_cast<size_t>(++group)];
         const int bits = native.state_bits;
         const double bound = bits == 8 ? efgs_adamw_ratio_bound(native.beta1, native.beta2) : 0.0;
         for (Py_ssize_t k = 0; k < PyList_GET_SIZE(params); k++) {
@@ -322,7 +327,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, const py::dict& states,
             t.param = param.data_ptr();
             t.n_elements = n;
             t.step = step_entry(state) + 1;
-            t.group = static_cast<int32_t>(native_groups.size()) - 1;
+            t.group = group;
             if (max_grad_norm) norms.push_back({t.grad, n, t.grad_type, 0});
             tensors.push_back(t);
             entries.push_back({param, state, t.step, written});

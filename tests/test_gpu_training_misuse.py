@@ -118,3 +118,24 @@ def test_a_resumed_run_of_8_bit_states_is_the_same_run():
     opt.step()
     other.step()
     assert torch.equal(q, p) and all(torch.equal(x, y) for x, y in zip(other.moments(q), opt.moments(p)))
+
+
+@pytest.mark.parametrize('change', [dict(betas=(0.95, 0.9)), dict(betas=(0.9, 0.81)), dict(state_bits=16), dict(lr=float('nan')), dict(eps=-1.0)])
+def test_a_refused_group_leaves_no_state_behind(change):
+    """Values that a program set between steps: the refused step makes no states that a later one could not read."""
+    import efgs
+    p, q = (torch.ones(300, device=DEVICE).requires_grad_() for _ in range(2))
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    opt = efgs.AdamW([{'params': [p]}, {'params': [q], 'state_bits': 8}], seed=5)
+    group = opt.param_groups[1]
+    kept = dict(group)
+    group.update(change)
+    with pytest.raises((RuntimeError, ValueError), match='efgs'):
+        opt.step()
+    assert torch.equal(p, torch.ones_like(p)) and len(opt.state) == 0
+    group.update(kept)
+    opt.step()
+    other = torch.ones(300, device=DEVICE).requires_grad_()
+    other.grad = torch.ones_like(other)
+    efgs.AdamW([other], state_bits=8, seed=5).step()
+    assert torch.equal(q, other) and opt.state[q]['step'] == 1
