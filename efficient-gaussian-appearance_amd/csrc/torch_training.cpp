@@ -204,13 +204,17 @@ PyObject* state_of(PyObject* states, PyObject* key, const Tensor& param, int bit
     if (PyDict_GET_SIZE(state) > 0) return state;
     const c10::DeviceGuard guard(param.device());
     const auto options = at::TensorOptions().device(param.device());
+    // (all of them made before the first is kept: memory may run out)
+    const auto type = options.dtype(bits == 32 ? at::kFloat : at::kByte);
+    const Tensor first = at::zeros(param.sizes(), type), second = at::zeros(param.sizes(), type);
     if (bits == 32) {
-        set_entry(state, exp_avg_name, THPVariable_Wrap(at::zeros(param.sizes(), options.dtype(at::kFloat))));
-        set_entry(state, exp_avg_sq_name, THPVariable_Wrap(at::zeros(param.sizes(), options.dtype(at::kFloat))));
+        set_entry(state, exp_avg_name, THPVariable_Wrap(first));
+        set_entry(state, exp_avg_sq_name, THPVariable_Wrap(second));
     } else {
-        set_entry(state, ratio_name, THPVariable_Wrap(at::zeros(param.sizes(), options.dtype(at::kByte))));
-        set_entry(state, root_name, THPVariable_Wrap(at::zeros(param.sizes(), options.dtype(at::kByte))));
-        set_entry(state, scale_name, THPVariable_Wrap(at::zeros({blocks_of(param.numel())}, options.dtype(at::kFloat))));
+        const Tensor scale = at::zeros({blocks_of(param.numel())}, options.dtype(at::kFloat));
+        set_entry(state, ratio_name, THPVariable_Wrap(first));
+        set_entry(state, root_name, THPVariable_Wrap(second));
+        set_entry(state, scale_name, THPVariable_Wrap(scale));
         set_entry(state, bound_name, PyFloat_FromDouble(bound));
     }
     set_entry(state, step_name, PyLong_FromLongLong(0));

@@ -139,3 +139,25 @@ def test_a_refused_group_leaves_no_state_behind(change):
     other.grad = torch.ones_like(other)
     efgs.AdamW([other], state_bits=8, seed=5).step()
     assert torch.equal(q, other) and opt.state[q]['step'] == 1
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_step_that_runs_out_of_memory_can_be_taken_again(bits):
+    """The second of a state's tensors does not fit (a limit on the process's memory): nothing half made stays."""
+    import efgs
+    torch.cuda.empty_cache()
+    p = torch.ones(96 << 20, dtype=torch.bfloat16, device=DEVICE).requires_grad_()
+    p.grad = torch.ones_like(p)
+    opt = efgs.AdamW([p], state_bits=bits)
+    one = p.numel() * (4 if bits == 32 else 1)
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + 1.5 * one) / total)
+    try:
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            opt.step()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    opt.step()
+    assert opt.state[p]['step'] == 1 and bool((p[:: 1 << 20] < 1.0).all())
+    del opt, p
+    torch.cuda.empty_cache()
