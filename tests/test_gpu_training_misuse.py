@@ -148,7 +148,7 @@ def test_a_step_that_runs_out_of_memory_can_be_taken_again(bits):
     torch.cuda.empty_cache()
     p = torch.ones(96 << 20, dtype=torch.bfloat16, device=DEVICE).requires_grad_()
     p.grad = torch.ones_like(p)
-    opt = efgs.AdamW([p], state_bits=bits)
+    opt = efgs.AdamW([p], lr=0.1, state_bits=bits)
     one = p.numel() * (4 if bits == 32 else 1)
     total = torch.cuda.get_device_properties(0).total_memory
     torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + 1.5 * one) / total)
