@@ -161,3 +161,17 @@ def test_a_step_that_runs_out_of_memory_can_be_taken_again(bits):
     assert opt.state[p]['step'] == 1 and bool((p[:: 1 << 20] < 1.0).all())
     del opt, p
     torch.cuda.empty_cache()
+
+
+def test_parameters_made_in_inference_mode():
+    """They have no version to count; a step updates them once, and counts."""
+    import efgs
+    with torch.inference_mode():
+        p = torch.ones(300, device=DEVICE)
+        p.grad = torch.ones_like(p)
+        opt = efgs.AdamW([p], lr=0.1)
+        opt.step()
+    q = torch.ones(300, device=DEVICE).requires_grad_()
+    q.grad = torch.ones_like(q)
+    efgs.AdamW([q], lr=0.1).step()
+    assert opt.state[p]['step'] == 1 and torch.equal(p, q)
