@@ -23,7 +23,7 @@ using torch::autograd::variable_list;
 // steady state a call makes a single allocation.
 class Workspace {
   public:
-    enum Kind { forward = 0, backward = 1, decode = 2, forward_no_backward = 3, embedding = 4, grad_norm = 5 };
+    enum Kind { forward = 0, backward = 1, decode = 2, forward_no_backward = 3 };
 
     Workspace(Kind kind, at::Device device) : key_(kind, device.index()), options_(at::TensorOptions().dtype(at::kByte).device(device)) {
         size_t capacity = 0;

@@ -24,6 +24,26 @@ int32_t element_type(const char* name, at::ScalarType type) {
     }
 }
 
+// Scratch of a call, as much as it asks for (in one request: a region that follows the largest call so far, as the rasterizer's does
+// to spare allocations, would save none and hold as much for a few rows as for the longest list).
+class Scratch {
+  public:
+    explicit Scratch(at::Device device) : options_(at::TensorOptions().dtype(at::kByte).device(device)) {}
+    static void* alloc(void* self, size_t bytes) noexcept {
+        try {
+            Scratch* s = static_cast<Scratch*>(self);
+            s->tensors_.push_back(at::empty({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, s->options_));
+            return s->tensors_.back().data_ptr();
+        } catch (...) {  // (out of memory: the library reports the failed allocation)
+            return nullptr;
+        }
+    }
+
+  private:
+    at::TensorOptions options_;
+    std::vector<Tensor> tensors_;
+};
+
 // ---- rows of a table by index ------------------------------------------------------------------------------------------
 
 struct Rows {
@@ -79,13 +99,12 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const c10::DeviceGuard guard(device);
         const Tensor indices = saved.contiguous(), grad_out = upstream.contiguous();
         const Tensor out = at::empty({rows, columns}, grad_out.options());
-        Workspace workspace(Workspace::embedding, device);
+        Scratch scratch(device);
         check_status(efgs_embedding_backward(indices.numel() > 0 ? indices.data_ptr() : nullptr, static_cast<int>(indices.element_size()),
                                              indices.numel(), grad_out.numel() > 0 ? grad_out.data_ptr() : nullptr, rows, columns,
                                              element_type("the gradient", grad_out.scalar_type()), static_cast<float>(ctx->saved_data["scale"].toDouble()),
-                                             ctx->saved_data["padding"].toInt(), out.numel() > 0 ? out.data_ptr() : nullptr, efgs_workspace_alloc,
-                                             workspace.context(), current_stream(device)));
-        workspace.finish();
+                                             ctx->saved_data["padding"].toInt(), out.numel() > 0 ? out.data_ptr() : nullptr, &Scratch::alloc, &scratch,
+                                             current_stream(device)));
         return out;
     }
 };
@@ -123,10 +142,9 @@ Tensor embedding(const Tensor& indices, const Tensor& table, double scale, const
 Tensor norm_of(const std::vector<efgs_norm_tensor>& tensors, at::Device device) {
     const c10::DeviceGuard guard(device);
     const Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
-    Workspace workspace(Workspace::grad_norm, device);
-    check_status(efgs_grad_norm(tensors.data(), static_cast<int64_t>(tensors.size()), static_cast<float*>(norm.data_ptr()), efgs_workspace_alloc,
-                                workspace.context(), current_stream(device)));
-    workspace.finish();
+    Scratch scratch(device);
+    check_status(efgs_grad_norm(tensors.data(), static_cast<int64_t>(tensors.size()), static_cast<float*>(norm.data_ptr()), &Scratch::alloc, &scratch,
+                                current_stream(device)));
     return norm;
 }
 

@@ -175,3 +175,24 @@ def test_parameters_made_in_inference_mode():
     q.grad = torch.ones_like(q)
     efgs.AdamW([q], lr=0.1).step()
     assert opt.state[p]['step'] == 1 and torch.equal(p, q)
+
+
+def test_scratch_follows_the_call():
+    """A gradient of a few rows takes no more scratch after one of many has run: 12,288 indices into 5,000 rows of 8 floats need two lists of
+    8 bytes a key, a table of 512 KB and a few KB of open rows; 2 MB are allowed beside the gradient itself."""
+    import efgs
+
+    def peak(n, rows, columns):
+        table = torch.zeros(rows, columns, device=DEVICE, requires_grad=True)
+        indices = torch.randint(0, rows, (n,), device=DEVICE)
+        out = efgs.embedding(indices, table)
+        upstream = torch.ones_like(out)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        torch.autograd.grad(out, table, upstream)
+        return torch.cuda.max_memory_allocated() - before - table.numel() * 4
+
+    assert peak(400_000, 50_000, 1024) > 40 << 20
+    assert peak(12_288, 5_000, 8) < 2 << 20
+    assert peak(500, 100, 8) < 2 << 20
