@@ -204,8 +204,8 @@ __device__ __forceinline__ Rates rates_of(const AdamWGroupDevice& G, const float
 // elements, 1,652 MB, in 280 us (5.9 TB/s; a large copy reaches 5.1, a sum of two arrays 5.9). 590k, 17 MB, take 6 us, of which
 // 3.2 would be memory at a large copy's rate.
 template <bool WHOLE, bool CYCLE, int PIECES, typename P, typename D>
-__device__ __forceinline__ void step_pieces(const AdamWTensor& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
-                                            Clip clip) {
+__device__ __forceinline__ void step_block(const AdamWTensor& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
+                                           Clip clip) {
     float p[PIECES][4], g[PIECES][4], m[PIECES][4], v[PIECES][4];
     Four four[PIECES];
 #pragma unroll
@@ -233,12 +233,6 @@ __device__ __forceinline__ void step_pieces(const AdamWTensor& T, const AdamWGro
         store4<WHOLE>(static_cast<float*>(T.v) + four[q].at, four[q].count, v[q]);
         store4<WHOLE>(static_cast<P*>(T.param) + four[q].at, four[q].count, p[q]);
     }
-}
-
-template <bool WHOLE, bool CYCLE, int PIECES, typename P, typename D>
-__device__ __forceinline__ void step_block(const AdamWTensor& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
-                                           Clip clip) {
-    step_pieces<WHOLE, CYCLE, PIECES, P, D>(T, G, cycle, base, n, column, clip);
 }
 
 // ---- 8-bit codes -----------------------------------------------------------------------------------------------------
@@ -295,6 +289,7 @@ __device__ __forceinline__ uint32_t recoded_ratios(uint32_t codes, const AdamWGr
 template <bool WHOLE, bool CYCLE, int PIECES, typename P, typename D>
 __device__ __forceinline__ void step_block(const AdamWTensor8& T, const AdamWGroupDevice& G, const float2* cycle, uint64_t base, uint64_t n, uint32_t column,
                                            Clip clip) {
+    static_assert(PIECES == 1, "a wave takes one block of 256");
     const uint32_t lane = threadIdx.x & 63u;
     const uint64_t first = base + (threadIdx.x - lane) * 4u;  // of the wave's block
     if (!WHOLE && first >= n) return;
