@@ -92,10 +92,9 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const at::Device device = upstream.device();
         TORCH_CHECK_VALUE(device.is_cuda() && saved.device() == device && (saved.scalar_type() == at::kInt || saved.scalar_type() == at::kLong),
                           "efgs: the embedding's indices must be int32 or int64 on the gradient's device, got ", saved.dtype(), " on ", saved.device());
-        std::vector<int64_t> shape = saved.sizes().vec();
-        shape.push_back(columns);
-        TORCH_CHECK_VALUE(upstream.sizes() == at::IntArrayRef(shape), "efgs: the embedding's gradient must have the output's shape ", at::IntArrayRef(shape),
-                          ", got ", upstream.sizes());
+        const at::IntArrayRef sizes = upstream.sizes();
+        TORCH_CHECK_VALUE(!sizes.empty() && sizes.back() == columns && sizes.slice(0, sizes.size() - 1) == saved.sizes(),
+                          "efgs: the embedding's gradient must have the output's shape, the indices' ", saved.sizes(), " and ", columns, " columns, got ", sizes);
         const c10::DeviceGuard guard(device);
         const Tensor indices = saved.contiguous(), grad_out = upstream.contiguous();
         const Tensor out = at::empty({rows, columns}, grad_out.options());
