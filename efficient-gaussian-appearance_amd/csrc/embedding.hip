@@ -564,9 +564,10 @@ __global__ __launch_bounds__(sum_block) void embedding_sum_kernel(SumArgs a) {
 }
 
 constexpr uint32_t join_block = 256, chunk = 64;
-// Blocks of the sums from which the chunks have a kernel of their own, which costs 2.5 to 4 us: without and with it, us, 130k indices into 40 rows of
-// 2,048 bfloat16 (2,032 blocks) 157 and 166 over even rows, 198 and 165 where one row has half of them; 200k into 50k of 1,024 (3,907) 136 and 139,
-// 181 and 150, and with one row for all 212 and 143.
+// Blocks of the sums from which the chunks have a kernel of their own, which costs 2.5 to 9 us: without and with it, us, 130k indices into 40 rows of
+// 2,048 bfloat16 (2,032 blocks) 157 and 166 over even rows, 198 and 165 where one row has half of them, 225 and 155 where it has all; 200k into 50k
+// of 1,024 (3,907) 136 and 139, 181 and 150, 212 and 143; 200k into 50k of 256 floats 75 and 77, 102 and 83, 125 and 82; 200k into 3,000 of 1,024
+// bfloat16 113 and 116, 161 and 122, 189 and 116. Even rows pay 2 to 6 % for it; just below the limit a row that has all pays 45 % without it.
 constexpr uint32_t chunks_from = 2048;
 
 // The last of closed[floor, at) that is set, or floor and `found` unset. Every wave looks at 256 at once.
@@ -694,8 +695,11 @@ __device__ __forceinline__ void load_floats(const float* p, float* x) {
 // table of its own (every row, in 32 bits), and a second kernel adds the partial tables up. grad_out is read a tile at a time,
 // where the long list's runs gather rows from all over it, 128-byte lines for 32 bytes; two launches stand for five to seven. What it
 // costs is the partial tables, written and read once, so they decide: at most 32 MB of them, 256 KB each (us by the list and by tiles: 1M
-// indices into 4,096 rows of 8 floats, 32 MB, 56 and 37; 200k into 257 rows of 45 30 and 20, 20k into 500 of 8 18 and 11; past that 100k
+// indices into 4,096 rows of 8 floats, 32 MB, 57 and 37, of 8 bfloat16 56 and 43; 200k into 257 rows of 45 30 and 20, 20k into 500 of 8 18 and 11; past that 100k
 // into 4,096 rows of 64 28 and 46, 200k into 700 rows of 64, 35 MB, 31 and 33, 4,000 into 4,096 rows of 64, 1 MB each, 14 and 23).
+// The bytes are where rows of 64 floats cross. Narrow rows cross later, past 8,192 rows, and pay the list's price from 4,097 on: 1M
+// into 5,000 rows of 8 floats 58 and 39, 8,192 57 and 45, 16,384 63 and 65, 32,768 64 and 124; 16,384 rows of 4 62 and 46; 100k
+// into 5,000 rows of 8 27 and 19, 16,384 31 and 31, 8,192 rows of 16 27 and 31; 1M into 8,192 of 8 bfloat16 56 and 52.
 
 constexpr uint32_t tile_rows = 4096, tile_lanes = 16, tile_position_bits = 12;
 constexpr uint32_t tile_most_blocks = 256;
@@ -712,8 +716,8 @@ struct TileSumArgs {
 
 // Groups of G lanes take the ordered entries evenly, whatever the runs; the group that holds a run's last entry writes its sum, with what
 // earlier groups had of it by a segmented scan. Rows that no entry meets keep the zeros that the block wrote first. A block's chain of
-// steps bounds it: 1M indices into 4,096 rows of 8 floats take 30 us, and of a block's cycles 39 % went to the tile's sort, 31 % to loads and
-// sums, 17 % to the scan (read at one block). The tables' sum takes 7.
+// steps bounds it, one block of 1,024 threads to a CU with nothing beside it: 1M indices into 4,096 rows of 8 floats take 31 us (35 over even
+// rows), and of a block's cycles 39 % went to the tile's sort, 31 % to loads and sums, 17 % to the scan (read at one block). The tables' sum takes 7.
 template <typename T, int W, int G, uint32_t STEPS>
 __global__ __launch_bounds__(sort_block) void embedding_tile_sum_kernel(TileSumArgs a) {
     constexpr uint32_t tile_size = sort_block * STEPS, groups = sort_block / G, batch = 8;

@@ -311,7 +311,7 @@ typedef struct efgs_adamw_tensor {
     float* root_scale;       /* 8 bits: ceil(n / 256) floats, updated */
     double ratio_bound;      /* 8 bits: of the state as it is */
     int64_t n_elements;      /* up to 2^33 */
-    int64_t step;
+    int64_t step;            /* t, the caller's to count; a step left out for its norm does not see it */
     int32_t group;
     int32_t param_type, grad_type;
     int32_t pad_;
@@ -349,7 +349,7 @@ int efgs_grad_norm(const efgs_norm_tensor* tensors, int64_t n_tensors, float* no
 int efgs_embedding_forward(const void* indices, int index_bytes, int64_t n, const void* table, int64_t rows, int64_t columns, int64_t row_stride,
                            int type, float scale, void* out, void* stream);
 /* grad_table (rows x columns, every row written) = per row scale times the sum of grad_out's rows (n x columns) whose index it is, in
- * 32 bits in an order that the indices give (the same results every time); rows that no index meets are zero, and so is
+ * 32 bits in a fixed order that the indices and sizes give (the same results every time); rows that no index meets are zero, and so is
  * padding_row (outside [0, rows): none). Scratch from `alloc`. Stream-ordered, no host synchronisation. */
 int efgs_embedding_backward(const void* indices, int index_bytes, int64_t n, const void* grad_out, int64_t rows, int64_t columns, int type,
                             float scale, int64_t padding_row, void* grad_table, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
