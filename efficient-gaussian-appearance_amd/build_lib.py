@@ -29,6 +29,9 @@ SOURCES = [
     ('adam.hip', ['-ffp-contract=off']),
     ('adamw.hip', ['-ffp-contract=off']),
     ('embedding.hip', []),
+    ('cross_entropy.hip', []),
+    ('dropout.hip', ['-ffp-contract=off']),
+    ('balance.hip', []),
     ('densification.hip', ['-ffp-contract=off']),
     ('ngsplat.hip', ['-ffp-contract=off']),
 ]
@@ -53,7 +56,7 @@ def _run(what: str, cmd: list[str]) -> None:
 
 
 # sources of the Python extension (host code only)
-BINDING_SOURCES = ('torch_binding.cpp', 'torch_training.cpp')
+BINDING_SOURCES = ('torch_binding.cpp', 'torch_training.cpp', 'torch_losses.cpp')
 
 
 def _compile_binding(src: str) -> str:

@@ -1,0 +1,401 @@
+// The loss that balances how often codes (or experts) are chosen, and their counts.
+//
+//   count_e = choices of e, share_e = count_e / all choices, p_n = softmax(z_n), P_e = mean of p_ne over the rows that count
+//   loss = E sum_e share_e P_e,  d loss / d z_ne = E / rows p_ne (share_e - sum_j share_j p_nj)
+//
+// A choice outside [0, E) counts nowhere, a row without any other is left out. Rows of nothing but -inf have no
+// probabilities and no gradient. One pass over the logits either way: TPR lanes share a row (a wave takes several short rows, a
+// block one long row), each holds the same columns of every row that it meets, so that the sums over rows stay in registers until
+// the block's end. The forward leaves a table of the blocks' sums, which a second kernel adds up in the blocks' order
+// (64 bits) and a third makes the loss of: no atomics on floats, the same bits from call to call.
+#include <algorithm>
+
+#include "internal.h"
+
+namespace efgs {
+
+namespace {
+
+constexpr uint32_t balance_block = 256, balance_waves = balance_block / 64;
+constexpr uint32_t balance_max_blocks = 1024;   // of the forward: rows of the table of sums
+constexpr float log2_e = 1.4426950408889634f;
+
+template <typename T, int W> struct Part { typedef T type __attribute__((ext_vector_type(W), aligned(sizeof(T)))); };
+template <typename T> struct Part<T, 1> { using type = T; };
+
+struct BalanceKernelArgs {
+    const void* logits;
+    const void* indices;
+    uint64_t n;
+    uint32_t experts, chosen, index_bytes;
+    float* sums;          // blocks x experts
+    uint32_t* counts;     // blocks x (experts + 1): choices of each, then rows that count
+    const float* share;   // backward: experts, then E / rows
+    const float* upstream;
+    void* gradient;
+};
+
+template <uint32_t TPR, typename F>
+__device__ __forceinline__ float across(float v, float* lds, F&& join) {
+    constexpr uint32_t lanes = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (uint32_t o = 1; o < lanes; o <<= 1) v = join(v, __shfl_xor(v, o));
+    if constexpr (TPR > 64) {  // (a row to the block: a slot for each wave, one set of slots for each reduction of a row)
+        if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = lds[0];
+#pragma unroll
+        for (uint32_t w = 1; w < balance_waves; w++) v = join(v, lds[w]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ int64_t choice_at(const BalanceKernelArgs& a, uint64_t i) {
+    return a.index_bytes == 8 ? static_cast<const int64_t*>(a.indices)[i] : static_cast<const int32_t*>(a.indices)[i];
+}
+
+// the lane's columns of a row; what lies past the row is -inf
+template <typename T, int W, uint32_t TPR, int ITEMS>
+__device__ __forceinline__ void load_row(const BalanceKernelArgs& a, uint64_t row, uint32_t lane, float (&z)[ITEMS][W]) {
+    const T* const p = static_cast<const T*>(a.logits) + row * a.experts;
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const uint32_t column = (k * TPR + lane) * W;
+        const typename Part<T, W>::type v = *reinterpret_cast<const typename Part<T, W>::type*>(p + min(column, a.experts - W));
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            float x;
+            if constexpr (W == 1) x = static_cast<float>(v);
+            else x = static_cast<float>(v[j]);
+            z[k][j] = column < a.experts ? x : -__builtin_inff();
+        }
+    }
+}
+
+// z becomes exp(z - max); the reciprocal of their sum, 0 for a row of nothing but -inf
+template <int W, uint32_t TPR, int ITEMS>
+__device__ __forceinline__ float exponentials(float (&z)[ITEMS][W], float (*lds)[balance_waves]) {
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+        for (int j = 0; j < W; j++) top = fmaxf(top, z[k][j]);
+    top = across<TPR>(top, lds[0], [](float x, float y) { return fmaxf(x, y); });
+    if (top == -__builtin_inff()) top = 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            z[k][j] = __builtin_amdgcn_exp2f((z[k][j] - top) * log2_e);
+            sum += z[k][j];
+        }
+    sum = across<TPR>(sum, lds[1], [](float x, float y) { return x + y; });
+    return sum == 0.0f ? 0.0f : 1.0f / sum;
+}
+
+template <uint32_t TPR>
+__device__ __forceinline__ bool row_counts(const BalanceKernelArgs& a, uint64_t row, uint32_t lane, bool active, uint32_t* histogram) {
+    bool any = false;
+    for (uint32_t k = lane; k < a.chosen; k += TPR) {
+        const int64_t e = choice_at(a, row * a.chosen + k);
+        const bool valid = active && e >= 0 && e < static_cast<int64_t>(a.experts);
+        if (valid && histogram) atomicAdd(&histogram[e], 1u);
+        any |= valid;
+    }
+    if constexpr (TPR > 64) return __syncthreads_or(any);
+    const uint64_t ballot = __ballot(any), mask = TPR >= 64 ? ~0ull : (1ull << (TPR & 63u)) - 1ull;
+    return (ballot >> (threadIdx.x & 63u & ~(TPR - 1u)) & mask) != 0;
+}
+
+// LDS: choices of each expert (experts x 4 bytes), then, where several groups share the block, their sums (waves x experts x 4)
+template <typename T, int W, uint32_t TPR, int ITEMS>
+__global__ __launch_bounds__(balance_block) void balance_forward_kernel(BalanceKernelArgs a) {
+    extern __shared__ uint32_t histogram[];
+    __shared__ float slots[2][balance_waves];
+    __shared__ uint32_t rows_of_wave[balance_waves];
+    constexpr uint32_t groups = balance_block / TPR;
+    const uint32_t lane = threadIdx.x & (TPR - 1u), group = threadIdx.x / TPR, wave = threadIdx.x >> 6;
+    for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) histogram[e] = 0;
+    __syncthreads();
+    float sums[ITEMS][W] = {};
+    uint32_t rows = 0;
+    for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups; first < a.n; first += static_cast<uint64_t>(gridDim.x) * groups) {
+        const uint64_t row = min(first + group, a.n - 1);
+        float z[ITEMS][W];
+        load_row<T, W, TPR, ITEMS>(a, row, lane, z);
+        const bool counts = row_counts<TPR>(a, row, lane, first + group < a.n, histogram);
+        const float inverse = exponentials<W, TPR, ITEMS>(z, slots);
+        rows += counts && lane == 0;
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++) sums[k][j] += counts ? z[k][j] * inverse : 0.0f;
+        if constexpr (TPR > 64) __syncthreads();  // (the slots are written again)
+    }
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) rows += __shfl_xor(rows, o);
+    if ((threadIdx.x & 63u) == 0) rows_of_wave[wave] = rows;
+    float* const out = a.sums + static_cast<uint64_t>(blockIdx.x) * a.experts;
+    float* const shared = reinterpret_cast<float*>(histogram + a.experts);
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            float x = sums[k][j];
+#pragma unroll
+            for (uint32_t o = TPR; o < 64; o <<= 1) x += __shfl_xor(x, o);
+            const uint32_t column = (k * TPR + lane) * W + j;
+            if (column >= a.experts) continue;
+            if constexpr (TPR > 64) out[column] = x;
+            else if ((threadIdx.x & 63u) < TPR) shared[wave * a.experts + column] = x;
+        }
+    __syncthreads();
+    uint32_t* const counts = a.counts + static_cast<uint64_t>(blockIdx.x) * (a.experts + 1);
+    for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) {
+        counts[e] = histogram[e];
+        if constexpr (TPR <= 64) {
+            float x = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < balance_waves; w++) x += shared[w * a.experts + e];
+            out[e] = x;
+        }
+    }
+    if (threadIdx.x == 0) {
+        uint32_t all = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < balance_waves; w++) all += rows_of_wave[w];
+        counts[a.experts] = all;
+    }
+}
+
+struct BalanceTotals {
+    const float* sums;
+    const uint32_t* counts;
+    uint32_t blocks, experts;
+    double* totals;       // experts + 1: sums of probabilities; rows
+    int64_t* count;       // experts
+    float* share;         // experts, then E / rows
+    float* loss;
+};
+
+constexpr uint32_t totals_columns = 16, totals_parts = balance_block / totals_columns;
+
+// sixteen columns a block, the table's rows in sixteen parts, joined in their order; column `experts` is the number of rows
+__global__ __launch_bounds__(balance_block) void balance_totals_kernel(BalanceTotals a) {
+    __shared__ double sums[totals_parts][totals_columns];
+    __shared__ uint64_t counts[totals_parts][totals_columns];
+    const uint32_t c = threadIdx.x & (totals_columns - 1u), part = threadIdx.x / totals_columns, column = blockIdx.x * totals_columns + c;
+    const uint32_t each = (a.blocks + totals_parts - 1) / totals_parts, last = min(a.blocks, (part + 1) * each);
+    double sum = 0.0;
+    uint64_t count = 0;
+    if (column <= a.experts)
+        for (uint32_t b = part * each; b < last; b++) {
+            if (column < a.experts) sum += static_cast<double>(a.sums[static_cast<uint64_t>(b) * a.experts + column]);
+            count += a.counts[static_cast<uint64_t>(b) * (a.experts + 1) + column];
+        }
+    sums[part][c] = sum;
+    counts[part][c] = count;
+    __syncthreads();
+    if (part != 0 || column > a.experts) return;
+    for (uint32_t p = 1; p < totals_parts; p++) {
+        sum += sums[p][c];
+        count += counts[p][c];
+    }
+    a.totals[column] = column < a.experts ? sum : static_cast<double>(count);
+    if (column < a.experts) a.count[column] = static_cast<int64_t>(count);
+}
+
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double sum = 0.0;
+#pragma unroll
+    for (uint32_t w = 0; w < balance_waves; w++) sum += lds[w];
+    return sum;
+}
+
+__global__ __launch_bounds__(balance_block) void balance_loss_kernel(BalanceTotals a) {
+    __shared__ double lds[balance_waves];
+    double choices = 0.0;
+    for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) choices += static_cast<double>(a.count[e]);
+    choices = block_sum(choices, lds);
+    const double rows = a.totals[a.experts], per_choice = choices > 0.0 ? 1.0 / choices : 0.0, per_row = rows > 0.0 ? a.experts / rows : 0.0;
+    double loss = 0.0;
+    for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) {
+        const double share = static_cast<double>(a.count[e]) * per_choice;
+        a.share[e] = static_cast<float>(share);
+        if (a.count[e] > 0) loss += share * a.totals[e];
+    }
+    loss = block_sum(loss, lds);
+    if (threadIdx.x == 0) {
+        a.share[a.experts] = static_cast<float>(per_row);
+        *a.loss = static_cast<float>(loss * per_row);
+    }
+}
+
+template <typename T, int W, uint32_t TPR, int ITEMS>
+__global__ __launch_bounds__(balance_block) void balance_backward_kernel(BalanceKernelArgs a) {
+    __shared__ float slots[3][balance_waves];
+    constexpr uint32_t groups = balance_block / TPR;
+    const uint32_t lane = threadIdx.x & (TPR - 1u), group = threadIdx.x / TPR;
+    const float factor = a.share[a.experts] * *a.upstream;
+    float share[ITEMS][W];
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+        for (int j = 0; j < W; j++) share[k][j] = a.share[min((k * TPR + lane) * W + j, a.experts - 1)];
+    for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups; first < a.n; first += static_cast<uint64_t>(gridDim.x) * groups) {
+        const bool active = first + group < a.n;
+        const uint64_t row = min(first + group, a.n - 1);
+        float z[ITEMS][W];
+        load_row<T, W, TPR, ITEMS>(a, row, lane, z);
+        const bool counts = row_counts<TPR>(a, row, lane, active, nullptr);
+        const float inverse = exponentials<W, TPR, ITEMS>(z, slots);
+        float mean = 0.0f;
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                z[k][j] *= inverse;
+                mean += z[k][j] * share[k][j];
+            }
+        mean = across<TPR>(mean, slots[2], [](float x, float y) { return x + y; });
+        T* const out = static_cast<T*>(a.gradient) + row * a.experts;
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++) {
+            const uint32_t column = (k * TPR + lane) * W;
+            typename Part<T, W>::type v;
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                const T y = static_cast<T>(counts ? z[k][j] * (share[k][j] - mean) * factor : 0.0f);
+                if constexpr (W == 1) v = y;
+                else v[j] = y;
+            }
+            if (active && column < a.experts) *reinterpret_cast<typename Part<T, W>::type*>(out + column) = v;
+        }
+        if constexpr (TPR > 64) __syncthreads();
+    }
+}
+
+// calls f with a part's width, the lanes of a row and the parts of a lane (up to balance_max_experts)
+template <typename T, int W, typename F>
+void with_shape(uint32_t experts, F&& f) {
+    const uint32_t parts = (experts + W - 1) / W;
+    auto lanes = [&](auto tpr, auto items) { f(std::integral_constant<int, W>{}, tpr, items); };
+#define EFGS_LANES(TPR, ITEMS) lanes(std::integral_constant<uint32_t, TPR>{}, std::integral_constant<int, ITEMS>{})
+    if (parts <= 1) EFGS_LANES(1, 1);
+    else if (parts <= 2) EFGS_LANES(2, 1);
+    else if (parts <= 4) EFGS_LANES(4, 1);
+    else if (parts <= 8) EFGS_LANES(8, 1);
+    else if (parts <= 16) EFGS_LANES(16, 1);
+    else if (parts <= 32) EFGS_LANES(32, 1);
+    else if (parts <= 64) EFGS_LANES(64, 1);
+    else if (parts <= 128) EFGS_LANES(64, 2);
+    else if (parts <= 256) EFGS_LANES(64, 4);
+    else if (parts <= 512) EFGS_LANES(256, 2);
+    else if (parts <= 1024) EFGS_LANES(256, 4);
+    else if (parts <= 2048) EFGS_LANES(256, 8);
+    else if constexpr (W == 1) {
+        if (parts <= 4096) EFGS_LANES(256, 16);
+        else EFGS_LANES(256, 32);
+    }
+#undef EFGS_LANES
+}
+
+template <typename T, typename F>
+void with_type(uint32_t experts, F&& f) {
+    constexpr int widest = 16 / sizeof(T);
+    if (experts % widest == 0) with_shape<T, widest>(experts, [&](auto w, auto tpr, auto items) { f(T{}, w, tpr, items); });
+    else with_shape<T, 1>(experts, [&](auto w, auto tpr, auto items) { f(T{}, w, tpr, items); });
+}
+
+template <typename F>
+void dispatch(int type, uint32_t experts, F&& f) {
+    if (type == type_float) with_type<float>(experts, f);
+    else if (type == type_bfloat16) with_type<__bf16>(experts, f);
+    else with_type<_Float16>(experts, f);
+}
+
+BalanceKernelArgs kernel_args(const BalanceArgs& a) {
+    BalanceKernelArgs k{};
+    k.logits = a.logits;
+    k.indices = a.indices;
+    k.n = a.n;
+    k.experts = a.experts;
+    k.chosen = a.chosen;
+    k.index_bytes = static_cast<uint32_t>(a.index_bytes);
+    return k;
+}
+
+uint32_t rows_at_once(const BalanceArgs& a) {
+    uint32_t rows = 1;
+    dispatch(a.type, a.experts, [&](auto, auto, auto tpr, auto) { rows = balance_block / decltype(tpr)::value; });
+    return rows;
+}
+
+uint32_t forward_blocks(const BalanceArgs& a) {
+    const uint64_t rows = rows_at_once(a);
+    return static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>((a.n + rows - 1) / rows, 1), balance_max_blocks));
+}
+
+}  // namespace
+
+size_t balance_scratch_bytes(const BalanceArgs& a) {
+    const uint64_t blocks = forward_blocks(a);
+    return (a.experts + 1ull) * sizeof(double) + blocks * a.experts * sizeof(float) + blocks * (a.experts + 1ull) * sizeof(uint32_t);
+}
+
+bool launch_balance_forward(const BalanceArgs& a, int64_t* counts, float* share, float* loss, void* scratch, hipStream_t s) {
+    const uint32_t blocks = forward_blocks(a);
+    BalanceTotals t{};
+    t.totals = static_cast<double*>(scratch);
+    float* const sums = reinterpret_cast<float*>(t.totals + a.experts + 1);
+    uint32_t* const table = reinterpret_cast<uint32_t*>(sums + static_cast<uint64_t>(blocks) * a.experts);
+    t.sums = sums;
+    t.counts = table;
+    t.blocks = blocks;
+    t.experts = a.experts;
+    t.count = counts;
+    t.share = share;
+    t.loss = loss;
+    BalanceKernelArgs k = kernel_args(a);
+    k.sums = sums;
+    k.counts = table;
+    if (a.n > 0) {
+        dispatch(a.type, a.experts, [&](auto type, auto w, auto tpr, auto items) {
+            constexpr uint32_t lanes = decltype(tpr)::value;
+            const size_t lds = a.experts * sizeof(uint32_t) * (lanes > 64 ? 1 : 1 + balance_waves);
+            hipLaunchKernelGGL((balance_forward_kernel<decltype(type), decltype(w)::value, lanes, decltype(items)::value>), dim3(blocks),
+                               dim3(balance_block), lds, s, k);
+        });
+    } else {
+        t.blocks = 0;
+    }
+    hipLaunchKernelGGL(balance_totals_kernel, dim3(div_up(a.experts + 1ull, totals_columns)), dim3(balance_block), 0, s, t);
+    hipLaunchKernelGGL(balance_loss_kernel, dim3(1), dim3(balance_block), 0, s, t);
+    EFGS_HIP_CHECK(hipGetLastError());
+    return true;
+}
+
+bool launch_balance_backward(const BalanceArgs& a, const float* share, const float* upstream, void* gradient, hipStream_t s) {
+    if (a.n == 0) return true;
+    BalanceKernelArgs k = kernel_args(a);
+    k.share = share;
+    k.upstream = upstream;
+    k.gradient = gradient;
+    dispatch(a.type, a.experts, [&](auto type, auto w, auto tpr, auto items) {
+        constexpr uint32_t lanes = decltype(tpr)::value;
+        const uint64_t rows = balance_block / lanes;
+        const uint32_t blocks = static_cast<uint32_t>(std::min<uint64_t>((a.n + rows - 1) / rows, 1u << 23));
+        hipLaunchKernelGGL((balance_backward_kernel<decltype(type), decltype(w)::value, lanes, decltype(items)::value>), dim3(blocks),
+                           dim3(balance_block), 0, s, k);
+    });
+    EFGS_HIP_CHECK(hipGetLastError());
+    return true;
+}
+
+}  // namespace efgs

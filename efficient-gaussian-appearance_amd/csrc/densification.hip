@@ -8,13 +8,10 @@
 //                       primitive (counter = (offset / 4, primitive index, 0), key = seed) and two Box-Muller
 //                       transforms; quaternions with |q|^2 < 1e-8 leave their mean unchanged
 //
-// Philox4x32-10 is the counter-based generator of Salmon, Moraes, Dror and Shaw ("Parallel random numbers: as
-// easy as 1, 2, 3", SC 2011; Random123): ten rounds of two 32x32 -> 64-bit multiplications (0xD2511F53,
-// 0xCD9E8D57) with the key bumped by the Weyl constants (0x9E3779B9, 0xBB67AE85) between rounds.
-//
 // Reference: B/densification/include/kernels_mcmc.cuh:11-146, B/densification/src/mcmc.cu:1-56,
 // B/densification/src/densification_api.cu:13-72.
 #include "internal.h"
+#include "philox.h"
 
 #include <cmath>
 #include <mutex>
@@ -26,20 +23,6 @@ namespace {
 constexpr uint32_t densify_block = 256;
 
 __constant__ float c_relocation[mcmc_max_samples * mcmc_max_samples];
-
-__device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k) {
-#pragma unroll
-    for (int r = 0; r < 10; r++) {
-        if (r > 0) {
-            k.x += 0x9E3779B9u;
-            k.y += 0xBB67AE85u;
-        }
-        const uint32_t lo0 = 0xD2511F53u * c.x, hi0 = __umulhi(0xD2511F53u, c.x);
-        const uint32_t lo1 = 0xCD9E8D57u * c.z, hi1 = __umulhi(0xCD9E8D57u, c.z);
-        c = make_uint4(hi1 ^ c.y ^ k.x, lo1, hi0 ^ c.w ^ k.y, lo0);
-    }
-    return c;
-}
 
 // two standard normal samples from two uniform 32-bit words: u = (bits_u + 1/2) 2^-32 in (0, 1], angle =
 // bits_v 2 pi 2^-32

@@ -283,6 +283,55 @@ size_t embedding_gradient_bytes(const EmbeddingArgs& a);  // of `workspace`
 // every row of `gradient` is written; `padding`: a row that gets no gradient (>= rows: none)
 bool launch_embedding_gradient(const EmbeddingArgs& a, const void* grad_out, uint32_t padding, void* gradient, void* workspace, hipStream_t s);
 
+// ---- dropout -------------------------------------------------------------------------------------------------------
+struct DropoutArgs {
+    const void* x;
+    const void* residual;     // or null
+    void* out;
+    uint64_t n;
+    uint64_t seed, offset;
+    const uint64_t* seed_at;  // on the device, or null: `seed`
+    uint32_t threshold;       // round(2^16 p)
+    int type;
+};
+bool launch_dropout(const DropoutArgs& a, hipStream_t s);
+
+// ---- balance loss ----------------------------------------------------------------------------------------------------
+struct BalanceArgs {
+    const void* logits;       // n x experts
+    const void* indices;      // n x chosen
+    int index_bytes;          // 4 or 8 (signed)
+    int type;
+    uint64_t n;
+    uint32_t experts, chosen;
+};
+constexpr int64_t balance_max_experts = 8192;
+size_t balance_scratch_bytes(const BalanceArgs& a);
+// share: experts + 1 floats for the backward
+bool launch_balance_forward(const BalanceArgs& a, int64_t* counts, float* share, float* loss, void* scratch, hipStream_t s);
+bool launch_balance_backward(const BalanceArgs& a, const float* share, const float* upstream, void* gradient, hipStream_t s);
+
+// ---- cross entropy against the rows of a table -------------------------------------------------------------------------
+struct EntropyArgs {
+    const void* features;     // n x columns, feature_stride elements apart (forward)
+    const void* table;        // rows x columns, table_stride elements apart
+    const void* targets;      // n (forward)
+    uint64_t feature_stride, table_stride;
+    uint32_t n, rows, columns;
+    int target_bytes;         // 4 or 8 (signed)
+    int type;
+    float scale;
+    bool mean, each;          // the loss: mean over the rows that count, every row's, or their sum
+};
+constexpr int64_t entropy_max = (1ll << 31) - 1024;  // rows of either side, columns
+bool entropy_fits(const EntropyArgs& a);             // whether the launches can count their blocks
+size_t entropy_saved_bytes(const EntropyArgs& a);    // what a backward needs of its forward
+size_t entropy_forward_bytes(const EntropyArgs& a);  // of `scratch`
+size_t entropy_backward_bytes(const EntropyArgs& a);
+bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void* scratch, hipStream_t s);
+bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const void* saved, void* grad_features, void* grad_table, void* scratch,
+                             hipStream_t s);
+
 // ---- MCMC densification ---------------------------------------------------------------------------------------
 constexpr uint32_t mcmc_max_samples = 50;  // samples per relocated Gaussian (larger counts are clamped)
 bool launch_add_noise(const float* raw_scales, const float* raw_rotations, const float* raw_opacities, float* means, uint32_t n, float lr,

@@ -16,6 +16,7 @@
 
 namespace efgs_torch {
 void register_training(pybind11::module_& m);  // torch_training.cpp
+void register_losses(pybind11::module_& m);    // torch_losses.cpp
 }
 
 namespace {
@@ -266,4 +267,5 @@ PYBIND11_MODULE(_native, m) {
     m.def("diff_rasterize", torch::wrap_pybind_function_no_gil(diff_rasterize));
     m.def("neural_decode", torch::wrap_pybind_function_no_gil(neural_decode));
     efgs_torch::register_training(m);
+    efgs_torch::register_losses(m);
 }

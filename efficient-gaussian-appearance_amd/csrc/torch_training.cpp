@@ -15,35 +15,6 @@ namespace efgs_torch {
 
 namespace {
 
-int32_t element_type(const char* name, at::ScalarType type) {
-    switch (type) {
-        case at::kFloat: return EFGS_FLOAT;
-        case at::kBFloat16: return EFGS_BFLOAT16;
-        case at::kHalf: return EFGS_HALF;
-        default: TORCH_CHECK_VALUE(false, "efgs: ", name, " must be float32, bfloat16 or float16, got ", type);
-    }
-}
-
-// Scratch of a call, as much as it asks for (in one request: a region that follows the largest call so far, as the rasterizer's does
-// to spare allocations, would save none and hold as much for a few rows as for the longest list).
-class Scratch {
-  public:
-    explicit Scratch(at::Device device) : options_(at::TensorOptions().dtype(at::kByte).device(device)) {}
-    static void* alloc(void* self, size_t bytes) noexcept {
-        try {
-            Scratch* s = static_cast<Scratch*>(self);
-            s->tensors_.push_back(at::empty({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, s->options_));
-            return s->tensors_.back().data_ptr();
-        } catch (...) {  // (out of memory: the library reports the failed allocation)
-            return nullptr;
-        }
-    }
-
-  private:
-    at::TensorOptions options_;
-    std::vector<Tensor> tensors_;
-};
-
 // ---- rows of a table by index ------------------------------------------------------------------------------------------
 
 struct Rows {

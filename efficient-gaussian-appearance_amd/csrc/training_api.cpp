@@ -1,5 +1,6 @@
 // C entry points of the training operators beside the rasterizer: AdamW over many tensors with 32-bit and 8-bit states,
-// the gradient norm, and rows of a table by index with their gradient (include/efgs.h). Arguments are checked here, before
+// the gradient norm, rows of a table by index with their gradient, the cross entropy of rows against a table, dropout and the
+// balance loss (include/efgs.h). Arguments are checked here, before
 // any device work; nothing thrown leaves an entry point.
 #include <cmath>
 #include <exception>
@@ -125,6 +126,50 @@ const char* embedding_fault(const void* indices, int index_bytes, int64_t n, int
     return nullptr;
 }
 
+// the fault of a call's values, or null
+const char* entropy_fault(const efgs_entropy* e) {
+    if (!e) return "null cross entropy arguments";
+    if (e->n < 0 || e->rows < 0 || e->columns < 0 || e->n > entropy_max || e->rows > entropy_max || e->columns > entropy_max)
+        return "cross entropy sizes must lie between 0 and 2^31 - 1024";
+    if (e->target_bytes != 4 && e->target_bytes != 8) return "cross entropy targets have 4 or 8 bytes";
+    if (!known_type(e->type)) return "unknown element type";
+    if (!std::isfinite(e->scale)) return "the cross entropy's scale must be finite";
+    if (e->reduction < EFGS_EACH || e->reduction > EFGS_MEAN) return "unknown reduction";
+    if (e->feature_stride < 0 || e->table_stride < 0) return "negative row stride";
+    return nullptr;
+}
+
+EntropyArgs entropy_args(const efgs_entropy& e) {
+    EntropyArgs a{};
+    a.features = e.features;
+    a.table = e.table;
+    a.targets = e.targets;
+    a.feature_stride = static_cast<uint64_t>(e.feature_stride);
+    a.table_stride = static_cast<uint64_t>(e.table_stride);
+    a.n = static_cast<uint32_t>(e.n);
+    a.rows = static_cast<uint32_t>(e.rows);
+    a.columns = static_cast<uint32_t>(e.columns);
+    a.target_bytes = e.target_bytes;
+    a.type = e.type;
+    a.scale = e.scale;
+    a.mean = e.reduction == EFGS_MEAN;
+    a.each = e.reduction == EFGS_EACH;
+    return a;
+}
+
+const char* balance_fault(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type) {
+    if (experts < 1 || experts > balance_max_experts) return "between 1 and 8192 experts are supported";
+    if (n < 0 || n > embedding_max || chosen < 0 || chosen > embedding_max) return "balance loss sizes must lie between 0 and 2^31 - 1";
+    if (index_bytes != 4 && index_bytes != 8) return "balance loss indices have 4 or 8 bytes";
+    if (!known_type(type)) return "unknown element type";
+    if (n > 0 && (!logits || (chosen > 0 && !indices))) return "null balance loss tensor";
+    return nullptr;
+}
+
+BalanceArgs balance_args(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type) {
+    return BalanceArgs{logits, indices, index_bytes, type, static_cast<uint64_t>(n), static_cast<uint32_t>(experts), static_cast<uint32_t>(chosen)};
+}
+
 }  // namespace
 
 extern "C" {
@@ -245,6 +290,84 @@ int efgs_embedding_backward(const void* indices, int index_bytes, int64_t n, con
         void* workspace = alloc(alloc_ctx, embedding_gradient_bytes(a));
         if (!workspace) return fail(EFGS_ERR_ALLOC, "allocation of the embedding gradient's workspace failed");
         return launch_embedding_gradient(a, grad_out, padding, grad_table, workspace, static_cast<hipStream_t>(stream)) ? EFGS_OK : EFGS_ERR_HIP;
+    });
+}
+
+int64_t efgs_linear_cross_entropy_saved_bytes(const efgs_entropy* e) {
+    int64_t bytes = -1;
+    guarded([&]() -> int {
+        if (const char* fault = entropy_fault(e)) return fail(EFGS_ERR_INVALID_ARGUMENT, fault);
+        const EntropyArgs a = entropy_args(*e);
+        if (!entropy_fits(a)) return fail(EFGS_ERR_INVALID_ARGUMENT, "too many rows and columns in the cross entropy");
+        bytes = static_cast<int64_t>(entropy_saved_bytes(a));
+        return EFGS_OK;
+    });
+    return bytes;
+}
+
+int efgs_linear_cross_entropy_forward(const efgs_entropy* e, float* loss, void* saved, efgs_alloc_fn alloc, void* alloc_ctx, void* stream) {
+    return guarded([&]() -> int {
+        if (const char* fault = entropy_fault(e)) return fail(EFGS_ERR_INVALID_ARGUMENT, fault);
+        const EntropyArgs a = entropy_args(*e);
+        if (!entropy_fits(a)) return fail(EFGS_ERR_INVALID_ARGUMENT, "too many rows and columns in the cross entropy");
+        if ((!loss && !(a.each && a.n == 0)) || !alloc || (a.n > 0 && (!a.targets || (a.columns > 0 && !a.features))) || (a.rows > 0 && a.columns > 0 && !a.table))
+            return fail(EFGS_ERR_INVALID_ARGUMENT, "null cross entropy tensor");
+        const size_t own = saved ? 0 : entropy_saved_bytes(a);  // (a forward without a backward: scratch)
+        char* const scratch = static_cast<char*>(alloc(alloc_ctx, own + entropy_forward_bytes(a)));
+        if (!scratch) return fail(EFGS_ERR_ALLOC, "allocation of the cross entropy's workspace failed");
+        return launch_entropy_forward(a, loss, saved ? saved : scratch, scratch + own, static_cast<hipStream_t>(stream)) ? EFGS_OK : EFGS_ERR_HIP;
+    });
+}
+
+int efgs_linear_cross_entropy_backward(const efgs_entropy* e, const float* upstream, const void* saved, void* grad_features, void* grad_table,
+                                       efgs_alloc_fn alloc, void* alloc_ctx, void* stream) {
+    return guarded([&]() -> int {
+        if (const char* fault = entropy_fault(e)) return fail(EFGS_ERR_INVALID_ARGUMENT, fault);
+        const EntropyArgs a = entropy_args(*e);
+        if (!entropy_fits(a)) return fail(EFGS_ERR_INVALID_ARGUMENT, "too many rows and columns in the cross entropy");
+        if (a.rows == 0) grad_table = nullptr;
+        if (a.n == 0) grad_features = nullptr;
+        if (a.columns == 0 || (!grad_features && !grad_table)) return EFGS_OK;
+        if (!saved || !alloc || (!upstream && !(a.each && a.n == 0)) || (a.rows > 0 && !a.table)) return fail(EFGS_ERR_INVALID_ARGUMENT, "null cross entropy tensor");
+        void* const scratch = alloc(alloc_ctx, entropy_backward_bytes(a));
+        if (!scratch) return fail(EFGS_ERR_ALLOC, "allocation of the cross entropy's workspace failed");
+        return launch_entropy_backward(a, upstream, saved, grad_features, grad_table, scratch, static_cast<hipStream_t>(stream)) ? EFGS_OK : EFGS_ERR_HIP;
+    });
+}
+
+int efgs_dropout(const void* x, const void* residual, void* out, int64_t n, int type, double p, uint64_t seed, const uint64_t* seed_at, uint64_t offset,
+                 void* stream) {
+    return guarded([&]() -> int {
+        if (n < 0) return fail(EFGS_ERR_INVALID_ARGUMENT, "negative dropout size");
+        if (!known_type(type)) return fail(EFGS_ERR_INVALID_ARGUMENT, "unknown element type");
+        if (!(p >= 0.0 && p <= 1.0)) return fail(EFGS_ERR_INVALID_ARGUMENT, "the dropout probability must lie in [0, 1]");
+        if (n == 0) return EFGS_OK;
+        if (!x || !out) return fail(EFGS_ERR_INVALID_ARGUMENT, "null dropout tensor");
+        const DropoutArgs a{x, residual, out, static_cast<uint64_t>(n), seed, offset, seed_at, static_cast<uint32_t>(std::nearbyint(p * 65536.0)), type};
+        return launch_dropout(a, static_cast<hipStream_t>(stream)) ? EFGS_OK : EFGS_ERR_HIP;
+    });
+}
+
+int efgs_balance_loss_forward(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type,
+                              float* loss, int64_t* counts, float* share, efgs_alloc_fn alloc, void* alloc_ctx, void* stream) {
+    return guarded([&]() -> int {
+        if (const char* fault = balance_fault(logits, indices, index_bytes, n, experts, chosen, type)) return fail(EFGS_ERR_INVALID_ARGUMENT, fault);
+        if (!loss || !counts || !share || !alloc) return fail(EFGS_ERR_INVALID_ARGUMENT, "null balance loss tensor");
+        const BalanceArgs a = balance_args(logits, indices, index_bytes, n, experts, chosen, type);
+        void* const scratch = alloc(alloc_ctx, balance_scratch_bytes(a));
+        if (!scratch) return fail(EFGS_ERR_ALLOC, "allocation of the balance loss's workspace failed");
+        return launch_balance_forward(a, counts, share, loss, scratch, static_cast<hipStream_t>(stream)) ? EFGS_OK : EFGS_ERR_HIP;
+    });
+}
+
+int efgs_balance_loss_backward(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type,
+                               const float* share, const float* upstream, void* gradient, void* stream) {
+    return guarded([&]() -> int {
+        if (const char* fault = balance_fault(logits, indices, index_bytes, n, experts, chosen, type)) return fail(EFGS_ERR_INVALID_ARGUMENT, fault);
+        if (n == 0) return EFGS_OK;
+        if (!share || !upstream || !gradient) return fail(EFGS_ERR_INVALID_ARGUMENT, "null balance loss tensor");
+        const BalanceArgs a = balance_args(logits, indices, index_bytes, n, experts, chosen, type);
+        return launch_balance_backward(a, share, upstream, gradient, static_cast<hipStream_t>(stream)) ? EFGS_OK : EFGS_ERR_HIP;
     });
 }
 

@@ -66,6 +66,12 @@ class AdamWState(ctypes.Structure):
                 ('exp_avg_sq', ctypes.c_void_p), ('ratio_bound', ctypes.c_double), ('n_elements', ctypes.c_int64)]
 
 
+class Entropy(ctypes.Structure):
+    _fields_ = [('features', ctypes.c_void_p), ('table', ctypes.c_void_p), ('targets', ctypes.c_void_p), ('n', ctypes.c_int64), ('rows', ctypes.c_int64),
+                ('columns', ctypes.c_int64), ('feature_stride', ctypes.c_int64), ('table_stride', ctypes.c_int64), ('target_bytes', ctypes.c_int32),
+                ('type', ctypes.c_int32), ('reduction', ctypes.c_int32), ('scale', ctypes.c_float)]
+
+
 class NormTensor(ctypes.Structure):
     _fields_ = [('data', ctypes.c_void_p), ('n_elements', ctypes.c_int64), ('type', ctypes.c_int32), ('pad_', ctypes.c_int32)]
 
@@ -102,7 +108,8 @@ EXPORTED = ('efgs_last_error', 'efgs_set_rtc_dirs', 'efgs_rasterizer_create', 'e
             'efgs_get_frame_views', 'efgs_get_frame_tile_views', 'efgs_precompile', 'efgs_set_stage_timing', 'efgs_get_stage_times', 'efgs_workspace_alloc',
             'efgs_neural_decode_forward', 'efgs_neural_decode_backward', 'efgs_neural_decode_backward_no_alloc', 'efgs_add_noise', 'efgs_relocation_adjustment', 'efgs_render', 'efgs_update_pruning_scores',
             'efgs_ngsplat_layout', 'efgs_ngsplat_pack', 'efgs_adamw_step', 'efgs_adamw_moments', 'efgs_adamw_ratio_bound', 'efgs_grad_norm',
-            'efgs_embedding_forward', 'efgs_embedding_backward')
+            'efgs_embedding_forward', 'efgs_embedding_backward', 'efgs_linear_cross_entropy_saved_bytes', 'efgs_linear_cross_entropy_forward',
+            'efgs_linear_cross_entropy_backward', 'efgs_dropout', 'efgs_balance_loss_forward', 'efgs_balance_loss_backward')
 
 # stage ids of efgs_get_stage_times, in order (include/efgs.h)
 STAGES = ('preprocess_forward', 'compact', 'counter_read', 'create_instances', 'tile_offsets', 'tile_buckets', 'tile_sort',
@@ -157,6 +164,16 @@ lib.efgs_embedding_forward.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_i
 lib.efgs_embedding_backward.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                         ctypes.c_int, ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, ALLOC_FN, ctypes.c_void_p,
                                         ctypes.c_void_p]
+
+lib.efgs_linear_cross_entropy_saved_bytes.restype = ctypes.c_int64
+lib.efgs_linear_cross_entropy_saved_bytes.argtypes = [ctypes.POINTER(Entropy)]
+lib.efgs_linear_cross_entropy_forward.argtypes = [ctypes.POINTER(Entropy), ctypes.c_void_p, ctypes.c_void_p, ALLOC_FN, ctypes.c_void_p, ctypes.c_void_p]
+lib.efgs_linear_cross_entropy_backward.argtypes = [ctypes.POINTER(Entropy)] + [ctypes.c_void_p] * 4 + [ALLOC_FN, ctypes.c_void_p, ctypes.c_void_p]
+lib.efgs_dropout.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_int64, ctypes.c_int, ctypes.c_double, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_uint64,
+                                                     ctypes.c_void_p]
+lib.efgs_balance_loss_forward.argtypes = ([ctypes.c_void_p] * 2 + [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_int] + [ctypes.c_void_p] * 3 +
+                                          [ALLOC_FN, ctypes.c_void_p, ctypes.c_void_p])
+lib.efgs_balance_loss_backward.argtypes = ([ctypes.c_void_p] * 2 + [ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_int] + [ctypes.c_void_p] * 4)
 
 
 def check(rc: int) -> None:

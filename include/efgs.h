@@ -354,6 +354,44 @@ int efgs_embedding_forward(const void* indices, int index_bytes, int64_t n, cons
 int efgs_embedding_backward(const void* indices, int index_bytes, int64_t n, const void* grad_out, int64_t rows, int64_t columns, int type,
                             float scale, int64_t padding_row, void* grad_table, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
 
+/* Softmax cross entropy of n rows x against every row w of a table, without the logits in memory: z = scale x . w,
+ * loss = log sum exp z - z[target]. A target outside [0, rows) leaves its row out: loss and gradient 0, whatever its features hold.
+ * Logits, sums and statistics are in 32 bits. EFGS_MEAN is over the rows that count (0 if none does). Rows lie feature_stride and
+ * table_stride elements apart. */
+enum { EFGS_EACH = 0, EFGS_SUM = 1, EFGS_MEAN = 2 };
+typedef struct efgs_entropy {
+    const void* features; /* n x columns */
+    const void* table;    /* rows x columns */
+    const void* targets;  /* n int32 or int64 (target_bytes 4 or 8) */
+    int64_t n, rows, columns, feature_stride, table_stride;
+    int32_t target_bytes, type, reduction;
+    float scale;
+} efgs_entropy;
+/* bytes of `saved`, or -1 with an error set; features, table and targets are not read */
+int64_t efgs_linear_cross_entropy_saved_bytes(const efgs_entropy* e);
+/* loss: one float, or n with EFGS_EACH. saved (256-byte aligned): what the backward needs, or NULL where none follows. Scratch from `alloc`.
+ * Stream-ordered, no host synchronisation. */
+int efgs_linear_cross_entropy_forward(const efgs_entropy* e, float* loss, void* saved, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
+/* grad_features (n x columns) and grad_table (rows x columns), contiguous, in `type`, every row written; either may be NULL. upstream: one float, or n with
+ * EFGS_EACH. `e` as in the forward (features and targets are not read: they are in `saved`). The upstream gradients of the logits are held by pieces of
+ * the table in `type`; sums in 32 bits in a fixed order. Scratch from `alloc`. Stream-ordered, no host synchronisation. */
+int efgs_linear_cross_entropy_backward(const efgs_entropy* e, const float* upstream, const void* saved, void* grad_features, void* grad_table,
+                                       efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
+
+/* out = keep x / (1 - t / 2^16) (+ residual, or NULL), t = round(2^16 p), in 32 bits, rounded once to `type`. Element i has 16 bits of Philox4x32-10
+ * (counter: i / 8, offset; key: the seed; bits 16 (i mod 8) of the four words) and is kept where they are not below t; a dropped one is 0 whatever x held.
+ * The gradient with respect to x is the same call on the upstream gradient without the residual. seed_at: the seed on the device, or NULL for `seed`. */
+int efgs_dropout(const void* x, const void* residual, void* out, int64_t n, int type, double p, uint64_t seed, const uint64_t* seed_at, uint64_t offset,
+                 void* stream);
+
+/* Balance of choices: counts (int64) of each of `experts` (1 to 8192) among indices (n x chosen; outside [0, experts): none),
+ * loss = experts sum_e share_e P_e, share_e = counts_e / all choices, P_e the mean of softmax(logits)_e over the rows with a choice (0 without one).
+ * share (experts + 1 floats) is kept for the backward, which writes gradient (n x experts, in `type`). Sums in a fixed order. Stream-ordered. */
+int efgs_balance_loss_forward(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type,
+                              float* loss, int64_t* counts, float* share, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
+int efgs_balance_loss_backward(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type,
+                               const float* share, const float* upstream, void* gradient, void* stream);
+
 /* Standalone neural decode: the configured residual MLP (efgs_set_residual_mlp, model 5) on n primitives'
  * features (n x n_features, the learned latents), base colours (n x 3, read with base input only) and unit
  * view directions (n x 3; not read, and may be NULL, when the encoding has no SH degree), encoded as in the

@@ -99,3 +99,55 @@ def embedding_gradient(indices, grad_out, rows: int, scale: float, padding=None)
     np.add.at(total, indices[inside], grad_out[inside])
     np.add.at(magnitude, indices[inside], np.abs(grad_out[inside]))
     return total * scale, magnitude * abs(scale), np.bincount(indices[inside], minlength=rows)
+
+
+def cross_entropy(features, table, targets, scale, weights):
+    """(losses, p, g, grad_features, grad_table): g = weights (p - onehot) of the rows whose target lies in the table, zeros elsewhere."""
+    x, w = np.asarray(features, np.float64), np.asarray(table, np.float64)
+    targets, n = np.asarray(targets, np.int64), len(targets)
+    inside = (targets >= 0) & (targets < len(w))
+    x = np.where(inside[:, None], x, 0.0)
+    z = scale * (x @ w.T)
+    top = z.max(1, keepdims=True) if len(w) else np.zeros((n, 1))
+    p = np.exp(z - top)
+    total = p.sum(1, keepdims=True)
+    rows = np.arange(n)[inside]
+    losses = np.zeros(n)
+    losses[rows] = (np.log(total) + top)[rows, 0] - z[rows, targets[rows]]
+    p = np.where(inside[:, None], p / np.where(total > 0, total, 1.0), 0.0)
+    g = p.copy()
+    g[rows, targets[rows]] -= 1.0
+    g *= np.asarray(weights, np.float64)[:, None]
+    return losses, p, g, scale * (g @ w), scale * (g.T @ x)
+
+
+def philox_bits(n: int, seed: int, offset: int, first: int = 0):
+    """16 bits of each of the elements first..first + n (first a multiple of 8): Philox4x32-10 of (i / 8, offset) and the seed, in Python's whole numbers."""
+    mask, out = 0xffffffff, []
+    for group in range(first // 8, (first + n + 7) // 8):
+        c, k = [group & mask, group >> 32, offset & mask, offset >> 32], [seed & mask, seed >> 32]
+        for _ in range(10):
+            a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+            c = [b >> 32 ^ c[1] ^ k[0], b & mask, a >> 32 ^ c[3] ^ k[1], a & mask]
+            k = [(k[0] + 0x9E3779B9) & mask, (k[1] + 0xBB67AE85) & mask]
+        for word in c:
+            out += [word & 0xffff, word >> 16]
+    return np.array(out[:n])
+
+
+def balance(logits, indices, upstream=1.0):
+    """(loss, counts, gradient) of (N, E) logits and (N, k) indices."""
+    z, indices = np.asarray(logits, np.float64), np.asarray(indices, np.int64)
+    n, experts = z.shape
+    valid = (indices >= 0) & (indices < experts)
+    rows = valid.any(1)
+    counts = np.bincount(indices[valid], minlength=experts)
+    share = counts / max(1, counts.sum())
+    z = np.where(rows[:, None], z, 0.0)
+    top = z.max(1, keepdims=True)
+    p = np.exp(z - np.where(np.isneginf(top), 0.0, top))
+    total = p.sum(1, keepdims=True)
+    p = np.where(rows[:, None] & (total > 0), p / np.where(total > 0, total, 1.0), 0.0)
+    number = max(1, rows.sum())
+    loss = experts * (share * p.sum(0)).sum() / number
+    return loss, counts, upstream * experts / number * p * (share - (p @ share)[:, None])

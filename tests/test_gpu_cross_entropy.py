@@ -1,0 +1,335 @@
+"""efgs.linear_cross_entropy on the GPU against the 64-bit oracle (oracle/training_ref.py).
+
+Bars, e = 2^-24, u = half a step of the inputs' type relative to the value (2^-24, 2^-8, 2^-11): a logit is a float32 sum of D exact or
+once-rounded products, off by dz <= 2 (D + 4) e scale sum |x w|, the 2 for matrix instructions that may cut where they align, and the product with
+scale log2 e and its rounding 3 e |z|. A sum of exponentials of V table rows goes through at most 64 + V / 16 additions in a row, each exponential 4 e
+off; so a loss is off by 2 max dz + (80 + V / 16) e + 4 e (|lse| + |z|), and a probability by that relative to it. g = weight (p - onehot) is rounded to the
+type (u |g|, and 2^-38 for float16, whose g is held times 2^15), a gradient is a float32 sum of K values (at most 2 (K + 4) e of their magnitudes), scaled, and
+rounded to the type: u of the value, float16 half its least step, 2^-25.
+"""
+import numpy as np
+import pytest
+import torch
+
+import training_ref as R
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+TYPES = {'f32': (torch.float32, E, 0.0, 0.0), 'bf16': (torch.bfloat16, 2.0 ** -8, 0.0, 0.0), 'f16': (torch.float16, 2.0 ** -11, 2.0 ** -25, 2.0 ** -38)}
+DEVICE = 'cuda:0'
+
+
+def inputs(n, rows, columns, dtype, seed=0, left_out=0.1, index=torch.int64, sharp=8.0, scale=1.0):
+    rng = np.random.default_rng(seed)
+    kind = TYPES[dtype][0]
+    table = torch.tensor(rng.normal(size=(rows, columns)) * 2.0 / (scale * np.sqrt(columns)), device=DEVICE).to(kind)
+    targets = rng.integers(0, rows, n)
+    pull = torch.tensor(rng.random((n, 1)) * sharp * scale / 4.0, device=DEVICE)
+    features = (torch.tensor(rng.normal(size=(n, columns)), device=DEVICE) + pull * table[torch.tensor(targets, device=DEVICE)].double()).to(kind)
+    wrong = np.array([-1, -100, rows, rows + 7, -(1 << 31), (1 << 31) - 1])
+    pick = rng.random(n) < left_out
+    targets[pick] = wrong[rng.integers(0, 6, int(pick.sum()))]
+    return features, table, torch.tensor(targets, device=DEVICE).to(index), torch.tensor(rng.normal(size=n), dtype=torch.float32, device=DEVICE)
+
+
+def bounds(features, table, targets, weights, scale, dtype, gradient=True):
+    """(losses and their bars, gradients and their bars) as numpy arrays."""
+    _, u, least, held = TYPES[dtype]
+    x, w = features.detach().double().cpu().numpy(), table.detach().double().cpu().numpy()
+    y = targets.cpu().numpy()
+    weights = np.asarray(weights, np.float64)
+    inside = (y >= 0) & (y < len(w))
+    x = np.where(inside[:, None], x, 0.0)
+    losses, p, g, dx, dw = R.cross_entropy(x, w, y, scale, weights)
+    size, z = abs(scale) * (np.abs(x) @ np.abs(w).T), scale * (x @ w.T)
+    dz = 2 * (x.shape[1] + 4) * E * size + 3 * E * np.abs(z)
+    off = 2 * dz.max(1) + (80 + len(w) / 16) * E + 8 * E * (np.abs(z).max(1) + np.log(len(w)) + 1)
+    loss_bar = np.where(inside, off, 0.0)
+    if not gradient:
+        return losses, loss_bar
+    dg = np.abs(weights)[:, None] * (p * off[:, None] * 1.01 + 2 * E) * inside[:, None] + u * np.abs(g) * 1.02 + held * np.abs(weights).max(initial=1.0)
+    dg *= inside[:, None]
+    aw, ax, ag, s = np.abs(w), np.abs(x), np.abs(g) + dg, abs(scale)
+    bar_x = s * (dg @ aw + 2 * (len(w) + 4) * E * (ag @ aw)) * (1 + 4 * E)
+    bar_w = s * (dg.T @ ax + 2 * (len(x) + 4) * E * (ag.T @ ax)) * (1 + 4 * E)
+    bar_x += u * (np.abs(dx) + bar_x) + least
+    bar_w += u * (np.abs(dw) + bar_w) + least
+    return losses, loss_bar, dx, bar_x, dw, bar_w
+
+
+def within(name, got, want, bar):
+    got = got.detach().double().cpu().numpy()
+    off = np.abs(got - want)
+    assert got.shape == want.shape and np.all(off <= bar), (name, float(np.max(off / np.maximum(bar, 1e-300))), np.unravel_index(np.argmax(off - bar), off.shape))
+
+
+def check(n, rows, columns, dtype, scale=1.0, reduction='mean', grads=(True, True), **how):
+    import efgs
+    print(f'case cross entropy n={n} rows={rows} columns={columns} {dtype} {reduction} {how}', flush=True)
+    features, table, targets, upstream = inputs(n, rows, columns, dtype, scale=scale, **how)
+    features.requires_grad_(grads[0])
+    table.requires_grad_(grads[1])
+    inside = int(((targets >= 0) & (targets < rows)).sum())
+    if reduction == 'none':
+        weights, up = upstream.double().cpu().numpy(), upstream
+    else:
+        up = upstream[0] if n else torch.tensor(0.7, device=DEVICE)
+        weights = np.full(n, float(up) / (max(inside, 1) if reduction == 'mean' else 1))
+    losses, loss_bar, dx, bar_x, dw, bar_w = bounds(features, table, targets, weights, scale, dtype)
+    loss = efgs.linear_cross_entropy(features, table, targets, scale, reduction)
+    with torch.no_grad():
+        assert torch.equal(efgs.linear_cross_entropy(features, table, targets, scale, reduction), loss)
+    assert loss.dtype == torch.float32
+    if reduction == 'none':
+        within('losses', loss, losses, loss_bar)
+        assert np.all(loss.detach().cpu().numpy()[loss_bar == 0] == 0)
+    else:
+        share = max(inside, 1) if reduction == 'mean' else 1
+        within('loss', loss, np.asarray(losses.sum() / share), np.asarray((loss_bar.sum() + 2 * E * losses.sum()) / share + 1e-300))
+    loss.backward(up)
+    if grads[0]:
+        assert features.grad.dtype == features.dtype
+        within('features', features.grad, dx, bar_x)
+    else:
+        assert features.grad is None
+    if grads[1]:
+        within('table', table.grad, dw, bar_w)
+    else:
+        assert table.grad is None
+    return features, table, targets, up, loss
+
+
+COLUMNS = [1, 3, 8, 15, 16, 33, 45, 64, 65, 72, 128, 136, 200, 257, 333, 512]
+
+
+@pytest.mark.parametrize('columns', COLUMNS)
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+def test_widths(columns, dtype):
+    check(301, 1003, columns, dtype, seed=columns)
+
+
+@pytest.mark.parametrize('n', [1, 2, 15, 16, 17, 64, 65, 255, 256, 257, 1025])
+@pytest.mark.parametrize('columns,dtype', [(8, 'f32'), (96, 'bf16'), (200, 'f32'), (130, 'f16')])
+def test_row_counts(n, columns, dtype):
+    check(n, 517, columns, dtype, seed=n, reduction='none')
+
+
+@pytest.mark.parametrize('rows', [1, 2, 15, 16, 17, 127, 128, 129, 255, 256, 257, 2049, 5003])
+@pytest.mark.parametrize('columns,dtype', [(8, 'f32'), (64, 'bf16'), (300, 'f16')])
+def test_table_sizes(rows, columns, dtype):
+    check(133, rows, columns, dtype, seed=rows, reduction='sum')
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+@pytest.mark.parametrize('scale', [0.25, -1.5, 10.0])
+def test_reductions_and_scales(dtype, reduction, scale):
+    check(260, 700, 72, dtype, scale=scale, reduction=reduction, index=torch.int32)
+
+
+@pytest.mark.parametrize('grads', [(True, False), (False, True)])
+@pytest.mark.parametrize('dtype,columns', [('f32', 8), ('f32', 150), ('bf16', 256)])
+def test_one_gradient_alone(dtype, columns, grads):
+    check(100, 400, columns, dtype, grads=grads)
+
+
+@pytest.mark.parametrize('dtype,columns', [('f32', 8), ('f32', 150), ('bf16', 8), ('bf16', 256), ('f16', 77)])
+@pytest.mark.parametrize('left_out', [0.0, 0.9, 1.0])
+def test_rows_left_out(dtype, columns, left_out):
+    for reduction in ('mean', 'none'):
+        f, t, targets, up, loss = check(600, 300, columns, dtype, left_out=left_out, reduction=reduction)
+        out = (targets < 0) | (targets >= 300)
+        assert torch.all(f.grad[out] == 0)
+        if left_out == 1.0:
+            assert torch.all(loss == 0) and torch.all(t.grad == 0)
+
+
+@pytest.mark.parametrize('dtype,columns', [('f32', 8), ('f32', 150), ('bf16', 8), ('bf16', 256), ('f16', 77)])
+def test_what_stands_in_rows_left_out_reaches_nothing(dtype, columns):
+    import efgs
+    features, table, targets, upstream = inputs(300, 500, columns, dtype, seed=3, left_out=0.3)
+    out = (targets < 0) | (targets >= 500)
+    assert int(out.sum()) > 10
+    results = []
+    for value in (0.0, float('nan'), float('inf'), -float('inf')):
+        x, w, up = features.clone(), table.clone().requires_grad_(), upstream.clone()
+        x[out] = value
+        up[out] = value
+        x.requires_grad_()
+        loss = efgs.linear_cross_entropy(x, w, targets, reduction='none')
+        loss.backward(up)
+        results.append((loss.detach(), x.grad, w.grad))
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('n,rows,columns', [(0, 5, 4), (4, 0, 4), (4, 5, 0), (0, 0, 3), (0, 5, 200)])
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+def test_empty_sides(n, rows, columns, reduction):
+    import efgs
+    x, w = torch.randn(n, columns, device=DEVICE, requires_grad=True), torch.randn(rows, columns, device=DEVICE, requires_grad=True)
+    y = torch.zeros(n, dtype=torch.int64, device=DEVICE)
+    loss = efgs.linear_cross_entropy(x, w, y, reduction=reduction)
+    counted = n if rows else 0   # (rows that count have no columns here: equal logits)
+    each = np.full(n, np.log(rows) if rows else 0.0)
+    want = each if reduction == 'none' else each.sum() / (max(counted, 1) if reduction == 'mean' else 1)
+    assert np.allclose(loss.detach().cpu().numpy(), want, atol=1e-6)
+    loss.sum().backward()
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape and torch.all(x.grad == 0) and torch.all(w.grad == 0)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('columns', [16, 136])
+def test_shapes_strides_and_alignment(dtype, columns):
+    """Leading dimensions, transposed and offset views: the same bits as of contiguous copies."""
+    import efgs
+    kind = TYPES[dtype][0]
+    rng = torch.Generator(DEVICE).manual_seed(5)
+    base = torch.randn(3, columns + 3, 40, generator=rng, device=DEVICE).to(kind)
+    wide = torch.randn(301, columns + 5, generator=rng, device=DEVICE).to(kind)
+    targets = torch.randint(-1, 300, (40, 3), generator=rng, device=DEVICE).t()
+    for x, w in ((base[:, 1:columns + 1].transpose(1, 2), wide[1:, 3:columns + 3]), (base[:, 1:columns + 1].transpose(1, 2), wide[1:, :columns].t().contiguous().t())):
+        results = []
+        for a, b, y in ((x, w, targets), (x.contiguous(), w.contiguous(), targets.contiguous())):
+            a, b = a.detach().requires_grad_(), b.detach().requires_grad_()
+            loss = efgs.linear_cross_entropy(a, b, y, reduction='none')
+            assert loss.shape == (3, 40)
+            results.append((loss.detach(), *torch.autograd.grad(loss, (a, b), torch.ones_like(loss))))
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+def test_far_logits(dtype):
+    """Logits of hundreds, equal ones, and a target that no probability is left for."""
+    import efgs
+    x = torch.zeros(4, 80, device=DEVICE)
+    x[0, 0], x[1, 0], x[2, 1] = 30.0, -30.0, 30.0
+    w = torch.zeros(50, 80, device=DEVICE)
+    w[:, 0] = torch.linspace(-16, 16, 50, device=DEVICE).to(TYPES[dtype][0]).float()
+    y = torch.tensor([0, 0, 7, 49], device=DEVICE)
+    x, w = x.to(TYPES[dtype][0]).requires_grad_(), w.to(TYPES[dtype][0]).requires_grad_()
+    loss = efgs.linear_cross_entropy(x, w, y, reduction='none')
+    losses, bar, dx, bar_x, dw, bar_w = bounds(x, w, y, np.ones(4), 1.0, dtype)
+    within('losses', loss, losses, bar)
+    loss.sum().backward()
+    within('features', x.grad, dx, bar_x)
+    within('table', w.grad, dw, bar_w)
+
+
+@pytest.mark.parametrize('dtype,columns', [('f32', 8), ('f32', 150), ('bf16', 8), ('bf16', 256), ('f16', 256)])
+def test_infinities_and_nan_are_passed_on(dtype, columns):
+    import efgs
+    features, table, targets, _ = inputs(70, 300, columns, dtype, left_out=0.0)
+    features[3, 0] = float('nan')
+    features.requires_grad_()
+    loss = efgs.linear_cross_entropy(features, table, targets, reduction='none')
+    assert bool(torch.isnan(loss[3])) and int(torch.isnan(loss).sum()) == 1
+    loss.sum().backward()
+    assert torch.all(torch.isnan(features.grad[3])) and int(torch.isnan(features.grad).any(1).sum()) == 1
+
+
+@pytest.mark.parametrize('dtype,columns', [('f32', 8), ('f32', 150), ('bf16', 16), ('bf16', 256), ('f16', 256)])
+def test_the_same_bits_every_time(dtype, columns):
+    import efgs
+    features, table, targets, upstream = inputs(777, 3001, columns, dtype)
+    features.requires_grad_()
+    table.requires_grad_()
+    first = None
+    for _ in range(3):
+        loss = efgs.linear_cross_entropy(features, table, targets, reduction='none')
+        now = (loss.detach(), *torch.autograd.grad(loss, (features, table), upstream))
+        first = first or now
+        for a, b in zip(first, now):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dtype,columns', [('f32', 8), ('f32', 150), ('bf16', 256)])
+def test_a_captured_step_replays(dtype, columns):
+    import efgs
+    features, table, targets, _ = inputs(300, 1000, columns, dtype)
+    features.requires_grad_()
+    table.requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            efgs.linear_cross_entropy(features, table, targets).backward()
+            features.grad = table.grad = None
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = efgs.linear_cross_entropy(features, table, targets)
+        loss.backward()
+    held = (features.grad, table.grad)
+    for seed in range(4):
+        other = inputs(300, 1000, columns, dtype, seed=seed + 10, left_out=0.2 * seed)
+        with torch.no_grad():
+            features.copy_(other[0])
+            table.copy_(other[1])
+            targets.copy_(other[2])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (loss.detach(), *held)]
+        a, b = features.detach().clone().requires_grad_(), table.detach().clone().requires_grad_()
+        eager = efgs.linear_cross_entropy(a, b, targets)
+        eager.backward()
+        for x, y in zip(got, (eager.detach(), a.grad, b.grad)):
+            assert torch.equal(x, y)
+
+
+def test_two_calls_on_two_streams():
+    import efgs
+    work = [inputs(500, 2000, c, d, seed=k) for k, (c, d) in enumerate(((8, 'f32'), (256, 'bf16'), (150, 'f32'), (128, 'f16')))]
+    def step(features, table, targets, upstream):
+        a, b = features.detach().requires_grad_(), table.detach().requires_grad_()
+        loss = efgs.linear_cross_entropy(a, b, targets, reduction='none')
+        return (loss.detach(), *torch.autograd.grad(loss, (a, b), upstream))
+    alone = [step(*w) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    together = []
+    for s, w in zip(streams, work):
+        with torch.cuda.stream(s):
+            together.append(step(*w))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, together):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+def test_an_in_place_change_of_the_table_is_refused_and_of_the_features_does_not_matter():
+    import efgs
+    features, table, targets, _ = inputs(50, 100, 16, 'f32')
+    x, w = features.clone().requires_grad_(), table.clone().requires_grad_()
+    want = torch.autograd.grad(efgs.linear_cross_entropy(x, w, targets), (x, w))
+    y = x * 1.0
+    loss = efgs.linear_cross_entropy(y, w, targets)
+    with torch.no_grad():
+        y.zero_()
+    got = torch.autograd.grad(loss, (y, w), retain_graph=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        w.zero_()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(loss, (y, w))
+
+
+def test_second_derivatives_raise():
+    import efgs
+    features, table, targets, _ = inputs(20, 30, 16, 'f32')
+    features.requires_grad_()
+    up = torch.ones((), device=DEVICE, requires_grad=True)
+    grad = torch.autograd.grad(efgs.linear_cross_entropy(features, table, targets), features, up, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        torch.autograd.grad(grad.sum(), up)
+
+
+def test_pieces_and_lists_of_many_rows():
+    """More rows than a block counts by itself, more of the table than a piece holds."""
+    check(20_001, 600, 8, 'f32', seed=9)
+    check(17_000, 300, 130, 'f32', seed=9, reduction='none')
+    check(17_000, 300, 64, 'bf16', seed=10)
