@@ -30,6 +30,7 @@ SOURCES = [
     ('adamw.hip', ['-ffp-contract=off']),
     ('embedding.hip', []),
     ('cross_entropy.hip', []),
+    ('cross_entropy_16.hip', []),
     ('dropout.hip', ['-ffp-contract=off']),
     ('balance.hip', []),
     ('densification.hip', ['-ffp-contract=off']),

@@ -1,0 +1,47 @@
+// What the sources of the cross entropy share: the products' arguments and tiles.
+#pragma once
+#include "internal.h"
+
+namespace efgs {
+
+constexpr uint32_t entropy_none = 0xffffffffu;
+constexpr uint32_t entropy_row_tile = 256;     // packed rows come in multiples of it
+constexpr uint32_t entropy_column_tile = 64;   // so do their columns
+constexpr float entropy_half_range = 32768.0f; // float16: what upstream gradients of the logits are held times
+
+// C(i, j) = sum_k A(i, k) B(k, j); i is the table row in the first two products and the column in the gradients, j the packed row and, in
+// the table's gradient, the table row.
+enum EntropyProduct { entropy_logits, entropy_upstream, entropy_features_gradient, entropy_table_gradient };
+
+struct EntropyProductArgs {
+    const void* a;
+    const void* b;
+    uint64_t a_stride, b_stride;   // elements from row to row as they lie in memory
+    uint32_t i_end, j_end, k_end;  // (j of all but the table's gradient, and its k: at most *count)
+    uint32_t a_columns;            // of a's rows in memory (wide products: a multiple of 8)
+    uint32_t i_tiles;
+    uint32_t j_first;              // of the launch
+    uint32_t splits;               // of k, over gridDim.y
+    const uint32_t* count;         // packed rows
+    float to_log2;                 // scale log2 e
+    float2* partial;               // logits: i_tiles x slab_rows (maximum, sum of exponentials), from row j_first on
+    float* target_logit;
+    const uint32_t* target;
+    const float* lse;
+    const float* weight;
+    uint32_t first_row;            // of the piece in the table
+    void* piece;                   // upstream gradients of the logits: padded rows x piece_stride
+    uint64_t piece_stride;
+    float* slab;                   // splits x slab_rows x slab_stride
+    uint64_t slab_stride, slab_rows;
+    bool add;
+    void* out;                     // table's gradient without splits: its rows from the piece's first
+    uint64_t out_stride;
+    const float* factor;
+};
+
+// 16-bit types, tiles of 256 x 256: rows of 16-byte aligned memory, strides in multiples of 8 elements
+constexpr uint32_t entropy_wide_tile = 256;
+void launch_entropy_wide(EntropyProduct product, int type, const EntropyProductArgs& a, uint32_t j_tiles, hipStream_t s);
+
+}  // namespace efgs

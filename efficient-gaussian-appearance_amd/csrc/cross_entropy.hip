@@ -11,7 +11,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "internal.h"
+#include "cross_entropy.h"
 
 namespace efgs {
 
@@ -20,9 +20,7 @@ namespace {
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr float log2_e = 1.4426950408889634f, ln_2 = 0.6931471805599453f, infinity = __builtin_inff();
-constexpr uint32_t none = 0xffffffffu;
-constexpr uint32_t row_tile = 256;        // packed rows come in multiples of it
-constexpr uint32_t column_tile = 64;      // so do their columns
+constexpr uint32_t none = entropy_none, row_tile = entropy_row_tile, column_tile = entropy_column_tile;
 constexpr uint32_t rank_block = 1024;
 constexpr uint32_t count_alone = 16384;   // largest list that every block counts by itself
 
@@ -34,15 +32,12 @@ uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 
 struct Packing {
     const void* targets;
-    const void* features;
-    uint64_t feature_stride;
-    uint32_t n, padded, rows, columns, padded_columns, target_bytes;
+    uint32_t n, padded, rows, target_bytes;
     uint32_t* chunk_counts;  // null: short lists
     uint32_t* count;         // rows that count
     uint32_t* row_of;        // packed row -> row
     uint32_t* packed_of;     // row -> packed row, or none
     uint32_t* target;        // of a packed row; none past them
-    void* packed;            // padded x padded_columns
 };
 
 __device__ __forceinline__ uint32_t target_at(const Packing& a, uint32_t i) {
@@ -106,62 +101,43 @@ __global__ __launch_bounds__(rank_block) void entropy_rank_kernel(Packing a) {
     if (i == 0) *a.count = all;
 }
 
-// Sixteen bytes a thread; rows past those that count are zeros, up to a whole tile.
+struct Copying {
+    const void* from;
+    uint64_t stride;
+    uint32_t rows, columns, padded_columns;
+    const uint32_t* count;   // packed rows, or null: all
+    const uint32_t* row_of;
+    void* to;
+};
+
+// Rows with their columns padded by zeros, sixteen bytes a thread. Of packed rows, those past the ones that count are zeros, up to a whole tile.
 template <typename T>
-__global__ __launch_bounds__(256) void entropy_pack_kernel(Packing a) {
+__global__ __launch_bounds__(256) void entropy_copy_kernel(Copying a) {
     constexpr uint32_t W = 16 / sizeof(T);
-    const uint32_t parts = a.padded_columns / W, end = (*a.count + row_tile - 1) / row_tile * row_tile;
+    const uint32_t parts = a.padded_columns / W, end = a.count ? (*a.count + row_tile - 1) / row_tile * row_tile : a.rows;
     const uint64_t items = static_cast<uint64_t>(end) * parts, step = static_cast<uint64_t>(gridDim.x) * 256u;
     for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < items; t += step) {
         const uint32_t m = static_cast<uint32_t>(t / parts), column = static_cast<uint32_t>(t - static_cast<uint64_t>(m) * parts) * W;
-        const uint32_t row = a.row_of[m];
+        const uint32_t row = a.row_of ? a.row_of[m] : m;
         Part<T, W> v{};
         if (row != none && column < a.columns) {
-            const T* const p = static_cast<const T*>(a.features) + row * a.feature_stride + column;
+            const T* const p = static_cast<const T*>(a.from) + row * a.stride + column;
             if (column + W <= a.columns) v = *reinterpret_cast<const Part<T, W>*>(p);
             else
 #pragma unroll
                 for (uint32_t k = 0; k < W; k++)
                     if (column + k < a.columns) v[k] = p[k];
         }
-        *reinterpret_cast<Part<T, W>*>(static_cast<T*>(a.packed) + t * W) = v;
+        *reinterpret_cast<Part<T, W>*>(static_cast<T*>(a.to) + t * W) = v;
     }
 }
 
 // ---- matrix products in 32 bits ----------------------------------------------------------------------------------------
-// C(i, j) = sum_k A(i, k) B(k, j), 128 x 128 to a block of four waves (64 x 64 each), v_mfma_f32_16x16x4_f32. A lane's results are
+// 128 x 128 results to a block of four waves (64 x 64 each), v_mfma_f32_16x16x4_f32. A lane's results are
 // four consecutive i at one j: i is the table row in the logits, so that a row's maximum and sum stay mostly in
 // registers, and the column in the gradients, which are stored along it.
 
 constexpr uint32_t tile = 128, tile_k = 16, tile_pitch = tile + 4, tile_block = 256;
-
-enum Product { logits, upstream_piece, features_gradient, table_gradient };
-
-struct ProductArgs {
-    const void* a;
-    const void* b;
-    uint64_t a_stride, b_stride;   // elements from row to row as they lie in memory
-    uint32_t i_end, j_end, k_end;  // (j of the logits and of the rows' gradient, k of the table's: at most *count)
-    uint32_t i_tiles;
-    uint32_t j_first;              // of the launch
-    uint32_t splits;               // of k, over gridDim.y
-    const uint32_t* count;
-    float to_log2;                 // scale log2 e
-    float2* partial;               // logits: i_tiles x slab_rows (maximum, sum of exponentials), from row j_first on
-    float* target_logit;
-    const uint32_t* target;
-    const float* lse;
-    const float* weight;
-    uint32_t first_row;            // of the piece in the table
-    float* piece;                  // upstream_piece: padded x piece_stride
-    uint64_t piece_stride;
-    float* slab;                   // splits x j_slab x slab_stride
-    uint64_t slab_stride, slab_rows;
-    bool add;
-    void* out;                     // table_gradient without splits: the gradient's rows from the piece's first
-    uint64_t out_stride;
-    const float* factor;
-};
 
 // eight consecutive values, those from `valid` on zero
 template <typename T>
@@ -196,17 +172,17 @@ __device__ __forceinline__ void store_tile(float (*lds)[tile_pitch], const float
     }
 }
 
-template <typename T, Product P>
-__global__ __launch_bounds__(tile_block) void entropy_product_kernel(ProductArgs a) {
-    using B = std::conditional_t<P == logits || P == upstream_piece, T, float>;
-    constexpr bool a_along_k = P == logits || P == upstream_piece, b_along_k = P != table_gradient;
+template <typename T, EntropyProduct P>
+__global__ __launch_bounds__(tile_block) void entropy_product_kernel(EntropyProductArgs a) {
+    using B = std::conditional_t<P == entropy_logits || P == entropy_upstream, T, float>;
+    constexpr bool a_along_k = P == entropy_logits || P == entropy_upstream, b_along_k = P != entropy_table_gradient;
     __shared__ float lds_a[tile_k][tile_pitch], lds_b[tile_k][tile_pitch];
     __shared__ float2 joined[2][tile];
     const uint32_t i0 = blockIdx.x % a.i_tiles * tile, j0 = a.j_first + blockIdx.x / a.i_tiles * tile;
     const uint32_t count = *a.count;
-    const uint32_t j_end = P == table_gradient ? a.j_end : count;
-    if (j0 >= (P == upstream_piece ? (count + row_tile - 1) / row_tile * row_tile : j_end)) return;
-    const uint32_t k_all = P == table_gradient ? count : a.k_end;
+    const uint32_t j_end = P == entropy_table_gradient ? a.j_end : count;
+    if (j0 >= (P == entropy_upstream ? (count + row_tile - 1) / row_tile * row_tile : j_end)) return;
+    const uint32_t k_all = P == entropy_table_gradient ? count : a.k_end;
     const uint32_t k_each = (k_all / a.splits + tile_k) / tile_k * tile_k, k_first = min(blockIdx.y * k_each, k_all), k_end = min(k_first + k_each, k_all);
     const uint32_t lane = threadIdx.x & 63u, e = lane & 15u, q = lane >> 4, wave = threadIdx.x >> 6, wi = wave & 1u, wj = wave >> 1;
     floatx4 acc[4][4] = {};
@@ -239,7 +215,7 @@ __global__ __launch_bounds__(tile_block) void entropy_product_kernel(ProductArgs
         }
     }
     const uint32_t i_lane = i0 + wi * 64 + 4 * q, j_lane = j0 + wj * 64 + e;  // results: i_lane + 16 ti + r, j_lane + 16 tj
-    if constexpr (P == logits) {
+    if constexpr (P == entropy_logits) {
 #pragma unroll
         for (uint32_t tj = 0; tj < 4; tj++) {
             const uint32_t j = j_lane + tj * 16, target = a.target[j];
@@ -272,7 +248,7 @@ __global__ __launch_bounds__(tile_block) void entropy_product_kernel(ProductArgs
             const float sum = x.y * __builtin_amdgcn_exp2f(x.x - from) + y.y * __builtin_amdgcn_exp2f(y.x - from);
             a.partial[(i0 / tile) * a.slab_rows + (j0 - a.j_first) + threadIdx.x] = make_float2(top, sum);
         }
-    } else if constexpr (P == upstream_piece) {
+    } else if constexpr (P == entropy_upstream) {
 #pragma unroll
         for (uint32_t tj = 0; tj < 4; tj++) {
             const uint32_t j = j_lane + tj * 16, target = a.target[j];
@@ -287,11 +263,11 @@ __global__ __launch_bounds__(tile_block) void entropy_product_kernel(ProductArgs
                     const float p = __builtin_amdgcn_exp2f(acc[ti][tj][r] * a.to_log2 - lse) - (a.first_row + i + r == target ? 1.0f : 0.0f);
                     g[r] = counts && i + r < a.i_end ? p * weight : 0.0f;
                 }
-                *reinterpret_cast<floatx4*>(a.piece + j * a.piece_stride + i) = g;
+                *reinterpret_cast<floatx4*>(static_cast<float*>(a.piece) + j * a.piece_stride + i) = g;
             }
         }
     } else {
-        const bool direct = P == table_gradient && a.out;
+        const bool direct = P == entropy_table_gradient && a.out;
         const float factor = direct ? *a.factor : 1.0f;
 #pragma unroll
         for (uint32_t tj = 0; tj < 4; tj++) {
@@ -392,14 +368,34 @@ struct WeightArgs {
     uint32_t padded;
     bool each, mean;
     float scale;
-    float* weight;           // of packed rows
+    float held;              // what the logits' gradients are held times
+    float* weight;           // of packed rows, times `held`
     float* factor;           // of the sums
 };
 
 __global__ __launch_bounds__(256) void entropy_weights_kernel(WeightArgs a) {
     const uint32_t m = blockIdx.x * 256 + threadIdx.x, count = *a.count;
-    if (m < a.padded) a.weight[m] = m >= count ? 0.0f : a.each ? a.upstream[a.row_of[m]] : 1.0f;
-    if (m == 0) *a.factor = a.each ? a.scale : a.scale * *a.upstream / (a.mean ? static_cast<float>(max(count, 1u)) : 1.0f);
+    if (m < a.padded) a.weight[m] = m >= count ? 0.0f : (a.each ? a.upstream[a.row_of[m]] : 1.0f) * a.held;
+    if (m == 0) *a.factor = (a.each ? a.scale : a.scale * *a.upstream / (a.mean ? static_cast<float>(max(count, 1u)) : 1.0f)) / a.held;
+}
+
+// float16, a weight for each row: the weights over the power of two at or above the largest, so that a product of weight and probability
+// keeps to the type's range. One block.
+__global__ __launch_bounds__(1024) void entropy_half_weights_kernel(WeightArgs a) {
+    __shared__ float lds[16];
+    const uint32_t count = *a.count;
+    float top = 0.0f;
+    for (uint32_t m = threadIdx.x; m < count; m += 1024) top = fmaxf(top, fabsf(a.upstream[a.row_of[m]]));
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = top;
+    __syncthreads();
+    for (uint32_t w = 0; w < 16; w++) top = fmaxf(top, lds[w]);
+    int exponent = 0;
+    if (top > 0.0f && top < infinity) frexpf(top, &exponent);  // (else zeros, or infinities and NaN either way)
+    for (uint32_t m = threadIdx.x; m < a.padded; m += 1024)
+        a.weight[m] = m < count ? ldexpf(a.upstream[a.row_of[m]], -exponent) * a.held : 0.0f;
+    if (threadIdx.x == 0) *a.factor = ldexpf(a.scale / a.held, exponent);
 }
 
 // sums of the splits, scaled; rows without a packed one are zeros
@@ -439,6 +435,11 @@ class Carver {
 
 uint32_t type_bytes(int type) { return type == type_float ? 4 : 2; }
 
+bool wide(const EntropyArgs& a) { return a.type != type_float; }
+bool table_is_copied(const EntropyArgs& a);
+
+uint32_t tile_of(const EntropyArgs& a) { return wide(a) ? entropy_wide_tile : tile; }
+
 struct Saved {
     uint32_t* count;
     uint32_t* row_of;
@@ -471,51 +472,67 @@ struct ForwardScratch {
     float2* partial;
     float* target_logit;
     double* sums;
+    void* copy;        // of the table, or null
+    bool copied;
     uint32_t tiles, rows_at_once;
     size_t bytes;
     ForwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
-        tiles = div_up(a.rows, tile);
+        tiles = div_up(a.rows, tile_of(a));
         chunk_counts = c.take<uint32_t>(div_up(s.padded, rank_block));
         const uint64_t most = std::min(partial_bytes / sizeof(float2), most_blocks * tile) / std::max(tiles, 1u);
         rows_at_once = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(most / row_tile * row_tile, row_tile), s.padded));
         partial = c.take<float2>(static_cast<uint64_t>(tiles) * rows_at_once);
         target_logit = c.take<float>(s.padded);
         sums = c.take<double>(s.padded / join_rows);
+        copy = table_is_copied(a) ? c.take<char>(static_cast<uint64_t>(a.rows) * s.padded_columns * type_bytes(a.type)) : nullptr;
+        copied = table_is_copied(a);
         bytes = c.used();
     }
 };
 
-// how often a product's k is split so that its blocks fill the GPU
-uint32_t splits_for(uint64_t tiles, uint64_t k) {
-    const uint64_t wanted = tiles >= 512 ? 1 : (1024 + tiles - 1) / std::max<uint64_t>(tiles, 1);
-    return static_cast<uint32_t>(std::max<uint64_t>(1, std::min({wanted, k / 256, static_cast<uint64_t>(64)})));
+// How often a product's k is split so that its blocks fill the GPU: `at_once` blocks run together, a split costs its partial results once more.
+uint32_t splits_for(uint64_t tiles, uint64_t k, uint64_t at_once) {
+    uint32_t best = 1;
+    double least = 1e30;
+    for (uint32_t s = 1; s <= 64 && (s == 1 || k / s >= 256); s++) {
+        const double cost = static_cast<double>((tiles * s + at_once - 1) / at_once) / s * (1.0 + 0.02 * (s - 1));
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
 }
 
 struct BackwardScratch {
     float* weight;
     float* factor;
-    float* piece;
+    void* piece;
     float* features_slab;
     float* table_slab;
+    void* copy;              // of the table, or null
+    bool copied;
     uint32_t piece_rows, pieces;
     uint32_t features_splits, table_splits;
     size_t bytes;
     BackwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
-        const uint64_t most = std::max<uint64_t>(piece_bytes / (static_cast<uint64_t>(s.padded) * sizeof(float)) / 256 * 256, 256);
+        const uint64_t most = std::max<uint64_t>(piece_bytes / (static_cast<uint64_t>(s.padded) * type_bytes(a.type)) / 256 * 256, 256);
         const uint64_t all = round_up(std::max(a.rows, 1u), 256);
         pieces = div_up(all, std::min(most, all));
         piece_rows = static_cast<uint32_t>(round_up(div_up(all, pieces), 256));
         pieces = div_up(all, piece_rows);
-        const uint64_t column_tiles = div_up(std::max(a.columns, 1u), tile);
-        features_splits = splits_for(s.padded / tile * column_tiles, piece_rows);
-        table_splits = splits_for(piece_rows / tile * column_tiles, s.padded);
+        const uint64_t side = tile_of(a), column_tiles = div_up(std::max(a.columns, 1u), side), at_once = wide(a) ? 256 : 512;
+        features_splits = splits_for(s.padded / side * column_tiles, piece_rows, at_once);
+        table_splits = splits_for(piece_rows / side * column_tiles, s.padded, at_once);
         weight = c.take<float>(s.padded);
         factor = c.take<float>(1);
-        piece = c.take<float>(static_cast<uint64_t>(s.padded) * piece_rows);
+        piece = c.take<char>(static_cast<uint64_t>(s.padded) * piece_rows * type_bytes(a.type));
         features_slab = c.take<float>(static_cast<uint64_t>(features_splits) * s.padded * s.padded_columns);
         table_slab = table_splits > 1 ? c.take<float>(static_cast<uint64_t>(table_splits) * piece_rows * s.padded_columns) : nullptr;
+        copied = table_is_copied(a);
+        copy = copied ? c.take<char>(static_cast<uint64_t>(a.rows) * s.padded_columns * type_bytes(a.type)) : nullptr;
         bytes = c.used();
     }
 };
@@ -531,29 +548,62 @@ constexpr uint32_t copy_blocks = 1u << 16;
 
 uint32_t copy_grid(uint64_t items) { return static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>((items + 255) / 256, 1), copy_blocks)); }
 
+void launch_copy(const EntropyArgs& a, const Copying& c, uint64_t most_rows, hipStream_t stream) {
+    if (c.padded_columns == 0 || most_rows == 0) return;
+    const uint32_t blocks = copy_grid(most_rows * c.padded_columns * type_bytes(a.type) / 16);
+    with_type(a.type, [&](auto t) { hipLaunchKernelGGL(entropy_copy_kernel<decltype(t)>, dim3(blocks), dim3(256), 0, stream, c); });
+}
+
 void launch_packing(const EntropyArgs& a, const Saved& s, uint32_t* chunk_counts, hipStream_t stream) {
     Packing p{};
     p.targets = a.targets;
-    p.features = a.features;
-    p.feature_stride = a.feature_stride;
     p.n = a.n;
     p.padded = s.padded;
     p.rows = a.rows;
-    p.columns = a.columns;
-    p.padded_columns = s.padded_columns;
     p.target_bytes = static_cast<uint32_t>(a.target_bytes);
     p.chunk_counts = a.n > count_alone ? chunk_counts : nullptr;
     p.count = s.count;
     p.row_of = s.row_of;
     p.packed_of = s.packed_of;
     p.target = s.target;
-    p.packed = s.packed;
     const dim3 chunks(div_up(s.padded, rank_block));
     if (p.chunk_counts) hipLaunchKernelGGL(entropy_count_kernel, chunks, dim3(rank_block), 0, stream, p);
     hipLaunchKernelGGL(entropy_rank_kernel, chunks, dim3(rank_block), 0, stream, p);
-    if (a.columns == 0) return;
-    const uint32_t blocks = copy_grid(static_cast<uint64_t>(s.padded) * s.padded_columns * type_bytes(a.type) / 16);
-    with_type(a.type, [&](auto t) { hipLaunchKernelGGL(entropy_pack_kernel<decltype(t)>, dim3(blocks), dim3(256), 0, stream, p); });
+    launch_copy(a, Copying{a.features, a.feature_stride, a.n, a.columns, s.padded_columns, s.count, s.row_of, s.packed}, s.padded, stream);
+}
+
+// A table whose rows the wide products cannot read as they lie: another alignment than 16 bytes, columns that 16 bytes do not divide, rows that
+// overlap, or so far apart that 32 bits of bytes do not reach over a tile. A copy takes its place.
+bool table_is_copied(const EntropyArgs& a) {
+    return wide(a) && a.rows > 0 && (reinterpret_cast<uintptr_t>(a.table) % 16 != 0 || a.columns % 8 != 0 || a.table_stride % 8 != 0 ||
+                                     a.table_stride < a.columns || a.table_stride >= 1ull << 22);
+}
+
+// the table, or its copy in `room`
+struct Table {
+    const void* rows;
+    uint64_t stride;
+    uint32_t columns;
+};
+
+Table table_of(const EntropyArgs& a, const Saved& s, void* room, hipStream_t stream) {
+    if (!room) return {a.table, a.table_stride, a.columns};
+    launch_copy(a, Copying{a.table, a.table_stride, a.rows, a.columns, s.padded_columns, nullptr, nullptr, room}, a.rows, stream);
+    return {room, s.padded_columns, s.padded_columns};
+}
+
+void launch_product(EntropyProduct product, const EntropyArgs& a, const EntropyProductArgs& p, uint32_t j, hipStream_t stream) {
+    if (wide(a)) {
+        launch_entropy_wide(product, a.type, p, div_up(j, entropy_wide_tile), stream);
+        return;
+    }
+    const dim3 grid(p.i_tiles * div_up(j, tile), p.splits);
+    switch (product) {
+        case entropy_logits: hipLaunchKernelGGL((entropy_product_kernel<float, entropy_logits>), grid, dim3(tile_block), 0, stream, p); break;
+        case entropy_upstream: hipLaunchKernelGGL((entropy_product_kernel<float, entropy_upstream>), grid, dim3(tile_block), 0, stream, p); break;
+        case entropy_features_gradient: hipLaunchKernelGGL((entropy_product_kernel<float, entropy_features_gradient>), grid, dim3(tile_block), 0, stream, p); break;
+        case entropy_table_gradient: hipLaunchKernelGGL((entropy_product_kernel<float, entropy_table_gradient>), grid, dim3(tile_block), 0, stream, p); break;
+    }
 }
 
 }  // namespace
@@ -573,16 +623,19 @@ bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void
     const Saved s(a, saved);
     const ForwardScratch f(a, s, scratch);
     launch_packing(a, s, f.chunk_counts, stream);
+    const Table table = table_of(a, s, f.copied ? f.copy : nullptr, stream);
     for (uint32_t first = 0; first < s.padded; first += f.rows_at_once) {
         const uint32_t rows = std::min(s.padded - first, f.rows_at_once);
         if (a.rows > 0) {
-            ProductArgs p{};
-            p.a = a.table;
-            p.a_stride = a.table_stride;
+            EntropyProductArgs p{};
+            p.a = table.rows;
+            p.a_stride = table.stride;
+            p.a_columns = table.columns;
             p.b = s.packed;
             p.b_stride = s.padded_columns;
             p.i_end = a.rows;
-            p.k_end = a.columns;
+            p.j_end = rows;
+            p.k_end = table.columns;
             p.i_tiles = f.tiles;
             p.j_first = first;
             p.splits = 1;
@@ -592,9 +645,7 @@ bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void
             p.slab_rows = rows;
             p.target_logit = f.target_logit;
             p.target = s.target;
-            with_type(a.type, [&](auto t) {
-                hipLaunchKernelGGL((entropy_product_kernel<decltype(t), logits>), dim3(f.tiles * (rows / tile)), dim3(tile_block), 0, stream, p);
-            });
+            launch_product(entropy_logits, a, p, rows, stream);
         }
         const JoinArgs j{f.partial, f.tiles, first, rows, a.n, s.count, s.row_of, s.packed_of, f.target_logit, s.lse, a.each ? loss : nullptr, f.sums};
         hipLaunchKernelGGL(entropy_join_kernel, dim3(rows / join_rows), dim3(join_rows * join_parts), 0, stream, j);
@@ -609,70 +660,75 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
     if (a.columns == 0) return true;
     const Saved s(a, const_cast<void*>(saved));
     const BackwardScratch w(a, s, scratch);
-    const WeightArgs weights{upstream, s.count, s.row_of, s.padded, a.each, a.mean, a.scale, w.weight, w.factor};
-    hipLaunchKernelGGL(entropy_weights_kernel, dim3(div_up(s.padded, 256)), dim3(256), 0, stream, weights);
-    const uint32_t row_tiles = s.padded / tile, column_tiles = div_up(a.columns, tile);
+    const Table table = table_of(a, s, w.copied ? w.copy : nullptr, stream);
+    const bool half = a.type == type_half;
+    const WeightArgs weights{upstream, s.count, s.row_of, s.padded, a.each, a.mean, a.scale, half ? entropy_half_range : 1.0f, w.weight, w.factor};
+    if (half && a.each) hipLaunchKernelGGL(entropy_half_weights_kernel, dim3(1), dim3(1024), 0, stream, weights);
+    else hipLaunchKernelGGL(entropy_weights_kernel, dim3(div_up(s.padded, 256)), dim3(256), 0, stream, weights);
+    const uint32_t side = tile_of(a), column_tiles = div_up(a.columns, side), bytes = type_bytes(a.type);
     for (uint32_t piece = 0; piece < w.pieces && a.rows > 0; piece++) {
         const uint32_t first = piece * w.piece_rows, rows = std::min(a.rows - first, w.piece_rows);
-        with_type(a.type, [&](auto t) {
-            using T = decltype(t);
-            const T* const table = static_cast<const T*>(a.table) + first * a.table_stride;
-            ProductArgs p{};
-            p.a = table;
-            p.a_stride = a.table_stride;
-            p.b = s.packed;
-            p.b_stride = s.padded_columns;
-            p.i_end = rows;
-            p.k_end = a.columns;
-            p.i_tiles = w.piece_rows / tile;
-            p.splits = 1;
-            p.count = s.count;
-            p.to_log2 = a.scale * log2_e;
-            p.target = s.target;
-            p.lse = s.lse;
-            p.weight = w.weight;
-            p.first_row = first;
-            p.piece = w.piece;
-            p.piece_stride = w.piece_rows;
-            hipLaunchKernelGGL((entropy_product_kernel<T, upstream_piece>), dim3(p.i_tiles * row_tiles), dim3(tile_block), 0, stream, p);
-            ProductArgs x{};
-            x.count = s.count;
-            x.i_end = a.columns;
-            x.i_tiles = column_tiles;
-            x.slab_stride = s.padded_columns;
-            if (grad_features) {
-                x.a = table;
-                x.a_stride = a.table_stride;
-                x.b = w.piece;
-                x.b_stride = w.piece_rows;
-                x.k_end = rows;
-                x.splits = w.features_splits;
-                x.slab = w.features_slab;
-                x.slab_rows = s.padded;
-                x.add = piece > 0;
-                hipLaunchKernelGGL((entropy_product_kernel<T, features_gradient>), dim3(column_tiles * row_tiles, x.splits), dim3(tile_block), 0, stream, x);
-            }
-            if (grad_table) {
-                T* const out = static_cast<T*>(grad_table) + static_cast<uint64_t>(first) * a.columns;
-                x.a = s.packed;
-                x.a_stride = s.padded_columns;
-                x.b = w.piece;
-                x.b_stride = w.piece_rows;
-                x.j_end = rows;
-                x.splits = w.table_splits;
-                x.slab = w.table_slab;
-                x.slab_rows = w.piece_rows;
-                x.add = false;
-                x.out = x.splits > 1 ? nullptr : out;
-                x.out_stride = a.columns;
-                x.factor = w.factor;
-                hipLaunchKernelGGL((entropy_product_kernel<T, table_gradient>), dim3(column_tiles * div_up(rows, tile), x.splits), dim3(tile_block), 0,
-                                   stream, x);
-                if (x.splits > 1)
+        const void* const part = static_cast<const char*>(table.rows) + first * table.stride * bytes;
+        EntropyProductArgs p{};
+        p.a = part;
+        p.a_stride = table.stride;
+        p.a_columns = table.columns;
+        p.b = s.packed;
+        p.b_stride = s.padded_columns;
+        p.i_end = rows;
+        p.j_end = s.padded;
+        p.k_end = table.columns;
+        p.i_tiles = div_up(rows, side);
+        p.splits = 1;
+        p.count = s.count;
+        p.to_log2 = a.scale * log2_e;
+        p.target = s.target;
+        p.lse = s.lse;
+        p.weight = w.weight;
+        p.first_row = first;
+        p.piece = w.piece;
+        p.piece_stride = w.piece_rows;
+        launch_product(entropy_upstream, a, p, s.padded, stream);
+        EntropyProductArgs x{};
+        x.count = s.count;
+        x.i_end = a.columns;
+        x.i_tiles = column_tiles;
+        x.slab_stride = s.padded_columns;
+        x.b = w.piece;
+        x.b_stride = w.piece_rows;
+        if (grad_features) {
+            x.a = part;
+            x.a_stride = table.stride;
+            x.a_columns = table.columns;
+            x.j_end = s.padded;
+            x.k_end = rows;
+            x.splits = w.features_splits;
+            x.slab = w.features_slab;
+            x.slab_rows = s.padded;
+            x.add = piece > 0;
+            launch_product(entropy_features_gradient, a, x, s.padded, stream);
+        }
+        if (grad_table) {
+            void* const out = static_cast<char*>(grad_table) + static_cast<uint64_t>(first) * a.columns * bytes;
+            x.a = s.packed;
+            x.a_stride = s.padded_columns;
+            x.a_columns = s.padded_columns;
+            x.j_end = rows;
+            x.splits = w.table_splits;
+            x.slab = w.table_slab;
+            x.slab_rows = w.piece_rows;
+            x.add = false;
+            x.out = x.splits > 1 ? nullptr : out;
+            x.out_stride = a.columns;
+            x.factor = w.factor;
+            launch_product(entropy_table_gradient, a, x, rows, stream);
+            if (x.splits > 1)
+                with_type(a.type, [&](auto t) {
+                    using T = decltype(t);
                     hipLaunchKernelGGL(entropy_gather_kernel<T>, dim3(copy_grid(static_cast<uint64_t>(rows) * a.columns)), dim3(256), 0, stream,
-                                       w.table_slab, w.piece_rows, s.padded_columns, x.splits, nullptr, rows, a.columns, w.factor, out);
-            }
-        });
+                                       w.table_slab, w.piece_rows, s.padded_columns, x.splits, nullptr, rows, a.columns, w.factor, static_cast<T*>(out));
+                });
+        }
     }
     if (grad_features && a.n > 0)
         with_type(a.type, [&](auto t) {

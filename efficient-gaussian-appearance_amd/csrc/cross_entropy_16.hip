@@ -1,0 +1,304 @@
+// The cross entropy's matrix products for bfloat16 and float16 on v_mfma_f32_16x16x32: 256 x 256 results to a block of eight waves (2 along i,
+// 4 along j, 128 x 64 each), 64 of k at a time.
+//
+// Operand tiles go from memory to LDS past the registers (16 bytes a lane), two stages of 64 KB: while a stage is multiplied
+// the next one is on its way, with one barrier a stage. An operand whose memory runs along k lies in rows of 64 k (128 bytes), its 16-byte
+// chunks exchanged by the row's low bits, so that the reads of eight rows meet all banks; one whose memory runs along i (or j) lies as it
+// is, 256 to a row of k, and is read by the transposing read, four rows of k by 16 columns to 16 lanes, its pairs of chunks
+// exchanged by k's bits. What lies past an operand's end is read as zero by the buffer's bounds.
+//
+// A lane's results are four consecutive i at one j: in the logits i is the table row, so that a row's maximum and sum
+// stay mostly in registers; the gradients are stored along i.
+#include <algorithm>
+#include <type_traits>
+
+#include "cross_entropy.h"
+
+namespace efgs {
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef short shortx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t tile = entropy_wide_tile, step_k = 64, block = 512, waves = 8;
+constexpr uint32_t operand_bytes = tile * step_k * 2, stage_bytes = 2 * operand_bytes;
+constexpr uint32_t wave_chunks = operand_bytes / 1024 / waves;  // transfers of 1 KB by a wave to an operand's tile
+constexpr uint32_t outside = 0xfffffff0u;                       // an offset past every bound
+constexpr float infinity = __builtin_inff();
+
+template <typename T>
+__device__ __forceinline__ floatx4 multiply(shortx8 a, shortx8 b, floatx4 c) {
+    if constexpr (std::is_same_v<T, __bf16>) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+}
+
+// 64 lanes' 16 bytes each to 1 KB of LDS at `to`. (The builtin of this transfer makes the compiler wait for it before the next
+// transposing read of whatever address; the waits stand in the loop instead.)
+__device__ __forceinline__ void to_lds(uint32_t to, uintx4 buffer, uint32_t lane_offset, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer), "s"(offset) : "memory");
+}
+
+__device__ __forceinline__ uint32_t scalar(uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x))); }
+
+__device__ __forceinline__ uintx4 buffer_of(const void* base, uint64_t bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    return uintx4{scalar(static_cast<uint32_t>(at)), scalar(static_cast<uint32_t>(at >> 32)), scalar(bytes < 0xffffff00u ? static_cast<uint32_t>(bytes) : 0xffffff00u),
+                  0x00020000u};
+}
+
+// An operand: ALONG_K, `first` its first row of the tile (of `rows`), k along them; otherwise `first` the tile's first column, k the row.
+template <bool ALONG_K>
+struct Operand {
+    const char* base;
+    uint64_t stride;         // bytes
+    uint32_t rows, columns;  // as they lie in memory
+    uint32_t first, k_end;
+    uintx4 buffer;
+    uint32_t offsets[wave_chunks];
+    uint32_t chunk_k;        // ALONG_K: k of the lane's 16 bytes within a step
+
+    __device__ __forceinline__ void begin(const void* p, uint64_t stride_elements, uint32_t rows_, uint32_t columns_, uint32_t first_, uint32_t k_end_) {
+        const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        base = static_cast<const char*>(p);
+        stride = stride_elements * 2;
+        rows = rows_;
+        columns = columns_;
+        first = first_;
+        k_end = k_end_;
+        if constexpr (ALONG_K) {
+            const uint64_t left = min(rows - first, tile);
+            buffer = buffer_of(base + first * stride, (left - 1) * stride + columns * 2ull);
+            chunk_k = ((lane & 7u) ^ (lane >> 3)) * 8;
+#pragma unroll
+            for (uint32_t u = 0; u < wave_chunks; u++)
+                offsets[u] = ((wave * wave_chunks + u) * 8 + (lane >> 3)) * static_cast<uint32_t>(stride) + chunk_k * 2;
+        } else {
+#pragma unroll
+            for (uint32_t u = 0; u < wave_chunks; u++) {
+                const uint32_t k = (wave * wave_chunks + u) * 2 + (lane >> 5), exchange = (k & 3u) | (k >> 3 & 1u) << 2;
+                offsets[u] = k * static_cast<uint32_t>(stride) + (first + ((lane & 31u) ^ 2 * exchange) * 8) * 2;
+            }
+        }
+    }
+
+    // the tile of k..k + 63 on its way to LDS at `to`
+    __device__ __forceinline__ void load(uint32_t to, uint32_t k) {
+        const uint32_t wave = scalar(threadIdx.x >> 6);
+        if constexpr (ALONG_K) {
+            const bool inside = k + chunk_k < k_end;
+#pragma unroll
+            for (uint32_t u = 0; u < wave_chunks; u++) to_lds(to + (wave * wave_chunks + u) * 1024, buffer, inside ? offsets[u] : outside, k * 2);
+        } else {
+            const uint64_t left = min(k_end - k, step_k);
+            const uintx4 here = buffer_of(base + k * stride, (left - 1) * stride + columns * 2ull);
+#pragma unroll
+            for (uint32_t u = 0; u < wave_chunks; u++) to_lds(to + (wave * wave_chunks + u) * 1024, here, offsets[u], 0);
+        }
+    }
+};
+
+// Fragments of a step: lane (e, q) holds k = 8 q..8 q + 7 of each half step of 32 at column e of each 16.
+template <bool ALONG_K, uint32_t N>
+struct Fragments {
+    uint32_t at[ALONG_K ? 2 : N];
+
+    __device__ __forceinline__ void begin(uint32_t first) {
+        const uint32_t lane = threadIdx.x & 63u, e = lane & 15u, q = lane >> 4;
+        if constexpr (ALONG_K) {
+#pragma unroll
+            for (uint32_t half = 0; half < 2; half++) at[half] = (first + e) * 128 + ((half * 4 + q) ^ (e & 7u)) * 16;
+        } else {
+            const uint32_t exchange = (e >> 2) | (q & 1u) << 2;
+#pragma unroll
+            for (uint32_t t = 0; t < N; t++) at[t] = (8 * q + (e >> 2)) * 512 + ((first / 16 + t) ^ exchange) * 32 + (e & 3u) * 8;
+        }
+    }
+
+    __device__ __forceinline__ shortx8 read(const char* lds, uint32_t half, uint32_t t) const {
+        if constexpr (ALONG_K) {
+            return *reinterpret_cast<const shortx8*>(lds + at[half] + t * 2048);
+        } else {
+            using Part = __attribute__((address_space(3))) shortx4;
+            const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Part*)(lds + at[t] + half * 32 * 512));
+            const shortx4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Part*)(lds + at[t] + half * 32 * 512 + 4 * 512));
+            return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+template <typename T, EntropyProduct P>
+__global__ __launch_bounds__(block) void entropy_wide_kernel(EntropyProductArgs a) {
+    constexpr bool first_two = P == entropy_logits || P == entropy_upstream, a_along_k = first_two, b_along_k = P != entropy_table_gradient;
+    constexpr uint32_t wave_i = 8, wave_j = 4;  // tiles of 16 a wave
+    __shared__ __attribute__((aligned(1024))) char lds[2 * stage_bytes];
+    const uint32_t count = scalar(*a.count);
+    // Blocks go round the eight XCDs one by one: each XCD takes a run of the tiles, four rows of j at a time along i, so that the tiles that
+    // are under way on it share their operands in its L2.
+    const uint32_t j_tiles = P == entropy_table_gradient ? (a.j_end + tile - 1) / tile
+                                                         : (min(count - min(count, a.j_first), a.j_end) + tile - 1) / tile;
+    const uint32_t tiles = a.i_tiles * j_tiles, each = (tiles + 7) / 8, at = (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= each || at >= tiles) return;
+    const uint32_t band = at / (4 * a.i_tiles), in_band = at - band * 4 * a.i_tiles, width = min(4u, j_tiles - band * 4);
+    const uint32_t i0 = in_band / width * tile, j0 = a.j_first + (band * 4 + in_band % width) * tile;
+    const uint32_t k_all = P == entropy_table_gradient ? (count + step_k - 1) / step_k * step_k : a.k_end;
+    const uint32_t k_each = ((k_all + a.splits - 1) / a.splits + step_k - 1) / step_k * step_k;
+    const uint32_t k_first = min(blockIdx.y * k_each, k_all), k_end = min(k_first + k_each, k_all);
+
+    const uint32_t lane = threadIdx.x & 63u, e = lane & 15u, q = lane >> 4, wave = threadIdx.x >> 6, wi = wave & 1u, wj = wave >> 1;
+    Operand<a_along_k> operand_a;
+    Operand<b_along_k> operand_b;
+    if constexpr (first_two) {
+        operand_a.begin(a.a, a.a_stride, a.i_end, a.a_columns, i0, a.a_columns);
+        operand_b.begin(a.b, a.b_stride, j0 + tile, static_cast<uint32_t>(a.b_stride), j0, static_cast<uint32_t>(a.b_stride));
+    } else if constexpr (P == entropy_features_gradient) {
+        operand_a.begin(a.a, a.a_stride, k_all, a.a_columns, i0, k_all);
+        operand_b.begin(a.b, a.b_stride, j0 + tile, static_cast<uint32_t>(a.b_stride), j0, static_cast<uint32_t>(a.b_stride));
+    } else {
+        operand_a.begin(a.a, a.a_stride, k_all, a.a_columns, i0, k_all);
+        operand_b.begin(a.b, a.b_stride, k_all, static_cast<uint32_t>(a.b_stride), j0, k_all);
+    }
+    Fragments<a_along_k, wave_i> fragments_a;
+    Fragments<b_along_k, wave_j> fragments_b;
+    fragments_a.begin(wi * 128);
+    fragments_b.begin(wj * 64);
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uint64_t>((__attribute__((address_space(3))) char*)lds));
+
+    floatx4 acc[wave_i][wave_j] = {};
+    if (k_first < k_end) {
+        operand_a.load(lds_at, k_first);
+        operand_b.load(lds_at + operand_bytes, k_first);
+    }
+    uint32_t stage = 0;
+    for (uint32_t k = k_first; k < k_end; k += step_k) {
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): this wave's part of the stage is there, the other stage is read
+        __builtin_amdgcn_s_barrier();        // and so for the other waves
+        if (k + step_k < k_end) {
+            operand_a.load(lds_at + (stage ^ stage_bytes), k + step_k);
+            operand_b.load(lds_at + (stage ^ stage_bytes) + operand_bytes, k + step_k);
+        }
+#pragma unroll
+        for (uint32_t half = 0; half < 2; half++) {
+            shortx8 fa[wave_i], fb[wave_j];
+#pragma unroll
+            for (uint32_t t = 0; t < wave_j; t++) fb[t] = fragments_b.read(lds + stage + operand_bytes, half, t);
+#pragma unroll
+            for (uint32_t t = 0; t < wave_i; t++) fa[t] = fragments_a.read(lds + stage, half, t);
+#pragma unroll
+            for (uint32_t ti = 0; ti < wave_i; ti++)
+#pragma unroll
+                for (uint32_t tj = 0; tj < wave_j; tj++) acc[ti][tj] = multiply<T>(fa[ti], fb[tj], acc[ti][tj]);
+        }
+        asm volatile("" ::: "memory");
+        stage ^= stage_bytes;
+    }
+
+    const uint32_t i_lane = i0 + wi * 128 + 4 * q, j_lane = j0 + wj * 64 + e;  // results: i_lane + 16 ti + r, j_lane + 16 tj
+    if constexpr (P == entropy_logits) {
+        __syncthreads();
+        float2* const joined = reinterpret_cast<float2*>(lds);
+#pragma unroll
+        for (uint32_t tj = 0; tj < wave_j; tj++) {
+            const uint32_t j = j_lane + tj * 16, target = a.target[j];
+            float top = -infinity, sum = 0.0f;
+#pragma unroll
+            for (uint32_t ti = 0; ti < wave_i; ti++)
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) {
+                    const uint32_t i = i_lane + ti * 16 + r;
+                    const float z = i < a.i_end ? acc[ti][tj][r] * a.to_log2 : -infinity;
+                    acc[ti][tj][r] = z;
+                    if (i == target) a.target_logit[j] = z;
+                    top = fmaxf(top, z);
+                }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float from = top == -infinity ? 0.0f : top;
+#pragma unroll
+            for (uint32_t ti = 0; ti < wave_i; ti++)
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) sum += __builtin_amdgcn_exp2f(acc[ti][tj][r] - from);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (q == 0) joined[wi * tile + wj * 64 + tj * 16 + e] = make_float2(top, sum);
+        }
+        __syncthreads();
+        if (threadIdx.x < tile) {
+            const float2 x = joined[threadIdx.x], y = joined[tile + threadIdx.x];
+            const float top = fmaxf(x.x, y.x), from = top == -infinity ? 0.0f : top;
+            const float sum = x.y * __builtin_amdgcn_exp2f(x.x - from) + y.y * __builtin_amdgcn_exp2f(y.x - from);
+            a.partial[(i0 / tile) * a.slab_rows + (j0 - a.j_first) + threadIdx.x] = make_float2(top, sum);
+        }
+    } else if constexpr (P == entropy_upstream) {
+        typedef T Four __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (uint32_t tj = 0; tj < wave_j; tj++) {
+            const uint32_t j = j_lane + tj * 16, target = a.target[j];
+            const bool counts = target != entropy_none;
+            const float lse = counts ? a.lse[j] : 0.0f, weight = counts ? a.weight[j] : 0.0f;
+#pragma unroll
+            for (uint32_t ti = 0; ti < wave_i; ti++) {
+                const uint32_t i = i_lane + ti * 16;
+                Four g;
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) {
+                    const float p = __builtin_amdgcn_exp2f(acc[ti][tj][r] * a.to_log2 - lse) - (a.first_row + i + r == target ? 1.0f : 0.0f);
+                    g[r] = static_cast<T>(counts && i + r < a.i_end ? p * weight : 0.0f);
+                }
+                *reinterpret_cast<Four*>(static_cast<T*>(a.piece) + j * a.piece_stride + i) = g;
+            }
+        }
+    } else {
+        typedef T Four __attribute__((ext_vector_type(4), aligned(2)));
+        const bool direct = P == entropy_table_gradient && a.out;
+        const float factor = direct ? *a.factor : 1.0f;
+        const uint32_t j_end = P == entropy_table_gradient ? a.j_end : count;
+#pragma unroll
+        for (uint32_t tj = 0; tj < wave_j; tj++) {
+            const uint32_t j = j_lane + tj * 16;
+            if (j >= j_end) continue;
+#pragma unroll
+            for (uint32_t ti = 0; ti < wave_i; ti++) {
+                const uint32_t i = i_lane + ti * 16;
+                if (direct) {
+                    T* const out = static_cast<T*>(a.out) + j * a.out_stride + i;
+                    Four y;
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) y[r] = static_cast<T>(acc[ti][tj][r] * factor);
+                    if (i + 4 <= a.i_end) *reinterpret_cast<Four*>(out) = y;
+                    else
+#pragma unroll
+                        for (uint32_t r = 0; r < 4; r++)
+                            if (i + r < a.i_end) out[r] = y[r];
+                } else if (i < a.slab_stride) {
+                    floatx4* const out = reinterpret_cast<floatx4*>(a.slab + (blockIdx.y * a.slab_rows + j) * a.slab_stride + i);
+                    *out = a.add ? *out + acc[ti][tj] : acc[ti][tj];
+                }
+            }
+        }
+    }
+}
+
+template <typename T>
+void launch(EntropyProduct product, const EntropyProductArgs& a, uint32_t j_tiles, hipStream_t s) {
+    const dim3 grid((a.i_tiles * j_tiles + 7) / 8 * 8, a.splits);
+    switch (product) {
+        case entropy_logits: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_logits>), grid, dim3(block), 0, s, a); break;
+        case entropy_upstream: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_upstream>), grid, dim3(block), 0, s, a); break;
+        case entropy_features_gradient: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_features_gradient>), grid, dim3(block), 0, s, a); break;
+        case entropy_table_gradient: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_table_gradient>), grid, dim3(block), 0, s, a); break;
+    }
+}
+
+}  // namespace
+
+void launch_entropy_wide(EntropyProduct product, int type, const EntropyProductArgs& a, uint32_t j_tiles, hipStream_t s) {
+    if (type == type_bfloat16) launch<__bf16>(product, a, j_tiles, s);
+    else launch<_Float16>(product, a, j_tiles, s);
+}
+
+}  // namespace efgs
