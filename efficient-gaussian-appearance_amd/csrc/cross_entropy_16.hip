@@ -86,19 +86,17 @@ struct Operand {
         }
     }
 
-    // the tile of k..k + 63 on its way to LDS at `to`
-    __device__ __forceinline__ void load(uint32_t to, uint32_t k) {
-        const uint32_t wave = scalar(threadIdx.x >> 6);
-        if constexpr (ALONG_K) {
-            const bool inside = k + chunk_k < k_end;
-#pragma unroll
-            for (uint32_t u = 0; u < wave_chunks; u++) to_lds(to + (wave * wave_chunks + u) * 1024, buffer, inside ? offsets[u] : outside, k * 2);
-        } else {
-            const uint64_t left = min(k_end - k, step_k);
-            const uintx4 here = buffer_of(base + k * stride, (left - 1) * stride + columns * 2ull);
-#pragma unroll
-            for (uint32_t u = 0; u < wave_chunks; u++) to_lds(to + (wave * wave_chunks + u) * 1024, here, offsets[u], 0);
-        }
+    // transfer u of the tile of k..k + 63, which `buffer_at` describes, on its way to LDS at `to` (past k's end: zeros)
+    __device__ __forceinline__ uintx4 buffer_at(uint32_t k) const {
+        if constexpr (ALONG_K) return buffer;
+        const uint64_t left = min(k_end - min(k, k_end), step_k);
+        return buffer_of(base + k * stride, left > 0 ? (left - 1) * stride + columns * 2ull : 0);
+    }
+
+    __device__ __forceinline__ void load(uint32_t to, uintx4 here, uint32_t k, uint32_t u) const {
+        const uint32_t at = to + (scalar(threadIdx.x >> 6) * wave_chunks + u) * 1024;
+        if constexpr (ALONG_K) to_lds(at, here, k + chunk_k < k_end ? offsets[u] : outside, k < k_end ? k * 2 : 0);
+        else to_lds(at, here, offsets[u], 0);
     }
 };
 
@@ -169,32 +167,61 @@ __global__ __launch_bounds__(block) void entropy_wide_kernel(EntropyProductArgs 
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uint64_t>((__attribute__((address_space(3))) char*)lds));
 
     floatx4 acc[wave_i][wave_j] = {};
+    shortx8 fa[2][wave_i], fb[2][wave_j];  // of the two halves of a step
+    // A half step: its products, and between them, so that both are under way at once, the reads of the fragments of the half step behind it
+    // and, in the second half, the transfers of the step after the next.
+    const auto half_step = [&](auto half, const char* from, uint32_t to, uint32_t k) {
+        constexpr uint32_t h = decltype(half)::value;
+        uintx4 buffer_a{}, buffer_b{};
+        if constexpr (h == 1) {
+            buffer_a = operand_a.buffer_at(k);
+            buffer_b = operand_b.buffer_at(k);
+        }
+#pragma unroll
+        for (uint32_t ti = 0; ti < wave_i; ti++) {
+            if (ti < wave_j) fb[1 - h][ti] = fragments_b.read(from + operand_bytes, 1 - h, ti);
+            fa[1 - h][ti] = fragments_a.read(from, 1 - h, ti);
+            if (h == 1 && ti < wave_chunks) {
+                operand_a.load(to, buffer_a, k, ti);
+                operand_b.load(to + operand_bytes, buffer_b, k, ti);
+            }
+#pragma unroll
+            for (uint32_t tj = 0; tj < wave_j; tj++) acc[ti][tj] = multiply<T>(fa[h][ti], fb[h][tj], acc[ti][tj]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const std::integral_constant<uint32_t, 0> first_half;
+    const std::integral_constant<uint32_t, 1> second_half;
+    // (Steps past the end are read as zeros, so that nothing stands in branches.) Half way through a step its second half is in the registers: its stage is free for the step after the next, and the next one's
+    // has to be there.
     if (k_first < k_end) {
-        operand_a.load(lds_at, k_first);
-        operand_b.load(lds_at + operand_bytes, k_first);
-    }
-    uint32_t stage = 0;
-    for (uint32_t k = k_first; k < k_end; k += step_k) {
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): this wave's part of the stage is there, the other stage is read
-        __builtin_amdgcn_s_barrier();        // and so for the other waves
-        if (k + step_k < k_end) {
-            operand_a.load(lds_at + (stage ^ stage_bytes), k + step_k);
-            operand_b.load(lds_at + (stage ^ stage_bytes) + operand_bytes, k + step_k);
-        }
+        const auto load = [&](uint32_t to, uint32_t k) {
+            const uintx4 buffer_a = operand_a.buffer_at(k), buffer_b = operand_b.buffer_at(k);
 #pragma unroll
-        for (uint32_t half = 0; half < 2; half++) {
-            shortx8 fa[wave_i], fb[wave_j];
-#pragma unroll
-            for (uint32_t t = 0; t < wave_j; t++) fb[t] = fragments_b.read(lds + stage + operand_bytes, half, t);
-#pragma unroll
-            for (uint32_t t = 0; t < wave_i; t++) fa[t] = fragments_a.read(lds + stage, half, t);
-#pragma unroll
-            for (uint32_t ti = 0; ti < wave_i; ti++)
-#pragma unroll
-                for (uint32_t tj = 0; tj < wave_j; tj++) acc[ti][tj] = multiply<T>(fa[ti], fb[tj], acc[ti][tj]);
-        }
+            for (uint32_t u = 0; u < wave_chunks; u++) {
+                operand_a.load(to, buffer_a, k, u);
+                operand_b.load(to + operand_bytes, buffer_b, k, u);
+            }
+        };
+        load(lds_at, k_first);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+        __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        stage ^= stage_bytes;
+        load(lds_at + stage_bytes, k_first + step_k);
+#pragma unroll
+        for (uint32_t t = 0; t < wave_j; t++) fb[0][t] = fragments_b.read(lds + operand_bytes, 0, t);
+#pragma unroll
+        for (uint32_t t = 0; t < wave_i; t++) fa[0][t] = fragments_a.read(lds, 0, t);
+        uint32_t stage = 0;
+        for (uint32_t k = k_first; k < k_end; k += step_k) {
+            half_step(first_half, lds + stage, 0, 0);
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): this wave's part of the next stage is there, its reads of this one are done
+            __builtin_amdgcn_s_barrier();        // and so for the other waves
+            asm volatile("" ::: "memory");
+            half_step(second_half, lds + (stage ^ stage_bytes), lds_at + stage, k + 2 * step_k);
+            stage ^= stage_bytes;
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the zeros that follow the last step
     }
 
     const uint32_t i_lane = i0 + wi * 128 + 4 * q, j_lane = j0 + wj * 64 + e;  // results: i_lane + 16 ti + r, j_lane + 16 tj
