@@ -44,4 +44,29 @@ struct EntropyProductArgs {
 constexpr uint32_t entropy_wide_tile = 256;
 void launch_entropy_wide(EntropyProduct product, int type, const EntropyProductArgs& a, uint32_t j_tiles, hipStream_t s);
 
+// few columns: products and exponentials of a tile in one kernel
+struct EntropyNarrowArgs {
+    const void* packed;
+    const void* table;
+    uint64_t packed_stride, table_stride;
+    uint32_t table_rows, columns, padded;
+    uint32_t own_waves;            // of a block's four that own different rows
+    const uint32_t* count;
+    const uint32_t* target;        // of packed rows, as the next two
+    const float* lse;
+    const float* weight;
+    float to_log2;
+    float2* partial;               // logits: splits x padded (reference, sum of exponentials)
+    float* target_logit;
+    float* slab;                   // gradients: splits x slab_rows x slab_stride
+    uint64_t slab_rows, slab_stride;
+};
+struct EntropyNarrowPlan {
+    uint32_t own_waves, blocks, stream_blocks;
+    uint32_t splits;               // partial results of an owned row
+};
+constexpr uint32_t entropy_narrow_most = 128, entropy_narrow_most_16 = 32;  // columns of floats, of 16-bit types
+EntropyNarrowPlan entropy_narrow_plan(uint32_t own, uint32_t stream, uint32_t columns);
+void launch_entropy_narrow(EntropyProduct product, int type, const EntropyNarrowArgs& a, const EntropyNarrowPlan& p, hipStream_t s);
+
 }  // namespace efgs

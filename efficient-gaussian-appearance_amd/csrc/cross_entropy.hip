@@ -398,19 +398,40 @@ __global__ __launch_bounds__(1024) void entropy_half_weights_kernel(WeightArgs a
     if (threadIdx.x == 0) *a.factor = ldexpf(a.scale / a.held, exponent);
 }
 
-// sums of the splits, scaled; rows without a packed one are zeros
+struct Gathering {
+    const float* slab;           // splits x slab_rows x slab_stride
+    uint64_t slab_rows;
+    uint32_t slab_stride, splits;
+    const uint32_t* packed_of;   // or null: the rows themselves
+    const float* weight;         // of packed rows, or null
+    uint32_t rows, columns;
+    const float* factor;
+};
+
+// Sums of the splits, in their order, scaled; rows without a packed one are zeros. Four columns a thread.
 template <typename T>
-__global__ __launch_bounds__(256) void entropy_gather_kernel(const float* slab, uint64_t slab_rows, uint64_t slab_stride, uint32_t splits,
-                                                             const uint32_t* packed_of, uint32_t rows, uint32_t columns, const float* factor, T* out) {
-    const uint64_t items = static_cast<uint64_t>(rows) * columns, step = static_cast<uint64_t>(gridDim.x) * 256u;
-    const float f = *factor;
-    for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < items; t += step) {
-        const uint32_t row = static_cast<uint32_t>(t / columns), column = static_cast<uint32_t>(t - static_cast<uint64_t>(row) * columns);
-        const uint32_t m = packed_of ? packed_of[row] : row;
-        float sum = 0.0f;
-        if (m != none)
-            for (uint32_t s = 0; s < splits; s++) sum += slab[(s * slab_rows + m) * slab_stride + column];
-        out[t] = static_cast<T>(m == none ? 0.0f : sum * f);
+__global__ __launch_bounds__(256) void entropy_gather_kernel(Gathering a, T* out) {
+    const uint32_t parts = (a.columns + 3) / 4, lanes = min(parts, 256u), rows = 256u / lanes, r = threadIdx.x / lanes, lane = threadIdx.x - r * lanes;
+    if (r >= rows) return;
+    const float factor = *a.factor;
+    for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * rows + r; row < a.rows; row += static_cast<uint64_t>(gridDim.x) * rows) {
+        const uint32_t m = a.packed_of ? a.packed_of[row] : static_cast<uint32_t>(row);
+        const float f = a.weight && m != none ? factor * a.weight[m] : factor;
+        for (uint32_t part = lane; part < parts; part += lanes) {
+            floatx4 sum{};
+            if (m != none)
+                for (uint32_t s = 0; s < a.splits; s++)
+                    sum += *reinterpret_cast<const floatx4*>(a.slab + (s * a.slab_rows + m) * a.slab_stride + part * 4);
+            Part<T, 4> y;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) y[k] = static_cast<T>(m == none ? 0.0f : sum[k] * f);
+            T* const to = out + row * a.columns + part * 4;
+            if (part * 4 + 4 <= a.columns) *reinterpret_cast<Part<T, 4>*>(to) = y;
+            else
+#pragma unroll
+                for (uint32_t k = 0; k < 4; k++)
+                    if (part * 4 + k < a.columns) to[k] = y[k];
+        }
     }
 }
 
@@ -435,7 +456,9 @@ class Carver {
 
 uint32_t type_bytes(int type) { return type == type_float ? 4 : 2; }
 
-bool wide(const EntropyArgs& a) { return a.type != type_float; }
+// the three ways: few columns, 16-bit types, floats
+bool narrow(const EntropyArgs& a) { return a.columns > 0 && a.columns <= (a.type == type_float ? entropy_narrow_most : entropy_narrow_most_16); }
+bool wide(const EntropyArgs& a) { return a.type != type_float && !narrow(a); }
 bool table_is_copied(const EntropyArgs& a);
 
 uint32_t tile_of(const EntropyArgs& a) { return wide(a) ? entropy_wide_tile : tile; }
@@ -452,7 +475,7 @@ struct Saved {
     Saved(const EntropyArgs& a, void* base) {
         Carver c(base);
         padded = static_cast<uint32_t>(round_up(std::max(a.n, 1u), row_tile));
-        padded_columns = static_cast<uint32_t>(round_up(a.columns, column_tile));
+        padded_columns = static_cast<uint32_t>(round_up(a.columns, narrow(a) ? 16 / type_bytes(a.type) : column_tile));
         count = c.take<uint32_t>(1);
         row_of = c.take<uint32_t>(padded);
         packed_of = c.take<uint32_t>(padded);
@@ -474,14 +497,16 @@ struct ForwardScratch {
     double* sums;
     void* copy;        // of the table, or null
     bool copied;
+    EntropyNarrowPlan plan;
     uint32_t tiles, rows_at_once;
     size_t bytes;
     ForwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
-        tiles = div_up(a.rows, tile_of(a));
+        plan = entropy_narrow_plan(std::max(a.n, 1u), a.rows, a.columns);
+        tiles = narrow(a) ? (a.rows > 0 ? plan.splits : 0) : div_up(a.rows, tile_of(a));
         chunk_counts = c.take<uint32_t>(div_up(s.padded, rank_block));
         const uint64_t most = std::min(partial_bytes / sizeof(float2), most_blocks * tile) / std::max(tiles, 1u);
-        rows_at_once = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(most / row_tile * row_tile, row_tile), s.padded));
+        rows_at_once = narrow(a) ? s.padded : static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(most / row_tile * row_tile, row_tile), s.padded));
         partial = c.take<float2>(static_cast<uint64_t>(tiles) * rows_at_once);
         target_logit = c.take<float>(s.padded);
         sums = c.take<double>(s.padded / join_rows);
@@ -504,6 +529,25 @@ uint32_t splits_for(uint64_t tiles, uint64_t k, uint64_t at_once) {
     }
     return best;
 }
+
+struct NarrowBackwardScratch {
+    float* weight;
+    float* factor;
+    float* slab;             // of one gradient after the other
+    EntropyNarrowPlan features, table;
+    uint32_t slab_stride;
+    size_t bytes;
+    NarrowBackwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
+        Carver c(base);
+        features = entropy_narrow_plan(std::max(a.n, 1u), a.rows, a.columns);
+        table = entropy_narrow_plan(a.rows, std::max(a.n, 1u), a.columns);
+        slab_stride = static_cast<uint32_t>(round_up(a.columns, 4));
+        weight = c.take<float>(s.padded);
+        factor = c.take<float>(1);
+        slab = c.take<float>(std::max(static_cast<uint64_t>(features.splits) * s.padded, static_cast<uint64_t>(table.splits) * a.rows) * slab_stride);
+        bytes = c.used();
+    }
+};
 
 struct BackwardScratch {
     float* weight;
@@ -592,6 +636,54 @@ Table table_of(const EntropyArgs& a, const Saved& s, void* room, hipStream_t str
     return {room, s.padded_columns, s.padded_columns};
 }
 
+EntropyNarrowArgs narrow_args(const EntropyArgs& a, const Saved& s) {
+    EntropyNarrowArgs p{};
+    p.packed = s.packed;
+    p.packed_stride = s.padded_columns;
+    p.table = a.table;
+    p.table_stride = a.table_stride;
+    p.table_rows = a.rows;
+    p.columns = a.columns;
+    p.padded = s.padded;
+    p.count = s.count;
+    p.target = s.target;
+    p.lse = s.lse;
+    p.to_log2 = a.scale * log2_e;
+    return p;
+}
+
+void launch_gathering(int type, const Gathering& g, void* out, hipStream_t stream) {
+    if (g.rows == 0 || g.columns == 0) return;
+    const uint32_t blocks = copy_grid(static_cast<uint64_t>(g.rows) * ((g.columns + 3) / 4));
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(entropy_gather_kernel<T>, dim3(blocks), dim3(256), 0, stream, g, static_cast<T*>(out));
+    });
+}
+
+bool launch_narrow_backward(const EntropyArgs& a, const float* upstream, const Saved& s, void* grad_features, void* grad_table, void* scratch,
+                            hipStream_t stream) {
+    const NarrowBackwardScratch w(a, s, scratch);
+    const WeightArgs weights{upstream, s.count, s.row_of, s.padded, a.each, a.mean, a.scale, 1.0f, w.weight, w.factor};
+    hipLaunchKernelGGL(entropy_weights_kernel, dim3(div_up(s.padded, 256)), dim3(256), 0, stream, weights);
+    EntropyNarrowArgs p = narrow_args(a, s);
+    p.weight = w.weight;
+    p.slab = w.slab;
+    p.slab_stride = w.slab_stride;
+    if (grad_features) {
+        p.slab_rows = s.padded;
+        if (a.rows > 0) launch_entropy_narrow(entropy_features_gradient, a.type, p, w.features, stream);
+        launch_gathering(a.type, {w.slab, s.padded, w.slab_stride, w.features.splits, s.packed_of, w.weight, a.n, a.columns, w.factor}, grad_features, stream);
+    }
+    if (grad_table) {
+        p.slab_rows = a.rows;
+        launch_entropy_narrow(entropy_table_gradient, a.type, p, w.table, stream);
+        launch_gathering(a.type, {w.slab, a.rows, w.slab_stride, w.table.splits, nullptr, nullptr, a.rows, a.columns, w.factor}, grad_table, stream);
+    }
+    EFGS_HIP_CHECK(hipGetLastError());
+    return true;
+}
+
 void launch_product(EntropyProduct product, const EntropyArgs& a, const EntropyProductArgs& p, uint32_t j, hipStream_t stream) {
     if (wide(a)) {
         launch_entropy_wide(product, a.type, p, div_up(j, entropy_wide_tile), stream);
@@ -617,7 +709,9 @@ bool entropy_fits(const EntropyArgs& a) {
 
 size_t entropy_saved_bytes(const EntropyArgs& a) { return Saved(a, nullptr).bytes; }
 size_t entropy_forward_bytes(const EntropyArgs& a) { return ForwardScratch(a, Saved(a, nullptr), nullptr).bytes; }
-size_t entropy_backward_bytes(const EntropyArgs& a) { return BackwardScratch(a, Saved(a, nullptr), nullptr).bytes; }
+size_t entropy_backward_bytes(const EntropyArgs& a) {
+    return narrow(a) ? NarrowBackwardScratch(a, Saved(a, nullptr), nullptr).bytes : BackwardScratch(a, Saved(a, nullptr), nullptr).bytes;
+}
 
 bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void* scratch, hipStream_t stream) {
     const Saved s(a, saved);
@@ -626,7 +720,12 @@ bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void
     const Table table = table_of(a, s, f.copied ? f.copy : nullptr, stream);
     for (uint32_t first = 0; first < s.padded; first += f.rows_at_once) {
         const uint32_t rows = std::min(s.padded - first, f.rows_at_once);
-        if (a.rows > 0) {
+        if (a.rows > 0 && narrow(a)) {
+            EntropyNarrowArgs p = narrow_args(a, s);
+            p.partial = f.partial;
+            p.target_logit = f.target_logit;
+            launch_entropy_narrow(entropy_logits, a.type, p, f.plan, stream);
+        } else if (a.rows > 0) {
             EntropyProductArgs p{};
             p.a = table.rows;
             p.a_stride = table.stride;
@@ -659,6 +758,7 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
                              hipStream_t stream) {
     if (a.columns == 0) return true;
     const Saved s(a, const_cast<void*>(saved));
+    if (narrow(a)) return launch_narrow_backward(a, upstream, s, grad_features, grad_table, scratch, stream);
     const BackwardScratch w(a, s, scratch);
     const Table table = table_of(a, s, w.copied ? w.copy : nullptr, stream);
     const bool half = a.type == type_half;
@@ -723,19 +823,12 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
             x.factor = w.factor;
             launch_product(entropy_table_gradient, a, x, rows, stream);
             if (x.splits > 1)
-                with_type(a.type, [&](auto t) {
-                    using T = decltype(t);
-                    hipLaunchKernelGGL(entropy_gather_kernel<T>, dim3(copy_grid(static_cast<uint64_t>(rows) * a.columns)), dim3(256), 0, stream,
-                                       w.table_slab, w.piece_rows, s.padded_columns, x.splits, nullptr, rows, a.columns, w.factor, static_cast<T*>(out));
-                });
+                launch_gathering(a.type, {w.table_slab, w.piece_rows, s.padded_columns, x.splits, nullptr, nullptr, rows, a.columns, w.factor}, out, stream);
         }
     }
-    if (grad_features && a.n > 0)
-        with_type(a.type, [&](auto t) {
-            using T = decltype(t);
-            hipLaunchKernelGGL(entropy_gather_kernel<T>, dim3(copy_grid(static_cast<uint64_t>(a.n) * a.columns)), dim3(256), 0, stream, w.features_slab,
-                               s.padded, s.padded_columns, w.features_splits, s.packed_of, a.n, a.columns, w.factor, static_cast<T*>(grad_features));
-        });
+    if (grad_features)
+        launch_gathering(a.type, {w.features_slab, s.padded, s.padded_columns, w.features_splits, s.packed_of, nullptr, a.n, a.columns, w.factor},
+                         grad_features, stream);
     EFGS_HIP_CHECK(hipGetLastError());
     return true;
 }
