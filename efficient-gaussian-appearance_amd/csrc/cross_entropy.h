@@ -9,6 +9,9 @@ constexpr uint32_t entropy_row_tile = 256;     // packed rows come in multiples 
 constexpr uint32_t entropy_column_tile = 64;   // so do their columns
 constexpr float entropy_half_range = 32768.0f; // float16: what upstream gradients of the logits are held times
 
+// The log sum of a row's exponentials (log 2) is held in two parts, the first near the largest logit and the second small: a probability is
+// exp2((z - first) - second), exact to the rounding of z alone also where z and the sum are large.
+
 // C(i, j) = sum_k A(i, k) B(k, j); i is the table row in the first two products and the column in the gradients, j the packed row and, in
 // the table's gradient, the table row.
 enum EntropyProduct { entropy_logits, entropy_upstream, entropy_features_gradient, entropy_table_gradient };
@@ -27,7 +30,7 @@ struct EntropyProductArgs {
     float2* partial;               // logits: i_tiles x slab_rows (maximum, sum of exponentials), from row j_first on
     float* target_logit;
     const uint32_t* target;
-    const float* lse;
+    const float2* lse;
     const float* weight;
     uint32_t first_row;            // of the piece in the table
     void* piece;                   // upstream gradients of the logits: padded rows x piece_stride
@@ -53,7 +56,7 @@ struct EntropyNarrowArgs {
     uint32_t own_waves;            // of a block's four that own different rows
     const uint32_t* count;
     const uint32_t* target;        // of packed rows, as the next two
-    const float* lse;
+    const float2* lse;
     const float* weight;
     float to_log2;
     float2* partial;               // logits: splits x padded (reference, sum of exponentials)

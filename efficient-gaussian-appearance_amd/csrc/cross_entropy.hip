@@ -172,6 +172,12 @@ __device__ __forceinline__ void store_tile(float (*lds)[tile_pitch], const float
     }
 }
 
+// a product that is rounded before it is subtracted from, as the forward has it
+__device__ __forceinline__ float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+
 template <typename T, EntropyProduct P>
 __global__ __launch_bounds__(tile_block) void entropy_product_kernel(EntropyProductArgs a) {
     using B = std::conditional_t<P == entropy_logits || P == entropy_upstream, T, float>;
@@ -253,14 +259,15 @@ __global__ __launch_bounds__(tile_block) void entropy_product_kernel(EntropyProd
         for (uint32_t tj = 0; tj < 4; tj++) {
             const uint32_t j = j_lane + tj * 16, target = a.target[j];
             const bool counts = target != none;
-            const float lse = counts ? a.lse[j] : 0.0f, weight = counts ? a.weight[j] : 0.0f;
+            const float2 lse = counts ? a.lse[j] : make_float2(0.0f, 0.0f);
+            const float weight = counts ? a.weight[j] : 0.0f;
 #pragma unroll
             for (uint32_t ti = 0; ti < 4; ti++) {
                 const uint32_t i = i_lane + ti * 16;
                 floatx4 g;
 #pragma unroll
                 for (uint32_t r = 0; r < 4; r++) {
-                    const float p = __builtin_amdgcn_exp2f(acc[ti][tj][r] * a.to_log2 - lse) - (a.first_row + i + r == target ? 1.0f : 0.0f);
+                    const float p = __builtin_amdgcn_exp2f((rounded(acc[ti][tj][r] * a.to_log2) - lse.x) - lse.y) - (a.first_row + i + r == target ? 1.0f : 0.0f);
                     g[r] = counts && i + r < a.i_end ? p * weight : 0.0f;
                 }
                 *reinterpret_cast<floatx4*>(static_cast<float*>(a.piece) + j * a.piece_stride + i) = g;
@@ -301,7 +308,7 @@ struct JoinArgs {
     const uint32_t* row_of;
     const uint32_t* packed_of;
     const float* target_logit;
-    float* lse;
+    float2* lse;
     float* losses;         // of each row, or null
     double* sums;          // of each block's rows
 };
@@ -331,9 +338,12 @@ __global__ __launch_bounds__(join_rows * join_parts) void entropy_join_kernel(Jo
         sum = sum * __builtin_amdgcn_exp2f(top - from) + x.y * __builtin_amdgcn_exp2f(x.x - from);
         top = higher;
     }
-    const float lse = top + log2f(sum);
-    const float loss = counts ? (lse - a.target_logit[row]) * ln_2 : 0.0f;
-    if (counts) a.lse[row] = lse;
+    // the sum's power of two joins the reference, with what that sum rounds off
+    int exponent = 0;
+    const float fraction = sum > 0.0f && sum < infinity ? frexpf(sum, &exponent) : sum;
+    const float power = static_cast<float>(exponent), first = top + power, second = log2f(fraction) + (exponent != 0 ? top - (first - power) : 0.0f);
+    const float loss = counts ? ((first - a.target_logit[row]) + second) * ln_2 : 0.0f;
+    if (counts) a.lse[row] = make_float2(first, second);
     if (a.losses) {
         if (counts) a.losses[a.row_of[row]] = loss;
         if (row < a.n && a.packed_of[row] == none) a.losses[row] = 0.0f;
@@ -468,7 +478,7 @@ struct Saved {
     uint32_t* row_of;
     uint32_t* packed_of;
     uint32_t* target;
-    float* lse;
+    float2* lse;
     void* packed;
     uint32_t padded, padded_columns;
     size_t bytes;
@@ -480,7 +490,7 @@ struct Saved {
         row_of = c.take<uint32_t>(padded);
         packed_of = c.take<uint32_t>(padded);
         target = c.take<uint32_t>(padded);
-        lse = c.take<float>(padded);
+        lse = c.take<float2>(padded);
         packed = c.take<char>(static_cast<uint64_t>(padded) * padded_columns * type_bytes(a.type));
         bytes = c.used();
     }

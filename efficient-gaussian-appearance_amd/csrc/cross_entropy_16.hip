@@ -31,6 +31,12 @@ constexpr uint32_t wave_chunks = operand_bytes / 1024 / waves;  // transfers of 
 constexpr uint32_t outside = 0xfffffff0u;                       // an offset past every bound
 constexpr float infinity = __builtin_inff();
 
+// a product that is rounded before it is subtracted from, as the forward has it
+__device__ __forceinline__ float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+
 template <typename T>
 __device__ __forceinline__ floatx4 multiply(shortx8 a, shortx8 b, floatx4 c) {
     if constexpr (std::is_same_v<T, __bf16>) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -266,14 +272,15 @@ __global__ __launch_bounds__(block) void entropy_wide_kernel(EntropyProductArgs 
         for (uint32_t tj = 0; tj < wave_j; tj++) {
             const uint32_t j = j_lane + tj * 16, target = a.target[j];
             const bool counts = target != entropy_none;
-            const float lse = counts ? a.lse[j] : 0.0f, weight = counts ? a.weight[j] : 0.0f;
+            const float2 lse = counts ? a.lse[j] : make_float2(0.0f, 0.0f);
+            const float weight = counts ? a.weight[j] : 0.0f;
 #pragma unroll
             for (uint32_t ti = 0; ti < wave_i; ti++) {
                 const uint32_t i = i_lane + ti * 16;
                 Four g;
 #pragma unroll
                 for (uint32_t r = 0; r < 4; r++) {
-                    const float p = __builtin_amdgcn_exp2f(acc[ti][tj][r] * a.to_log2 - lse) - (a.first_row + i + r == target ? 1.0f : 0.0f);
+                    const float p = __builtin_amdgcn_exp2f((rounded(acc[ti][tj][r] * a.to_log2) - lse.x) - lse.y) - (a.first_row + i + r == target ? 1.0f : 0.0f);
                     g[r] = static_cast<T>(counts && i + r < a.i_end ? p * weight : 0.0f);
                 }
                 *reinterpret_cast<Four*>(static_cast<T*>(a.piece) + j * a.piece_stride + i) = g;

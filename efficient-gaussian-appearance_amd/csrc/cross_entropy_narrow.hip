@@ -3,9 +3,8 @@
 // A wave owns up to 64 rows of one side, 16 to a tile, and meets the rows of the other side 16 at a time, from LDS:
 //   logits      S(m, o) = sum_k stream(m, k) own(o, k)        v_mfma_f32_16x16x4_f32, a lane has four m at one o
 //   gradient    out(d, o) += sum_m stream(m, d) g(m, o)       g's registers as they lie are this product's operand: register r of lane (o, q) is row 4 q + r
-// The forward and the rows' gradient own packed rows and meet the table; the table's gradient owns table rows and meets the packed rows. The products
-// begin from minus the row's log sum (or, in the forward, from minus the lane's reference), so that a result goes into the exponential as it
-// is. Sums that several blocks or waves share are left as partial ones, joined in their order.
+// The forward and the rows' gradient own packed rows and meet the table; the table's gradient owns table rows and meets the packed rows. The owned side
+// comes times scale log2 e, so that a product goes into the exponential less its row's log sum (in the forward, less the lane's reference). Sums that several blocks or waves share are left as partial ones, joined in their order.
 #include <algorithm>
 
 #include "cross_entropy.h"
@@ -47,7 +46,7 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
     constexpr uint32_t pitch = DT * 16 + 4, quads = KS <= 4 ? 1 : KS / 4;  // (row 4 q + r: four q in four parts of the banks)
     __shared__ float logit_tiles[chunk * KS * 4];                                          // tile, step, lane
     __shared__ __attribute__((aligned(16))) float rows[gradient ? chunk * pitch : 4];       // row-major, of the table's gradient times their weights
-    __shared__ __attribute__((aligned(16))) float row_start[own_table ? chunk : 4];         // minus the log sums
+    __shared__ __attribute__((aligned(16))) float row_lse[2][own_table ? chunk : 4];
     __shared__ __attribute__((aligned(16))) uint32_t row_target[own_table ? chunk : 4];
     const uint32_t count = scalar(*a.count), own_end = own_table ? a.table_rows : count, stream_end = own_table ? count : a.table_rows;
     const uint32_t lane = threadIdx.x & 63u, e = lane & 15u, q = lane >> 4, wave = scalar(threadIdx.x >> 6);
@@ -55,16 +54,17 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
     const uint32_t own_first = (blockIdx.x * a.own_waves + own_wave) * TILES * 16;
     if (blockIdx.x * a.own_waves * TILES * 16 >= own_end) return;
     const uint32_t chunks = (stream_end + chunk - 1) / chunk, chunks_each = (chunks + gridDim.y - 1) / gridDim.y;
-    const uint32_t first = min(blockIdx.y * chunks_each, chunks) * chunk, end = min(stream_end, first + chunks_each * chunk);
+    const uint32_t begin = min(blockIdx.y * chunks_each, chunks) * chunk, end = min(stream_end, begin + chunks_each * chunk);
     const T* const own = static_cast<const T*>(own_table ? a.table : a.packed);
     const T* const stream = static_cast<const T*>(own_table ? a.packed : a.table);
     const uint64_t own_stride = own_table ? a.table_stride : a.packed_stride, stream_stride = own_table ? a.packed_stride : a.table_stride;
 
     float fo[TILES][KS];
-    floatx4 start[TILES];
+    float2 lse[TILES];
     uint32_t target[TILES];
     floatx4 out[TILES][DT];
     float reference[TILES], sum[TILES];
+    bool begun[TILES];
 #pragma unroll
     for (uint32_t t = 0; t < TILES; t++) {
         const uint32_t o = own_first + t * 16 + e;
@@ -72,10 +72,10 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
 #pragma unroll
         for (uint32_t s = 0; s < KS; s++)
             fo[t][s] = inside && 4 * s + q < a.columns ? static_cast<float>(own[o * own_stride + 4 * s + q]) * a.to_log2 : 0.0f;
-        const float lse = P == entropy_features_gradient && inside ? a.lse[o] : 0.0f;
-        start[t] = floatx4{-lse, -lse, -lse, -lse};
+        lse[t] = P == entropy_features_gradient && inside ? a.lse[o] : make_float2(0.0f, 0.0f);
         target[t] = !own_table && inside ? a.target[o] : entropy_none;
-        reference[t] = -infinity;
+        reference[t] = 0.0f;
+        begun[t] = false;
         sum[t] = 0.0f;
 #pragma unroll
         for (uint32_t d = 0; d < DT; d++) out[t][d] = floatx4{};
@@ -84,7 +84,8 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
     // a chunk of the streamed rows on its way to the registers: row threadIdx.x / 4, every fourth quad of its columns
     const uint32_t row = threadIdx.x / 4, quad = threadIdx.x % 4;
     floatx4 next[quads];
-    float next_lse = 0.0f, next_weight = 0.0f;
+    float2 next_lse{};
+    float next_weight = 0.0f;
     uint32_t next_target = entropy_none;
     const auto fetch = [&](uint32_t from) {
         const uint32_t m = from + row;
@@ -94,13 +95,13 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
             next[j] = load4<T>(stream + static_cast<uint64_t>(m) * stream_stride + column, m < stream_end ? static_cast<int32_t>(a.columns) - static_cast<int32_t>(column) : 0);
         }
         if constexpr (own_table) {
-            next_lse = m < stream_end ? a.lse[m] : infinity;
+            next_lse = m < stream_end ? a.lse[m] : make_float2(infinity, 0.0f);  // (no probability)
             next_weight = m < stream_end ? a.weight[m] : 0.0f;
             next_target = m < stream_end ? a.target[m] : entropy_none;
         }
     };
-    if (first < end) fetch(first);
-    for (uint32_t from = first; from < end; from += chunk) {
+    if (begin < end) fetch(begin);
+    for (uint32_t from = begin; from < end; from += chunk) {
         __syncthreads();
 #pragma unroll
         for (uint32_t j = 0; j < quads; j++) {
@@ -113,7 +114,8 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
         }
         if constexpr (own_table) {
             if (quad == 0) {
-                row_start[row] = -next_lse;
+                row_lse[0][row] = next_lse.x;
+                row_lse[1][row] = next_lse.y;
                 row_target[row] = next_target;
             }
         }
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
                 bool above = false;
 #pragma unroll
                 for (uint32_t t = 0; t < TILES; t++) {
-                    z[t] = start[t];
+                    z[t] = floatx4{};
 #pragma unroll
                     for (uint32_t s = 0; s < KS; s++) z[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(fs[s], fo[t][s], z[t], 0, 0, 0);
                 }
@@ -140,22 +142,23 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
                         for (uint32_t r = 0; r < 4; r++)
                             if (from + mt * 16 + 4 * q + r >= end) z[t][r] = -infinity;
                 }
-                float top[TILES];
+                float top[TILES];  // above the reference, or the first logits
 #pragma unroll
                 for (uint32_t t = 0; t < TILES; t++) {
+                    z[t] -= reference[t];
                     top[t] = fmaxf(fmaxf(z[t][0], z[t][1]), fmaxf(z[t][2], z[t][3]));
-                    above |= top[t] > far_above || (reference[t] == -infinity && top[t] > -infinity);
+                    above |= top[t] > far_above || (!begun[t] && top[t] > -infinity);
                 }
                 // a lane's first logits, or ones far above its reference: they become the reference
                 if (__any(above)) {
 #pragma unroll
                     for (uint32_t t = 0; t < TILES; t++) {
-                        const bool begin = reference[t] == -infinity;
-                        const float by = top[t] > far_above || (begin && top[t] > -infinity) ? top[t] : 0.0f;
-                        reference[t] = begin ? (by == 0.0f && !(top[t] > -infinity) ? -infinity : by) : reference[t] + by;
-                        sum[t] = begin ? sum[t] : sum[t] * __builtin_amdgcn_exp2f(-by);
-                        z[t] -= by;
-                        start[t] -= by;
+                        const bool begins = !begun[t] && top[t] > -infinity, moves = begins || top[t] > far_above;
+                        const float to = reference[t] + top[t];
+                        if (begun[t] && moves) sum[t] *= __builtin_amdgcn_exp2f(reference[t] - to);
+                        if (moves) z[t] -= to - reference[t];
+                        reference[t] = moves ? to : reference[t];
+                        begun[t] |= begins;
                     }
                 }
 #pragma unroll
@@ -173,11 +176,12 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
                 for (uint32_t r = 0; r < 4; r++)
 #pragma unroll
                     for (uint32_t d = 0; d < DT; d++) fr[r][d] = rows[(mt * 16 + 4 * q + r) * pitch + d * 16 + e];
-                floatx4 begin{};
+                floatx4 first{}, second{};
                 uintx4 hits{};
                 bool hit = false;
                 if constexpr (own_table) {
-                    begin = *reinterpret_cast<const floatx4*>(row_start + mt * 16 + 4 * q);
+                    first = *reinterpret_cast<const floatx4*>(row_lse[0] + mt * 16 + 4 * q);
+                    second = *reinterpret_cast<const floatx4*>(row_lse[1] + mt * 16 + 4 * q);
                     hits = *reinterpret_cast<const uintx4*>(row_target + mt * 16 + 4 * q);
 #pragma unroll
                     for (uint32_t r = 0; r < 4; r++) hit |= hits[r] - own_first < TILES * 16u;
@@ -188,15 +192,15 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
                 floatx4 p[TILES];
 #pragma unroll
                 for (uint32_t t = 0; t < TILES; t++) {
-                    p[t] = own_table ? begin : start[t];
+                    p[t] = floatx4{};
 #pragma unroll
                     for (uint32_t s = 0; s < KS; s++) p[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(fs[s], fo[t][s], p[t], 0, 0, 0);
                 }
 #pragma unroll
                 for (uint32_t t = 0; t < TILES; t++)
 #pragma unroll
-                    for (uint32_t r = 0; r < 4; r++) p[t][r] = __builtin_amdgcn_exp2f(p[t][r]);
-                if (!own_table && m0 + 16 > end) {  // (past the table: the log sum alone may be an exponential without bounds)
+                    for (uint32_t r = 0; r < 4; r++) p[t][r] = __builtin_amdgcn_exp2f((p[t][r] - (own_table ? first[r] : lse[t].x)) - (own_table ? second[r] : lse[t].y));
+                if (!own_table && m0 + 16 > end) {  // (past the table: a zero less the log sum may be an exponential without bounds)
 #pragma unroll
                     for (uint32_t t = 0; t < TILES; t++)
 #pragma unroll
@@ -227,7 +231,7 @@ __global__ __launch_bounds__(block) void entropy_narrow_kernel(EntropyNarrowArgs
     for (uint32_t t = 0; t < TILES; t++) {
         const uint32_t o = own_first + t * 16 + e;
         if constexpr (!gradient) {
-            float top = reference[t], total = sum[t];
+            float top = begun[t] ? reference[t] : -infinity, total = sum[t];
 #pragma unroll
             for (uint32_t x = 16; x < 64; x <<= 1) {
                 const float other = __shfl_xor(top, x), other_total = __shfl_xor(total, x);
@@ -285,9 +289,12 @@ EntropyNarrowPlan entropy_narrow_plan(uint32_t own, uint32_t stream, uint32_t co
     EntropyNarrowPlan p{};
     p.own_waves = own > 2 * wave_rows ? 4 : own > wave_rows ? 2 : 1;
     p.blocks = std::max(div_up(own, p.own_waves * wave_rows), 1u);
-    // blocks for four to a CU, unless a block would meet fewer than four chunks
-    const uint32_t chunks = std::max(div_up(stream, chunk), 1u);
-    p.stream_blocks = std::max(1u, std::min({1024u / p.blocks, div_up(chunks, 4), 1024u}));
+    // Blocks for four to a CU, unless one would meet fewer than four chunks; and none that meets many more than 64 (sums of 4,096 rows; one of 15,000 in a row
+    // cost as much precision as all else: table gradient of 1M x 4,096 x 8 1.8e-6 off in 64 parts), where the partial sums take 128 MB at most.
+    const uint64_t chunks = std::max(div_up(stream, chunk), 1u), waves_beside = waves / p.own_waves;
+    const uint64_t wanted = std::max<uint64_t>(1024u / p.blocks, (chunks + 63) / 64);
+    const uint64_t room = (128ull << 20) / (static_cast<uint64_t>(own) * std::max(columns, 4u) * sizeof(float) * waves_beside + 1);
+    p.stream_blocks = static_cast<uint32_t>(std::max<uint64_t>(1, std::min({wanted, (chunks + 3) / 4, std::max<uint64_t>(room, 1024u / p.blocks), uint64_t{1024}})));
     p.splits = p.stream_blocks * (waves / p.own_waves);
     return p;
 }
