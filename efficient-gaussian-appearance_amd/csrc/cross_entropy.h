@@ -10,7 +10,7 @@ constexpr uint32_t entropy_column_tile = 64;   // so do their columns
 constexpr float entropy_half_range = 32768.0f; // float16: what upstream gradients of the logits are held times
 
 // The log sum of a row's exponentials (log 2) is held in two parts, the first near the largest logit and the second small: a probability is
-// exp2((z - first) - second), exact to the rounding of z alone also where z and the sum are large.
+// exp2(z - first) exp2(-second), exact to the rounding of z alone also where z and the sum are large.
 
 // C(i, j) = sum_k A(i, k) B(k, j); i is the table row in the first two products and the column in the gradients, j the packed row and, in
 // the table's gradient, the table row.
@@ -68,8 +68,8 @@ struct EntropyNarrowPlan {
     uint32_t own_waves, blocks, stream_blocks;
     uint32_t splits;               // partial results of an owned row
 };
-constexpr uint32_t entropy_narrow_most = 128, entropy_narrow_most_16 = 32;  // columns of floats, of 16-bit types
-EntropyNarrowPlan entropy_narrow_plan(uint32_t own, uint32_t stream, uint32_t columns);
+constexpr uint32_t entropy_narrow_most = 64;  // columns
+EntropyNarrowPlan entropy_narrow_plan(uint32_t own, uint32_t stream, uint32_t columns, int type);
 void launch_entropy_narrow(EntropyProduct product, int type, const EntropyNarrowArgs& a, const EntropyNarrowPlan& p, hipStream_t s);
 
 }  // namespace efgs

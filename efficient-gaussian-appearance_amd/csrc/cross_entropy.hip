@@ -467,7 +467,7 @@ class Carver {
 uint32_t type_bytes(int type) { return type == type_float ? 4 : 2; }
 
 // the three ways: few columns, 16-bit types, floats
-bool narrow(const EntropyArgs& a) { return a.columns > 0 && a.columns <= (a.type == type_float ? entropy_narrow_most : entropy_narrow_most_16); }
+bool narrow(const EntropyArgs& a) { return a.columns > 0 && a.columns <= entropy_narrow_most; }
 bool wide(const EntropyArgs& a) { return a.type != type_float && !narrow(a); }
 bool table_is_copied(const EntropyArgs& a);
 
@@ -512,7 +512,7 @@ struct ForwardScratch {
     size_t bytes;
     ForwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
-        plan = entropy_narrow_plan(std::max(a.n, 1u), a.rows, a.columns);
+        plan = entropy_narrow_plan(std::max(a.n, 1u), a.rows, a.columns, a.type);
         tiles = narrow(a) ? (a.rows > 0 ? plan.splits : 0) : div_up(a.rows, tile_of(a));
         chunk_counts = c.take<uint32_t>(div_up(s.padded, rank_block));
         const uint64_t most = std::min(partial_bytes / sizeof(float2), most_blocks * tile) / std::max(tiles, 1u);
@@ -549,8 +549,8 @@ struct NarrowBackwardScratch {
     size_t bytes;
     NarrowBackwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
-        features = entropy_narrow_plan(std::max(a.n, 1u), a.rows, a.columns);
-        table = entropy_narrow_plan(a.rows, std::max(a.n, 1u), a.columns);
+        features = entropy_narrow_plan(std::max(a.n, 1u), a.rows, a.columns, a.type);
+        table = entropy_narrow_plan(a.rows, std::max(a.n, 1u), a.columns, a.type);
         slab_stride = static_cast<uint32_t>(round_up(a.columns, 4));
         weight = c.take<float>(s.padded);
         factor = c.take<float>(1);
