@@ -31,6 +31,7 @@ SOURCES = [
     ('embedding.hip', []),
     ('cross_entropy.hip', []),
     ('cross_entropy_16.hip', []),
+    ('cross_entropy_few.hip', []),
     ('cross_entropy_narrow.hip', []),
     ('dropout.hip', ['-ffp-contract=off']),
     ('balance.hip', []),

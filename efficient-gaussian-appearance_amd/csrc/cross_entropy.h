@@ -72,4 +72,9 @@ constexpr uint32_t entropy_narrow_most = 64;  // columns
 EntropyNarrowPlan entropy_narrow_plan(uint32_t own, uint32_t stream, uint32_t columns, int type);
 void launch_entropy_narrow(EntropyProduct product, int type, const EntropyNarrowArgs& a, const EntropyNarrowPlan& p, hipStream_t s);
 
+// up to 64 rows without a gradient (n, rows and columns at least 1)
+constexpr uint32_t entropy_few_most = 64;
+size_t entropy_few_bytes(const EntropyArgs& a);
+void launch_entropy_few(const EntropyArgs& a, float* loss, void* scratch, hipStream_t s);
+
 }  // namespace efgs

@@ -466,7 +466,8 @@ class Carver {
 
 uint32_t type_bytes(int type) { return type == type_float ? 4 : 2; }
 
-// the three ways: few columns, 16-bit types, floats
+// the ways: few rows without a gradient; few columns; 16-bit types; floats
+bool few(const EntropyArgs& a) { return a.n > 0 && a.n <= entropy_few_most && a.rows > 0 && a.columns > 0; }
 bool narrow(const EntropyArgs& a) { return a.columns > 0 && a.columns <= entropy_narrow_most; }
 bool wide(const EntropyArgs& a) { return a.type != type_float && !narrow(a); }
 bool table_is_copied(const EntropyArgs& a);
@@ -718,14 +719,23 @@ bool entropy_fits(const EntropyArgs& a) {
 }
 
 size_t entropy_saved_bytes(const EntropyArgs& a) { return Saved(a, nullptr).bytes; }
-size_t entropy_forward_bytes(const EntropyArgs& a) { return ForwardScratch(a, Saved(a, nullptr), nullptr).bytes; }
+size_t entropy_forward_bytes(const EntropyArgs& a, bool backward) {
+    if (!backward && few(a)) return entropy_few_bytes(a);
+    const Saved s(a, nullptr);
+    return (backward ? 0 : s.bytes) + ForwardScratch(a, s, nullptr).bytes;
+}
 size_t entropy_backward_bytes(const EntropyArgs& a) {
     return narrow(a) ? NarrowBackwardScratch(a, Saved(a, nullptr), nullptr).bytes : BackwardScratch(a, Saved(a, nullptr), nullptr).bytes;
 }
 
 bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void* scratch, hipStream_t stream) {
-    const Saved s(a, saved);
-    const ForwardScratch f(a, s, scratch);
+    if (!saved && few(a)) {
+        launch_entropy_few(a, loss, scratch, stream);
+        EFGS_HIP_CHECK(hipGetLastError());
+        return true;
+    }
+    const Saved s(a, saved ? saved : scratch);
+    const ForwardScratch f(a, s, saved ? scratch : static_cast<char*>(scratch) + s.bytes);
     launch_packing(a, s, f.chunk_counts, stream);
     const Table table = table_of(a, s, f.copied ? f.copy : nullptr, stream);
     for (uint32_t first = 0; first < s.padded; first += f.rows_at_once) {

@@ -326,8 +326,9 @@ struct EntropyArgs {
 constexpr int64_t entropy_max = (1ll << 31) - 1024;  // rows of either side, columns
 bool entropy_fits(const EntropyArgs& a);             // whether the launches can count their blocks
 size_t entropy_saved_bytes(const EntropyArgs& a);    // what a backward needs of its forward
-size_t entropy_forward_bytes(const EntropyArgs& a);  // of `scratch`
+size_t entropy_forward_bytes(const EntropyArgs& a, bool backward);  // of `scratch`, with a backward to follow or without
 size_t entropy_backward_bytes(const EntropyArgs& a);
+// saved: null without a backward
 bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void* scratch, hipStream_t s);
 bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const void* saved, void* grad_features, void* grad_table, void* scratch,
                              hipStream_t s);

@@ -312,10 +312,9 @@ int efgs_linear_cross_entropy_forward(const efgs_entropy* e, float* loss, void* 
         if (!entropy_fits(a)) return fail(EFGS_ERR_INVALID_ARGUMENT, "too many rows and columns in the cross entropy");
         if ((!loss && !(a.each && a.n == 0)) || !alloc || (a.n > 0 && (!a.targets || (a.columns > 0 && !a.features))) || (a.rows > 0 && a.columns > 0 && !a.table))
             return fail(EFGS_ERR_INVALID_ARGUMENT, "null cross entropy tensor");
-        const size_t own = saved ? 0 : entropy_saved_bytes(a);  // (a forward without a backward: scratch)
-        char* const scratch = static_cast<char*>(alloc(alloc_ctx, own + entropy_forward_bytes(a)));
+        void* const scratch = alloc(alloc_ctx, entropy_forward_bytes(a, saved != nullptr));
         if (!scratch) return fail(EFGS_ERR_ALLOC, "allocation of the cross entropy's workspace failed");
-        return launch_entropy_forward(a, loss, saved ? saved : scratch, scratch + own, static_cast<hipStream_t>(stream)) ? EFGS_OK : EFGS_ERR_HIP;
+        return launch_entropy_forward(a, loss, saved, scratch, static_cast<hipStream_t>(stream)) ? EFGS_OK : EFGS_ERR_HIP;
     });
 }
 

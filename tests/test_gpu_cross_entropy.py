@@ -79,14 +79,15 @@ def check(n, rows, columns, dtype, scale=1.0, reduction='mean', grads=(True, Tru
     losses, loss_bar, dx, bar_x, dw, bar_w = bounds(features, table, targets, weights, scale, dtype)
     loss = efgs.linear_cross_entropy(features, table, targets, scale, reduction)
     with torch.no_grad():
-        assert torch.equal(efgs.linear_cross_entropy(features, table, targets, scale, reduction), loss)
-    assert loss.dtype == torch.float32
-    if reduction == 'none':
-        within('losses', loss, losses, loss_bar)
-        assert np.all(loss.detach().cpu().numpy()[loss_bar == 0] == 0)
-    else:
-        share = max(inside, 1) if reduction == 'mean' else 1
-        within('loss', loss, np.asarray(losses.sum() / share), np.asarray((loss_bar.sum() + 2 * E * losses.sum()) / share + 1e-300))
+        alone = efgs.linear_cross_entropy(features, table, targets, scale, reduction)
+    for value in (loss, alone):  # (without a gradient a few rows take another way)
+        assert value.dtype == torch.float32
+        if reduction == 'none':
+            within('losses', value, losses, loss_bar)
+            assert np.all(value.detach().cpu().numpy()[loss_bar == 0] == 0)
+        else:
+            share = max(inside, 1) if reduction == 'mean' else 1
+            within('loss', value, np.asarray(losses.sum() / share), np.asarray((loss_bar.sum() + 2 * E * losses.sum()) / share + 1e-300))
     loss.backward(up)
     if grads[0]:
         assert features.grad.dtype == features.dtype
@@ -326,6 +327,40 @@ def test_second_derivatives_raise():
     grad = torch.autograd.grad(efgs.linear_cross_entropy(features, table, targets), features, up, create_graph=True)[0]
     with pytest.raises(RuntimeError, match='once_differentiable'):
         torch.autograd.grad(grad.sum(), up)
+
+
+@pytest.mark.parametrize('n', [1, 2, 3, 16, 17, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize('columns', [1, 5, 31, 32, 33, 63, 64, 65, 127, 129, 200, 1000, 1024])
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+def test_a_few_rows_without_a_gradient(n, columns, dtype):
+    import efgs
+    rows = 37 * n + columns % 97 + 1
+    features, table, targets, _ = inputs(n, rows, columns, dtype, seed=n + columns, left_out=0.2)
+    losses, bar = bounds(features, table, targets, np.ones(n), 0.8, dtype, gradient=False)
+    within('losses', efgs.linear_cross_entropy(features, table, targets, 0.8, 'none'), losses, bar)
+    count = max(1, int(((targets >= 0) & (targets < rows)).sum()))
+    mean = efgs.linear_cross_entropy(features, table, targets, 0.8)
+    within('mean', mean, np.asarray(losses.sum() / count), np.asarray((bar.sum() + 2 * E * losses.sum()) / count + 1e-300))
+    odd = torch.empty(rows * (columns + 3) + 1, dtype=table.dtype, device=DEVICE)[1:].view(rows, columns + 3)[:, 2:columns + 2]
+    odd.copy_(table)
+    assert torch.equal(efgs.linear_cross_entropy(features, odd, targets, 0.8), mean)
+
+
+def test_what_stands_in_few_rows_left_out_reaches_nothing():
+    import efgs
+    features, table, targets, _ = inputs(40, 500, 100, 'bf16', left_out=0.3)
+    out = (targets < 0) | (targets >= 500)
+    results = []
+    for value in (0.0, float('nan'), float('inf')):
+        x = features.clone()
+        x[out] = value
+        results.append((efgs.linear_cross_entropy(x, table, targets, reduction='none'), efgs.linear_cross_entropy(x, table, targets)))
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.equal(a, b)
+    features[3] = float('nan')
+    targets[3] = 1
+    assert bool(torch.isnan(efgs.linear_cross_entropy(features, table, targets, reduction='none')[3]))
 
 
 def test_pieces_and_lists_of_many_rows():
