@@ -313,26 +313,31 @@ struct JoinArgs {
     double* sums;          // of each block's rows
 };
 
-constexpr uint32_t join_rows = 64, join_parts = 16;
+constexpr uint32_t join_rows = 64;
+constexpr uint32_t join_parts = 16, join_alone = 4;  // parts of the tiles; up to so many tiles: one, four times the rows
 
-// 64 packed rows a block, the tiles of the table in sixteen parts
-__global__ __launch_bounds__(join_rows * join_parts) void entropy_join_kernel(JoinArgs a) {
-    __shared__ float2 parts[join_parts][join_rows];
-    const uint32_t lane = threadIdx.x & (join_rows - 1u), part = threadIdx.x / join_rows, at = blockIdx.x * join_rows + lane, row = a.first_row + at;
+// 64 packed rows a wave, the tiles of the table in PARTS parts
+template <uint32_t PARTS>
+__global__ __launch_bounds__(PARTS > 1 ? join_rows * PARTS : 256) void entropy_join_kernel(JoinArgs a) {
+    __shared__ float2 parts[PARTS][join_rows];
+    const uint32_t lane = threadIdx.x & (join_rows - 1u), wave = threadIdx.x / join_rows, part = PARTS > 1 ? wave : 0;
+    const uint32_t at = PARTS > 1 ? blockIdx.x * join_rows + lane : blockIdx.x * 256 + threadIdx.x, row = a.first_row + at;
     const uint32_t count = *a.count;
     const bool counts = row < count;
     float top = -infinity, sum = 0.0f;
     if (counts)
-        for (uint32_t t = part; t < a.tiles; t += join_parts) {
+        for (uint32_t t = part; t < a.tiles; t += PARTS) {
             const float2 x = a.partial[static_cast<uint64_t>(t) * a.rows + at];
             const float higher = fmaxf(top, x.x), from = higher == -infinity ? 0.0f : higher;
             sum = sum * __builtin_amdgcn_exp2f(top - from) + x.y * __builtin_amdgcn_exp2f(x.x - from);
             top = higher;
         }
-    parts[part][lane] = make_float2(top, sum);
-    __syncthreads();
-    if (part != 0) return;
-    for (uint32_t k = 1; k < join_parts; k++) {
+    if constexpr (PARTS > 1) {
+        parts[part][lane] = make_float2(top, sum);
+        __syncthreads();
+        if (part != 0) return;
+    }
+    for (uint32_t k = 1; k < PARTS; k++) {
         const float2 x = parts[k][lane];
         const float higher = fmaxf(top, x.x), from = higher == -infinity ? 0.0f : higher;
         sum = sum * __builtin_amdgcn_exp2f(top - from) + x.y * __builtin_amdgcn_exp2f(x.x - from);
@@ -355,16 +360,19 @@ __global__ __launch_bounds__(join_rows * join_parts) void entropy_join_kernel(Jo
     if (lane == 0) a.sums[row / join_rows] = total;
 }
 
-__global__ __launch_bounds__(256) void entropy_total_kernel(const double* sums, uint32_t blocks, const uint32_t* count, bool mean, float* loss) {
-    __shared__ double lds[4];
+constexpr uint32_t total_block = 1024;
+
+__global__ __launch_bounds__(total_block) void entropy_total_kernel(const double* sums, uint32_t waves, const uint32_t* count, bool mean, float* loss) {
+    __shared__ double lds[total_block / 64];
     double total = 0.0;
-    for (uint32_t b = threadIdx.x; b < blocks; b += 256) total += sums[b];
+    for (uint32_t b = threadIdx.x; b < waves; b += total_block) total += sums[b];
 #pragma unroll
     for (uint32_t o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
     if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = total;
     __syncthreads();
     if (threadIdx.x == 0) {
-        total = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+        total = 0.0;
+        for (uint32_t w = 0; w < total_block / 64; w++) total += lds[w];
         *loss = static_cast<float>(mean ? total / max(*count, 1u) : total);
     }
 }
@@ -443,6 +451,27 @@ __global__ __launch_bounds__(256) void entropy_gather_kernel(Gathering a, T* out
                     if (part * 4 + k < a.columns) to[k] = y[k];
         }
     }
+}
+
+// The same where there are many splits of few rows: sixteen items of four columns a block, their splits in sixteen parts.
+template <typename T>
+__global__ __launch_bounds__(256) void entropy_gather_splits_kernel(Gathering a, T* out) {
+    __shared__ floatx4 lds[16][16];
+    const uint32_t parts = (a.columns + 3) / 4, item = threadIdx.x & 15u, part = threadIdx.x >> 4;
+    const uint64_t items = static_cast<uint64_t>(a.rows) * parts, t = min(blockIdx.x * 16ull + item, items - 1);
+    const uint64_t row = t / parts;
+    const uint32_t column = static_cast<uint32_t>(t - row * parts) * 4, m = a.packed_of ? a.packed_of[row] : static_cast<uint32_t>(row);
+    floatx4 sum{};
+    if (m != none)
+        for (uint32_t s = part; s < a.splits; s += 16) sum += *reinterpret_cast<const floatx4*>(a.slab + (s * a.slab_rows + m) * a.slab_stride + column);
+    lds[part][item] = sum;
+    __syncthreads();
+    if (part != 0 || blockIdx.x * 16ull + item >= items) return;
+    for (uint32_t k = 1; k < 16; k++) sum += lds[k][item];
+    const float f = m == none ? 0.0f : a.weight ? *a.factor * a.weight[m] : *a.factor;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++)
+        if (column + k < a.columns) out[row * a.columns + column + k] = static_cast<T>(m == none ? 0.0f : sum[k] * f);
 }
 
 // ---- sizes and buffers -------------------------------------------------------------------------------------------------
@@ -527,14 +556,17 @@ struct ForwardScratch {
     }
 };
 
-// How often a product's k is split so that its blocks fill the GPU: `at_once` blocks run together, a split costs its partial results once more.
-uint32_t splits_for(uint64_t tiles, uint64_t k, uint64_t at_once) {
+// How often a product's k is split: where its tiles leave much of the GPU idle, more blocks, at the price of partial results (`results` floats) written and
+// read once more for each. A CU takes about 1.7 us for a step of a wide tile (64 of k), and for one of 16 of a float tile beside another; partial results move at 4 TB/s.
+uint32_t splits_for(uint64_t tiles, uint64_t k, uint64_t results, bool wide) {
+    const uint64_t at_once = wide ? 256 : 512, step = wide ? 64 : 16;
     uint32_t best = 1;
     double least = 1e30;
-    for (uint32_t s = 1; s <= 64 && (s == 1 || k / s >= 256); s++) {
-        const double cost = static_cast<double>((tiles * s + at_once - 1) / at_once) / s * (1.0 + 0.02 * (s - 1));
-        if (cost < least) {
-            least = cost;
+    for (uint32_t s = 1; s <= 64 && (s == 1 || k / s >= 2 * step); s++) {
+        const double rounds = static_cast<double>((tiles * s + at_once - 1) / at_once), steps = static_cast<double>((k + s * step - 1) / (s * step));
+        const double us = rounds * steps * 1.7 + (s > 1 ? s * static_cast<double>(results) * 8.0 / 4e6 : 0.0);
+        if (us < least) {
+            least = us;
             best = s;
         }
     }
@@ -578,9 +610,9 @@ struct BackwardScratch {
         pieces = div_up(all, std::min(most, all));
         piece_rows = static_cast<uint32_t>(round_up(div_up(all, pieces), 256));
         pieces = div_up(all, piece_rows);
-        const uint64_t side = tile_of(a), column_tiles = div_up(std::max(a.columns, 1u), side), at_once = wide(a) ? 256 : 512;
-        features_splits = splits_for(s.padded / side * column_tiles, piece_rows, at_once);
-        table_splits = splits_for(piece_rows / side * column_tiles, s.padded, at_once);
+        const uint64_t side = tile_of(a), column_tiles = div_up(std::max(a.columns, 1u), side);
+        features_splits = splits_for(s.padded / side * column_tiles, piece_rows, static_cast<uint64_t>(s.padded) * s.padded_columns, wide(a));
+        table_splits = splits_for(piece_rows / side * column_tiles, s.padded, static_cast<uint64_t>(piece_rows) * s.padded_columns, wide(a));
         weight = c.take<float>(s.padded);
         factor = c.take<float>(1);
         piece = c.take<char>(static_cast<uint64_t>(s.padded) * piece_rows * type_bytes(a.type));
@@ -665,10 +697,12 @@ EntropyNarrowArgs narrow_args(const EntropyArgs& a, const Saved& s) {
 
 void launch_gathering(int type, const Gathering& g, void* out, hipStream_t stream) {
     if (g.rows == 0 || g.columns == 0) return;
-    const uint32_t blocks = copy_grid(static_cast<uint64_t>(g.rows) * ((g.columns + 3) / 4));
+    const uint64_t items = static_cast<uint64_t>(g.rows) * ((g.columns + 3) / 4);
+    const uint32_t blocks = copy_grid(items);
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(entropy_gather_kernel<T>, dim3(blocks), dim3(256), 0, stream, g, static_cast<T*>(out));
+        if (g.splits >= 16 && items <= 1u << 18) hipLaunchKernelGGL(entropy_gather_splits_kernel<T>, dim3(div_up(items, 16)), dim3(256), 0, stream, g, static_cast<T*>(out));
+        else hipLaunchKernelGGL(entropy_gather_kernel<T>, dim3(blocks), dim3(256), 0, stream, g, static_cast<T*>(out));
     });
 }
 
@@ -767,9 +801,10 @@ bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void
             launch_product(entropy_logits, a, p, rows, stream);
         }
         const JoinArgs j{f.partial, f.tiles, first, rows, a.n, s.count, s.row_of, s.packed_of, f.target_logit, s.lse, a.each ? loss : nullptr, f.sums};
-        hipLaunchKernelGGL(entropy_join_kernel, dim3(rows / join_rows), dim3(join_rows * join_parts), 0, stream, j);
+        if (f.tiles <= join_alone) hipLaunchKernelGGL(entropy_join_kernel<1>, dim3(rows / 256), dim3(256), 0, stream, j);
+        else hipLaunchKernelGGL(entropy_join_kernel<join_parts>, dim3(rows / join_rows), dim3(join_rows * join_parts), 0, stream, j);
     }
-    if (!a.each) hipLaunchKernelGGL(entropy_total_kernel, dim3(1), dim3(256), 0, stream, f.sums, s.padded / join_rows, s.count, a.mean, loss);
+    if (!a.each) hipLaunchKernelGGL(entropy_total_kernel, dim3(1), dim3(total_block), 0, stream, f.sums, s.padded / join_rows, s.count, a.mean, loss);
     EFGS_HIP_CHECK(hipGetLastError());
     return true;
 }
