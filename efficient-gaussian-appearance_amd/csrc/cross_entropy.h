@@ -43,9 +43,8 @@ struct EntropyProductArgs {
     const float* factor;
 };
 
-// 16-bit types, tiles of 256 x 256: rows of 16-byte aligned memory, strides in multiples of 8 elements
-constexpr uint32_t entropy_wide_tile = 256;
-void launch_entropy_wide(EntropyProduct product, int type, const EntropyProductArgs& a, uint32_t j_tiles, hipStream_t s);
+// 16-bit types, tiles of side x side (256 or 128): rows of 16-byte aligned memory, strides in multiples of 8 elements; j of them at most
+void launch_entropy_wide(EntropyProduct product, int type, uint32_t side, const EntropyProductArgs& a, uint32_t j, hipStream_t s);
 
 // few columns: products and exponentials of a tile in one kernel
 struct EntropyNarrowArgs {

@@ -501,7 +501,6 @@ bool narrow(const EntropyArgs& a) { return a.columns > 0 && a.columns <= entropy
 bool wide(const EntropyArgs& a) { return a.type != type_float && !narrow(a); }
 bool table_is_copied(const EntropyArgs& a);
 
-uint32_t tile_of(const EntropyArgs& a) { return wide(a) ? entropy_wide_tile : tile; }
 
 struct Saved {
     uint32_t* count;
@@ -526,6 +525,33 @@ struct Saved {
     }
 };
 
+// The side of a product's tiles, and how often its k is split: where tiles leave much of the GPU idle, smaller ones and more blocks, at the price of less reuse, or of
+// partial results (`results` floats) written and read once more for each split. Measured: a CU takes 1.7 us for 64 of k of a tile of 256, 1.2 for those of two of 128 (0.8 for
+// one alone), 1.8 for 16 of k of two float tiles; partial results move at 4 TB/s.
+struct ProductPlan {
+    uint32_t side, splits;
+};
+
+ProductPlan plan_product(const EntropyArgs& a, uint64_t i, uint64_t j, uint64_t k, uint64_t results) {
+    ProductPlan best{tile, 1};
+    double least = 1e30;
+    for (const uint32_t side : {256u, 128u}) {
+        if (side == 256 && !wide(a)) continue;
+        const uint64_t tiles = ((i + side - 1) / side) * ((j + side - 1) / side), at_once = side == 256 ? 256 : 512, step = wide(a) ? 64 : 16;
+        for (uint32_t s = 1; s <= 64 && (s == 1 || (results > 0 && k / s >= 2 * step)); s++) {
+            const uint64_t blocks = tiles * s;
+            const double step_us = !wide(a) ? 1.8 : side == 256 ? 1.7 : blocks <= 256 ? 0.8 : 1.2;
+            const double rounds = static_cast<double>((blocks + at_once - 1) / at_once), steps = static_cast<double>((k + s * step - 1) / (s * step));
+            const double us = rounds * (steps + 2.0) * step_us + (s > 1 ? s * static_cast<double>(results) * 8.0 / 4e6 : 0.0);
+            if (us < least) {
+                least = us;
+                best = {side, s};
+            }
+        }
+    }
+    return best;
+}
+
 constexpr uint64_t partial_bytes = 256ull << 20;  // of the tiles' statistics at once
 constexpr uint64_t piece_bytes = 256ull << 20;    // of a piece's upstream gradients
 constexpr uint64_t most_blocks = 1ull << 23;      // of a launch of 256 threads (32 bits of threads)
@@ -538,12 +564,13 @@ struct ForwardScratch {
     void* copy;        // of the table, or null
     bool copied;
     EntropyNarrowPlan plan;
-    uint32_t tiles, rows_at_once;
+    uint32_t side, tiles, rows_at_once;
     size_t bytes;
     ForwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
         plan = entropy_narrow_plan(std::max(a.n, 1u), a.rows, a.columns, a.type);
-        tiles = narrow(a) ? (a.rows > 0 ? plan.splits : 0) : div_up(a.rows, tile_of(a));
+        side = plan_product(a, a.rows, s.padded, a.columns, 0).side;
+        tiles = narrow(a) ? (a.rows > 0 ? plan.splits : 0) : div_up(a.rows, side);
         chunk_counts = c.take<uint32_t>(div_up(s.padded, rank_block));
         const uint64_t most = std::min(partial_bytes / sizeof(float2), most_blocks * tile) / std::max(tiles, 1u);
         rows_at_once = narrow(a) ? s.padded : static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(most / row_tile * row_tile, row_tile), s.padded));
@@ -555,23 +582,6 @@ struct ForwardScratch {
         bytes = c.used();
     }
 };
-
-// How often a product's k is split: where its tiles leave much of the GPU idle, more blocks, at the price of partial results (`results` floats) written and
-// read once more for each. A CU takes about 1.7 us for a step of a wide tile (64 of k), and for one of 16 of a float tile beside another; partial results move at 4 TB/s.
-uint32_t splits_for(uint64_t tiles, uint64_t k, uint64_t results, bool wide) {
-    const uint64_t at_once = wide ? 256 : 512, step = wide ? 64 : 16;
-    uint32_t best = 1;
-    double least = 1e30;
-    for (uint32_t s = 1; s <= 64 && (s == 1 || k / s >= 2 * step); s++) {
-        const double rounds = static_cast<double>((tiles * s + at_once - 1) / at_once), steps = static_cast<double>((k + s * step - 1) / (s * step));
-        const double us = rounds * steps * 1.7 + (s > 1 ? s * static_cast<double>(results) * 8.0 / 4e6 : 0.0);
-        if (us < least) {
-            least = us;
-            best = s;
-        }
-    }
-    return best;
-}
 
 struct NarrowBackwardScratch {
     float* weight;
@@ -601,7 +611,7 @@ struct BackwardScratch {
     void* copy;              // of the table, or null
     bool copied;
     uint32_t piece_rows, pieces;
-    uint32_t features_splits, table_splits;
+    ProductPlan upstream, features, table;
     size_t bytes;
     BackwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
@@ -610,14 +620,14 @@ struct BackwardScratch {
         pieces = div_up(all, std::min(most, all));
         piece_rows = static_cast<uint32_t>(round_up(div_up(all, pieces), 256));
         pieces = div_up(all, piece_rows);
-        const uint64_t side = tile_of(a), column_tiles = div_up(std::max(a.columns, 1u), side);
-        features_splits = splits_for(s.padded / side * column_tiles, piece_rows, static_cast<uint64_t>(s.padded) * s.padded_columns, wide(a));
-        table_splits = splits_for(piece_rows / side * column_tiles, s.padded, static_cast<uint64_t>(piece_rows) * s.padded_columns, wide(a));
+        upstream = plan_product(a, piece_rows, s.padded, a.columns, 0);
+        features = plan_product(a, a.columns, s.padded, piece_rows, static_cast<uint64_t>(s.padded) * s.padded_columns);
+        table = plan_product(a, a.columns, piece_rows, s.padded, static_cast<uint64_t>(piece_rows) * s.padded_columns);
         weight = c.take<float>(s.padded);
         factor = c.take<float>(1);
         piece = c.take<char>(static_cast<uint64_t>(s.padded) * piece_rows * type_bytes(a.type));
-        features_slab = c.take<float>(static_cast<uint64_t>(features_splits) * s.padded * s.padded_columns);
-        table_slab = table_splits > 1 ? c.take<float>(static_cast<uint64_t>(table_splits) * piece_rows * s.padded_columns) : nullptr;
+        features_slab = c.take<float>(static_cast<uint64_t>(features.splits) * s.padded * s.padded_columns);
+        table_slab = table.splits > 1 ? c.take<float>(static_cast<uint64_t>(table.splits) * piece_rows * s.padded_columns) : nullptr;
         copied = table_is_copied(a);
         copy = copied ? c.take<char>(static_cast<uint64_t>(a.rows) * s.padded_columns * type_bytes(a.type)) : nullptr;
         bytes = c.used();
@@ -729,9 +739,9 @@ bool launch_narrow_backward(const EntropyArgs& a, const float* upstream, const S
     return true;
 }
 
-void launch_product(EntropyProduct product, const EntropyArgs& a, const EntropyProductArgs& p, uint32_t j, hipStream_t stream) {
+void launch_product(EntropyProduct product, const EntropyArgs& a, uint32_t side, const EntropyProductArgs& p, uint32_t j, hipStream_t stream) {
     if (wide(a)) {
-        launch_entropy_wide(product, a.type, p, div_up(j, entropy_wide_tile), stream);
+        launch_entropy_wide(product, a.type, side, p, j, stream);
         return;
     }
     const dim3 grid(p.i_tiles * div_up(j, tile), p.splits);
@@ -798,7 +808,7 @@ bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void
             p.slab_rows = rows;
             p.target_logit = f.target_logit;
             p.target = s.target;
-            launch_product(entropy_logits, a, p, rows, stream);
+            launch_product(entropy_logits, a, f.side, p, rows, stream);
         }
         const JoinArgs j{f.partial, f.tiles, first, rows, a.n, s.count, s.row_of, s.packed_of, f.target_logit, s.lse, a.each ? loss : nullptr, f.sums};
         if (f.tiles <= join_alone) hipLaunchKernelGGL(entropy_join_kernel<1>, dim3(rows / 256), dim3(256), 0, stream, j);
@@ -820,7 +830,7 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
     const WeightArgs weights{upstream, s.count, s.row_of, s.padded, a.each, a.mean, a.scale, half ? entropy_half_range : 1.0f, w.weight, w.factor};
     if (half && a.each) hipLaunchKernelGGL(entropy_half_weights_kernel, dim3(1), dim3(1024), 0, stream, weights);
     else hipLaunchKernelGGL(entropy_weights_kernel, dim3(div_up(s.padded, 256)), dim3(256), 0, stream, weights);
-    const uint32_t side = tile_of(a), column_tiles = div_up(a.columns, side), bytes = type_bytes(a.type);
+    const uint32_t bytes = type_bytes(a.type);
     for (uint32_t piece = 0; piece < w.pieces && a.rows > 0; piece++) {
         const uint32_t first = piece * w.piece_rows, rows = std::min(a.rows - first, w.piece_rows);
         const void* const part = static_cast<const char*>(table.rows) + first * table.stride * bytes;
@@ -833,7 +843,7 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
         p.i_end = rows;
         p.j_end = s.padded;
         p.k_end = table.columns;
-        p.i_tiles = div_up(rows, side);
+        p.i_tiles = div_up(rows, w.upstream.side);
         p.splits = 1;
         p.count = s.count;
         p.to_log2 = a.scale * log2_e;
@@ -843,11 +853,10 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
         p.first_row = first;
         p.piece = w.piece;
         p.piece_stride = w.piece_rows;
-        launch_product(entropy_upstream, a, p, s.padded, stream);
+        launch_product(entropy_upstream, a, w.upstream.side, p, s.padded, stream);
         EntropyProductArgs x{};
         x.count = s.count;
         x.i_end = a.columns;
-        x.i_tiles = column_tiles;
         x.slab_stride = s.padded_columns;
         x.b = w.piece;
         x.b_stride = w.piece_rows;
@@ -855,34 +864,36 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
             x.a = part;
             x.a_stride = table.stride;
             x.a_columns = table.columns;
+            x.i_tiles = div_up(a.columns, w.features.side);
             x.j_end = s.padded;
             x.k_end = rows;
-            x.splits = w.features_splits;
+            x.splits = w.features.splits;
             x.slab = w.features_slab;
             x.slab_rows = s.padded;
             x.add = piece > 0;
-            launch_product(entropy_features_gradient, a, x, s.padded, stream);
+            launch_product(entropy_features_gradient, a, w.features.side, x, s.padded, stream);
         }
         if (grad_table) {
             void* const out = static_cast<char*>(grad_table) + static_cast<uint64_t>(first) * a.columns * bytes;
             x.a = s.packed;
             x.a_stride = s.padded_columns;
             x.a_columns = s.padded_columns;
+            x.i_tiles = div_up(a.columns, w.table.side);
             x.j_end = rows;
-            x.splits = w.table_splits;
+            x.splits = w.table.splits;
             x.slab = w.table_slab;
             x.slab_rows = w.piece_rows;
             x.add = false;
             x.out = x.splits > 1 ? nullptr : out;
             x.out_stride = a.columns;
             x.factor = w.factor;
-            launch_product(entropy_table_gradient, a, x, rows, stream);
+            launch_product(entropy_table_gradient, a, w.table.side, x, rows, stream);
             if (x.splits > 1)
                 launch_gathering(a.type, {w.table_slab, w.piece_rows, s.padded_columns, x.splits, nullptr, nullptr, rows, a.columns, w.factor}, out, stream);
         }
     }
     if (grad_features)
-        launch_gathering(a.type, {w.features_slab, s.padded, s.padded_columns, w.features_splits, s.packed_of, nullptr, a.n, a.columns, w.factor},
+        launch_gathering(a.type, {w.features_slab, s.padded, s.padded_columns, w.features.splits, s.packed_of, nullptr, a.n, a.columns, w.factor},
                          grad_features, stream);
     EFGS_HIP_CHECK(hipGetLastError());
     return true;

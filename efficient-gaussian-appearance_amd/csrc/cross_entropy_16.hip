@@ -1,10 +1,10 @@
 // The cross entropy's matrix products for bfloat16 and float16 on v_mfma_f32_16x16x32: 256 x 256 results to a block of eight waves (2 along i,
-// 4 along j, 128 x 64 each), 64 of k at a time.
+// 4 along j, 128 x 64 each), or, where those would leave most of the GPU idle, 128 x 128 to one of four (64 x 64 each); 64 of k at a time.
 //
-// Operand tiles go from memory to LDS past the registers (16 bytes a lane), two stages of 64 KB: while a stage is multiplied
+// Operand tiles go from memory to LDS past the registers (16 bytes a lane), two stages of 64 KB (32): while a stage is multiplied
 // the next one is on its way, with one barrier a stage. An operand whose memory runs along k lies in rows of 64 k (128 bytes), its 16-byte
 // chunks exchanged by the row's low bits, so that the reads of eight rows meet all banks; one whose memory runs along i (or j) lies as it
-// is, 256 to a row of k, and is read by the transposing read, four rows of k by 16 columns to 16 lanes, its pairs of chunks
+// is, 256 (128) to a row of k, and is read by the transposing read, four rows of k by 16 columns to 16 lanes, its pairs of chunks
 // exchanged by k's bits. What lies past an operand's end is read as zero by the buffer's bounds.
 //
 // A lane's results are four consecutive i at one j: in the logits i is the table row, so that a row's maximum and sum
@@ -25,9 +25,8 @@ typedef short shortx8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 
-constexpr uint32_t tile = entropy_wide_tile, step_k = 64, block = 512, waves = 8;
-constexpr uint32_t operand_bytes = tile * step_k * 2, stage_bytes = 2 * operand_bytes;
-constexpr uint32_t wave_chunks = operand_bytes / 1024 / waves;  // transfers of 1 KB by a wave to an operand's tile
+constexpr uint32_t step_k = 64, wave_chunks = 4;                // transfers of 1 KB by a wave to an operand's tile
+template <uint32_t SIDE> constexpr uint32_t block_of = SIDE * 2;
 constexpr uint32_t outside = 0xfffffff0u;                       // an offset past every bound
 constexpr float infinity = __builtin_inff();
 
@@ -58,7 +57,7 @@ __device__ __forceinline__ uintx4 buffer_of(const void* base, uint64_t bytes) {
 }
 
 // An operand: ALONG_K, `first` its first row of the tile (of `rows`), k along them; otherwise `first` the tile's first column, k the row.
-template <bool ALONG_K>
+template <uint32_t SIDE, bool ALONG_K>
 struct Operand {
     const char* base;
     uint64_t stride;         // bytes
@@ -77,7 +76,7 @@ struct Operand {
         first = first_;
         k_end = k_end_;
         if constexpr (ALONG_K) {
-            const uint64_t left = min(rows - first, tile);
+            const uint64_t left = min(rows - first, SIDE);
             buffer = buffer_of(base + first * stride, (left - 1) * stride + columns * 2ull);
             chunk_k = ((lane & 7u) ^ (lane >> 3)) * 8;
 #pragma unroll
@@ -86,8 +85,9 @@ struct Operand {
         } else {
 #pragma unroll
             for (uint32_t u = 0; u < wave_chunks; u++) {
-                const uint32_t k = (wave * wave_chunks + u) * 2 + (lane >> 5), exchange = (k & 3u) | (k >> 3 & 1u) << 2;
-                offsets[u] = k * static_cast<uint32_t>(stride) + (first + ((lane & 31u) ^ 2 * exchange) * 8) * 2;
+                constexpr uint32_t lanes = SIDE / 8;  // of a row
+                const uint32_t k = (wave * wave_chunks + u) * (64 / lanes) + lane / lanes, exchange = (k & 3u) | (k >> 3 & 1u) << 2;
+                offsets[u] = k * static_cast<uint32_t>(stride) + (first + (lane % lanes ^ 2 * exchange) * 8) * 2;
             }
         }
     }
@@ -107,8 +107,9 @@ struct Operand {
 };
 
 // Fragments of a step: lane (e, q) holds k = 8 q..8 q + 7 of each half step of 32 at column e of each 16.
-template <bool ALONG_K, uint32_t N>
+template <uint32_t SIDE, bool ALONG_K, uint32_t N>
 struct Fragments {
+    static constexpr uint32_t row_bytes = SIDE * 2;  // of k
     uint32_t at[ALONG_K ? 2 : N];
 
     __device__ __forceinline__ void begin(uint32_t first) {
@@ -119,7 +120,7 @@ struct Fragments {
         } else {
             const uint32_t exchange = (e >> 2) | (q & 1u) << 2;
 #pragma unroll
-            for (uint32_t t = 0; t < N; t++) at[t] = (8 * q + (e >> 2)) * 512 + ((first / 16 + t) ^ exchange) * 32 + (e & 3u) * 8;
+            for (uint32_t t = 0; t < N; t++) at[t] = (8 * q + (e >> 2)) * row_bytes + ((first / 16 + t) ^ exchange) * 32 + (e & 3u) * 8;
         }
     }
 
@@ -128,17 +129,18 @@ struct Fragments {
             return *reinterpret_cast<const shortx8*>(lds + at[half] + t * 2048);
         } else {
             using Part = __attribute__((address_space(3))) shortx4;
-            const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Part*)(lds + at[t] + half * 32 * 512));
-            const shortx4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Part*)(lds + at[t] + half * 32 * 512 + 4 * 512));
+            const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Part*)(lds + at[t] + half * 32 * row_bytes));
+            const shortx4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Part*)(lds + at[t] + (half * 32 + 4) * row_bytes));
             return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
 };
 
-template <typename T, EntropyProduct P>
-__global__ __launch_bounds__(block) void entropy_wide_kernel(EntropyProductArgs a) {
+template <typename T, EntropyProduct P, uint32_t SIDE>
+__global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(EntropyProductArgs a) {
     constexpr bool first_two = P == entropy_logits || P == entropy_upstream, a_along_k = first_two, b_along_k = P != entropy_table_gradient;
-    constexpr uint32_t wave_i = 8, wave_j = 4;  // tiles of 16 a wave
+    constexpr uint32_t tile = SIDE, operand_bytes = tile * step_k * 2, stage_bytes = 2 * operand_bytes;
+    constexpr uint32_t wave_i = SIDE / 32, wave_j = 4;  // tiles of 16 a wave
     __shared__ __attribute__((aligned(1024))) char lds[2 * stage_bytes];
     const uint32_t count = scalar(*a.count);
     // Blocks go round the eight XCDs one by one: each XCD takes a run of the tiles, four rows of j at a time along i, so that the tiles that
@@ -154,8 +156,8 @@ __global__ __launch_bounds__(block) void entropy_wide_kernel(EntropyProductArgs 
     const uint32_t k_first = min(blockIdx.y * k_each, k_all), k_end = min(k_first + k_each, k_all);
 
     const uint32_t lane = threadIdx.x & 63u, e = lane & 15u, q = lane >> 4, wave = threadIdx.x >> 6, wi = wave & 1u, wj = wave >> 1;
-    Operand<a_along_k> operand_a;
-    Operand<b_along_k> operand_b;
+    Operand<SIDE, a_along_k> operand_a;
+    Operand<SIDE, b_along_k> operand_b;
     if constexpr (first_two) {
         operand_a.begin(a.a, a.a_stride, a.i_end, a.a_columns, i0, a.a_columns);
         operand_b.begin(a.b, a.b_stride, j0 + tile, static_cast<uint32_t>(a.b_stride), j0, static_cast<uint32_t>(a.b_stride));
@@ -166,9 +168,9 @@ __global__ __launch_bounds__(block) void entropy_wide_kernel(EntropyProductArgs 
         operand_a.begin(a.a, a.a_stride, k_all, a.a_columns, i0, k_all);
         operand_b.begin(a.b, a.b_stride, k_all, static_cast<uint32_t>(a.b_stride), j0, k_all);
     }
-    Fragments<a_along_k, wave_i> fragments_a;
-    Fragments<b_along_k, wave_j> fragments_b;
-    fragments_a.begin(wi * 128);
+    Fragments<SIDE, a_along_k, wave_i> fragments_a;
+    Fragments<SIDE, b_along_k, wave_j> fragments_b;
+    fragments_a.begin(wi * (SIDE / 2));
     fragments_b.begin(wj * 64);
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uint64_t>((__attribute__((address_space(3))) char*)lds));
 
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(block) void entropy_wide_kernel(EntropyProductArgs 
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the zeros that follow the last step
     }
 
-    const uint32_t i_lane = i0 + wi * 128 + 4 * q, j_lane = j0 + wj * 64 + e;  // results: i_lane + 16 ti + r, j_lane + 16 tj
+    const uint32_t i_lane = i0 + wi * (SIDE / 2) + 4 * q, j_lane = j0 + wj * 64 + e;  // results: i_lane + 16 ti + r, j_lane + 16 tj
     if constexpr (P == entropy_logits) {
         __syncthreads();
         float2* const joined = reinterpret_cast<float2*>(lds);
@@ -317,22 +319,27 @@ __global__ __launch_bounds__(block) void entropy_wide_kernel(EntropyProductArgs 
     }
 }
 
-template <typename T>
-void launch(EntropyProduct product, const EntropyProductArgs& a, uint32_t j_tiles, hipStream_t s) {
-    const dim3 grid((a.i_tiles * j_tiles + 7) / 8 * 8, a.splits);
+template <typename T, uint32_t SIDE>
+void launch(EntropyProduct product, const EntropyProductArgs& a, uint32_t j, hipStream_t s) {
+    const dim3 grid((a.i_tiles * div_up(j, SIDE) + 7) / 8 * 8, a.splits), block(block_of<SIDE>);
     switch (product) {
-        case entropy_logits: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_logits>), grid, dim3(block), 0, s, a); break;
-        case entropy_upstream: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_upstream>), grid, dim3(block), 0, s, a); break;
-        case entropy_features_gradient: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_features_gradient>), grid, dim3(block), 0, s, a); break;
-        case entropy_table_gradient: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_table_gradient>), grid, dim3(block), 0, s, a); break;
+        case entropy_logits: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_logits, SIDE>), grid, block, 0, s, a); break;
+        case entropy_upstream: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_upstream, SIDE>), grid, block, 0, s, a); break;
+        case entropy_features_gradient: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_features_gradient, SIDE>), grid, block, 0, s, a); break;
+        case entropy_table_gradient: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_table_gradient, SIDE>), grid, block, 0, s, a); break;
     }
 }
 
 }  // namespace
 
-void launch_entropy_wide(EntropyProduct product, int type, const EntropyProductArgs& a, uint32_t j_tiles, hipStream_t s) {
-    if (type == type_bfloat16) launch<__bf16>(product, a, j_tiles, s);
-    else launch<_Float16>(product, a, j_tiles, s);
+void launch_entropy_wide(EntropyProduct product, int type, uint32_t side, const EntropyProductArgs& a, uint32_t j, hipStream_t s) {
+    if (type == type_bfloat16) {
+        if (side == 256) launch<__bf16, 256>(product, a, j, s);
+        else launch<__bf16, 128>(product, a, j, s);
+    } else {
+        if (side == 256) launch<_Float16, 256>(product, a, j, s);
+        else launch<_Float16, 128>(product, a, j, s);
+    }
 }
 
 }  // namespace efgs
