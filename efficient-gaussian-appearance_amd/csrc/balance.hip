@@ -17,7 +17,7 @@ namespace efgs {
 namespace {
 
 constexpr uint32_t balance_block = 256, balance_waves = balance_block / 64;
-constexpr uint32_t balance_max_blocks = 1024;   // of the forward: rows of the table of sums
+constexpr uint32_t balance_max_blocks = 2048;   // eight to a CU; of the forward: rows of the table of sums
 constexpr float log2_e = 1.4426950408889634f;
 
 template <typename T, int W> struct Part { typedef T type __attribute__((ext_vector_type(W), aligned(sizeof(T)))); };
@@ -35,11 +35,21 @@ struct BalanceKernelArgs {
     void* gradient;
 };
 
+// v of another lane, without LDS: its neighbour, the other pair of its four, its mirror image in eight or in sixteen lanes
+template <int CONTROL>
+__device__ __forceinline__ float exchanged(float v) {
+    const int x = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, CONTROL, 0xf, 0xf, true));
+}
+
 template <uint32_t TPR, typename F>
 __device__ __forceinline__ float across(float v, float* lds, F&& join) {
-    constexpr uint32_t lanes = TPR < 64 ? TPR : 64;
-#pragma unroll
-    for (uint32_t o = 1; o < lanes; o <<= 1) v = join(v, __shfl_xor(v, o));
+    if constexpr (TPR >= 2) v = join(v, exchanged<0xb1>(v));
+    if constexpr (TPR >= 4) v = join(v, exchanged<0x4e>(v));
+    if constexpr (TPR >= 8) v = join(v, exchanged<0x141>(v));
+    if constexpr (TPR >= 16) v = join(v, exchanged<0x140>(v));
+    if constexpr (TPR >= 32) v = join(v, __shfl_xor(v, 16));
+    if constexpr (TPR >= 64) v = join(v, __shfl_xor(v, 32));
     if constexpr (TPR > 64) {  // (a row to the block: a slot for each wave, one set of slots for each reduction of a row)
         if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -91,26 +101,84 @@ __device__ __forceinline__ float exponentials(float (&z)[ITEMS][W], float (*lds)
             sum += z[k][j];
         }
     sum = across<TPR>(sum, lds[1], [](float x, float y) { return x + y; });
-    return sum == 0.0f ? 0.0f : 1.0f / sum;
+    return sum == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum);  // (to a step of the last place)
 }
 
+// The lane's first choice of a row (-1 where it has none). Loaded beside the logits: a load that only follows them costs their latency again.
 template <uint32_t TPR>
-__device__ __forceinline__ bool row_counts(const BalanceKernelArgs& a, uint64_t row, uint32_t lane, bool active, uint32_t* histogram) {
+__device__ __forceinline__ int64_t first_choice(const BalanceKernelArgs& a, uint64_t row, uint32_t lane) {
+    if (a.chosen == 0) return -1;
+    const int64_t e = choice_at(a, row * a.chosen + min(lane, a.chosen - 1));
+    return lane < a.chosen ? e : -1;
+}
+
+// whether the row has a choice; counts its choices in `histogram`, if there is one
+template <uint32_t TPR>
+__device__ __forceinline__ bool row_counts(const BalanceKernelArgs& a, uint64_t row, uint32_t lane, bool active, int64_t first, uint32_t* histogram) {
     bool any = false;
-    for (uint32_t k = lane; k < a.chosen; k += TPR) {
-        const int64_t e = choice_at(a, row * a.chosen + k);
-        const bool valid = active && e >= 0 && e < static_cast<int64_t>(a.experts);
+    int64_t e = first;
+    for (uint32_t k = lane;;) {
+        const bool valid = active && static_cast<uint64_t>(e) < a.experts;
         if (valid && histogram) atomicAdd(&histogram[e], 1u);
         any |= valid;
+        k += TPR;
+        if (k >= a.chosen) break;
+        e = choice_at(a, row * a.chosen + k);
     }
     if constexpr (TPR > 64) return __syncthreads_or(any);
     const uint64_t ballot = __ballot(any), mask = TPR >= 64 ? ~0ull : (1ull << (TPR & 63u)) - 1ull;
     return (ballot >> (threadIdx.x & 63u & ~(TPR - 1u)) & mask) != 0;
 }
 
+struct BalanceTotals {
+    const float* sums;
+    const uint32_t* counts;
+    uint32_t blocks, experts;
+    double* totals;       // experts + 1: sums of probabilities; rows
+    int64_t* count;       // experts
+    float* share;         // experts, then E / rows
+    float* loss;
+};
+
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double sum = 0.0;
+#pragma unroll
+    for (uint32_t w = 0; w < balance_waves; w++) sum += lds[w];
+    return sum;
+}
+
+// one block: shares and the loss from the totals
+__device__ __forceinline__ void loss_of_totals(const BalanceTotals& a) {
+    __shared__ double lds[balance_waves];
+    double choices = 0.0;
+    for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) choices += static_cast<double>(a.count[e]);
+    choices = block_sum(choices, lds);
+    const double rows = a.totals[a.experts], per_choice = choices > 0.0 ? 1.0 / choices : 0.0, per_row = rows > 0.0 ? a.experts / rows : 0.0;
+    double loss = 0.0;
+    for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) {
+        const double share = static_cast<double>(a.count[e]) * per_choice;
+        a.share[e] = static_cast<float>(share);
+        if (a.count[e] > 0) loss += share * a.totals[e];
+    }
+    loss = block_sum(loss, lds);
+    if (threadIdx.x == 0) {
+        a.share[a.experts] = static_cast<float>(per_row);
+        *a.loss = static_cast<float>(loss * per_row);
+    }
+}
+
+// rows of a group of lanes whose loads are under way at once: several where a lane has few values of each
+template <int W, uint32_t TPR, int ITEMS>
+constexpr uint32_t rows_under_way = TPR > 64 || ITEMS * W > 8 ? 1 : ITEMS * W > 4 ? 2 : 4;
+
 // LDS: choices of each expert (experts x 4 bytes), then, where several groups share the block, their sums (waves x experts x 4)
 template <typename T, int W, uint32_t TPR, int ITEMS>
-__global__ __launch_bounds__(balance_block) void balance_forward_kernel(BalanceKernelArgs a) {
+__global__ __launch_bounds__(balance_block) void balance_forward_kernel(BalanceKernelArgs a, BalanceTotals totals) {
     extern __shared__ uint32_t histogram[];
     __shared__ float slots[2][balance_waves];
     __shared__ uint32_t rows_of_wave[balance_waves];
@@ -120,17 +188,28 @@ __global__ __launch_bounds__(balance_block) void balance_forward_kernel(BalanceK
     __syncthreads();
     float sums[ITEMS][W] = {};
     uint32_t rows = 0;
-    for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups; first < a.n; first += static_cast<uint64_t>(gridDim.x) * groups) {
-        const uint64_t row = min(first + group, a.n - 1);
-        float z[ITEMS][W];
-        load_row<T, W, TPR, ITEMS>(a, row, lane, z);
-        const bool counts = row_counts<TPR>(a, row, lane, first + group < a.n, histogram);
-        const float inverse = exponentials<W, TPR, ITEMS>(z, slots);
-        rows += counts && lane == 0;
+    constexpr uint32_t at_once = rows_under_way<W, TPR, ITEMS>;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * groups;
+    for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups; first < a.n; first += at_once * step) {
+        float z[at_once][ITEMS][W];
+        int64_t choice[at_once];
 #pragma unroll
-        for (int k = 0; k < ITEMS; k++)
+        for (uint32_t u = 0; u < at_once; u++) {
+            const uint64_t row = min(first + u * step + group, a.n - 1);
+            choice[u] = first_choice<TPR>(a, row, lane);
+            load_row<T, W, TPR, ITEMS>(a, row, lane, z[u]);
+        }
 #pragma unroll
-            for (int j = 0; j < W; j++) sums[k][j] += counts ? z[k][j] * inverse : 0.0f;
+        for (uint32_t u = 0; u < at_once; u++) {
+            const uint64_t row = first + u * step + group;
+            const bool counts = row_counts<TPR>(a, min(row, a.n - 1), lane, row < a.n, choice[u], histogram);
+            const float inverse = exponentials<W, TPR, ITEMS>(z[u], slots);
+            rows += counts && lane == 0;
+#pragma unroll
+            for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+                for (int j = 0; j < W; j++) sums[k][j] += counts ? z[u][k][j] * inverse : 0.0f;
+        }
         if constexpr (TPR > 64) __syncthreads();  // (the slots are written again)
     }
 #pragma unroll
@@ -167,33 +246,46 @@ __global__ __launch_bounds__(balance_block) void balance_forward_kernel(BalanceK
         for (uint32_t w = 0; w < balance_waves; w++) all += rows_of_wave[w];
         counts[a.experts] = all;
     }
+    if (gridDim.x > 1) return;
+    // few rows: the only block's sums are the totals, which spares two launches
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e <= a.experts; e += balance_block) {
+        totals.totals[e] = e < a.experts ? static_cast<double>(out[e]) : static_cast<double>(counts[e]);
+        if (e < a.experts) totals.count[e] = static_cast<int64_t>(counts[e]);
+    }
+    __syncthreads();
+    loss_of_totals(totals);
 }
 
-struct BalanceTotals {
-    const float* sums;
-    const uint32_t* counts;
-    uint32_t blocks, experts;
-    double* totals;       // experts + 1: sums of probabilities; rows
-    int64_t* count;       // experts
-    float* share;         // experts, then E / rows
-    float* loss;
-};
+constexpr uint32_t totals_block = 1024, totals_columns = 16, totals_parts = totals_block / totals_columns;
 
-constexpr uint32_t totals_columns = 16, totals_parts = balance_block / totals_columns;
-
-// sixteen columns a block, the table's rows in sixteen parts, joined in their order; column `experts` is the number of rows
-__global__ __launch_bounds__(balance_block) void balance_totals_kernel(BalanceTotals a) {
+// sixteen columns a block, the table's rows in 64 parts, joined in their order; column `experts` is the number of rows
+__global__ __launch_bounds__(totals_block) void balance_totals_kernel(BalanceTotals a) {
     __shared__ double sums[totals_parts][totals_columns];
     __shared__ uint64_t counts[totals_parts][totals_columns];
     const uint32_t c = threadIdx.x & (totals_columns - 1u), part = threadIdx.x / totals_columns, column = blockIdx.x * totals_columns + c;
     const uint32_t each = (a.blocks + totals_parts - 1) / totals_parts, last = min(a.blocks, (part + 1) * each);
     double sum = 0.0;
     uint64_t count = 0;
-    if (column <= a.experts)
-        for (uint32_t b = part * each; b < last; b++) {
-            if (column < a.experts) sum += static_cast<double>(a.sums[static_cast<uint64_t>(b) * a.experts + column]);
-            count += a.counts[static_cast<uint64_t>(b) * (a.experts + 1) + column];
+    if (column <= a.experts) {
+        const uint32_t sum_column = min(column, a.experts - 1);
+        constexpr uint32_t at_once = 4;
+        for (uint32_t b = part * each; b < last; b += at_once) {
+            float x[at_once];
+            uint32_t n[at_once];
+#pragma unroll
+            for (uint32_t k = 0; k < at_once; k++) {
+                const uint64_t row = min(b + k, last - 1);
+                x[k] = a.sums[row * a.experts + sum_column];
+                n[k] = a.counts[row * (a.experts + 1) + column];
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < at_once; k++) {
+                sum += b + k < last ? static_cast<double>(x[k]) : 0.0;
+                count += b + k < last ? n[k] : 0u;
+            }
         }
+    }
     sums[part][c] = sum;
     counts[part][c] = count;
     __syncthreads();
@@ -206,36 +298,7 @@ __global__ __launch_bounds__(balance_block) void balance_totals_kernel(BalanceTo
     if (column < a.experts) a.count[column] = static_cast<int64_t>(count);
 }
 
-__device__ __forceinline__ double block_sum(double v, double* lds) {
-#pragma unroll
-    for (uint32_t o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double sum = 0.0;
-#pragma unroll
-    for (uint32_t w = 0; w < balance_waves; w++) sum += lds[w];
-    return sum;
-}
-
-__global__ __launch_bounds__(balance_block) void balance_loss_kernel(BalanceTotals a) {
-    __shared__ double lds[balance_waves];
-    double choices = 0.0;
-    for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) choices += static_cast<double>(a.count[e]);
-    choices = block_sum(choices, lds);
-    const double rows = a.totals[a.experts], per_choice = choices > 0.0 ? 1.0 / choices : 0.0, per_row = rows > 0.0 ? a.experts / rows : 0.0;
-    double loss = 0.0;
-    for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) {
-        const double share = static_cast<double>(a.count[e]) * per_choice;
-        a.share[e] = static_cast<float>(share);
-        if (a.count[e] > 0) loss += share * a.totals[e];
-    }
-    loss = block_sum(loss, lds);
-    if (threadIdx.x == 0) {
-        a.share[a.experts] = static_cast<float>(per_row);
-        *a.loss = static_cast<float>(loss * per_row);
-    }
-}
+__global__ __launch_bounds__(balance_block) void balance_loss_kernel(BalanceTotals a) { loss_of_totals(a); }
 
 template <typename T, int W, uint32_t TPR, int ITEMS>
 __global__ __launch_bounds__(balance_block) void balance_backward_kernel(BalanceKernelArgs a) {
@@ -248,34 +311,44 @@ __global__ __launch_bounds__(balance_block) void balance_backward_kernel(Balance
     for (int k = 0; k < ITEMS; k++)
 #pragma unroll
         for (int j = 0; j < W; j++) share[k][j] = a.share[min((k * TPR + lane) * W + j, a.experts - 1)];
-    for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups; first < a.n; first += static_cast<uint64_t>(gridDim.x) * groups) {
-        const bool active = first + group < a.n;
-        const uint64_t row = min(first + group, a.n - 1);
-        float z[ITEMS][W];
-        load_row<T, W, TPR, ITEMS>(a, row, lane, z);
-        const bool counts = row_counts<TPR>(a, row, lane, active, nullptr);
-        const float inverse = exponentials<W, TPR, ITEMS>(z, slots);
-        float mean = 0.0f;
+    constexpr uint32_t at_once = rows_under_way<W, TPR, ITEMS>;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * groups;
+    for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups; first < a.n; first += at_once * step) {
+        float z[at_once][ITEMS][W];
+        int64_t choice[at_once];
 #pragma unroll
-        for (int k = 0; k < ITEMS; k++)
+        for (uint32_t u = 0; u < at_once; u++) {
+            const uint64_t row = min(first + u * step + group, a.n - 1);
+            choice[u] = first_choice<TPR>(a, row, lane);
+            load_row<T, W, TPR, ITEMS>(a, row, lane, z[u]);
+        }
 #pragma unroll
-            for (int j = 0; j < W; j++) {
-                z[k][j] *= inverse;
-                mean += z[k][j] * share[k][j];
+        for (uint32_t u = 0; u < at_once; u++) {
+            const uint64_t row = first + u * step + group;
+            const bool active = row < a.n, counts = row_counts<TPR>(a, min(row, a.n - 1), lane, active, choice[u], nullptr);
+            const float inverse = exponentials<W, TPR, ITEMS>(z[u], slots);
+            float mean = 0.0f;
+#pragma unroll
+            for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    z[u][k][j] *= inverse;
+                    mean += z[u][k][j] * share[k][j];
+                }
+            mean = across<TPR>(mean, slots[2], [](float x, float y) { return x + y; });
+            T* const out = static_cast<T*>(a.gradient) + row * a.experts;
+#pragma unroll
+            for (int k = 0; k < ITEMS; k++) {
+                const uint32_t column = (k * TPR + lane) * W;
+                typename Part<T, W>::type v;
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    const T y = static_cast<T>(counts ? z[u][k][j] * (share[k][j] - mean) * factor : 0.0f);
+                    if constexpr (W == 1) v = y;
+                    else v[j] = y;
+                }
+                if (active && column < a.experts) *reinterpret_cast<typename Part<T, W>::type*>(out + column) = v;
             }
-        mean = across<TPR>(mean, slots[2], [](float x, float y) { return x + y; });
-        T* const out = static_cast<T*>(a.gradient) + row * a.experts;
-#pragma unroll
-        for (int k = 0; k < ITEMS; k++) {
-            const uint32_t column = (k * TPR + lane) * W;
-            typename Part<T, W>::type v;
-#pragma unroll
-            for (int j = 0; j < W; j++) {
-                const T y = static_cast<T>(counts ? z[k][j] * (share[k][j] - mean) * factor : 0.0f);
-                if constexpr (W == 1) v = y;
-                else v[j] = y;
-            }
-            if (active && column < a.experts) *reinterpret_cast<typename Part<T, W>::type*>(out + column) = v;
         }
         if constexpr (TPR > 64) __syncthreads();
     }
@@ -310,6 +383,7 @@ template <typename T, typename F>
 void with_type(uint32_t experts, F&& f) {
     constexpr int widest = 16 / sizeof(T);
     if (experts % widest == 0) with_shape<T, widest>(experts, [&](auto w, auto tpr, auto items) { f(T{}, w, tpr, items); });
+    else if (sizeof(T) == 2 && experts % 2 == 0) with_shape<T, 2>(experts, [&](auto w, auto tpr, auto items) { f(T{}, w, tpr, items); });
     else with_shape<T, 1>(experts, [&](auto w, auto tpr, auto items) { f(T{}, w, tpr, items); });
 }
 
@@ -331,26 +405,27 @@ BalanceKernelArgs kernel_args(const BalanceArgs& a) {
     return k;
 }
 
-uint32_t rows_at_once(const BalanceArgs& a) {
-    uint32_t rows = 1;
-    dispatch(a.type, a.experts, [&](auto, auto, auto tpr, auto) { rows = balance_block / decltype(tpr)::value; });
-    return rows;
-}
-
-uint32_t forward_blocks(const BalanceArgs& a) {
-    const uint64_t rows = rows_at_once(a);
-    return static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>((a.n + rows - 1) / rows, 1), balance_max_blocks));
+// blocks whose groups all have the rows that they take at once, but enough of them where there are few rows
+uint32_t blocks_for(const BalanceArgs& a) {
+    uint64_t rows = 1, at_once = 1;
+    dispatch(a.type, a.experts, [&](auto, auto w, auto tpr, auto items) {
+        rows = balance_block / decltype(tpr)::value;
+        at_once = rows_under_way<decltype(w)::value, decltype(tpr)::value, decltype(items)::value>;
+    });
+    if (a.n <= rows * at_once) return 1;
+    const uint64_t full = (a.n + rows * at_once - 1) / (rows * at_once), most = (a.n + rows - 1) / rows;
+    return static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>({full, std::min<uint64_t>(most, 512), 1}), balance_max_blocks));
 }
 
 }  // namespace
 
 size_t balance_scratch_bytes(const BalanceArgs& a) {
-    const uint64_t blocks = forward_blocks(a);
+    const uint64_t blocks = blocks_for(a);
     return (a.experts + 1ull) * sizeof(double) + blocks * a.experts * sizeof(float) + blocks * (a.experts + 1ull) * sizeof(uint32_t);
 }
 
 bool launch_balance_forward(const BalanceArgs& a, int64_t* counts, float* share, float* loss, void* scratch, hipStream_t s) {
-    const uint32_t blocks = forward_blocks(a);
+    const uint32_t blocks = blocks_for(a);
     BalanceTotals t{};
     t.totals = static_cast<double*>(scratch);
     float* const sums = reinterpret_cast<float*>(t.totals + a.experts + 1);
@@ -370,12 +445,16 @@ bool launch_balance_forward(const BalanceArgs& a, int64_t* counts, float* share,
             constexpr uint32_t lanes = decltype(tpr)::value;
             const size_t lds = a.experts * sizeof(uint32_t) * (lanes > 64 ? 1 : 1 + balance_waves);
             hipLaunchKernelGGL((balance_forward_kernel<decltype(type), decltype(w)::value, lanes, decltype(items)::value>), dim3(blocks),
-                               dim3(balance_block), lds, s, k);
+                               dim3(balance_block), lds, s, k, t);
         });
+        if (blocks == 1) {
+            EFGS_HIP_CHECK(hipGetLastError());
+            return true;
+        }
     } else {
         t.blocks = 0;
     }
-    hipLaunchKernelGGL(balance_totals_kernel, dim3(div_up(a.experts + 1ull, totals_columns)), dim3(balance_block), 0, s, t);
+    hipLaunchKernelGGL(balance_totals_kernel, dim3(div_up(a.experts + 1ull, totals_columns)), dim3(totals_block), 0, s, t);
     hipLaunchKernelGGL(balance_loss_kernel, dim3(1), dim3(balance_block), 0, s, t);
     EFGS_HIP_CHECK(hipGetLastError());
     return true;
@@ -383,14 +462,13 @@ bool launch_balance_forward(const BalanceArgs& a, int64_t* counts, float* share,
 
 bool launch_balance_backward(const BalanceArgs& a, const float* share, const float* upstream, void* gradient, hipStream_t s) {
     if (a.n == 0) return true;
+    const uint32_t blocks = blocks_for(a);
     BalanceKernelArgs k = kernel_args(a);
     k.share = share;
     k.upstream = upstream;
     k.gradient = gradient;
     dispatch(a.type, a.experts, [&](auto type, auto w, auto tpr, auto items) {
         constexpr uint32_t lanes = decltype(tpr)::value;
-        const uint64_t rows = balance_block / lanes;
-        const uint32_t blocks = static_cast<uint32_t>(std::min<uint64_t>((a.n + rows - 1) / rows, 1u << 23));
         hipLaunchKernelGGL((balance_backward_kernel<decltype(type), decltype(w)::value, lanes, decltype(items)::value>), dim3(blocks),
                            dim3(balance_block), 0, s, k);
     });

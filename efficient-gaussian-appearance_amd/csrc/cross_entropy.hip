@@ -538,7 +538,8 @@ ProductPlan plan_product(const EntropyArgs& a, uint64_t i, uint64_t j, uint64_t 
     for (const uint32_t side : {256u, 128u}) {
         if (side == 256 && !wide(a)) continue;
         const uint64_t tiles = ((i + side - 1) / side) * ((j + side - 1) / side), at_once = side == 256 ? 256 : 512, step = wide(a) ? 64 : 16;
-        for (uint32_t s = 1; s <= 64 && (s == 1 || (results > 0 && k / s >= 2 * step)); s++) {
+        for (const uint32_t s : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u, 24u, 32u, 48u, 64u}) {
+            if (s > 1 && (results == 0 || k / s < 2 * step)) break;
             const uint64_t blocks = tiles * s;
             const double step_us = !wide(a) ? 1.8 : side == 256 ? 1.7 : blocks <= 256 ? 0.8 : 1.2;
             const double rounds = static_cast<double>((blocks + at_once - 1) / at_once), steps = static_cast<double>((k + s * step - 1) / (s * step));

@@ -323,7 +323,8 @@ struct EntropyArgs {
     float scale;
     bool mean, each;          // the loss: mean over the rows that count, every row's, or their sum
 };
-constexpr int64_t entropy_max = (1ll << 31) - 1024;  // rows of either side, columns
+constexpr int64_t entropy_max = (1ll << 31) - 1024;  // rows of either side
+constexpr int64_t entropy_max_columns = 1ll << 22;   // (bytes of a tile's rows are counted in 32 bits)
 bool entropy_fits(const EntropyArgs& a);             // whether the launches can count their blocks
 size_t entropy_saved_bytes(const EntropyArgs& a);    // what a backward needs of its forward
 size_t entropy_forward_bytes(const EntropyArgs& a, bool backward);  // of `scratch`, with a backward to follow or without

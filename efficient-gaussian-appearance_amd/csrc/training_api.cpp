@@ -129,8 +129,8 @@ const char* embedding_fault(const void* indices, int index_bytes, int64_t n, int
 // the fault of a call's values, or null
 const char* entropy_fault(const efgs_entropy* e) {
     if (!e) return "null cross entropy arguments";
-    if (e->n < 0 || e->rows < 0 || e->columns < 0 || e->n > entropy_max || e->rows > entropy_max || e->columns > entropy_max)
-        return "cross entropy sizes must lie between 0 and 2^31 - 1024";
+    if (e->n < 0 || e->rows < 0 || e->n > entropy_max || e->rows > entropy_max) return "the cross entropy's rows must lie between 0 and 2^31 - 1024";
+    if (e->columns < 0 || e->columns > entropy_max_columns) return "the cross entropy's columns must lie between 0 and 2^22";
     if (e->target_bytes != 4 && e->target_bytes != 8) return "cross entropy targets have 4 or 8 bytes";
     if (!known_type(e->type)) return "unknown element type";
     if (!std::isfinite(e->scale)) return "the cross entropy's scale must be finite";

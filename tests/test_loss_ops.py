@@ -98,7 +98,7 @@ def _entropy(**how):
     return e
 
 
-@pytest.mark.parametrize('how', [dict(n=-1), dict(rows=1 << 31), dict(columns=-2), dict(target_bytes=2), dict(type=3), dict(reduction=3), dict(scale=float('inf')),
+@pytest.mark.parametrize('how', [dict(n=-1), dict(rows=1 << 31), dict(columns=-2), dict(columns=(1 << 22) + 1), dict(target_bytes=2), dict(type=3), dict(reduction=3), dict(scale=float('inf')),
                                  dict(scale=float('nan')), dict(table_stride=-1), dict(n=1 << 30, columns=1 << 30), dict(rows=1 << 30, columns=1 << 30)])
 def test_refusals_of_the_c_cross_entropy(how):
     from efgs import _lib
