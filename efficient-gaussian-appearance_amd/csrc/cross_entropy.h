@@ -35,6 +35,7 @@ struct EntropyProductArgs {
     uint32_t first_row;            // of the piece in the table
     void* piece;                   // upstream gradients of the logits: padded rows x piece_stride
     uint64_t piece_stride;
+    float* residual;               // 16-bit types: what a row's own target's gradient lost as it was rounded to the piece
     float* slab;                   // splits x slab_rows x slab_stride
     uint64_t slab_stride, slab_rows;
     bool add;

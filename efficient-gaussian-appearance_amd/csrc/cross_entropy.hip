@@ -422,9 +422,29 @@ struct Gathering {
     uint32_t slab_stride, splits;
     const uint32_t* packed_of;   // or null: the rows themselves
     const float* weight;         // of packed rows, or null
+    const float* residual;       // of packed rows, times their target's table row, or null
+    const uint32_t* target;
+    const void* table;
+    uint64_t table_stride;
     uint32_t rows, columns;
     const float* factor;
 };
+
+// four columns of a packed row's own target's table row
+template <typename T>
+__device__ __forceinline__ floatx4 target_columns(const Gathering& a, uint32_t m, uint32_t column) {
+    const T* const p = static_cast<const T*>(a.table) + a.target[m] * a.table_stride + column;
+    floatx4 x{};
+    if (column + 4 <= a.columns) {
+        const Part<T, 4> v = *reinterpret_cast<const Part<T, 4>*>(p);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) x[k] = static_cast<float>(v[k]);
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) x[k] = column + k < a.columns ? static_cast<float>(p[k]) : 0.0f;
+    }
+    return x;
+}
 
 // Sums of the splits, in their order, scaled; rows without a packed one are zeros. Four columns a thread.
 template <typename T>
@@ -440,6 +460,7 @@ __global__ __launch_bounds__(256) void entropy_gather_kernel(Gathering a, T* out
             if (m != none)
                 for (uint32_t s = 0; s < a.splits; s++)
                     sum += *reinterpret_cast<const floatx4*>(a.slab + (s * a.slab_rows + m) * a.slab_stride + part * 4);
+            if (a.residual && m != none) sum += a.residual[m] * target_columns<T>(a, m, part * 4);
             Part<T, 4> y;
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++) y[k] = static_cast<T>(m == none ? 0.0f : sum[k] * f);
@@ -468,6 +489,7 @@ __global__ __launch_bounds__(256) void entropy_gather_splits_kernel(Gathering a,
     __syncthreads();
     if (part != 0 || blockIdx.x * 16ull + item >= items) return;
     for (uint32_t k = 1; k < 16; k++) sum += lds[k][item];
+    if (a.residual && m != none) sum += a.residual[m] * target_columns<T>(a, m, column);
     const float f = m == none ? 0.0f : a.weight ? *a.factor * a.weight[m] : *a.factor;
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++)
@@ -606,6 +628,7 @@ struct NarrowBackwardScratch {
 struct BackwardScratch {
     float* weight;
     float* factor;
+    float* residual;         // 16-bit types: of packed rows, or null
     void* piece;
     float* features_slab;
     float* table_slab;
@@ -626,6 +649,7 @@ struct BackwardScratch {
         table = plan_product(a, a.columns, piece_rows, s.padded, static_cast<uint64_t>(piece_rows) * s.padded_columns);
         weight = c.take<float>(s.padded);
         factor = c.take<float>(1);
+        residual = wide(a) ? c.take<float>(s.padded) : nullptr;
         piece = c.take<char>(static_cast<uint64_t>(s.padded) * piece_rows * type_bytes(a.type));
         features_slab = c.take<float>(static_cast<uint64_t>(features.splits) * s.padded * s.padded_columns);
         table_slab = table.splits > 1 ? c.take<float>(static_cast<uint64_t>(table.splits) * piece_rows * s.padded_columns) : nullptr;
@@ -729,12 +753,12 @@ bool launch_narrow_backward(const EntropyArgs& a, const float* upstream, const S
     if (grad_features) {
         p.slab_rows = s.padded;
         if (a.rows > 0) launch_entropy_narrow(entropy_features_gradient, a.type, p, w.features, stream);
-        launch_gathering(a.type, {w.slab, s.padded, w.slab_stride, w.features.splits, s.packed_of, w.weight, a.n, a.columns, w.factor}, grad_features, stream);
+        launch_gathering(a.type, {w.slab, s.padded, w.slab_stride, w.features.splits, s.packed_of, w.weight, nullptr, nullptr, nullptr, 0, a.n, a.columns, w.factor}, grad_features, stream);
     }
     if (grad_table) {
         p.slab_rows = a.rows;
         launch_entropy_narrow(entropy_table_gradient, a.type, p, w.table, stream);
-        launch_gathering(a.type, {w.slab, a.rows, w.slab_stride, w.table.splits, nullptr, nullptr, a.rows, a.columns, w.factor}, grad_table, stream);
+        launch_gathering(a.type, {w.slab, a.rows, w.slab_stride, w.table.splits, nullptr, nullptr, nullptr, nullptr, nullptr, 0, a.rows, a.columns, w.factor}, grad_table, stream);
     }
     EFGS_HIP_CHECK(hipGetLastError());
     return true;
@@ -853,6 +877,7 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
         p.weight = w.weight;
         p.first_row = first;
         p.piece = w.piece;
+        p.residual = w.residual;
         p.piece_stride = w.piece_rows;
         launch_product(entropy_upstream, a, w.upstream.side, p, s.padded, stream);
         EntropyProductArgs x{};
@@ -861,6 +886,9 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
         x.slab_stride = s.padded_columns;
         x.b = w.piece;
         x.b_stride = w.piece_rows;
+        x.target = s.target;
+        x.first_row = first;
+        x.residual = w.residual;
         if (grad_features) {
             x.a = part;
             x.a_stride = table.stride;
@@ -890,11 +918,11 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
             x.factor = w.factor;
             launch_product(entropy_table_gradient, a, w.table.side, x, rows, stream);
             if (x.splits > 1)
-                launch_gathering(a.type, {w.table_slab, w.piece_rows, s.padded_columns, x.splits, nullptr, nullptr, rows, a.columns, w.factor}, out, stream);
+                launch_gathering(a.type, {w.table_slab, w.piece_rows, s.padded_columns, x.splits, nullptr, nullptr, nullptr, nullptr, nullptr, 0, rows, a.columns, w.factor}, out, stream);
         }
     }
     if (grad_features)
-        launch_gathering(a.type, {w.features_slab, s.padded, s.padded_columns, w.features.splits, s.packed_of, nullptr, a.n, a.columns, w.factor},
+        launch_gathering(a.type, {w.features_slab, s.padded, s.padded_columns, w.features.splits, s.packed_of, nullptr, w.residual, s.target, table.rows, table.stride, a.n, a.columns, w.factor},
                          grad_features, stream);
     EFGS_HIP_CHECK(hipGetLastError());
     return true;

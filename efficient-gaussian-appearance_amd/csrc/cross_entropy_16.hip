@@ -136,6 +136,87 @@ struct Fragments {
     }
 };
 
+// The logits' gradients are rounded to the type. A row's own target's is mostly the largest by far, and its rounding would be most of what the gradients lose;
+// so what it lost is added to them, in the rows' gradient as they are gathered, and in the table's here: the packed rows whose target is one of the tile's
+// table rows are looked up, and 64 of them at a time make one more step of k, their features one operand and the residuals, each in its
+// row and target's column of zeros, the other. (8,192 rows against 128,000: sixteen of them to a tile, mostly one step after 128.)
+template <typename T, uint32_t SIDE, typename FA, typename FB, typename Acc>
+__device__ __forceinline__ void add_residuals(const EntropyProductArgs& a, char* lds, uint32_t count, uint32_t i0, uint32_t j0, const FA& fragments_a,
+                                              const FB& fragments_b, Acc& acc) {
+    constexpr uint32_t block = block_of<SIDE>, operand_bytes = SIDE * step_k * 2, row_bytes = SIDE * 2, at_once = 4, most = SIDE * 32;
+    constexpr uint32_t wave_i = SIDE / 32, wave_j = 4;
+    uint32_t* const list = reinterpret_cast<uint32_t*>(lds + 2 * operand_bytes);   // the second stage: packed rows, then the waves' counts
+    uint32_t* const wave_counts = list + most;
+    static_assert((most + at_once * block / 64) * sizeof(uint32_t) <= 2 * operand_bytes, "the list fits a stage");
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, first = a.first_row + j0;
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    uint32_t listed = 0;
+    __syncthreads();
+    for (uint32_t from = 0; from < count; from += at_once * block) {
+        bool hit[at_once];
+#pragma unroll
+        for (uint32_t k = 0; k < at_once; k++) {
+            const uint32_t m = from + k * block + threadIdx.x;
+            hit[k] = m < count && a.target[m] - first < SIDE;
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < at_once; k++) {
+            const uint64_t ballot = __ballot(hit[k]);
+            if (lane == 0) wave_counts[k * (block / 64) + wave] = static_cast<uint32_t>(__popcll(ballot));
+        }
+        __syncthreads();
+        uint32_t before[at_once] = {}, all = 0;
+        for (uint32_t w = 0; w < at_once * block / 64; w++) {
+            const uint32_t n = wave_counts[w];
+#pragma unroll
+            for (uint32_t k = 0; k < at_once; k++) before[k] += w < k * (block / 64) + wave ? n : 0u;
+            all += n;
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < at_once; k++) {
+            const uint64_t ballot = __ballot(hit[k]);
+            if (hit[k]) list[listed + before[k] + static_cast<uint32_t>(__popcll(ballot & ((1ull << lane) - 1ull)))] = from + k * block + threadIdx.x;
+        }
+        listed += all;
+        __syncthreads();
+        if (listed == 0 || (from + at_once * block < count && listed + at_once * block <= most)) continue;
+        for (uint32_t k0 = 0; k0 < listed; k0 += step_k) {
+            const uint32_t rows = min(listed - k0, step_k);
+            constexpr uint32_t chunks = operand_bytes / 16 / block;   // 16 bytes each, of both operands
+#pragma unroll
+            for (uint32_t c = 0; c < chunks; c++) {
+                const uint32_t at = c * block + threadIdx.x, k = at / (row_bytes / 16), chunk = at % (row_bytes / 16), exchange = (k & 3u) | (k >> 3 & 1u) << 2;
+                const uint32_t column = i0 + (chunk ^ 2 * exchange) * 8;
+                Words x{};
+                if (k < rows && column < a.a_columns)
+                    x = *reinterpret_cast<const Words*>(static_cast<const T*>(a.a) + list[k0 + k] * a.a_stride + column);
+                *reinterpret_cast<Words*>(lds + at * 16) = x;
+                *reinterpret_cast<Words*>(lds + operand_bytes + at * 16) = Words{};
+            }
+            __syncthreads();
+            if (threadIdx.x < rows) {
+                const uint32_t k = threadIdx.x, m = list[k0 + k], v = a.target[m] - first, exchange = (k & 3u) | (k >> 3 & 1u) << 2;
+                *reinterpret_cast<T*>(lds + operand_bytes + k * row_bytes + (v / 16 ^ exchange) * 32 + v % 16 * 2) = static_cast<T>(a.residual[m]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (uint32_t half = 0; half < 2; half++) {
+                shortx8 fa[wave_i], fb[wave_j];
+#pragma unroll
+                for (uint32_t t = 0; t < wave_j; t++) fb[t] = fragments_b.read(lds + operand_bytes, half, t);
+#pragma unroll
+                for (uint32_t t = 0; t < wave_i; t++) fa[t] = fragments_a.read(lds, half, t);
+#pragma unroll
+                for (uint32_t ti = 0; ti < wave_i; ti++)
+#pragma unroll
+                    for (uint32_t tj = 0; tj < wave_j; tj++) acc[ti][tj] = multiply<T>(fa[ti], fb[tj], acc[ti][tj]);
+            }
+            __syncthreads();
+        }
+        listed = 0;
+    }
+}
+
 template <typename T, EntropyProduct P, uint32_t SIDE>
 __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(EntropyProductArgs a) {
     constexpr bool first_two = P == entropy_logits || P == entropy_upstream, a_along_k = first_two, b_along_k = P != entropy_table_gradient;
@@ -232,6 +313,9 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the zeros that follow the last step
     }
 
+    if constexpr (P == entropy_table_gradient) {
+        if (blockIdx.y == 0) add_residuals<T, SIDE>(a, lds, count, i0, j0, fragments_a, fragments_b, acc);
+    }
     const uint32_t i_lane = i0 + wi * (SIDE / 2) + 4 * q, j_lane = j0 + wj * 64 + e;  // results: i_lane + 16 ti + r, j_lane + 16 tj
     if constexpr (P == entropy_logits) {
         __syncthreads();
@@ -276,14 +360,25 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
             const bool counts = target != entropy_none;
             const float2 lse = counts ? a.lse[j] : make_float2(0.0f, 0.0f);
             const float weight = counts ? a.weight[j] : 0.0f;
+            const bool hit = __any(target - (a.first_row + i0 + wi * (SIDE / 2)) < SIDE / 2);  // a target among the wave's table rows
 #pragma unroll
             for (uint32_t ti = 0; ti < wave_i; ti++) {
                 const uint32_t i = i_lane + ti * 16;
+                floatx4 p;
                 Four g;
 #pragma unroll
-                for (uint32_t r = 0; r < 4; r++) {
-                    const float p = __builtin_amdgcn_exp2f((rounded(acc[ti][tj][r] * a.to_log2) - lse.x) - lse.y) - (a.first_row + i + r == target ? 1.0f : 0.0f);
-                    g[r] = static_cast<T>(counts && i + r < a.i_end ? p * weight : 0.0f);
+                for (uint32_t r = 0; r < 4; r++) p[r] = __builtin_amdgcn_exp2f((rounded(acc[ti][tj][r] * a.to_log2) - lse.x) - lse.y);
+                if (hit) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++)
+                        if (a.first_row + i + r == target) p[r] -= 1.0f;
+                }
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) g[r] = static_cast<T>(counts && i + r < a.i_end ? p[r] * weight : 0.0f);
+                if (hit) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++)
+                        if (a.first_row + i + r == target) a.residual[j] = p[r] * weight - static_cast<float>(g[r]);
                 }
                 *reinterpret_cast<Four*>(static_cast<T*>(a.piece) + j * a.piece_stride + i) = g;
             }
