@@ -45,7 +45,7 @@ def check(n, experts, chosen, dtype, **how):
     finite = np.where(np.isfinite(z), z, 0.0)
     spread = (finite.max(1) - finite.min(1)).max(initial=0.0)
     r = (2 * spread + 60) * E
-    assert abs(float(loss) - want) <= (r + (np.ceil(n / 1024) + 40) * E) * abs(want) + 1e-300
+    assert abs(float(loss.detach()) - want) <= (r + (np.ceil(n / 1024) + 40) * E) * abs(want) + 1e-300
     grad = torch.autograd.grad(loss, logits, up)[0]
     assert grad.dtype == logits.dtype
     _, u, least = TYPES[dtype]
@@ -87,7 +87,7 @@ def test_choices(chosen):
 def test_rows_left_out(left_out, experts):
     _, _, loss, counts, grad = check(150, experts, 2, 'f32', left_out=left_out)
     if left_out == 1.0:
-        assert float(loss) == 0 and int(counts.sum()) == 0 and torch.all(grad == 0)
+        assert float(loss.detach()) == 0 and int(counts.sum()) == 0 and torch.all(grad == 0)
 
 
 @pytest.mark.parametrize('experts', [7, 64, 3000])
@@ -101,7 +101,7 @@ def test_masked_logits_and_rows_of_nothing_else(experts, dtype):
     logits.requires_grad_()
     loss, _ = efgs.balance_loss(logits, indices)
     want, _, gradient = R.balance(logits.detach().double().cpu().numpy(), indices.cpu().numpy())
-    assert abs(float(loss) - want) <= 1e-5 * want
+    assert abs(float(loss.detach()) - want) <= 1e-5 * want
     grad = torch.autograd.grad(loss, logits)[0]
     assert torch.all(grad[4] == 0) and torch.all(torch.isfinite(grad))
 
@@ -142,7 +142,7 @@ def test_shapes_and_strides():
     assert int(alone[1][3]) == 1
     empty = torch.empty(0, 6, device=DEVICE, requires_grad=True)
     loss, counts = efgs.balance_loss(empty, torch.empty(0, 2, dtype=torch.int64, device=DEVICE))
-    assert float(loss) == 0 and int(counts.sum()) == 0 and torch.autograd.grad(loss, empty)[0].shape == (0, 6)
+    assert float(loss.detach()) == 0 and int(counts.sum()) == 0 and torch.autograd.grad(loss, empty)[0].shape == (0, 6)
     off = torch.randn(1 + 40 * 64, device=DEVICE).to(torch.bfloat16)
     view, choice = off[1:].view(40, 64), torch.randint(0, 64, (40,), device=DEVICE)
     assert torch.equal(efgs.balance_loss(view, choice)[0], efgs.balance_loss(view.clone(), choice)[0])

@@ -368,3 +368,78 @@ def test_pieces_and_lists_of_many_rows():
     check(20_001, 600, 8, 'f32', seed=9)
     check(17_000, 300, 130, 'f32', seed=9, reduction='none')
     check(17_000, 300, 64, 'bf16', seed=10)
+
+
+@pytest.mark.parametrize('n,train', [(3, False), (300, False), (70, True)])
+def test_offsets_past_32_bits(n, train):
+    """A table of more than 4 GB: its last rows are met, and get their gradients."""
+    import efgs
+    rows, columns = 1_200_003, 2048
+    table = torch.zeros(rows, columns, dtype=torch.bfloat16, device=DEVICE)
+    rng = torch.Generator(DEVICE).manual_seed(1)
+    special = torch.tensor([0, 1, 524_287, 1_048_576, 1_048_577, rows - 2, rows - 1], device=DEVICE)
+    table[special] = (torch.randn(len(special), columns, generator=rng, device=DEVICE) / 32).bfloat16()
+    x = torch.randn(n, columns, generator=rng, device=DEVICE).bfloat16()
+    targets = special[torch.arange(n, device=DEVICE) % len(special)]
+    z = x.double() @ table[special].double().t()
+    total = torch.log(torch.exp(z).sum(1) + (rows - len(special)))
+    at = torch.arange(n, device=DEVICE) % len(special)
+    want = total - z[torch.arange(n, device=DEVICE), at]
+    if train:
+        table.requires_grad_()
+        x.requires_grad_()
+    loss = efgs.linear_cross_entropy(x, table, targets, reduction='none')
+    # (float32 logits of 2,048 products and 1.2 million exponentials: far inside of 1e-3)
+    assert torch.all((loss.detach().double() - want).abs() < 1e-3)
+    if train:
+        loss.sum().backward()
+        g = torch.exp(z - total[:, None])
+        g[torch.arange(n, device=DEVICE), at] -= 1.0
+        for got, exact in ((table.grad[special].double(), g.t() @ x.detach().double()), (x.grad.double(), g @ table.detach()[special].double())):
+            # (bfloat16 logits' gradients and one rounding: 2^-8 each of sums of 70 and 7 terms)
+            assert float((got - exact).abs().max()) <= 2.0 ** -6 * float(exact.abs().max())
+        rest = table.grad[2].double()
+        assert torch.all(torch.isfinite(rest)) and float(rest.abs().max()) < 1e-3
+
+
+def test_a_graph_kept_and_run_twice():
+    import efgs
+    features, table, targets, upstream = inputs(200, 300, 96, 'bf16')
+    features.requires_grad_()
+    table.requires_grad_()
+    loss = efgs.linear_cross_entropy(features, table, targets, reduction='none')
+    first = torch.autograd.grad(loss, (features, table), upstream, retain_graph=True)
+    second = torch.autograd.grad(loss, (features, table), upstream)
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('columns', [8, 96])
+def test_all_rows_of_one_target(columns):
+    """Every packed row's own target in one tile of the table, more of them than are listed at once."""
+    import efgs
+    n = 10_000
+    rng = torch.Generator(DEVICE).manual_seed(3)
+    x = torch.randn(n, columns, generator=rng, device=DEVICE).bfloat16().requires_grad_()
+    w = (torch.randn(600, columns, generator=rng, device=DEVICE) / 8).bfloat16().requires_grad_()
+    y = torch.full((n,), 333, device=DEVICE)
+    efgs.linear_cross_entropy(x, w, y, reduction='sum').backward()
+    _, _, g, dx, dw = R.cross_entropy(x.detach().double().cpu().numpy(), w.detach().double().cpu().numpy(), y.cpu().numpy(), 1.0, np.ones(n))
+    losses, _, dx, bar_x, dw, bar_w = bounds(x, w, y, np.ones(n), 1.0, 'bf16')
+    within('features', x.grad, dx, bar_x)
+    within('table', w.grad, dw, bar_w)
+    # the target's row itself: without its residuals the 10,000 roundings of about -1 would be most of its error
+    off = np.abs(w.grad.double().cpu().numpy()[333] - dw[333])
+    assert np.all(off <= 2.0 ** -8 * np.abs(dw[333]) * 1.01 + 2.0 ** -15 * (np.abs(g[:, 333]) @ np.abs(x.detach().double().cpu().numpy())))
+
+
+def test_saved_tensors_may_be_packed_by_hooks():
+    import efgs
+    features, table, targets, _ = inputs(100, 200, 64, 'f32')
+    features.requires_grad_()
+    table.requires_grad_()
+    want = torch.autograd.grad(efgs.linear_cross_entropy(features, table, targets), (features, table))
+    with torch.autograd.graph.save_on_cpu():
+        loss = efgs.linear_cross_entropy(features, table, targets)
+    for a, b in zip(want, torch.autograd.grad(loss, (features, table))):
+        assert torch.equal(a, b)
