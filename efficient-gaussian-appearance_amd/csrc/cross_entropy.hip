@@ -7,7 +7,13 @@
 // zeros), so that rows left out cost nothing behind that and nothing that stands in them reaches a sum. The forward is one
 // matrix product whose tiles leave, for each row, the maximum and the sum of exponentials over the tile's part of the table; a
 // second kernel joins them. The backward computes the logits again by pieces of the table, writes g of a piece, and multiplies
-// it by the piece and, transposed, by the rows. Statistics and sums are in 32 bits (logits in units of log 2), the sum over rows in 64.
+// it by the piece and, transposed, by the rows: four products where three would do if g could be kept (N x V of it), and no more memory than a piece.
+// Statistics and sums are in 32 bits (logits in units of log 2), the sum over rows in 64. g is held in the inputs' type, as the matrix unit takes it: its
+// rounding, 2^-9 of each, is as large as the gradients' own one only where one entry outweighs the others, which a row's target does; what that one loses is
+// added (cross_entropy_16.hip).
+//
+// This file: the packing, the joins and the launches, and the products of floats of more than 64 columns. Up to 64 columns: cross_entropy_narrow.hip. 16-bit types:
+// cross_entropy_16.hip. Up to 64 rows without a gradient: cross_entropy_few.hip.
 #include <algorithm>
 #include <type_traits>
 
@@ -132,34 +138,34 @@ __global__ __launch_bounds__(256) void entropy_copy_kernel(Copying a) {
     }
 }
 
-// ---- matrix products in 32 bits ----------------------------------------------------------------------------------------
-// 128 x 128 results to a block of four waves (64 x 64 each), v_mfma_f32_16x16x4_f32. A lane's results are
+// ---- matrix products of floats -----------------------------------------------------------------------------------------
+// 128 x 128 results to a block of four waves (64 x 64 each), v_mfma_f32_16x16x4_f32, operands through registers to LDS one step ahead. A lane's results are
 // four consecutive i at one j: i is the table row in the logits, so that a row's maximum and sum stay mostly in
-// registers, and the column in the gradients, which are stored along it.
+// registers, and the column in the gradients, which are stored along it. The matrix unit bounds it: 123 TFLOP/s of the four products of 8,192 x 128,000 x 4,096,
+// where a library's product of 8,192^3 reaches 146.
 
 constexpr uint32_t tile = 128, tile_k = 16, tile_pitch = tile + 4, tile_block = 256;
 
 // eight consecutive values, those from `valid` on zero
-template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p, int64_t valid) {
+__device__ __forceinline__ void load8(float (&x)[8], const float* p, int64_t valid) {
     if (valid >= 8) {
-        const Part<T, 8> v = *reinterpret_cast<const Part<T, 8>*>(p);
+        const Part<float, 8> v = *reinterpret_cast<const Part<float, 8>*>(p);
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = static_cast<float>(v[k]);
+        for (int k = 0; k < 8; k++) x[k] = v[k];
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = k < valid ? static_cast<float>(p[k]) : 0.0f;
+        for (int k = 0; k < 8; k++) x[k] = k < valid ? p[k] : 0.0f;
     }
 }
 
 // A tile of an operand: ALONG_K where its memory runs along k, else along i (or j).
-template <typename T, bool ALONG_K>
+template <bool ALONG_K>
 __device__ __forceinline__ void load_tile(float (&x)[8], const void* base, uint64_t stride, uint32_t first, uint32_t end, uint32_t k, uint32_t k_end) {
     const uint32_t t = threadIdx.x;
     const uint32_t row = ALONG_K ? first + t / 2 : k + t / 16, column = ALONG_K ? k + t % 2 * 8 : first + t % 16 * 8;
     const uint32_t rows = ALONG_K ? end : k_end, columns = ALONG_K ? k_end : end;
     const int64_t valid = row < rows ? static_cast<int64_t>(columns) - column : 0;
-    load8<T>(x, static_cast<const T*>(base) + static_cast<uint64_t>(row) * stride + column, valid);
+    load8(x, static_cast<const float*>(base) + static_cast<uint64_t>(row) * stride + column, valid);
 }
 
 template <bool ALONG_K>
@@ -178,9 +184,8 @@ __device__ __forceinline__ float rounded(float x) {
     return x;
 }
 
-template <typename T, EntropyProduct P>
+template <EntropyProduct P>
 __global__ __launch_bounds__(tile_block) void entropy_product_kernel(EntropyProductArgs a) {
-    using B = std::conditional_t<P == entropy_logits || P == entropy_upstream, T, float>;
     constexpr bool a_along_k = P == entropy_logits || P == entropy_upstream, b_along_k = P != entropy_table_gradient;
     __shared__ float lds_a[tile_k][tile_pitch], lds_b[tile_k][tile_pitch];
     __shared__ float2 joined[2][tile];
@@ -194,8 +199,8 @@ __global__ __launch_bounds__(tile_block) void entropy_product_kernel(EntropyProd
     floatx4 acc[4][4] = {};
     float xa[8], xb[8];
     if (k_first < k_end) {
-        load_tile<T, a_along_k>(xa, a.a, a.a_stride, i0, a.i_end, k_first, k_end);
-        load_tile<B, b_along_k>(xb, a.b, a.b_stride, j0, j_end, k_first, k_end);
+        load_tile<a_along_k>(xa, a.a, a.a_stride, i0, a.i_end, k_first, k_end);
+        load_tile<b_along_k>(xb, a.b, a.b_stride, j0, j_end, k_first, k_end);
     }
     for (uint32_t k = k_first; k < k_end; k += tile_k) {
         __syncthreads();
@@ -203,8 +208,8 @@ __global__ __launch_bounds__(tile_block) void entropy_product_kernel(EntropyProd
         store_tile<b_along_k>(lds_b, xb);
         __syncthreads();
         if (k + tile_k < k_end) {
-            load_tile<T, a_along_k>(xa, a.a, a.a_stride, i0, a.i_end, k + tile_k, k_end);
-            load_tile<B, b_along_k>(xb, a.b, a.b_stride, j0, j_end, k + tile_k, k_end);
+            load_tile<a_along_k>(xa, a.a, a.a_stride, i0, a.i_end, k + tile_k, k_end);
+            load_tile<b_along_k>(xb, a.b, a.b_stride, j0, j_end, k + tile_k, k_end);
         }
 #pragma unroll
         for (uint32_t s = 0; s < tile_k / 4; s++) {
@@ -284,10 +289,10 @@ __global__ __launch_bounds__(tile_block) void entropy_product_kernel(EntropyProd
             for (uint32_t ti = 0; ti < 4; ti++) {
                 const uint32_t i = i_lane + ti * 16;
                 if (direct) {
-                    T* const out = static_cast<T*>(a.out) + j * a.out_stride + i;
+                    float* const out = static_cast<float*>(a.out) + j * a.out_stride + i;
 #pragma unroll
                     for (uint32_t r = 0; r < 4; r++)
-                        if (i + r < a.i_end) out[r] = static_cast<T>(acc[ti][tj][r] * factor);
+                        if (i + r < a.i_end) out[r] = acc[ti][tj][r] * factor;
                 } else if (i < a.slab_stride) {
                     floatx4* const out = reinterpret_cast<floatx4*>(a.slab + (blockIdx.y * a.slab_rows + j) * a.slab_stride + i);
                     *out = a.add ? *out + acc[ti][tj] : acc[ti][tj];
@@ -397,20 +402,23 @@ __global__ __launch_bounds__(256) void entropy_weights_kernel(WeightArgs a) {
     if (m == 0) *a.factor = (a.each ? a.scale : a.scale * *a.upstream / (a.mean ? static_cast<float>(max(count, 1u)) : 1.0f)) / a.held;
 }
 
-// float16, a weight for each row: the weights over the power of two at or above the largest, so that a product of weight and probability
-// keeps to the type's range. One block.
+// float16, a weight for each row: the weights over the power of two at or above the largest finite one, so that a product of weight and
+// probability keeps to the type's range (a row of an infinite one or NaN alone, as the plain product would have it). One block.
 __global__ __launch_bounds__(1024) void entropy_half_weights_kernel(WeightArgs a) {
     __shared__ float lds[16];
     const uint32_t count = *a.count;
     float top = 0.0f;
-    for (uint32_t m = threadIdx.x; m < count; m += 1024) top = fmaxf(top, fabsf(a.upstream[a.row_of[m]]));
+    for (uint32_t m = threadIdx.x; m < count; m += 1024) {
+        const float weight = fabsf(a.upstream[a.row_of[m]]);
+        if (weight < infinity) top = fmaxf(top, weight);
+    }
 #pragma unroll
     for (uint32_t o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
     if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = top;
     __syncthreads();
     for (uint32_t w = 0; w < 16; w++) top = fmaxf(top, lds[w]);
     int exponent = 0;
-    if (top > 0.0f && top < infinity) frexpf(top, &exponent);  // (else zeros, or infinities and NaN either way)
+    if (top > 0.0f) frexpf(top, &exponent);
     for (uint32_t m = threadIdx.x; m < a.padded; m += 1024)
         a.weight[m] = m < count ? ldexpf(a.upstream[a.row_of[m]], -exponent) * a.held : 0.0f;
     if (threadIdx.x == 0) *a.factor = ldexpf(a.scale / a.held, exponent);
@@ -522,7 +530,6 @@ bool few(const EntropyArgs& a) { return a.n > 0 && a.n <= entropy_few_most && a.
 bool narrow(const EntropyArgs& a) { return a.columns > 0 && a.columns <= entropy_narrow_most; }
 bool wide(const EntropyArgs& a) { return a.type != type_float && !narrow(a); }
 bool table_is_copied(const EntropyArgs& a);
-
 
 struct Saved {
     uint32_t* count;
@@ -730,6 +737,19 @@ EntropyNarrowArgs narrow_args(const EntropyArgs& a, const Saved& s) {
     return p;
 }
 
+// of a slab's first `rows` rows, as they lie
+Gathering gathering_of(const float* slab, uint64_t slab_rows, uint32_t slab_stride, uint32_t splits, uint32_t rows, uint32_t columns, const float* factor) {
+    Gathering g{};
+    g.slab = slab;
+    g.slab_rows = slab_rows;
+    g.slab_stride = slab_stride;
+    g.splits = splits;
+    g.rows = rows;
+    g.columns = columns;
+    g.factor = factor;
+    return g;
+}
+
 void launch_gathering(int type, const Gathering& g, void* out, hipStream_t stream) {
     if (g.rows == 0 || g.columns == 0) return;
     const uint64_t items = static_cast<uint64_t>(g.rows) * ((g.columns + 3) / 4);
@@ -753,12 +773,15 @@ bool launch_narrow_backward(const EntropyArgs& a, const float* upstream, const S
     if (grad_features) {
         p.slab_rows = s.padded;
         if (a.rows > 0) launch_entropy_narrow(entropy_features_gradient, a.type, p, w.features, stream);
-        launch_gathering(a.type, {w.slab, s.padded, w.slab_stride, w.features.splits, s.packed_of, w.weight, nullptr, nullptr, nullptr, 0, a.n, a.columns, w.factor}, grad_features, stream);
+        Gathering g = gathering_of(w.slab, s.padded, w.slab_stride, w.features.splits, a.n, a.columns, w.factor);
+        g.packed_of = s.packed_of;
+        g.weight = w.weight;
+        launch_gathering(a.type, g, grad_features, stream);
     }
     if (grad_table) {
         p.slab_rows = a.rows;
         launch_entropy_narrow(entropy_table_gradient, a.type, p, w.table, stream);
-        launch_gathering(a.type, {w.slab, a.rows, w.slab_stride, w.table.splits, nullptr, nullptr, nullptr, nullptr, nullptr, 0, a.rows, a.columns, w.factor}, grad_table, stream);
+        launch_gathering(a.type, gathering_of(w.slab, a.rows, w.slab_stride, w.table.splits, a.rows, a.columns, w.factor), grad_table, stream);
     }
     EFGS_HIP_CHECK(hipGetLastError());
     return true;
@@ -771,10 +794,10 @@ void launch_product(EntropyProduct product, const EntropyArgs& a, uint32_t side,
     }
     const dim3 grid(p.i_tiles * div_up(j, tile), p.splits);
     switch (product) {
-        case entropy_logits: hipLaunchKernelGGL((entropy_product_kernel<float, entropy_logits>), grid, dim3(tile_block), 0, stream, p); break;
-        case entropy_upstream: hipLaunchKernelGGL((entropy_product_kernel<float, entropy_upstream>), grid, dim3(tile_block), 0, stream, p); break;
-        case entropy_features_gradient: hipLaunchKernelGGL((entropy_product_kernel<float, entropy_features_gradient>), grid, dim3(tile_block), 0, stream, p); break;
-        case entropy_table_gradient: hipLaunchKernelGGL((entropy_product_kernel<float, entropy_table_gradient>), grid, dim3(tile_block), 0, stream, p); break;
+        case entropy_logits: hipLaunchKernelGGL((entropy_product_kernel<entropy_logits>), grid, dim3(tile_block), 0, stream, p); break;
+        case entropy_upstream: hipLaunchKernelGGL((entropy_product_kernel<entropy_upstream>), grid, dim3(tile_block), 0, stream, p); break;
+        case entropy_features_gradient: hipLaunchKernelGGL((entropy_product_kernel<entropy_features_gradient>), grid, dim3(tile_block), 0, stream, p); break;
+        case entropy_table_gradient: hipLaunchKernelGGL((entropy_product_kernel<entropy_table_gradient>), grid, dim3(tile_block), 0, stream, p); break;
     }
 }
 
@@ -918,12 +941,18 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
             x.factor = w.factor;
             launch_product(entropy_table_gradient, a, w.table.side, x, rows, stream);
             if (x.splits > 1)
-                launch_gathering(a.type, {w.table_slab, w.piece_rows, s.padded_columns, x.splits, nullptr, nullptr, nullptr, nullptr, nullptr, 0, rows, a.columns, w.factor}, out, stream);
+                launch_gathering(a.type, gathering_of(w.table_slab, w.piece_rows, s.padded_columns, x.splits, rows, a.columns, w.factor), out, stream);
         }
     }
-    if (grad_features)
-        launch_gathering(a.type, {w.features_slab, s.padded, s.padded_columns, w.features.splits, s.packed_of, nullptr, w.residual, s.target, table.rows, table.stride, a.n, a.columns, w.factor},
-                         grad_features, stream);
+    if (grad_features) {
+        Gathering g = gathering_of(w.features_slab, s.padded, s.padded_columns, w.features.splits, a.n, a.columns, w.factor);
+        g.packed_of = s.packed_of;
+        g.residual = w.residual;
+        g.target = s.target;
+        g.table = table.rows;
+        g.table_stride = table.stride;
+        launch_gathering(a.type, g, grad_features, stream);
+    }
     EFGS_HIP_CHECK(hipGetLastError());
     return true;
 }

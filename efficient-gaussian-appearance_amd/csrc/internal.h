@@ -305,7 +305,7 @@ struct BalanceArgs {
     uint64_t n;
     uint32_t experts, chosen;
 };
-constexpr int64_t balance_max_experts = 8192;
+constexpr int64_t balance_max_experts = 8192, balance_max_chosen = 65536;
 size_t balance_scratch_bytes(const BalanceArgs& a);
 // share: experts + 1 floats for the backward
 bool launch_balance_forward(const BalanceArgs& a, int64_t* counts, float* share, float* loss, void* scratch, hipStream_t s);

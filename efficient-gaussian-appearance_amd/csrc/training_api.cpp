@@ -159,7 +159,8 @@ EntropyArgs entropy_args(const efgs_entropy& e) {
 
 const char* balance_fault(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type) {
     if (experts < 1 || experts > balance_max_experts) return "between 1 and 8192 experts are supported";
-    if (n < 0 || n > embedding_max || chosen < 0 || chosen > embedding_max) return "balance loss sizes must lie between 0 and 2^31 - 1";
+    if (n < 0 || n > embedding_max) return "balance loss sizes must lie between 0 and 2^31 - 1";
+    if (chosen < 0 || chosen > balance_max_chosen) return "between 0 and 65536 choices of a row are supported";  // (a block counts them in 32 bits)
     if (index_bytes != 4 && index_bytes != 8) return "balance loss indices have 4 or 8 bytes";
     if (!known_type(type)) return "unknown element type";
     if (n > 0 && (!logits || (chosen > 0 && !indices))) return "null balance loss tensor";

@@ -13,9 +13,12 @@ def linear_cross_entropy(features: torch.Tensor, table: torch.Tensor, targets: t
     features: (..., columns); table: (rows, columns), both float32, bfloat16 or float16; targets: int32 or int64 of the features' shape
     without columns. A target outside [0, rows) (say -1 or -100) leaves its row out: its loss and gradient are zero, whatever its features hold.
     reduction: 'none' (a loss for each target), 'sum', or 'mean' over the rows that count (0 if none does). Logits, sums and statistics are in 32
-    bits. Differentiable with respect to features and table, by pieces of the table whose logits are computed again; the logits' gradients are
-    held in the inputs' type between the two products, and every sum has a fixed order, the same bits from call to call; second and forward-mode
-    derivatives raise."""
+    bits. Differentiable with respect to features and table, by pieces of the table whose logits are computed again; above 64 columns the logits'
+    gradients are held in the inputs' type between the two products, but for what a row's own target's loses as it is rounded, which is added. Every sum
+    has a fixed order, the same bits from call to call; second and forward-mode derivatives raise.
+
+    Rows that count and the table should be finite: an infinity or NaN reaches the losses and gradients that its row has a part in, as NaN where
+    float32 arithmetic might have left an infinity."""
     return _native.linear_cross_entropy(features, table, targets, float(scale), reduction)
 
 
@@ -23,7 +26,7 @@ def balance_loss(logits: torch.Tensor, indices: torch.Tensor) -> tuple[torch.Ten
     """(loss, counts) of choosing experts (or codes): E * sum over the E experts of (share of the choices) * (mean softmax probability), float32, 1 where
     both are even; counts: int64 (E,), how often each was chosen.
 
-    logits: (..., E), E up to 8192, float32, bfloat16 or float16; indices: the chosen experts, int32 or int64, (...) or (..., choices). An index outside [0, E) counts
+    logits: (..., E), E up to 8192, float32, bfloat16 or float16; indices: the chosen experts, int32 or int64, (...) or (..., choices), up to 65536. An index outside [0, E) counts
     nowhere, and a row without any other is left out (0 and zero gradients if all are). Differentiable with respect to the logits; the counts
     are not. Rows of nothing but -inf have no probabilities. Sums over rows are in a fixed order; second and forward-mode derivatives raise."""
     return _native.balance_loss(logits, indices)

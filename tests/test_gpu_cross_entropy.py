@@ -168,9 +168,10 @@ def test_what_stands_in_rows_left_out_reaches_nothing(dtype, columns):
 
 @pytest.mark.parametrize('n,rows,columns', [(0, 5, 4), (4, 0, 4), (4, 5, 0), (0, 0, 3), (0, 5, 200)])
 @pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
-def test_empty_sides(n, rows, columns, reduction):
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_empty_sides(n, rows, columns, reduction, dtype):
     import efgs
-    x, w = torch.randn(n, columns, device=DEVICE, requires_grad=True), torch.randn(rows, columns, device=DEVICE, requires_grad=True)
+    x, w = (torch.randn(k, columns, device=DEVICE, dtype=TYPES[dtype][0], requires_grad=True) for k in (n, rows))
     y = torch.zeros(n, dtype=torch.int64, device=DEVICE)
     loss = efgs.linear_cross_entropy(x, w, y, reduction=reduction)
     counted = n if rows else 0   # (rows that count have no columns here: equal logits)
@@ -443,3 +444,53 @@ def test_saved_tensors_may_be_packed_by_hooks():
         loss = efgs.linear_cross_entropy(features, table, targets)
     for a, b in zip(want, torch.autograd.grad(loss, (features, table))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('columns', [32, 96])
+def test_an_infinite_gradient_of_one_row_leaves_the_others_theirs(columns):
+    """float16 gradients of the size a loss scale makes them, one overflowed to infinity: only its own row (and the table, which it has a part in) loses them."""
+    import efgs
+    features, table, targets, upstream = inputs(90, 300, columns, 'f16', left_out=0.0)
+    features.requires_grad_()
+    upstream = upstream * 1000.0
+    upstream[17] = float('inf')
+    grad, = torch.autograd.grad(efgs.linear_cross_entropy(features, table, targets, reduction='none'), features, upstream)
+    assert not bool(torch.isfinite(grad[17]).any())
+    weights = upstream.double().cpu().numpy()
+    weights[17] = 0.0
+    _, _, dx, bar_x, _, _ = bounds(features, table, targets, weights, 1.0, 'f16')
+    dx[17] = bar_x[17] = 0.0
+    grad[17] = 0.0
+    within('features', grad, dx, bar_x)
+
+
+@pytest.mark.parametrize('dtype,columns', [('f32', 24), ('f32', 96), ('bf16', 24), ('bf16', 96), ('f16', 136)])
+@pytest.mark.parametrize('n', [5, 150])
+def test_broadcast_rows_and_shared_tensors(dtype, columns, n):
+    """One feature row for all targets, one table row for all codes, and one tensor as both, with 32-bit targets: as of their copies."""
+    import efgs
+    rng = torch.Generator(DEVICE).manual_seed(9)
+    kind = TYPES[dtype][0]
+    rows = torch.randn(150, columns, generator=rng, device=DEVICE).to(kind)
+    one = torch.randn(1, columns, generator=rng, device=DEVICE).to(kind)
+    y = torch.randint(-1, 150, (n,), generator=rng, device=DEVICE, dtype=torch.int32)
+
+    def run(x, w, grads):
+        loss = efgs.linear_cross_entropy(x, w, y, 0.3)
+        with torch.no_grad():
+            alone = efgs.linear_cross_entropy(x, w, y, 0.3)
+        return loss.detach(), alone, *torch.autograd.grad(loss, grads)
+
+    for x, w in ((one.expand(n, columns), rows), (rows[:n], one.expand(150, columns))):
+        a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+        c, d = x.contiguous().requires_grad_(), w.contiguous().requires_grad_()
+        for got, want in zip(run(a, b, (a, b)), run(c, d, (c, d))):
+            assert torch.equal(got, want)
+    x, w = rows[:n].clone().requires_grad_(), rows.clone().requires_grad_()
+    both = rows.clone().requires_grad_()
+    loss, alone, dx, dw = run(x, w, (x, w))
+    got, got_alone, grad = run(both[:n], both, (both,))
+    assert torch.equal(got, loss) and torch.equal(got_alone, alone)
+    want = dw.clone()
+    want[:n] += dx
+    assert torch.equal(grad, want)

@@ -131,5 +131,8 @@ def test_null_pointers_and_failed_allocations_of_the_c_entry_points():
         assert lib.efgs_balance_loss_forward(one, one, 8, 4, experts, 1, 0, one, one, one, alloc, None, None) != 0
     assert lib.efgs_balance_loss_forward(one, one, 8, 4, 8, 1, 0, one, one, one, alloc, None, None) != 0 and b'allocation' in lib.efgs_last_error()
     assert lib.efgs_balance_loss_forward(one, one, 3, 4, 8, 1, 0, one, one, one, alloc, None, None) != 0
+    for chosen in (-1, 65537):
+        assert lib.efgs_balance_loss_forward(one, one, 8, 4, 8, chosen, 0, one, one, one, alloc, None, None) != 0
+        assert lib.efgs_balance_loss_backward(one, one, 8, 4, 8, chosen, 0, one, one, one, None) != 0
     assert lib.efgs_balance_loss_forward(one, None, 8, 4, 8, 1, 0, one, one, one, alloc, None, None) != 0
     assert lib.efgs_balance_loss_backward(one, one, 8, 4, 8, 1, 0, None, one, one, None) != 0
