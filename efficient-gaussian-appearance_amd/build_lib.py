@@ -30,7 +30,7 @@ SOURCES = [
     ('adamw.hip', ['-ffp-contract=off']),
     ('embedding.hip', []),
     ('cross_entropy.hip', []),
-    ('cross_entropy_16.hip', []),
+    ('cross_entropy_wide.hip', []),
     ('cross_entropy_few.hip', []),
     ('cross_entropy_narrow.hip', []),
     ('dropout.hip', ['-ffp-contract=off']),

@@ -10,10 +10,10 @@
 // it by the piece and, transposed, by the rows: four products where three would do if g could be kept (N x V of it), and no more memory than a piece.
 // Statistics and sums are in 32 bits (logits in units of log 2), the sum over rows in 64. g is held in the inputs' type, as the matrix unit takes it: its
 // rounding, 2^-9 of each, is as large as the gradients' own one only where one entry outweighs the others, which a row's target does; what that one loses is
-// added (cross_entropy_16.hip).
+// added (cross_entropy_wide.hip).
 //
 // This file: the packing, the joins and the launches, and the products of floats of more than 64 columns. Up to 64 columns: cross_entropy_narrow.hip. 16-bit types:
-// cross_entropy_16.hip. Up to 64 rows without a gradient: cross_entropy_few.hip.
+// cross_entropy_wide.hip. Up to 64 rows without a gradient: cross_entropy_few.hip.
 #include <algorithm>
 #include <type_traits>
 
@@ -138,167 +138,22 @@ __global__ __launch_bounds__(256) void entropy_copy_kernel(Copying a) {
     }
 }
 
-// ---- matrix products of floats -----------------------------------------------------------------------------------------
-// 128 x 128 results to a block of four waves (64 x 64 each), v_mfma_f32_16x16x4_f32, operands through registers to LDS one step ahead. A lane's results are
-// four consecutive i at one j: i is the table row in the logits, so that a row's maximum and sum stay mostly in
-// registers, and the column in the gradients, which are stored along it. The matrix unit bounds it: 123 TFLOP/s of the four products of 8,192 x 128,000 x 4,096,
-// where a library's product of 8,192^3 reaches 146.
-
-constexpr uint32_t tile = 128, tile_k = 16, tile_pitch = tile + 4, tile_block = 256;
-
-// eight consecutive values, those from `valid` on zero
-__device__ __forceinline__ void load8(float (&x)[8], const float* p, int64_t valid) {
-    if (valid >= 8) {
-        const Part<float, 8> v = *reinterpret_cast<const Part<float, 8>*>(p);
+// Rows of floats as three bfloat16 parts, one after the other, each padded by zeros: eight columns a thread.
+__global__ __launch_bounds__(256) void entropy_split_kernel(Copying a) {
+    typedef __bf16 Eight __attribute__((ext_vector_type(8)));
+    const uint32_t pieces = a.padded_columns / 8, end = a.count ? (*a.count + row_tile - 1) / row_tile * row_tile : a.rows;
+    const uint64_t items = static_cast<uint64_t>(end) * pieces, step = static_cast<uint64_t>(gridDim.x) * 256u;
+    for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < items; t += step) {
+        const uint32_t m = static_cast<uint32_t>(t / pieces), column = static_cast<uint32_t>(t - static_cast<uint64_t>(m) * pieces) * 8;
+        const uint32_t row = a.row_of ? a.row_of[m] : m;
+        float x[8];
+        entropy_load8(x, static_cast<const float*>(a.from) + row * a.stride + column,
+                      row != none && column < a.columns ? static_cast<int32_t>(a.columns - column) : 0);
+        Eight parts[3];
+        entropy_split<3>(parts, x);
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = v[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = k < valid ? p[k] : 0.0f;
-    }
-}
-
-// A tile of an operand: ALONG_K where its memory runs along k, else along i (or j).
-template <bool ALONG_K>
-__device__ __forceinline__ void load_tile(float (&x)[8], const void* base, uint64_t stride, uint32_t first, uint32_t end, uint32_t k, uint32_t k_end) {
-    const uint32_t t = threadIdx.x;
-    const uint32_t row = ALONG_K ? first + t / 2 : k + t / 16, column = ALONG_K ? k + t % 2 * 8 : first + t % 16 * 8;
-    const uint32_t rows = ALONG_K ? end : k_end, columns = ALONG_K ? k_end : end;
-    const int64_t valid = row < rows ? static_cast<int64_t>(columns) - column : 0;
-    load8(x, static_cast<const float*>(base) + static_cast<uint64_t>(row) * stride + column, valid);
-}
-
-template <bool ALONG_K>
-__device__ __forceinline__ void store_tile(float (*lds)[tile_pitch], const float (&x)[8]) {
-    const uint32_t t = threadIdx.x;
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        if constexpr (ALONG_K) lds[t % 2 * 8 + k][t / 2] = x[k];
-        else lds[t / 16][t % 16 * 8 + k] = x[k];
-    }
-}
-
-// a product that is rounded before it is subtracted from, as the forward has it
-__device__ __forceinline__ float rounded(float x) {
-    asm("" : "+v"(x));
-    return x;
-}
-
-template <EntropyProduct P>
-__global__ __launch_bounds__(tile_block) void entropy_product_kernel(EntropyProductArgs a) {
-    constexpr bool a_along_k = P == entropy_logits || P == entropy_upstream, b_along_k = P != entropy_table_gradient;
-    __shared__ float lds_a[tile_k][tile_pitch], lds_b[tile_k][tile_pitch];
-    __shared__ float2 joined[2][tile];
-    const uint32_t i0 = blockIdx.x % a.i_tiles * tile, j0 = a.j_first + blockIdx.x / a.i_tiles * tile;
-    const uint32_t count = *a.count;
-    const uint32_t j_end = P == entropy_table_gradient ? a.j_end : count;
-    if (j0 >= (P == entropy_upstream ? (count + row_tile - 1) / row_tile * row_tile : j_end)) return;
-    const uint32_t k_all = P == entropy_table_gradient ? count : a.k_end;
-    const uint32_t k_each = (k_all / a.splits + tile_k) / tile_k * tile_k, k_first = min(blockIdx.y * k_each, k_all), k_end = min(k_first + k_each, k_all);
-    const uint32_t lane = threadIdx.x & 63u, e = lane & 15u, q = lane >> 4, wave = threadIdx.x >> 6, wi = wave & 1u, wj = wave >> 1;
-    floatx4 acc[4][4] = {};
-    float xa[8], xb[8];
-    if (k_first < k_end) {
-        load_tile<a_along_k>(xa, a.a, a.a_stride, i0, a.i_end, k_first, k_end);
-        load_tile<b_along_k>(xb, a.b, a.b_stride, j0, j_end, k_first, k_end);
-    }
-    for (uint32_t k = k_first; k < k_end; k += tile_k) {
-        __syncthreads();
-        store_tile<a_along_k>(lds_a, xa);
-        store_tile<b_along_k>(lds_b, xb);
-        __syncthreads();
-        if (k + tile_k < k_end) {
-            load_tile<a_along_k>(xa, a.a, a.a_stride, i0, a.i_end, k + tile_k, k_end);
-            load_tile<b_along_k>(xb, a.b, a.b_stride, j0, j_end, k + tile_k, k_end);
-        }
-#pragma unroll
-        for (uint32_t s = 0; s < tile_k / 4; s++) {
-            float fa[4], fb[4];
-#pragma unroll
-            for (uint32_t t = 0; t < 4; t++) {
-                fa[t] = lds_a[4 * s + q][wi * 64 + t * 16 + e];
-                fb[t] = lds_b[4 * s + q][wj * 64 + t * 16 + e];
-            }
-#pragma unroll
-            for (uint32_t ti = 0; ti < 4; ti++)
-#pragma unroll
-                for (uint32_t tj = 0; tj < 4; tj++) acc[ti][tj] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[ti], fb[tj], acc[ti][tj], 0, 0, 0);
-        }
-    }
-    const uint32_t i_lane = i0 + wi * 64 + 4 * q, j_lane = j0 + wj * 64 + e;  // results: i_lane + 16 ti + r, j_lane + 16 tj
-    if constexpr (P == entropy_logits) {
-#pragma unroll
-        for (uint32_t tj = 0; tj < 4; tj++) {
-            const uint32_t j = j_lane + tj * 16, target = a.target[j];
-            float top = -infinity, sum = 0.0f;
-#pragma unroll
-            for (uint32_t ti = 0; ti < 4; ti++)
-#pragma unroll
-                for (uint32_t r = 0; r < 4; r++) {
-                    const uint32_t i = i_lane + ti * 16 + r;
-                    const float z = i < a.i_end ? acc[ti][tj][r] * a.to_log2 : -infinity;
-                    acc[ti][tj][r] = z;
-                    if (i == target) a.target_logit[j] = z;
-                    top = fmaxf(top, z);
-                }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float from = top == -infinity ? 0.0f : top;
-#pragma unroll
-            for (uint32_t ti = 0; ti < 4; ti++)
-#pragma unroll
-                for (uint32_t r = 0; r < 4; r++) sum += __builtin_amdgcn_exp2f(acc[ti][tj][r] - from);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (q == 0) joined[wi][wj * 64 + tj * 16 + e] = make_float2(top, sum);
-        }
-        __syncthreads();
-        if (threadIdx.x < tile) {
-            const float2 x = joined[0][threadIdx.x], y = joined[1][threadIdx.x];
-            const float top = fmaxf(x.x, y.x), from = top == -infinity ? 0.0f : top;
-            const float sum = x.y * __builtin_amdgcn_exp2f(x.x - from) + y.y * __builtin_amdgcn_exp2f(y.x - from);
-            a.partial[(i0 / tile) * a.slab_rows + (j0 - a.j_first) + threadIdx.x] = make_float2(top, sum);
-        }
-    } else if constexpr (P == entropy_upstream) {
-#pragma unroll
-        for (uint32_t tj = 0; tj < 4; tj++) {
-            const uint32_t j = j_lane + tj * 16, target = a.target[j];
-            const bool counts = target != none;
-            const float2 lse = counts ? a.lse[j] : make_float2(0.0f, 0.0f);
-            const float weight = counts ? a.weight[j] : 0.0f;
-#pragma unroll
-            for (uint32_t ti = 0; ti < 4; ti++) {
-                const uint32_t i = i_lane + ti * 16;
-                floatx4 g;
-#pragma unroll
-                for (uint32_t r = 0; r < 4; r++) {
-                    const float p = __builtin_amdgcn_exp2f((rounded(acc[ti][tj][r] * a.to_log2) - lse.x) - lse.y) - (a.first_row + i + r == target ? 1.0f : 0.0f);
-                    g[r] = counts && i + r < a.i_end ? p * weight : 0.0f;
-                }
-                *reinterpret_cast<floatx4*>(static_cast<float*>(a.piece) + j * a.piece_stride + i) = g;
-            }
-        }
-    } else {
-        const bool direct = P == entropy_table_gradient && a.out;
-        const float factor = direct ? *a.factor : 1.0f;
-#pragma unroll
-        for (uint32_t tj = 0; tj < 4; tj++) {
-            const uint32_t j = j_lane + tj * 16;
-            if (j >= j_end) continue;
-#pragma unroll
-            for (uint32_t ti = 0; ti < 4; ti++) {
-                const uint32_t i = i_lane + ti * 16;
-                if (direct) {
-                    float* const out = static_cast<float*>(a.out) + j * a.out_stride + i;
-#pragma unroll
-                    for (uint32_t r = 0; r < 4; r++)
-                        if (i + r < a.i_end) out[r] = acc[ti][tj][r] * factor;
-                } else if (i < a.slab_stride) {
-                    floatx4* const out = reinterpret_cast<floatx4*>(a.slab + (blockIdx.y * a.slab_rows + j) * a.slab_stride + i);
-                    *out = a.add ? *out + acc[ti][tj] : acc[ti][tj];
-                }
-            }
-        }
+        for (uint32_t k = 0; k < 3; k++)
+            *reinterpret_cast<Eight*>(static_cast<__bf16*>(a.to) + (static_cast<uint64_t>(m) * 3 + k) * a.padded_columns + column) = parts[k];
     }
 }
 
@@ -525,10 +380,12 @@ class Carver {
 
 uint32_t type_bytes(int type) { return type == type_float ? 4 : 2; }
 
-// the ways: few rows without a gradient; few columns; 16-bit types; floats
+// the ways: few rows without a gradient; few columns; the others
 bool few(const EntropyArgs& a) { return a.n > 0 && a.n <= entropy_few_most && a.rows > 0 && a.columns > 0; }
 bool narrow(const EntropyArgs& a) { return a.columns > 0 && a.columns <= entropy_narrow_most; }
-bool wide(const EntropyArgs& a) { return a.type != type_float && !narrow(a); }
+bool in_parts(const EntropyArgs& a) { return a.type == type_float && !narrow(a); }  // floats as three bfloat16
+uint32_t parts_of(const EntropyArgs& a) { return in_parts(a) ? 3 : 1; }
+uint32_t held_bytes(const EntropyArgs& a) { return in_parts(a) ? 6 : type_bytes(a.type); }  // of an element of the packed rows, of the table's copy and of a piece
 bool table_is_copied(const EntropyArgs& a);
 
 struct Saved {
@@ -549,29 +406,30 @@ struct Saved {
         packed_of = c.take<uint32_t>(padded);
         target = c.take<uint32_t>(padded);
         lse = c.take<float2>(padded);
-        packed = c.take<char>(static_cast<uint64_t>(padded) * padded_columns * type_bytes(a.type));
+        packed = c.take<char>(static_cast<uint64_t>(padded) * padded_columns * held_bytes(a));
         bytes = c.used();
     }
 };
 
 // The side of a product's tiles, and how often its k is split: where tiles leave much of the GPU idle, smaller ones and more blocks, at the price of less reuse, or of
-// partial results (`results` floats) written and read once more for each split. Measured: a CU takes 1.7 us for 64 of k of a tile of 256, 1.2 for those of two of 128 (0.8 for
-// one alone), 1.8 for 16 of k of two float tiles; partial results move at 4 TB/s.
+// partial results (`results` floats) written and read once more for each split. Measured: a CU takes 1.7 us for 64 of k of a tile of 256, 1.2 for those of
+// two of 128 (0.8 for one alone); partial results move at 4 TB/s. Floats: six times the steps, and with more than 2^21 columns small tiles, whose rows' parts
+// 32 bits of bytes reach over.
 struct ProductPlan {
     uint32_t side, splits;
 };
 
 ProductPlan plan_product(const EntropyArgs& a, uint64_t i, uint64_t j, uint64_t k, uint64_t results) {
-    ProductPlan best{tile, 1};
+    ProductPlan best{128, 1};
     double least = 1e30;
     for (const uint32_t side : {256u, 128u}) {
-        if (side == 256 && !wide(a)) continue;
-        const uint64_t tiles = ((i + side - 1) / side) * ((j + side - 1) / side), at_once = side == 256 ? 256 : 512, step = wide(a) ? 64 : 16;
+        if (side == 256 && in_parts(a) && a.columns > 1u << 21) continue;
+        const uint64_t tiles = ((i + side - 1) / side) * ((j + side - 1) / side), at_once = side == 256 ? 256 : 512, step = 64;
         for (const uint32_t s : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u, 24u, 32u, 48u, 64u}) {
             if (s > 1 && (results == 0 || k / s < 2 * step)) break;
             const uint64_t blocks = tiles * s;
-            const double step_us = !wide(a) ? 1.8 : side == 256 ? 1.7 : blocks <= 256 ? 0.8 : 1.2;
-            const double rounds = static_cast<double>((blocks + at_once - 1) / at_once), steps = static_cast<double>((k + s * step - 1) / (s * step));
+            const double step_us = side == 256 ? 1.7 : blocks <= 256 ? 0.8 : 1.2;
+            const double rounds = static_cast<double>((blocks + at_once - 1) / at_once), steps = static_cast<double>((k + s * step - 1) / (s * step) * (in_parts(a) ? 6 : 1));
             const double us = rounds * (steps + 2.0) * step_us + (s > 1 ? s * static_cast<double>(results) * 8.0 / 4e6 : 0.0);
             if (us < least) {
                 least = us;
@@ -585,6 +443,7 @@ ProductPlan plan_product(const EntropyArgs& a, uint64_t i, uint64_t j, uint64_t 
 constexpr uint64_t partial_bytes = 256ull << 20;  // of the tiles' statistics at once
 constexpr uint64_t piece_bytes = 256ull << 20;    // of a piece's upstream gradients
 constexpr uint64_t most_blocks = 1ull << 23;      // of a launch of 256 threads (32 bits of threads)
+constexpr uint32_t tile = 128;                    // the smaller tiles' side
 
 struct ForwardScratch {
     uint32_t* chunk_counts;
@@ -607,7 +466,7 @@ struct ForwardScratch {
         partial = c.take<float2>(static_cast<uint64_t>(tiles) * rows_at_once);
         target_logit = c.take<float>(s.padded);
         sums = c.take<double>(s.padded / join_rows);
-        copy = table_is_copied(a) ? c.take<char>(static_cast<uint64_t>(a.rows) * s.padded_columns * type_bytes(a.type)) : nullptr;
+        copy = table_is_copied(a) ? c.take<char>(static_cast<uint64_t>(a.rows) * s.padded_columns * held_bytes(a)) : nullptr;
         copied = table_is_copied(a);
         bytes = c.used();
     }
@@ -635,7 +494,7 @@ struct NarrowBackwardScratch {
 struct BackwardScratch {
     float* weight;
     float* factor;
-    float* residual;         // 16-bit types: of packed rows, or null
+    float* residual;         // of packed rows
     void* piece;
     float* features_slab;
     float* table_slab;
@@ -646,7 +505,7 @@ struct BackwardScratch {
     size_t bytes;
     BackwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
-        const uint64_t most = std::max<uint64_t>(piece_bytes / (static_cast<uint64_t>(s.padded) * type_bytes(a.type)) / 256 * 256, 256);
+        const uint64_t most = std::max<uint64_t>(piece_bytes / (static_cast<uint64_t>(s.padded) * held_bytes(a)) / 256 * 256, 256);
         const uint64_t all = round_up(std::max(a.rows, 1u), 256);
         pieces = div_up(all, std::min(most, all));
         piece_rows = static_cast<uint32_t>(round_up(div_up(all, pieces), 256));
@@ -656,12 +515,12 @@ struct BackwardScratch {
         table = plan_product(a, a.columns, piece_rows, s.padded, static_cast<uint64_t>(piece_rows) * s.padded_columns);
         weight = c.take<float>(s.padded);
         factor = c.take<float>(1);
-        residual = wide(a) ? c.take<float>(s.padded) : nullptr;
-        piece = c.take<char>(static_cast<uint64_t>(s.padded) * piece_rows * type_bytes(a.type));
+        residual = c.take<float>(s.padded);
+        piece = c.take<char>(static_cast<uint64_t>(s.padded) * piece_rows * held_bytes(a));
         features_slab = c.take<float>(static_cast<uint64_t>(features.splits) * s.padded * s.padded_columns);
         table_slab = table.splits > 1 ? c.take<float>(static_cast<uint64_t>(table.splits) * piece_rows * s.padded_columns) : nullptr;
         copied = table_is_copied(a);
-        copy = copied ? c.take<char>(static_cast<uint64_t>(a.rows) * s.padded_columns * type_bytes(a.type)) : nullptr;
+        copy = copied ? c.take<char>(static_cast<uint64_t>(a.rows) * s.padded_columns * held_bytes(a)) : nullptr;
         bytes = c.used();
     }
 };
@@ -679,6 +538,10 @@ uint32_t copy_grid(uint64_t items) { return static_cast<uint32_t>(std::min<uint6
 
 void launch_copy(const EntropyArgs& a, const Copying& c, uint64_t most_rows, hipStream_t stream) {
     if (c.padded_columns == 0 || most_rows == 0) return;
+    if (in_parts(a)) {
+        hipLaunchKernelGGL(entropy_split_kernel, dim3(copy_grid(most_rows * c.padded_columns / 8)), dim3(256), 0, stream, c);
+        return;
+    }
     const uint32_t blocks = copy_grid(most_rows * c.padded_columns * type_bytes(a.type) / 16);
     with_type(a.type, [&](auto t) { hipLaunchKernelGGL(entropy_copy_kernel<decltype(t)>, dim3(blocks), dim3(256), 0, stream, c); });
 }
@@ -702,9 +565,10 @@ void launch_packing(const EntropyArgs& a, const Saved& s, uint32_t* chunk_counts
 }
 
 // A table whose rows the wide products cannot read as they lie: another alignment than 16 bytes, columns that 16 bytes do not divide, rows that
-// overlap, or so far apart that 32 bits of bytes do not reach over a tile. A copy takes its place.
+// overlap, or so far apart that 32 bits of bytes do not reach over a tile; and one of floats, for their parts. A copy takes its place.
 bool table_is_copied(const EntropyArgs& a) {
-    return wide(a) && a.rows > 0 && (reinterpret_cast<uintptr_t>(a.table) % 16 != 0 || a.columns % 8 != 0 || a.table_stride % 8 != 0 ||
+    if (narrow(a) || a.rows == 0) return false;
+    return in_parts(a) || (reinterpret_cast<uintptr_t>(a.table) % 16 != 0 || a.columns % 8 != 0 || a.table_stride % 8 != 0 ||
                                      a.table_stride < a.columns || a.table_stride >= 1ull << 22);
 }
 
@@ -712,13 +576,13 @@ bool table_is_copied(const EntropyArgs& a) {
 struct Table {
     const void* rows;
     uint64_t stride;
-    uint32_t columns;
+    uint32_t columns;   // (of a part)
 };
 
 Table table_of(const EntropyArgs& a, const Saved& s, void* room, hipStream_t stream) {
     if (!room) return {a.table, a.table_stride, a.columns};
     launch_copy(a, Copying{a.table, a.table_stride, a.rows, a.columns, s.padded_columns, nullptr, nullptr, room}, a.rows, stream);
-    return {room, s.padded_columns, s.padded_columns};
+    return {room, static_cast<uint64_t>(s.padded_columns) * parts_of(a), s.padded_columns};
 }
 
 EntropyNarrowArgs narrow_args(const EntropyArgs& a, const Saved& s) {
@@ -736,6 +600,10 @@ EntropyNarrowArgs narrow_args(const EntropyArgs& a, const Saved& s) {
     p.to_log2 = a.scale * log2_e;
     return p;
 }
+
+// Whether what a target's rounding loses is added to the table's gradient. Where each table row is many rows' target, their roundings are a quarter of the result's
+// own or less (16 targets: 16 half steps' sum, a quarter of as many), and the rows to look up are many.
+bool targets_apart(const EntropyArgs& a) { return a.n / 64 <= a.rows; }
 
 // of a slab's first `rows` rows, as they lie
 Gathering gathering_of(const float* slab, uint64_t slab_rows, uint32_t slab_stride, uint32_t splits, uint32_t rows, uint32_t columns, const float* factor) {
@@ -787,20 +655,6 @@ bool launch_narrow_backward(const EntropyArgs& a, const float* upstream, const S
     return true;
 }
 
-void launch_product(EntropyProduct product, const EntropyArgs& a, uint32_t side, const EntropyProductArgs& p, uint32_t j, hipStream_t stream) {
-    if (wide(a)) {
-        launch_entropy_wide(product, a.type, side, p, j, stream);
-        return;
-    }
-    const dim3 grid(p.i_tiles * div_up(j, tile), p.splits);
-    switch (product) {
-        case entropy_logits: hipLaunchKernelGGL((entropy_product_kernel<entropy_logits>), grid, dim3(tile_block), 0, stream, p); break;
-        case entropy_upstream: hipLaunchKernelGGL((entropy_product_kernel<entropy_upstream>), grid, dim3(tile_block), 0, stream, p); break;
-        case entropy_features_gradient: hipLaunchKernelGGL((entropy_product_kernel<entropy_features_gradient>), grid, dim3(tile_block), 0, stream, p); break;
-        case entropy_table_gradient: hipLaunchKernelGGL((entropy_product_kernel<entropy_table_gradient>), grid, dim3(tile_block), 0, stream, p); break;
-    }
-}
-
 }  // namespace
 
 bool entropy_fits(const EntropyArgs& a) {
@@ -841,9 +695,11 @@ bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void
             EntropyProductArgs p{};
             p.a = table.rows;
             p.a_stride = table.stride;
-            p.a_columns = table.columns;
+            p.a_columns = table.columns * parts_of(a);
+            p.a_plane = table.columns;
             p.b = s.packed;
-            p.b_stride = s.padded_columns;
+            p.b_stride = static_cast<uint64_t>(s.padded_columns) * parts_of(a);
+            p.b_plane = s.padded_columns;
             p.i_end = a.rows;
             p.j_end = rows;
             p.k_end = table.columns;
@@ -856,7 +712,7 @@ bool launch_entropy_forward(const EntropyArgs& a, float* loss, void* saved, void
             p.slab_rows = rows;
             p.target_logit = f.target_logit;
             p.target = s.target;
-            launch_product(entropy_logits, a, f.side, p, rows, stream);
+            launch_entropy_wide(entropy_logits, a.type, f.side, p, rows, stream);
         }
         const JoinArgs j{f.partial, f.tiles, first, rows, a.n, s.count, s.row_of, s.packed_of, f.target_logit, s.lse, a.each ? loss : nullptr, f.sums};
         if (f.tiles <= join_alone) hipLaunchKernelGGL(entropy_join_kernel<1>, dim3(rows / 256), dim3(256), 0, stream, j);
@@ -878,16 +734,19 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
     const WeightArgs weights{upstream, s.count, s.row_of, s.padded, a.each, a.mean, a.scale, half ? entropy_half_range : 1.0f, w.weight, w.factor};
     if (half && a.each) hipLaunchKernelGGL(entropy_half_weights_kernel, dim3(1), dim3(1024), 0, stream, weights);
     else hipLaunchKernelGGL(entropy_weights_kernel, dim3(div_up(s.padded, 256)), dim3(256), 0, stream, weights);
-    const uint32_t bytes = type_bytes(a.type);
+    const uint32_t parts = parts_of(a);
+    const bool apart = targets_apart(a);
     for (uint32_t piece = 0; piece < w.pieces && a.rows > 0; piece++) {
         const uint32_t first = piece * w.piece_rows, rows = std::min(a.rows - first, w.piece_rows);
-        const void* const part = static_cast<const char*>(table.rows) + first * table.stride * bytes;
+        const void* const part = static_cast<const char*>(table.rows) + first * table.stride * (in_parts(a) ? 2 : type_bytes(a.type));
         EntropyProductArgs p{};
         p.a = part;
         p.a_stride = table.stride;
-        p.a_columns = table.columns;
+        p.a_columns = table.columns * parts;
+        p.a_plane = table.columns;
         p.b = s.packed;
-        p.b_stride = s.padded_columns;
+        p.b_stride = static_cast<uint64_t>(s.padded_columns) * parts;
+        p.b_plane = s.padded_columns;
         p.i_end = rows;
         p.j_end = s.padded;
         p.k_end = table.columns;
@@ -901,21 +760,25 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
         p.first_row = first;
         p.piece = w.piece;
         p.residual = w.residual;
-        p.piece_stride = w.piece_rows;
-        launch_product(entropy_upstream, a, w.upstream.side, p, s.padded, stream);
+        p.apart = apart;
+        p.piece_stride = static_cast<uint64_t>(w.piece_rows) * parts;
+        p.piece_plane = w.piece_rows;
+        launch_entropy_wide(entropy_upstream, a.type, w.upstream.side, p, s.padded, stream);
         EntropyProductArgs x{};
         x.count = s.count;
         x.i_end = a.columns;
         x.slab_stride = s.padded_columns;
         x.b = w.piece;
-        x.b_stride = w.piece_rows;
+        x.b_stride = p.piece_stride;
+        x.b_plane = w.piece_rows;
         x.target = s.target;
         x.first_row = first;
         x.residual = w.residual;
+        x.apart = apart;
         if (grad_features) {
             x.a = part;
             x.a_stride = table.stride;
-            x.a_columns = table.columns;
+            x.a_columns = x.a_plane = table.columns;
             x.i_tiles = div_up(a.columns, w.features.side);
             x.j_end = s.padded;
             x.k_end = rows;
@@ -923,13 +786,13 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
             x.slab = w.features_slab;
             x.slab_rows = s.padded;
             x.add = piece > 0;
-            launch_product(entropy_features_gradient, a, w.features.side, x, s.padded, stream);
+            launch_entropy_wide(entropy_features_gradient, a.type, w.features.side, x, s.padded, stream);
         }
         if (grad_table) {
-            void* const out = static_cast<char*>(grad_table) + static_cast<uint64_t>(first) * a.columns * bytes;
+            void* const out = static_cast<char*>(grad_table) + static_cast<uint64_t>(first) * a.columns * type_bytes(a.type);
             x.a = s.packed;
-            x.a_stride = s.padded_columns;
-            x.a_columns = s.padded_columns;
+            x.a_stride = p.b_stride;
+            x.a_columns = x.a_plane = s.padded_columns;
             x.i_tiles = div_up(a.columns, w.table.side);
             x.j_end = rows;
             x.splits = w.table.splits;
@@ -939,7 +802,7 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
             x.out = x.splits > 1 ? nullptr : out;
             x.out_stride = a.columns;
             x.factor = w.factor;
-            launch_product(entropy_table_gradient, a, w.table.side, x, rows, stream);
+            launch_entropy_wide(entropy_table_gradient, a.type, w.table.side, x, rows, stream);
             if (x.splits > 1)
                 launch_gathering(a.type, gathering_of(w.table_slab, w.piece_rows, s.padded_columns, x.splits, rows, a.columns, w.factor), out, stream);
         }
@@ -947,10 +810,10 @@ bool launch_entropy_backward(const EntropyArgs& a, const float* upstream, const 
     if (grad_features) {
         Gathering g = gathering_of(w.features_slab, s.padded, s.padded_columns, w.features.splits, a.n, a.columns, w.factor);
         g.packed_of = s.packed_of;
-        g.residual = w.residual;
+        g.residual = in_parts(a) && !apart ? nullptr : w.residual;
         g.target = s.target;
-        g.table = table.rows;
-        g.table_stride = table.stride;
+        g.table = in_parts(a) ? a.table : table.rows;
+        g.table_stride = in_parts(a) ? a.table_stride : table.stride;
         launch_gathering(a.type, g, grad_features, stream);
     }
     EFGS_HIP_CHECK(hipGetLastError());

@@ -26,8 +26,6 @@ typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-template <typename T, int W> using Part = T __attribute__((ext_vector_type(W), aligned(sizeof(T))));
-
 constexpr uint32_t block = 256, waves = 4, chunk = 64, chunk_tiles = chunk / 16;
 constexpr float infinity = __builtin_inff();
 constexpr float far_above = 64.0f;   // how far (log 2) a logit may lie above the lane's reference: what sums of 2^64 and below leave room for
@@ -39,43 +37,6 @@ template <typename T> constexpr uint32_t parts_of = std::is_same_v<T, float> ? 3
 template <uint32_t PARTS> constexpr uint32_t slots_of = PARTS == 3 ? 6 : PARTS == 2 ? 4 : 1;
 template <uint32_t PARTS> __device__ __forceinline__ uint32_t stream_part(uint32_t pair) { return PARTS == 1 ? 0 : PARTS == 2 ? pair >> 1 : 0x120100u >> 4 * pair & 3u; }
 template <uint32_t PARTS> __device__ __forceinline__ uint32_t own_part(uint32_t pair) { return PARTS == 1 ? 0 : PARTS == 2 ? pair & 1u : 0x102010u >> 4 * pair & 3u; }
-
-// eight consecutive values, those from `valid` on zero
-template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p, int32_t valid) {
-    if (valid >= 8) {
-        const Part<T, 8> v = *reinterpret_cast<const Part<T, 8>*>(p);
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = static_cast<float>(v[k]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = k < valid ? static_cast<float>(p[k]) : 0.0f;
-    }
-}
-
-// two values at a time: one conversion, and its halves back as floats by a shift and a mask (five instructions a pair and part)
-template <uint32_t PARTS, int N, typename V>
-__device__ __forceinline__ void split(V (&parts)[PARTS], const float (&x)[N]) {
-    typedef uint32_t Words __attribute__((ext_vector_type(N / 2)));
-    Words words[PARTS];
-#pragma unroll
-    for (int k = 0; k < N; k += 2) {
-        float low = x[k], high = x[k + 1];
-#pragma unroll
-        for (uint32_t part = 0; part < PARTS; part++) {
-            typedef float Floats __attribute__((ext_vector_type(2)));
-            typedef __bf16 Halves __attribute__((ext_vector_type(2)));
-            const uint32_t word = __builtin_bit_cast(uint32_t, __builtin_convertvector(Floats{low, high}, Halves));
-            words[part][k / 2] = word;
-            if (part + 1 < PARTS) {
-                low -= __builtin_bit_cast(float, word << 16);
-                high -= __builtin_bit_cast(float, word & 0xffff0000u);
-            }
-        }
-    }
-#pragma unroll
-    for (uint32_t part = 0; part < PARTS; part++) parts[part] = __builtin_bit_cast(V, words[part]);
-}
 
 __device__ __forceinline__ floatx4 multiply(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ bf16x8 pair(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
@@ -117,9 +78,9 @@ __global__ __launch_bounds__(block, 2) void entropy_narrow_kernel(EntropyNarrowA
         for (uint32_t s = 0; s < MS; s++) {
             const uint32_t slot = 4 * s + q, column = slot / SLOTS * 8, part = own_part<PARTS>(slot % SLOTS);
             float x[8];
-            load8<T>(x, own + o * own_stride + column, inside && slot < KB * SLOTS ? static_cast<int32_t>(a.columns) - static_cast<int32_t>(column) : 0);
+            entropy_load8<T>(x, own + o * own_stride + column, inside && slot < KB * SLOTS ? static_cast<int32_t>(a.columns) - static_cast<int32_t>(column) : 0);
             bf16x8 parts[PARTS];
-            split<PARTS>(parts, x);
+            entropy_split<PARTS>(parts, x);
             fo[t][s] = parts[0];
 #pragma unroll
             for (uint32_t k = 1; k < PARTS; k++) fo[t][s] = part == k ? parts[k] : fo[t][s];
@@ -157,7 +118,7 @@ __global__ __launch_bounds__(block, 2) void entropy_narrow_kernel(EntropyNarrowA
 #pragma unroll
         for (uint32_t j = 0; j < blocks; j++) {
             const uint32_t column = (first_block + 4 * j) * 8;
-            load8<T>(next[j], stream + static_cast<uint64_t>(m) * stream_stride + column,
+            entropy_load8<T>(next[j], stream + static_cast<uint64_t>(m) * stream_stride + column,
                      m < stream_end ? static_cast<int32_t>(a.columns) - static_cast<int32_t>(column) : 0);
         }
         if constexpr (own_table) {
@@ -174,7 +135,7 @@ __global__ __launch_bounds__(block, 2) void entropy_narrow_kernel(EntropyNarrowA
             const uint32_t b = first_block + 4 * j;
             if (b < KB) {
                 bf16x8 parts[PARTS];
-                split<PARTS>(parts, next[j]);
+                entropy_split<PARTS>(parts, next[j]);
 #pragma unroll
                 for (uint32_t part = 0; part < PARTS; part++) *reinterpret_cast<bf16x8*>(lds + part * part_bytes + (b * chunk + row) * 16) = parts[part];
             }
@@ -289,7 +250,7 @@ __global__ __launch_bounds__(block, 2) void entropy_narrow_kernel(EntropyNarrowA
                     constexpr uint32_t g_parts = PARTS == 3 ? 3 : 2;
                     bf16x4 g[g_parts];
                     const float x[4] = {z[t][0], z[t][1], z[t][2], z[t][3]};
-                    split<g_parts>(g, x);
+                    entropy_split<g_parts>(g, x);
 #pragma unroll
                     for (uint32_t d = 0; d < DT; d++) {
                         out[t][d] = multiply(pair(y[d][0], y[d][0]), pair(g[0], g[1]), out[t][d]);

@@ -27,6 +27,11 @@ typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t step_k = 64, wave_chunks = 4;                // transfers of 1 KB by a wave to an operand's tile
 template <uint32_t SIDE> constexpr uint32_t block_of = SIDE * 2;
+template <typename T> constexpr uint32_t parts_of = std::is_same_v<T, float> ? 3 : 1;   // a float: bfloat16 parts
+template <typename T> using Element = std::conditional_t<std::is_same_v<T, float>, __bf16, T>;
+constexpr uint32_t pairs = 6;                                   // of parts, the smallest products first; those below 2^-24 of the largest are left out
+__device__ __forceinline__ uint32_t a_part(uint32_t pair) { return 0x001012u >> 4 * pair & 3u; }
+__device__ __forceinline__ uint32_t b_part(uint32_t pair) { return 0x010210u >> 4 * pair & 3u; }
 constexpr uint32_t outside = 0xfffffff0u;                       // an offset past every bound
 constexpr float infinity = __builtin_inff();
 
@@ -92,16 +97,16 @@ struct Operand {
         }
     }
 
-    // transfer u of the tile of k..k + 63, which `buffer_at` describes, on its way to LDS at `to` (past k's end: zeros)
-    __device__ __forceinline__ uintx4 buffer_at(uint32_t k) const {
+    // transfer u of the tile of k..k + 63, `part` elements on, which `buffer_at` describes, on its way to LDS at `to` (past k's end: zeros)
+    __device__ __forceinline__ uintx4 buffer_at(uint32_t k, uint32_t part) const {
         if constexpr (ALONG_K) return buffer;
         const uint64_t left = min(k_end - min(k, k_end), step_k);
-        return buffer_of(base + k * stride, left > 0 ? (left - 1) * stride + columns * 2ull : 0);
+        return buffer_of(base + k * stride + part * 2ull, left > 0 ? (left - 1) * stride + columns * 2ull : 0);
     }
 
-    __device__ __forceinline__ void load(uint32_t to, uintx4 here, uint32_t k, uint32_t u) const {
+    __device__ __forceinline__ void load(uint32_t to, uintx4 here, uint32_t k, uint32_t part, uint32_t u) const {
         const uint32_t at = to + (scalar(threadIdx.x >> 6) * wave_chunks + u) * 1024;
-        if constexpr (ALONG_K) to_lds(at, here, k + chunk_k < k_end ? offsets[u] : outside, k < k_end ? k * 2 : 0);
+        if constexpr (ALONG_K) to_lds(at, here, k + chunk_k < k_end ? offsets[u] : outside, k < k_end ? (part + k) * 2 : 0);
         else to_lds(at, here, offsets[u], 0);
     }
 };
@@ -137,27 +142,33 @@ struct Fragments {
 };
 
 // The logits' gradients are rounded to the type. A row's own target's is mostly the largest by far, and its rounding would be most of what the gradients lose;
-// so what it lost is added to them, in the rows' gradient as they are gathered, and in the table's here: the packed rows whose target is one of the tile's
-// table rows are looked up, and 64 of them at a time make one more step of k, their features one operand and the residuals, each in its
-// row and target's column of zeros, the other. (8,192 rows against 128,000: sixteen of them to a tile, mostly one step after 128.)
+// so what it lost is added to them, in the rows' gradient as they are gathered, and in the table's here: the packed rows of the block's share of k whose target is
+// one of the tile's table rows are looked up, and 64 of them at a time make one more step of k, their features one operand and the residuals, each in its
+// row and target's column of zeros, the other; the next 64 rows' features are on their way meanwhile. (8,192 rows against 128,000: sixteen of them to a tile,
+// mostly one step after 128.) A float's target's gradient is left out of the piece as a whole and added here, by its parts: a sum over a long table that holds
+// one large value from early on rounds all that follow to it.
 template <typename T, uint32_t SIDE, typename FA, typename FB, typename Acc>
-__device__ __forceinline__ void add_residuals(const EntropyProductArgs& a, char* lds, uint32_t count, uint32_t i0, uint32_t j0, const FA& fragments_a,
+__device__ __forceinline__ void add_residuals(const EntropyProductArgs& a, char* lds, uint32_t begin, uint32_t end, uint32_t i0, uint32_t j0, const FA& fragments_a,
                                               const FB& fragments_b, Acc& acc) {
     constexpr uint32_t block = block_of<SIDE>, operand_bytes = SIDE * step_k * 2, row_bytes = SIDE * 2, at_once = 4, most = SIDE * 32;
-    constexpr uint32_t wave_i = SIDE / 32, wave_j = 4;
+    constexpr uint32_t wave_i = SIDE / 32, wave_j = 4, parts = parts_of<T>, chunks = operand_bytes / 16 / block;   // of 16 bytes, of an operand
+    using E = Element<T>;
     uint32_t* const list = reinterpret_cast<uint32_t*>(lds + 2 * operand_bytes);   // the second stage: packed rows, then the waves' counts
     uint32_t* const wave_counts = list + most;
     static_assert((most + at_once * block / 64) * sizeof(uint32_t) <= 2 * operand_bytes, "the list fits a stage");
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, first = a.first_row + j0;
     typedef uint32_t Words __attribute__((ext_vector_type(4)));
     uint32_t listed = 0;
+    E* place = reinterpret_cast<E*>(lds + operand_bytes);   // of the thread's row's residual
     __syncthreads();
-    for (uint32_t from = 0; from < count; from += at_once * block) {
+#pragma unroll
+    for (uint32_t c = 0; c < chunks; c++) *reinterpret_cast<Words*>(lds + operand_bytes + (c * block + threadIdx.x) * 16) = Words{};
+    for (uint32_t from = begin; from < end; from += at_once * block) {
         bool hit[at_once];
 #pragma unroll
         for (uint32_t k = 0; k < at_once; k++) {
             const uint32_t m = from + k * block + threadIdx.x;
-            hit[k] = m < count && a.target[m] - first < SIDE;
+            hit[k] = m < end && a.target[m] - first < SIDE;
         }
 #pragma unroll
         for (uint32_t k = 0; k < at_once; k++) {
@@ -179,49 +190,88 @@ __device__ __forceinline__ void add_residuals(const EntropyProductArgs& a, char*
         }
         listed += all;
         __syncthreads();
-        if (listed == 0 || (from + at_once * block < count && listed + at_once * block <= most)) continue;
-        for (uint32_t k0 = 0; k0 < listed; k0 += step_k) {
-            const uint32_t rows = min(listed - k0, step_k);
-            constexpr uint32_t chunks = operand_bytes / 16 / block;   // 16 bytes each, of both operands
+        if (listed == 0 || (from + at_once * block < end && listed + at_once * block <= most)) continue;
+        Words next[chunks];
+        float next_residual = 0.0f;
+        uint32_t next_column = 0;   // of the tile: the target's
+        const auto fetch = [&](uint32_t k0, uint32_t part) {
 #pragma unroll
             for (uint32_t c = 0; c < chunks; c++) {
                 const uint32_t at = c * block + threadIdx.x, k = at / (row_bytes / 16), chunk = at % (row_bytes / 16), exchange = (k & 3u) | (k >> 3 & 1u) << 2;
                 const uint32_t column = i0 + (chunk ^ 2 * exchange) * 8;
-                Words x{};
-                if (k < rows && column < a.a_columns)
-                    x = *reinterpret_cast<const Words*>(static_cast<const T*>(a.a) + list[k0 + k] * a.a_stride + column);
-                *reinterpret_cast<Words*>(lds + at * 16) = x;
-                *reinterpret_cast<Words*>(lds + operand_bytes + at * 16) = Words{};
+                next[c] = Words{};
+                if (k0 + k < listed && column < a.a_columns)
+                    next[c] = *reinterpret_cast<const Words*>(static_cast<const E*>(a.a) + list[k0 + k] * a.a_stride + part * a.a_plane + column);
             }
-            __syncthreads();
-            if (threadIdx.x < rows) {
-                const uint32_t k = threadIdx.x, m = list[k0 + k], v = a.target[m] - first, exchange = (k & 3u) | (k >> 3 & 1u) << 2;
-                *reinterpret_cast<T*>(lds + operand_bytes + k * row_bytes + (v / 16 ^ exchange) * 32 + v % 16 * 2) = static_cast<T>(a.residual[m]);
+            if (threadIdx.x < step_k) {
+                const bool inside = k0 + threadIdx.x < listed;
+                const uint32_t m = inside ? list[k0 + threadIdx.x] : 0;
+                next_residual = inside ? a.residual[m] : 0.0f;
+                next_column = inside ? a.target[m] - first : 0;
             }
-            __syncthreads();
+        };
+        fetch(0, 0);
+        for (uint32_t k0 = 0; k0 < listed; k0 += step_k) {
+            for (uint32_t part = 0; part < parts; part++) {
+                float left = next_residual;
 #pragma unroll
-            for (uint32_t half = 0; half < 2; half++) {
-                shortx8 fa[wave_i], fb[wave_j];
+                for (uint32_t c = 0; c < chunks; c++) *reinterpret_cast<Words*>(lds + (c * block + threadIdx.x) * 16) = next[c];
+                if (threadIdx.x < step_k) {
+                    const uint32_t k = threadIdx.x, v = next_column, exchange = (k & 3u) | (k >> 3 & 1u) << 2;
+                    *place = static_cast<E>(0.0f);
+                    place = reinterpret_cast<E*>(lds + operand_bytes + k * row_bytes + (v / 16 ^ exchange) * 32 + v % 16 * 2);
+                }
+                for (uint32_t other = 0; other < parts - part; other++) {  // the residual's parts that go with this one of the features
+                    if (other > 0) __syncthreads();
+                    if (threadIdx.x < step_k) *place = static_cast<E>(left);
+                    left -= static_cast<float>(static_cast<E>(left));
+                    __syncthreads();
+                    if (other == 0) fetch(part + 1 < parts ? k0 : k0 + step_k, part + 1 < parts ? part + 1 : 0);
 #pragma unroll
-                for (uint32_t t = 0; t < wave_j; t++) fb[t] = fragments_b.read(lds + operand_bytes, half, t);
+                    for (uint32_t half = 0; half < 2; half++) {
+                        shortx8 fa[wave_i], fb[wave_j];
 #pragma unroll
-                for (uint32_t t = 0; t < wave_i; t++) fa[t] = fragments_a.read(lds, half, t);
+                        for (uint32_t t = 0; t < wave_j; t++) fb[t] = fragments_b.read(lds + operand_bytes, half, t);
 #pragma unroll
-                for (uint32_t ti = 0; ti < wave_i; ti++)
+                        for (uint32_t t = 0; t < wave_i; t++) fa[t] = fragments_a.read(lds, half, t);
 #pragma unroll
-                    for (uint32_t tj = 0; tj < wave_j; tj++) acc[ti][tj] = multiply<T>(fa[ti], fb[tj], acc[ti][tj]);
+                        for (uint32_t ti = 0; ti < wave_i; ti++)
+#pragma unroll
+                            for (uint32_t tj = 0; tj < wave_j; tj++) acc[ti][tj] = multiply<E>(fa[ti], fb[tj], acc[ti][tj]);
+                    }
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
         listed = 0;
     }
 }
+
+// A step of k; of floats, the steps of one pair of parts follow those of another.
+template <uint32_t PARTS>
+struct Step {
+    uint32_t k, first, end, a_plane, b_plane, pair;
+
+    __device__ __forceinline__ void advance() {
+        k += step_k;
+        if constexpr (PARTS == 3) {
+            if (k >= end) {
+                pair++;
+                k = pair < pairs ? first : end;
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t of_a() const { return PARTS == 3 ? a_part(pair) * a_plane : 0; }
+    __device__ __forceinline__ uint32_t of_b() const { return PARTS == 3 ? b_part(pair) * b_plane : 0; }
+};
 
 template <typename T, EntropyProduct P, uint32_t SIDE>
 __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(EntropyProductArgs a) {
     constexpr bool first_two = P == entropy_logits || P == entropy_upstream, a_along_k = first_two, b_along_k = P != entropy_table_gradient;
     constexpr uint32_t tile = SIDE, operand_bytes = tile * step_k * 2, stage_bytes = 2 * operand_bytes;
     constexpr uint32_t wave_i = SIDE / 32, wave_j = 4;  // tiles of 16 a wave
+    constexpr uint32_t parts = parts_of<T>;
+    using E = Element<T>;
     __shared__ __attribute__((aligned(1024))) char lds[2 * stage_bytes];
     const uint32_t count = scalar(*a.count);
     // Blocks go round the eight XCDs one by one: each XCD takes a run of the tiles, four rows of j at a time along i, so that the tiles that
@@ -237,17 +287,18 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
     const uint32_t k_first = min(blockIdx.y * k_each, k_all), k_end = min(k_first + k_each, k_all);
 
     const uint32_t lane = threadIdx.x & 63u, e = lane & 15u, q = lane >> 4, wave = threadIdx.x >> 6, wi = wave & 1u, wj = wave >> 1;
+    const uint32_t b_columns = parts > 1 ? a.b_plane : static_cast<uint32_t>(a.b_stride);  // of a part
     Operand<SIDE, a_along_k> operand_a;
     Operand<SIDE, b_along_k> operand_b;
     if constexpr (first_two) {
-        operand_a.begin(a.a, a.a_stride, a.i_end, a.a_columns, i0, a.a_columns);
-        operand_b.begin(a.b, a.b_stride, j0 + tile, static_cast<uint32_t>(a.b_stride), j0, static_cast<uint32_t>(a.b_stride));
+        operand_a.begin(a.a, a.a_stride, a.i_end, a.a_columns, i0, parts > 1 ? a.a_plane : a.a_columns);
+        operand_b.begin(a.b, a.b_stride, j0 + tile, static_cast<uint32_t>(a.b_stride), j0, b_columns);
     } else if constexpr (P == entropy_features_gradient) {
         operand_a.begin(a.a, a.a_stride, k_all, a.a_columns, i0, k_all);
-        operand_b.begin(a.b, a.b_stride, j0 + tile, static_cast<uint32_t>(a.b_stride), j0, static_cast<uint32_t>(a.b_stride));
+        operand_b.begin(a.b, a.b_stride, j0 + tile, static_cast<uint32_t>(a.b_stride), j0, b_columns);
     } else {
         operand_a.begin(a.a, a.a_stride, k_all, a.a_columns, i0, k_all);
-        operand_b.begin(a.b, a.b_stride, k_all, static_cast<uint32_t>(a.b_stride), j0, k_all);
+        operand_b.begin(a.b, a.b_stride, k_all, b_columns, j0, k_all);
     }
     Fragments<SIDE, a_along_k, wave_i> fragments_a;
     Fragments<SIDE, b_along_k, wave_j> fragments_b;
@@ -259,62 +310,65 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
     shortx8 fa[2][wave_i], fb[2][wave_j];  // of the two halves of a step
     // A half step: its products, and between them, so that both are under way at once, the reads of the fragments of the half step behind it
     // and, in the second half, the transfers of the step after the next.
-    const auto half_step = [&](auto half, const char* from, uint32_t to, uint32_t k) {
+    const auto half_step = [&](auto half, const char* from, uint32_t to, const Step<parts>& s) {
         constexpr uint32_t h = decltype(half)::value;
         uintx4 buffer_a{}, buffer_b{};
         if constexpr (h == 1) {
-            buffer_a = operand_a.buffer_at(k);
-            buffer_b = operand_b.buffer_at(k);
+            buffer_a = operand_a.buffer_at(s.k, s.of_a());
+            buffer_b = operand_b.buffer_at(s.k, s.of_b());
         }
 #pragma unroll
         for (uint32_t ti = 0; ti < wave_i; ti++) {
             if (ti < wave_j) fb[1 - h][ti] = fragments_b.read(from + operand_bytes, 1 - h, ti);
             fa[1 - h][ti] = fragments_a.read(from, 1 - h, ti);
             if (h == 1 && ti < wave_chunks) {
-                operand_a.load(to, buffer_a, k, ti);
-                operand_b.load(to + operand_bytes, buffer_b, k, ti);
+                operand_a.load(to, buffer_a, s.k, s.of_a(), ti);
+                operand_b.load(to + operand_bytes, buffer_b, s.k, s.of_b(), ti);
             }
 #pragma unroll
-            for (uint32_t tj = 0; tj < wave_j; tj++) acc[ti][tj] = multiply<T>(fa[h][ti], fb[h][tj], acc[ti][tj]);
+            for (uint32_t tj = 0; tj < wave_j; tj++) acc[ti][tj] = multiply<E>(fa[h][ti], fb[h][tj], acc[ti][tj]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     const std::integral_constant<uint32_t, 0> first_half;
     const std::integral_constant<uint32_t, 1> second_half;
-    // (Steps past the end are read as zeros, so that nothing stands in branches.) Half way through a step its second half is in the registers: its stage is free for the step after the next, and the next one's
-    // has to be there.
+    // (Steps past the end are read as zeros, so that nothing stands in branches.) Half way through a step its second half is in the registers: its
+    // stage is free for the step after the next, and the next one's has to be there.
     if (k_first < k_end) {
-        const auto load = [&](uint32_t to, uint32_t k) {
-            const uintx4 buffer_a = operand_a.buffer_at(k), buffer_b = operand_b.buffer_at(k);
+        Step<parts> ahead{k_first, k_first, k_end, a.a_plane, a.b_plane, 0};
+        const auto load = [&](uint32_t to) {
+            const uintx4 buffer_a = operand_a.buffer_at(ahead.k, ahead.of_a()), buffer_b = operand_b.buffer_at(ahead.k, ahead.of_b());
 #pragma unroll
             for (uint32_t u = 0; u < wave_chunks; u++) {
-                operand_a.load(to, buffer_a, k, u);
-                operand_b.load(to + operand_bytes, buffer_b, k, u);
+                operand_a.load(to, buffer_a, ahead.k, ahead.of_a(), u);
+                operand_b.load(to + operand_bytes, buffer_b, ahead.k, ahead.of_b(), u);
             }
+            ahead.advance();
         };
-        load(lds_at, k_first);
+        load(lds_at);
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        load(lds_at + stage_bytes, k_first + step_k);
+        load(lds_at + stage_bytes);
 #pragma unroll
         for (uint32_t t = 0; t < wave_j; t++) fb[0][t] = fragments_b.read(lds + operand_bytes, 0, t);
 #pragma unroll
         for (uint32_t t = 0; t < wave_i; t++) fa[0][t] = fragments_a.read(lds, 0, t);
         uint32_t stage = 0;
-        for (uint32_t k = k_first; k < k_end; k += step_k) {
-            half_step(first_half, lds + stage, 0, 0);
+        for (uint32_t n = (k_end - k_first + step_k - 1) / step_k * (parts > 1 ? pairs : 1); n > 0; n--) {
+            half_step(first_half, lds + stage, 0, ahead);
             __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): this wave's part of the next stage is there, its reads of this one are done
             __builtin_amdgcn_s_barrier();        // and so for the other waves
             asm volatile("" ::: "memory");
-            half_step(second_half, lds + (stage ^ stage_bytes), lds_at + stage, k + 2 * step_k);
+            half_step(second_half, lds + (stage ^ stage_bytes), lds_at + stage, ahead);
+            ahead.advance();
             stage ^= stage_bytes;
         }
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the zeros that follow the last step
     }
 
     if constexpr (P == entropy_table_gradient) {
-        if (blockIdx.y == 0) add_residuals<T, SIDE>(a, lds, count, i0, j0, fragments_a, fragments_b, acc);
+        if (a.apart) add_residuals<T, SIDE>(a, lds, k_first, min(k_end, count), i0, j0, fragments_a, fragments_b, acc);
     }
     const uint32_t i_lane = i0 + wi * (SIDE / 2) + 4 * q, j_lane = j0 + wj * 64 + e;  // results: i_lane + 16 ti + r, j_lane + 16 tj
     if constexpr (P == entropy_logits) {
@@ -353,7 +407,7 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
             a.partial[(i0 / tile) * a.slab_rows + (j0 - a.j_first) + threadIdx.x] = make_float2(top, sum);
         }
     } else if constexpr (P == entropy_upstream) {
-        typedef T Four __attribute__((ext_vector_type(4)));
+        typedef E Four __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (uint32_t tj = 0; tj < wave_j; tj++) {
             const uint32_t j = j_lane + tj * 16, target = a.target[j];
@@ -365,7 +419,7 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
             for (uint32_t ti = 0; ti < wave_i; ti++) {
                 const uint32_t i = i_lane + ti * 16;
                 floatx4 p;
-                Four g;
+                E* const piece = static_cast<E*>(a.piece) + j * a.piece_stride + i;
 #pragma unroll
                 for (uint32_t r = 0; r < 4; r++) p[r] = __builtin_amdgcn_exp2f((rounded(acc[ti][tj][r] * a.to_log2) - lse.x) - lse.y);
                 if (hit) {
@@ -373,18 +427,35 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
                     for (uint32_t r = 0; r < 4; r++)
                         if (a.first_row + i + r == target) p[r] -= 1.0f;
                 }
+                if constexpr (parts == 1) {
+                    Four g;
 #pragma unroll
-                for (uint32_t r = 0; r < 4; r++) g[r] = static_cast<T>(counts && i + r < a.i_end ? p[r] * weight : 0.0f);
-                if (hit) {
+                    for (uint32_t r = 0; r < 4; r++) g[r] = static_cast<T>(counts && i + r < a.i_end ? p[r] * weight : 0.0f);
+                    if (hit) {
 #pragma unroll
-                    for (uint32_t r = 0; r < 4; r++)
-                        if (a.first_row + i + r == target) a.residual[j] = p[r] * weight - static_cast<float>(g[r]);
+                        for (uint32_t r = 0; r < 4; r++)
+                            if (a.first_row + i + r == target) a.residual[j] = p[r] * weight - static_cast<float>(g[r]);
+                    }
+                    *reinterpret_cast<Four*>(piece) = g;
+                } else {
+                    float g[4];
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) {
+                        g[r] = counts && i + r < a.i_end ? p[r] * weight : 0.0f;
+                        if (hit && a.apart && a.first_row + i + r == target) {
+                            a.residual[j] = g[r];
+                            g[r] = 0.0f;
+                        }
+                    }
+                    Four split[parts];
+                    entropy_split<parts>(split, g);
+#pragma unroll
+                    for (uint32_t part = 0; part < parts; part++) *reinterpret_cast<Four*>(piece + part * a.piece_plane) = split[part];
                 }
-                *reinterpret_cast<Four*>(static_cast<T*>(a.piece) + j * a.piece_stride + i) = g;
             }
         }
     } else {
-        typedef T Four __attribute__((ext_vector_type(4), aligned(2)));
+        typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
         const bool direct = P == entropy_table_gradient && a.out;
         const float factor = direct ? *a.factor : 1.0f;
         const uint32_t j_end = P == entropy_table_gradient ? a.j_end : count;
@@ -431,9 +502,12 @@ void launch_entropy_wide(EntropyProduct product, int type, uint32_t side, const 
     if (type == type_bfloat16) {
         if (side == 256) launch<__bf16, 256>(product, a, j, s);
         else launch<__bf16, 128>(product, a, j, s);
-    } else {
+    } else if (type == type_half) {
         if (side == 256) launch<_Float16, 256>(product, a, j, s);
         else launch<_Float16, 128>(product, a, j, s);
+    } else {
+        if (side == 256) launch<float, 256>(product, a, j, s);
+        else launch<float, 128>(product, a, j, s);
     }
 }
 
