@@ -25,7 +25,7 @@ struct EntropyProductArgs {
     uint32_t a_plane, b_plane;     // floats: elements from one part of a row to the next
     uint32_t i_tiles;
     uint32_t j_first;              // of the launch
-    uint32_t splits;               // of k, over gridDim.y
+    uint32_t splits;               // of k
     const uint32_t* count;         // packed rows
     float to_log2;                 // scale log2 e
     float2* partial;               // logits: i_tiles x slab_rows (maximum, sum of exponentials), from row j_first on

@@ -274,17 +274,18 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
     using E = Element<T>;
     __shared__ __attribute__((aligned(1024))) char lds[2 * stage_bytes];
     const uint32_t count = scalar(*a.count);
-    // Blocks go round the eight XCDs one by one: each XCD takes a run of the tiles, four rows of j at a time along i, so that the tiles that
-    // are under way on it share their operands in its L2.
+    // Blocks go round the eight XCDs one by one: each XCD takes a run of the tiles, split by split, four rows of j at a time along i, so that the tiles
+    // that are under way on it share their operands in its L2.
     const uint32_t j_tiles = P == entropy_table_gradient ? (a.j_end + tile - 1) / tile
                                                          : (min(count - min(count, a.j_first), a.j_end) + tile - 1) / tile;
-    const uint32_t tiles = a.i_tiles * j_tiles, each = (tiles + 7) / 8, at = (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= each || at >= tiles) return;
+    const uint32_t tiles = a.i_tiles * j_tiles, blocks = tiles * a.splits, each = (blocks + 7) / 8, in_all = (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= each || in_all >= blocks) return;
+    const uint32_t split = in_all / tiles, at = in_all - split * tiles;
     const uint32_t band = at / (4 * a.i_tiles), in_band = at - band * 4 * a.i_tiles, width = min(4u, j_tiles - band * 4);
     const uint32_t i0 = in_band / width * tile, j0 = a.j_first + (band * 4 + in_band % width) * tile;
     const uint32_t k_all = P == entropy_table_gradient ? (count + step_k - 1) / step_k * step_k : a.k_end;
     const uint32_t k_each = ((k_all + a.splits - 1) / a.splits + step_k - 1) / step_k * step_k;
-    const uint32_t k_first = min(blockIdx.y * k_each, k_all), k_end = min(k_first + k_each, k_all);
+    const uint32_t k_first = min(split * k_each, k_all), k_end = min(k_first + k_each, k_all);
 
     const uint32_t lane = threadIdx.x & 63u, e = lane & 15u, q = lane >> 4, wave = threadIdx.x >> 6, wi = wave & 1u, wj = wave >> 1;
     const uint32_t b_columns = parts > 1 ? a.b_plane : static_cast<uint32_t>(a.b_stride);  // of a part
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
                         for (uint32_t r = 0; r < 4; r++)
                             if (i + r < a.i_end) out[r] = y[r];
                 } else if (i < a.slab_stride) {
-                    floatx4* const out = reinterpret_cast<floatx4*>(a.slab + (blockIdx.y * a.slab_rows + j) * a.slab_stride + i);
+                    floatx4* const out = reinterpret_cast<floatx4*>(a.slab + (split * a.slab_rows + j) * a.slab_stride + i);
                     *out = a.add ? *out + acc[ti][tj] : acc[ti][tj];
                 }
             }
@@ -487,7 +488,7 @@ __global__ __launch_bounds__(block_of<SIDE>, 2) void entropy_wide_kernel(Entropy
 
 template <typename T, uint32_t SIDE>
 void launch(EntropyProduct product, const EntropyProductArgs& a, uint32_t j, hipStream_t s) {
-    const dim3 grid((a.i_tiles * div_up(j, SIDE) + 7) / 8 * 8, a.splits), block(block_of<SIDE>);
+    const dim3 grid((a.i_tiles * div_up(j, SIDE) * a.splits + 7) / 8 * 8), block(block_of<SIDE>);
     switch (product) {
         case entropy_logits: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_logits, SIDE>), grid, block, 0, s, a); break;
         case entropy_upstream: hipLaunchKernelGGL((entropy_wide_kernel<T, entropy_upstream, SIDE>), grid, block, 0, s, a); break;
