@@ -3,6 +3,9 @@
 //   count_e = choices of e, share_e = count_e / all choices, p_n = softmax(z_n), P_e = mean of p_ne over the rows that count
 //   loss = E sum_e share_e P_e,  d loss / d z_ne = E / rows p_ne (share_e - sum_j share_j p_nj)
 //
+// The probabilities of a row sum to one, so the gradient takes shares less the even one, 1 / E: even choices give zeros and not what the rounded sum of
+// probabilities leaves.
+//
 // A choice outside [0, E) counts nowhere, a row without any other is left out. Rows of nothing but -inf have no
 // probabilities and no gradient. One pass over the logits either way: TPR lanes share a row (a wave takes several short rows, a
 // block one long row), each holds the same columns of every row that it meets, so that the sums over rows stay in registers until
@@ -30,7 +33,7 @@ struct BalanceKernelArgs {
     uint32_t experts, chosen, index_bytes;
     float* sums;          // blocks x experts
     uint32_t* counts;     // blocks x (experts + 1): choices of each, then rows that count
-    const float* share;   // backward: experts, then E / rows
+    const float* share;   // backward: of each expert, less 1 / E; then E / rows
     const float* upstream;
     void* gradient;
 };
@@ -136,7 +139,7 @@ struct BalanceTotals {
     uint32_t blocks, experts;
     double* totals;       // experts + 1: sums of probabilities; rows
     int64_t* count;       // experts
-    float* share;         // experts, then E / rows
+    float* share;         // of each expert, less 1 / E; then E / rows
     float* loss;
 };
 
@@ -161,9 +164,9 @@ __device__ __forceinline__ void loss_of_totals(const BalanceTotals& a) {
     const double rows = a.totals[a.experts], per_choice = choices > 0.0 ? 1.0 / choices : 0.0, per_row = rows > 0.0 ? a.experts / rows : 0.0;
     double loss = 0.0;
     for (uint32_t e = threadIdx.x; e < a.experts; e += balance_block) {
-        const double share = static_cast<double>(a.count[e]) * per_choice;
-        a.share[e] = static_cast<float>(share);
-        if (a.count[e] > 0) loss += share * a.totals[e];
+        const double count = static_cast<double>(a.count[e]);
+        a.share[e] = static_cast<float>((count * a.experts - choices) * per_choice / a.experts);
+        if (a.count[e] > 0) loss += count * per_choice * a.totals[e];
     }
     loss = block_sum(loss, lds);
     if (threadIdx.x == 0) {

@@ -387,7 +387,7 @@ int efgs_dropout(const void* x, const void* residual, void* out, int64_t n, int 
 
 /* Balance of choices: counts (int64) of each of `experts` (1 to 8192) among indices (n x chosen, up to 65536 of a row; outside [0, experts): none),
  * loss = experts sum_e share_e P_e, share_e = counts_e / all choices, P_e the mean of softmax(logits)_e over the rows with a choice (0 without one).
- * share (experts + 1 floats) is kept for the backward, which writes gradient (n x experts, in `type`). Sums in a fixed order. Stream-ordered. */
+ * share (experts + 1 floats: shares less 1 / experts, experts / rows) is kept for the backward, which writes gradient (n x experts, in `type`). Sums in a fixed order. Stream-ordered. */
 int efgs_balance_loss_forward(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type,
                               float* loss, int64_t* counts, float* share, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
 int efgs_balance_loss_backward(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type,

@@ -172,3 +172,15 @@ def test_the_same_bits_every_time_and_captured():
         got = [t.detach().clone() for t in out]
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('experts', [3, 8, 300])
+def test_even_choices_have_no_gradient(experts):
+    """Every expert chosen as often as the others: the loss is 1 and its gradient zero, not what the probabilities' rounded sum leaves."""
+    import efgs
+    logits = torch.randn(7, experts, generator=torch.Generator(DEVICE).manual_seed(2), device=DEVICE).requires_grad_()
+    indices = torch.arange(experts, device=DEVICE).expand(7, experts)
+    loss, counts = efgs.balance_loss(logits, indices)
+    assert torch.all(counts == 7) and abs(float(loss) - 1.0) <= 2.0 ** -20
+    loss.backward()
+    assert torch.all(logits.grad == 0)
