@@ -65,7 +65,8 @@ __device__ __forceinline__ void entropy_load8(float (&x)[8], const T* p, int32_t
     }
 }
 
-// bfloat16 parts of values whose sum is each value (three of a float: to 2^-26 of it; two of a float16: exactly): two values at a time: one conversion, and its halves back as floats by a shift and a mask (five instructions a pair and part)
+// bfloat16 parts of values whose sum is each value (three of a float: to 2^-26 of it; two of a float16: exactly). Two values at a time: one conversion, and its
+// halves back as floats by a shift and a mask (five instructions a pair and part).
 template <uint32_t PARTS, int N, typename V>
 __device__ __forceinline__ void entropy_split(V (&parts)[PARTS], const float (&x)[N]) {
     typedef uint32_t Words __attribute__((ext_vector_type(N / 2)));

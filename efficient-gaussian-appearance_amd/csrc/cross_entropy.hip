@@ -8,12 +8,14 @@
 // matrix product whose tiles leave, for each row, the maximum and the sum of exponentials over the tile's part of the table; a
 // second kernel joins them. The backward computes the logits again by pieces of the table, writes g of a piece, and multiplies
 // it by the piece and, transposed, by the rows: four products where three would do if g could be kept (N x V of it), and no more memory than a piece.
-// Statistics and sums are in 32 bits (logits in units of log 2), the sum over rows in 64. g is held in the inputs' type, as the matrix unit takes it: its
-// rounding, 2^-9 of each, is as large as the gradients' own one only where one entry outweighs the others, which a row's target does; what that one loses is
-// added (cross_entropy_wide.hip).
+// Statistics and sums are in 32 bits (logits in units of log 2), the sum over rows in 64. g is held in the inputs' type, as the matrix unit takes it (floats: three
+// bfloat16 parts): its rounding, 2^-9 of each, is as large as the gradients' own one only where one entry outweighs the others, which a row's target does; what
+// that one loses is added (cross_entropy_wide.hip).
 //
-// This file: the packing, the joins and the launches, and the products of floats of more than 64 columns. Up to 64 columns: cross_entropy_narrow.hip. 16-bit types:
-// cross_entropy_wide.hip. Up to 64 rows without a gradient: cross_entropy_few.hip.
+// This file: the packing, the joins and the launches, most of them at the latency of a launch, 4 to 9 us each. The products: cross_entropy_narrow.hip up to 64
+// columns, where its kernels are the faster ones (32,768 x 4,096 x 64: float32 0.66 ms and 1.07 by the wide one, bfloat16 0.24 and 0.34; float16 0.41 and 0.35, for
+// no piece in memory); cross_entropy_wide.hip above, as a wave's rows would not fit the narrow ones' registers; up to 64 rows without a gradient
+// cross_entropy_few.hip, which no packing precedes (37 x 30,011 x 1,000 float16 40 us by the wide one, 24 so).
 #include <algorithm>
 #include <type_traits>
 
@@ -429,7 +431,8 @@ ProductPlan plan_product(const EntropyArgs& a, uint64_t i, uint64_t j, uint64_t 
             if (s > 1 && (results == 0 || k / s < 2 * step)) break;
             const uint64_t blocks = tiles * s;
             const double step_us = side == 256 ? 1.7 : blocks <= 256 ? 0.8 : 1.2;
-            const double rounds = static_cast<double>((blocks + at_once - 1) / at_once), steps = static_cast<double>((k + s * step - 1) / (s * step) * (in_parts(a) ? 6 : 1));
+            const double rounds = static_cast<double>((blocks + at_once - 1) / at_once);
+            const double steps = static_cast<double>((k + s * step - 1) / (s * step) * (in_parts(a) ? 6 : 1));
             const double us = rounds * (steps + 2.0) * step_us + (s > 1 ? s * static_cast<double>(results) * 8.0 / 4e6 : 0.0);
             if (us < least) {
                 least = us;
@@ -441,7 +444,11 @@ ProductPlan plan_product(const EntropyArgs& a, uint64_t i, uint64_t j, uint64_t 
 }
 
 constexpr uint64_t partial_bytes = 256ull << 20;  // of the tiles' statistics at once
-constexpr uint64_t piece_bytes = 256ull << 20;    // of a piece's upstream gradients
+// A piece's upstream gradients take what the memory-side cache holds, but at least 1,024 table rows if 8 GB are enough for them: with less the products' k is
+// short and every piece reads and writes the rows' gradient once more (256 and 1,024 rows: 1M x 4,096 x 72 bfloat16 17.3 and 11.6 ms, 200,000 x 4,096 x 200
+// float32 16.9 and 11.8; 100,000 x 20,000 x 136 bfloat16 7.1 either way).
+constexpr uint64_t piece_bytes = 256ull << 20, piece_most = 8ull << 30;
+constexpr uint32_t piece_least = 1024;
 constexpr uint64_t most_blocks = 1ull << 23;      // of a launch of 256 threads (32 bits of threads)
 constexpr uint32_t tile = 128;                    // the smaller tiles' side
 
@@ -505,7 +512,8 @@ struct BackwardScratch {
     size_t bytes;
     BackwardScratch(const EntropyArgs& a, const Saved& s, void* base) {
         Carver c(base);
-        const uint64_t most = std::max<uint64_t>(piece_bytes / (static_cast<uint64_t>(s.padded) * held_bytes(a)) / 256 * 256, 256);
+        const uint64_t row_bytes = static_cast<uint64_t>(s.padded) * held_bytes(a);   // of a table row's part of a piece
+        const uint64_t most = std::max<uint64_t>(std::max<uint64_t>(piece_bytes / row_bytes, std::min<uint64_t>(piece_least, piece_most / row_bytes)) / 256 * 256, 256);
         const uint64_t all = round_up(std::max(a.rows, 1u), 256);
         pieces = div_up(all, std::min(most, all));
         piece_rows = static_cast<uint32_t>(round_up(div_up(all, pieces), 256));
@@ -601,8 +609,8 @@ EntropyNarrowArgs narrow_args(const EntropyArgs& a, const Saved& s) {
     return p;
 }
 
-// Whether what a target's rounding loses is added to the table's gradient. Where each table row is many rows' target, their roundings are a quarter of the result's
-// own or less (16 targets: 16 half steps' sum, a quarter of as many), and the rows to look up are many.
+// Whether what a target's rounding loses is added to the table's gradient (of floats: whether the target's gradient goes apart). Not where each table row is the
+// target of more than 64: their roundings, unless all alike, make an eighth of one then, and the rows to look up are as many as those of a product's steps.
 bool targets_apart(const EntropyArgs& a) { return a.n / 64 <= a.rows; }
 
 // of a slab's first `rows` rows, as they lie
@@ -624,7 +632,8 @@ void launch_gathering(int type, const Gathering& g, void* out, hipStream_t strea
     const uint32_t blocks = copy_grid(items);
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (g.splits >= 16 && items <= 1u << 18) hipLaunchKernelGGL(entropy_gather_splits_kernel<T>, dim3(div_up(items, 16)), dim3(256), 0, stream, g, static_cast<T*>(out));
+        if (g.splits >= 16 && items <= 1u << 18)
+            hipLaunchKernelGGL(entropy_gather_splits_kernel<T>, dim3(div_up(items, 16)), dim3(256), 0, stream, g, static_cast<T*>(out));
         else hipLaunchKernelGGL(entropy_gather_kernel<T>, dim3(blocks), dim3(256), 0, stream, g, static_cast<T*>(out));
     });
 }
