@@ -413,6 +413,9 @@ struct Saved {
     }
 };
 
+constexpr uint64_t most_blocks = 1ull << 23;      // of a launch of 256 threads (32 bits of threads)
+constexpr uint32_t tile = 128;                    // the smaller tiles' side
+
 // The side of a product's tiles, and how often its k is split: where tiles leave much of the GPU idle, smaller ones and more blocks, at the price of less reuse, or of
 // partial results (`results` floats) written and read once more for each split. Measured: a CU takes 1.7 us for 64 of k of a tile of 256, 1.2 for those of
 // two of 128 (0.8 for one alone); partial results move at 4 TB/s. Floats: six times the steps, and with more than 2^21 columns small tiles, whose rows' parts
@@ -422,13 +425,13 @@ struct ProductPlan {
 };
 
 ProductPlan plan_product(const EntropyArgs& a, uint64_t i, uint64_t j, uint64_t k, uint64_t results) {
-    ProductPlan best{128, 1};
+    ProductPlan best{tile, 1};
     double least = 1e30;
     for (const uint32_t side : {256u, 128u}) {
         if (side == 256 && in_parts(a) && a.columns > 1u << 21) continue;
         const uint64_t tiles = ((i + side - 1) / side) * ((j + side - 1) / side), at_once = side == 256 ? 256 : 512, step = 64;
         for (const uint32_t s : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u, 24u, 32u, 48u, 64u}) {
-            if (s > 1 && (results == 0 || k / s < 2 * step)) break;
+            if (s > 1 && (results == 0 || k / s < 2 * step || tiles * s > most_blocks / 4)) break;
             const uint64_t blocks = tiles * s;
             const double step_us = side == 256 ? 1.7 : blocks <= 256 ? 0.8 : 1.2;
             const double rounds = static_cast<double>((blocks + at_once - 1) / at_once);
@@ -449,8 +452,6 @@ constexpr uint64_t partial_bytes = 256ull << 20;  // of the tiles' statistics at
 // float32 16.9 and 11.8; 100,000 x 20,000 x 136 bfloat16 7.1 either way).
 constexpr uint64_t piece_bytes = 256ull << 20, piece_most = 8ull << 30;
 constexpr uint32_t piece_least = 1024;
-constexpr uint64_t most_blocks = 1ull << 23;      // of a launch of 256 threads (32 bits of threads)
-constexpr uint32_t tile = 128;                    // the smaller tiles' side
 
 struct ForwardScratch {
     uint32_t* chunk_counts;

@@ -181,6 +181,6 @@ def test_even_choices_have_no_gradient(experts):
     logits = torch.randn(7, experts, generator=torch.Generator(DEVICE).manual_seed(2), device=DEVICE).requires_grad_()
     indices = torch.arange(experts, device=DEVICE).expand(7, experts)
     loss, counts = efgs.balance_loss(logits, indices)
-    assert torch.all(counts == 7) and abs(float(loss) - 1.0) <= 2.0 ** -20
+    assert torch.all(counts == 7) and abs(float(loss.detach()) - 1.0) <= 2.0 ** -20
     loss.backward()
     assert torch.all(logits.grad == 0)

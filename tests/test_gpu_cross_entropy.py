@@ -5,7 +5,7 @@ once-rounded products, off by dz <= 2 (D + 4) e scale sum |x w|, the 2 for matri
 scale log2 e and its rounding 3 e |z|. A sum of exponentials of V table rows goes through at most 64 + V / 16 additions in a row, each exponential 4 e
 off; so a loss is off by 2 max dz + (80 + V / 16) e + 4 e (|lse| + |z|), and a probability by that relative to it. g = weight (p - onehot) is rounded to the
 type (u |g|, and 2^-38 for float16, whose g is held times 2^15), a gradient is a float32 sum of K values (at most 2 (K + 4) e of their magnitudes), scaled, and
-rounded to the type: u of the value, float16 half its least step, 2^-25.
+rounded to the type: u of the value, float16 half its least step, 2^-25. Floats as three bfloat16 parts lose 2^-26 each and 2^-25 by the pairs left out, within the 4 beside D.
 """
 import numpy as np
 import pytest
@@ -494,3 +494,25 @@ def test_broadcast_rows_and_shared_tensors(dtype, columns, n):
     want = dw.clone()
     want[:n] += dx
     assert torch.equal(grad, want)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_rows_of_millions_of_columns(dtype):
+    """All but seven columns zero: as those columns alone."""
+    import efgs
+    columns, kind = (1 << 21) + 72, TYPES[dtype][0]
+    at = torch.tensor([0, 1, 63, 1 << 20, (1 << 21) - 1, 1 << 21, columns - 1], device=DEVICE)
+    rng = torch.Generator(DEVICE).manual_seed(4)
+    x, w = (torch.randn(k, 7, generator=rng, device=DEVICE).to(kind).requires_grad_() for k in (3, 5))
+    y = torch.tensor([4, -1, 2], device=DEVICE)
+    want = efgs.linear_cross_entropy(x, w, y, reduction='none')
+    want_x, want_w = torch.autograd.grad(want, (x, w), torch.ones_like(want))
+    wide_x, wide_w = (torch.zeros(len(t), columns, device=DEVICE, dtype=kind).index_copy_(1, at, t.detach()).requires_grad_() for t in (x, w))
+    loss = efgs.linear_cross_entropy(wide_x, wide_w, y, reduction='none')
+    grad_x, grad_w = torch.autograd.grad(loss, (wide_x, wide_w), torch.ones_like(loss))
+    # (logits of seven products of at most about 9; bf16: both ways round g and the result)
+    u = TYPES[dtype][1]
+    assert torch.all((loss - want).abs() <= 2.0 ** -18)
+    for got, value in ((grad_x, want_x), (grad_w, want_w)):
+        assert int((got != 0).sum()) == int((got[:, at] != 0).sum())
+        assert torch.all((got[:, at].float() - value.float()).abs() <= 4 * u * (value.float().abs() + 3.0 * 5) + 2.0 ** -16)
