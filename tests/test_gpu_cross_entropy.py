@@ -516,3 +516,40 @@ def test_rows_of_millions_of_columns(dtype):
     for got, value in ((grad_x, want_x), (grad_w, want_w)):
         assert int((got != 0).sum()) == int((got[:, at] != 0).sum())
         assert torch.all((got[:, at].float() - value.float()).abs() <= 4 * u * (value.float().abs() + 3.0 * 5) + 2.0 ** -16)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_more_rows_of_one_target_than_a_list_holds(dtype):
+    """Rows of one column each, all of one target, so many that a block looks them up in several parts: every one counts once. With n_c rows of column c and
+    p_c the softmax of the table's column, the table's gradient is n_c (p_c - onehot) and a row's the sum of (p_c - onehot) w.
+
+    Logits are single products (exact but for 2^-25), a sum of 4,096 exponentials is (64 + 4096 / 16) e off at most, so a probability by 2^-15 of it; the at
+    most five rows of a column add up exactly but for their roundings; a row's gradient is a float32 sum of at most 6 * 4096 / 32 steps, 2^-13 of its terms."""
+    import efgs
+    n, rows, columns, target = 20_000, 4_096, 4_096, 333
+    kind, u, _, _ = TYPES[dtype]
+    rng = torch.Generator(DEVICE).manual_seed(6)
+    column = torch.arange(n, device=DEVICE) % columns
+    x = torch.zeros(n, columns, device=DEVICE, dtype=kind).scatter_(1, column[:, None], 1.0).requires_grad_()
+    w = torch.randn(rows, columns, generator=rng, device=DEVICE).to(kind).requires_grad_()
+    efgs.linear_cross_entropy(x, w, torch.full((n,), target, device=DEVICE), reduction='sum').backward()
+    wide = w.detach().double()
+    g = torch.softmax(wide, 0)
+    p = g.clone()
+    g[target] -= 1.0
+    count = torch.bincount(column, minlength=columns)
+    dw, size = count * g, count * p
+    off = (w.grad.double() - dw).abs()
+    assert torch.all(off <= 2.0 ** -14 * size + 2.0 * u * (count * g.abs()) + u * dw.abs()), float((off / (size + dw.abs())).max())
+    some = torch.tensor([0, 1, 777, 4_095, 4_096, 8_191, 8_192, 16_384, n - 1], device=DEVICE)
+    c = column[some]
+    dx, size = g[:, c].t() @ wide, g[:, c].t().abs() @ wide.abs()
+    off = (x.grad[some].double() - dx).abs()
+    assert torch.all(off <= (2.0 ** -13 + 2.0 ** -14 + 2.0 * u) * size + u * dx.abs()), float((off / size).max())
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('n,rows', [(6_399, 100), (6_400, 100), (6_464, 100), (9_001, 17), (700, 2)])
+def test_many_rows_of_each_target(n, rows, dtype):
+    """About where the targets' gradients are no longer added to the table's apart (64 rows of each), and past it."""
+    check(n, rows, 136, dtype, reduction='none')
