@@ -213,7 +213,7 @@ __global__ __launch_bounds__(join_block) void entropy_few_join_kernel(FewArgs a,
     }
 }
 
-uint32_t tiles_of(uint32_t n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
+uint32_t tiles_of(uint32_t n) { return (n + 15) / 16; }
 uint32_t blocks_of(uint32_t rows) { return div_up(rows, waves * 16); }
 
 template <typename T>
@@ -222,6 +222,7 @@ void launch(const FewArgs& a, hipStream_t s) {
     switch (tiles_of(a.n)) {
         case 1: hipLaunchKernelGGL((entropy_few_kernel<T, 1>), grid, dim3(block), 0, s, a); break;
         case 2: hipLaunchKernelGGL((entropy_few_kernel<T, 2>), grid, dim3(block), 0, s, a); break;
+        case 3: hipLaunchKernelGGL((entropy_few_kernel<T, 3>), grid, dim3(block), 0, s, a); break;
         default: hipLaunchKernelGGL((entropy_few_kernel<T, 4>), grid, dim3(block), 0, s, a); break;
     }
 }

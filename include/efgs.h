@@ -374,8 +374,8 @@ int64_t efgs_linear_cross_entropy_saved_bytes(const efgs_entropy* e);
 int efgs_linear_cross_entropy_forward(const efgs_entropy* e, float* loss, void* saved, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
 /* grad_features (n x columns) and grad_table (rows x columns), contiguous, in `type`, every row written; either may be NULL. upstream: one float, or n with
  * EFGS_EACH. `e` as in the forward (features and targets are not read: they are in `saved`). Up to 64 columns the logits' gradients stay in registers, as
- * parts of bfloat16 (three of a float, two otherwise); above, they are held by pieces of the table in `type`, but for what a row's own target's loses as it is
- * rounded, which is added in 32 bits. Sums in 32 bits in a fixed order. Scratch from `alloc`. Stream-ordered, no host synchronisation. */
+ * parts of bfloat16 (three of a float, two otherwise); above, they are held by pieces of the table in `type` (floats in three parts), but for what a row's
+ * own target's loses as it is rounded, which is added in 32 bits. Sums in 32 bits in a fixed order. Scratch from `alloc`. Stream-ordered, no host synchronisation. */
 int efgs_linear_cross_entropy_backward(const efgs_entropy* e, const float* upstream, const void* saved, void* grad_features, void* grad_table,
                                        efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
 
@@ -387,7 +387,8 @@ int efgs_dropout(const void* x, const void* residual, void* out, int64_t n, int 
 
 /* Balance of choices: counts (int64) of each of `experts` (1 to 8192) among indices (n x chosen, up to 65536 of a row; outside [0, experts): none),
  * loss = experts sum_e share_e P_e, share_e = counts_e / all choices, P_e the mean of softmax(logits)_e over the rows with a choice (0 without one).
- * share (experts + 1 floats: shares less 1 / experts, experts / rows) is kept for the backward, which writes gradient (n x experts, in `type`). Sums in a fixed order. Stream-ordered. */
+ * share (experts + 1 floats: shares less 1 / experts, experts / rows) is kept for the backward, which writes gradient (n x experts, in `type`). Sums in a
+ * fixed order. Stream-ordered. */
 int efgs_balance_loss_forward(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type,
                               float* loss, int64_t* counts, float* share, efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
 int efgs_balance_loss_backward(const void* logits, const void* indices, int index_bytes, int64_t n, int64_t experts, int64_t chosen, int type,
