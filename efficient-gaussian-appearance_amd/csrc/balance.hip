@@ -361,10 +361,12 @@ __global__ __launch_bounds__(balance_block) void balance_backward_kernel(Balance
     }
 }
 
-// calls f with a part's width, the lanes of a row and the parts of a lane (up to balance_max_experts)
+// calls f with a part's width, the lanes of a row and the parts of a lane; the last shape of each width holds balance_max_experts, so that f is always called
 template <typename T, int W, typename F>
 void with_shape(uint32_t experts, F&& f) {
     const uint32_t parts = (experts + W - 1) / W;
+    constexpr uint32_t most_parts = (balance_max_experts + W - 1) / W;
+    static_assert(most_parts <= 8192, "the longest shape is 256 x 32 parts");
     auto lanes = [&](auto tpr, auto items) { f(std::integral_constant<int, W>{}, tpr, items); };
 #define EFGS_LANES(TPR, ITEMS) lanes(std::integral_constant<uint32_t, TPR>{}, std::integral_constant<int, ITEMS>{})
     if (parts <= 1) EFGS_LANES(1, 1);
@@ -378,11 +380,11 @@ void with_shape(uint32_t experts, F&& f) {
     else if (parts <= 256) EFGS_LANES(64, 4);
     else if (parts <= 512) EFGS_LANES(256, 2);
     else if (parts <= 1024) EFGS_LANES(256, 4);
+    else if constexpr (most_parts <= 2048) EFGS_LANES(256, 8);
     else if (parts <= 2048) EFGS_LANES(256, 8);
-    else if constexpr (W == 1) {
-        if (parts <= 4096) EFGS_LANES(256, 16);
-        else EFGS_LANES(256, 32);
-    }
+    else if constexpr (most_parts <= 4096) EFGS_LANES(256, 16);
+    else if (parts <= 4096) EFGS_LANES(256, 16);
+    else EFGS_LANES(256, 32);
 #undef EFGS_LANES
 }
 

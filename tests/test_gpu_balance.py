@@ -184,3 +184,11 @@ def test_even_choices_have_no_gradient(experts):
     assert torch.all(counts == 7) and abs(float(loss.detach()) - 1.0) <= 2.0 ** -20
     loss.backward()
     assert torch.all(logits.grad == 0)
+
+
+@pytest.mark.parametrize('n', [1, 2, 203])
+@pytest.mark.parametrize('experts', [4094, 4098, 4100, 4102, 4104, 6146, 8186, 8188, 8190])
+@pytest.mark.parametrize('dtype', list(TYPES))
+def test_even_widths_of_many_experts(experts, n, dtype):
+    """Multiples of two, four and eight up to the largest ones; one row, whose only block makes the loss too, and several."""
+    check(n, experts, 3, dtype, seed=experts + n, left_out=0.0 if n == 1 else 0.1)
