@@ -192,7 +192,8 @@ struct Dropout : torch::autograd::Function<Dropout> {
                               "efgs: dropout's gradient must have the output's type, on its device");
             const c10::DeviceGuard guard(g.device());
             if (ctx->needs_input_grad(0)) grads[0] = dropped(g.detach(), Tensor(), c);
-            if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1)) grads[1] = g.detach();
+            // (the upstream itself: a leaf takes a gradient that nobody else holds as its own, and a detached one would pass for such)
+            if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1)) grads[1] = g;
         }
         return first_order_only(std::move(grads), upstream[0]);
     }

@@ -157,3 +157,18 @@ def test_on_another_stream():
         got = efgs.dropout(x * 1.0, 0.5, seed=2)
     stream.synchronize()
     assert torch.equal(got, want)
+
+
+def test_the_residuals_gradient_is_its_own():
+    """Leaves that gather their gradients: none of them shares memory with the upstream gradient or with another's."""
+    import efgs
+    x, residual, other = (torch.randn(4096, device=DEVICE, requires_grad=True) for _ in range(3))
+    up = torch.ones(4096, device=DEVICE)
+    for k in range(1, 4):
+        efgs.dropout(x, 0.5, seed=k, residual=residual).backward(up)
+        assert torch.all(up == 1) and torch.all(residual.grad == k) and residual.grad.data_ptr() != up.data_ptr()
+    residual.grad = None
+    for k in range(1, 4):
+        ((efgs.dropout(x, 0.5, seed=k, residual=residual) + other) * 1.0).backward(up)
+        assert torch.all(residual.grad == k) and torch.all(other.grad == k)
+        assert len({t.data_ptr() for t in (x.grad, residual.grad, other.grad, up)}) == 4
