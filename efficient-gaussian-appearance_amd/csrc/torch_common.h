@@ -3,6 +3,7 @@
 #pragma once
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <map>
@@ -129,6 +130,24 @@ inline variable_list first_order_only(variable_list grads, const Tensor& upstrea
     if (at::GradMode::is_enabled() && upstream.requires_grad())
         for (Tensor& g : grads)
             if (g.defined()) g = FirstOrderOnly::apply(upstream, g);
+    return grads;
+}
+
+// The same for gradients that depend on the node's inputs too, as a loss's that is not linear in them: whenever the backward is being
+// recorded, they hang on everything that the node's inputs came from, so that no path back to them passes by the refusal.
+struct InputsOnce : torch::autograd::Node {
+    variable_list apply(variable_list&&) override { TORCH_CHECK(false, "trying to differentiate twice a function that was marked with @once_differentiable"); }
+};
+
+// called within the node's backward
+inline variable_list first_order_only_in_inputs(variable_list grads, const Tensor& upstream) {
+    if (!at::GradMode::is_enabled()) return grads;
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node(), refusal(new InputsOnce(), torch::autograd::deleteNode);
+    torch::autograd::edge_list edges = node ? node->next_edges() : torch::autograd::edge_list{};
+    if (upstream.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(upstream));
+    refusal->set_next_edges(std::move(edges));
+    for (Tensor& g : grads)
+        if (g.defined()) torch::autograd::set_history(g, refusal);
     return grads;
 }
 

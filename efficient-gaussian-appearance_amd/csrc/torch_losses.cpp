@@ -116,7 +116,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
                                                             grads[1].defined() ? pointer<void>(grads[1]) : nullptr, &Scratch::alloc, &scratch,
                                                             current_stream(device)));
         }
-        return first_order_only(std::move(grads), upstream[0]);
+        return first_order_only_in_inputs(std::move(grads), upstream[0]);
     }
 };
 
@@ -279,7 +279,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
                                                     element_type("logits", logits.scalar_type()), pointer<float>(share), pointer<float>(g),
                                                     pointer<void>(grads[0]), current_stream(device)));
         }
-        return first_order_only(std::move(grads), upstream[0]);
+        return first_order_only_in_inputs(std::move(grads), upstream[0]);
     }
 };
 

@@ -192,3 +192,18 @@ def test_even_choices_have_no_gradient(experts):
 def test_even_widths_of_many_experts(experts, n, dtype):
     """Multiples of two, four and eight up to the largest ones; one row, whose only block makes the loss too, and several."""
     check(n, experts, 3, dtype, seed=experts + n, left_out=0.0 if n == 1 else 0.1)
+
+
+def test_a_penalty_on_the_gradient_raises():
+    """The gradient depends on the logits themselves: what is differentiated through it raises, also where the upstream gradient asks for none."""
+    import efgs
+    logits, indices = inputs(40, 16, 2, 'f32')
+    logits.requires_grad_()
+    loss, _ = efgs.balance_loss(logits, indices)
+    grad, = torch.autograd.grad(loss, logits, create_graph=True)
+    want, = torch.autograd.grad(efgs.balance_loss(logits, indices)[0], logits)
+    assert grad.requires_grad and not want.requires_grad and torch.equal(grad, want)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        torch.autograd.grad(loss + grad.pow(2).sum(), logits, retain_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        (loss + grad.pow(2).sum()).backward()

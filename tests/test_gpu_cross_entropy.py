@@ -553,3 +553,23 @@ def test_more_rows_of_one_target_than_a_list_holds(dtype):
 def test_many_rows_of_each_target(n, rows, dtype):
     """About where the targets' gradients are no longer added to the table's apart (64 rows of each), and past it."""
     check(n, rows, 136, dtype, reduction='none')
+
+
+@pytest.mark.parametrize('dtype,columns', [('f32', 16), ('f32', 96), ('bf16', 96)])
+@pytest.mark.parametrize('grads', [(True, False), (False, True), (True, True)])
+def test_a_penalty_on_a_gradient_raises(dtype, columns, grads):
+    """The gradients depend on features and table themselves: what is differentiated through them raises, also where the upstream gradient asks for none."""
+    import efgs
+    features, table, targets, _ = inputs(20, 30, columns, dtype)
+    leaves = [t.requires_grad_() for t, wanted in zip((features, table), grads) if wanted]
+    x = features * 1.0   # (not a leaf: its own graph is part of what is differentiated)
+    loss = efgs.linear_cross_entropy(x, table, targets)
+    want = torch.autograd.grad(efgs.linear_cross_entropy(x, table, targets), leaves, retain_graph=True)
+    got = torch.autograd.grad(loss, leaves, create_graph=True)
+    for a, b in zip(got, want):
+        assert a.requires_grad and not b.requires_grad and torch.equal(a, b)
+        for leaf in leaves:
+            with pytest.raises(RuntimeError, match='once_differentiable'):
+                torch.autograd.grad(loss.float() + a.float().pow(2).sum(), leaf, retain_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        (loss + got[0].float().pow(2).sum()).backward()
