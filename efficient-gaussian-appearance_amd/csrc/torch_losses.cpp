@@ -228,6 +228,15 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, const c10::optional<Ten
     return Dropout::apply(x, residual, c);
 }
 
+// (seed, offset) of a torch generator for the draws of one call, which moves it on by four, as one step under its lock: what other threads draw meanwhile
+// has other offsets
+std::pair<uint64_t, uint64_t> draw_counters(at::Generator generator) {
+    const std::lock_guard<std::mutex> lock(generator.mutex());
+    const uint64_t seed = generator.current_seed(), offset = generator.get_offset();
+    generator.set_offset(offset + 4);
+    return {seed, offset};
+}
+
 // ---- balance loss ------------------------------------------------------------------------------------------------------
 
 struct BalanceCall {
@@ -314,6 +323,7 @@ std::pair<Tensor, Tensor> balance_loss(const Tensor& logits, const Tensor& indic
 void register_losses(py::module_& m) {
     m.def("linear_cross_entropy", torch::wrap_pybind_function_no_gil(linear_cross_entropy));
     m.def("dropout", torch::wrap_pybind_function_no_gil(dropout));
+    m.def("draw_counters", torch::wrap_pybind_function_no_gil(draw_counters));
     m.def("balance_loss", torch::wrap_pybind_function_no_gil(balance_loss));
 }
 

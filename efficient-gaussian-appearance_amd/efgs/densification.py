@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _native
 from ._lib import check, lib
 
 
@@ -60,9 +61,7 @@ def add_noise(raw_scales: torch.Tensor, raw_rotations: torch.Tensor, raw_opaciti
     if means.shape != (n, 3) or raw_scales.shape != (n, 3) or raw_rotations.shape != (n, 4) or raw_opacities.numel() != n:
         raise ValueError('efgs: add_noise expects scales (N, 3), rotations (N, 4), opacities (N, 1) and means (N, 3)')
     gen = torch.cuda.default_generators[device.index if device.index is not None else torch.cuda.current_device()]
-    seed = gen.initial_seed()
-    offset = gen.get_offset()
-    gen.set_offset(offset + 4)
+    seed, offset = _native.draw_counters(gen)
     if n == 0:
         return
     with torch.cuda.device(device):

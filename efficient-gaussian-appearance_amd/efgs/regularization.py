@@ -25,9 +25,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int | torch.Tensor | None = N
         with torch.cuda.device(x.device):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('efgs: a captured dropout needs its seed: the generator is read on the host')
-        generator = torch.cuda.default_generators[x.device.index]
-        seed, drawn = generator.initial_seed(), generator.get_offset()
-        generator.set_offset(drawn + 4)
+        seed, drawn = _native.draw_counters(torch.cuda.default_generators[x.device.index])
         offset = drawn | _STREAM
     if not 0 <= offset < 1 << 64:
         raise ValueError(f'efgs: the offset must lie in [0, 2^64), got {offset}')

@@ -172,3 +172,36 @@ def test_the_residuals_gradient_is_its_own():
         ((efgs.dropout(x, 0.5, seed=k, residual=residual) + other) * 1.0).backward(up)
         assert torch.all(residual.grad == k) and torch.all(other.grad == k)
         assert len({t.data_ptr() for t in (x.grad, residual.grad, other.grad, up)}) == 4
+
+
+def test_threads_draw_different_masks():
+    """Draws from the default generator by several threads at once: no two the same, and the generator advanced by all of them."""
+    import sys
+    import threading
+
+    import efgs
+    threads, calls = 8, 150
+    torch.cuda.manual_seed(5)
+    generator = torch.cuda.default_generators[0]
+    before, x = generator.get_offset(), torch.ones(256, device=DEVICE)
+    masks = [[] for _ in range(threads)]
+    start = threading.Barrier(threads)
+
+    def draw(out):
+        start.wait()
+        for _ in range(calls):
+            out.append(efgs.dropout(x, 0.5))
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        workers = [threading.Thread(target=draw, args=(out,)) for out in masks]
+        for w in workers:
+            w.start()
+        for w in workers:
+            w.join()
+    finally:
+        sys.setswitchinterval(interval)
+    kept = (torch.stack([m for out in masks for m in out]) != 0).cpu().numpy()
+    assert len({row.tobytes() for row in kept}) == threads * calls
+    assert generator.get_offset() == before + 4 * threads * calls
