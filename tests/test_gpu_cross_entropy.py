@@ -573,3 +573,24 @@ def test_a_penalty_on_a_gradient_raises(dtype, columns, grads):
                 torch.autograd.grad(loss.float() + a.float().pow(2).sum(), leaf, retain_graph=True)
     with pytest.raises(RuntimeError, match='once_differentiable'):
         (loss + got[0].float().pow(2).sum()).backward()
+
+
+@pytest.mark.parametrize('dtype,n,rows', [('bf16', 40_000, 520), ('bf16', 8_320, 130), ('bf16', 5_000, 520), ('f16', 270_000, 4_100)])
+def test_roundings_that_are_all_alike(dtype, n, rows):
+    """All rows of one target, many of them for each table row, and a table of zeros: every row's own gradient is 1 / rows - 1, which the type rounds the same
+    way every time. The target's row of the table's gradient is still one rounding off.
+
+    Features are 1, 2 or 3: the sum of p x is off by 2^-24 for each of its steps of 32 rows and a few more, (n / 32 + 64) e of its size, twice for what the matrix
+    instruction may cut; what a rounding lost, u of the whole, is itself held to u of it; then half a step of the result."""
+    import efgs
+    kind, u, _, _ = TYPES[dtype]
+    rng = torch.Generator(DEVICE).manual_seed(n)
+    columns, target = 96, 77
+    x = torch.randint(1, 4, (n, columns), generator=rng, device=DEVICE).to(kind)
+    w = torch.zeros(rows, columns, device=DEVICE, dtype=kind, requires_grad=True)
+    efgs.linear_cross_entropy(x, w, torch.full((n,), target, device=DEVICE)).backward()
+    dw = (1.0 / rows - 1.0) * x.double().mean(0)
+    off = (w.grad[target].double() - dw).abs()
+    inner = dw.abs() * (2 * (n / 32 + 64) * E + u * u)
+    step = 2.0 ** torch.floor(torch.log2(dw.abs() + inner)) * 2 * u   # of the result
+    assert torch.all(off <= step / 2 + inner), float((off / step).max())
