@@ -61,7 +61,7 @@ __device__ __forceinline__ floatx4 multiply(shortx8 a, shortx8 b, floatx4 c) {
 // 64 lanes' 16 bytes each to 1 KB of LDS at `to`. (The builtin of this transfer makes the compiler wait for it before the next
 // transposing read of whatever address; the waits stand in the loop instead.)
 __device__ __forceinline__ void to_lds(uint32_t to, uintx4 buffer, uint32_t lane_offset, uint32_t offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer), "s"(offset) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer), "s"(offset) : "memory", "m0");
 }
 
 __device__ __forceinline__ uint32_t scalar(uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x))); }
