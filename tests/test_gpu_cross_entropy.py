@@ -594,3 +594,59 @@ def test_roundings_that_are_all_alike(dtype, n, rows):
     inner = dw.abs() * (2 * (n / 32 + 64) * E + u * u)
     step = 2.0 ** torch.floor(torch.log2(dw.abs() + inner)) * 2 * u   # of the result
     assert torch.all(off <= step / 2 + inner), float((off / step).max())
+
+
+def check_on_device(n, rows, columns, dtype, seed):
+    """`check` with a weight for each row, oracle and bars in 64 bits on the GPU (the same formulas): sizes that would take long on the CPU."""
+    import efgs
+    print(f'case cross entropy on the device n={n} rows={rows} columns={columns} {dtype}', flush=True)
+    _, u, least, held = TYPES[dtype]
+    features, table, targets, weights = inputs(n, rows, columns, dtype, seed=seed)
+    loss = efgs.linear_cross_entropy(features.requires_grad_(), table.requires_grad_(), targets, reduction='none')
+    grad_x, grad_w = torch.autograd.grad(loss, (features, table), weights)
+    inside = (targets >= 0) & (targets < rows)
+    x, w = features.detach().double() * inside[:, None], table.detach().double()
+    ax, aw, up, at = x.abs(), w.abs(), (weights.double() * inside)[:, None], inside.nonzero()[:, 0]
+    z = x @ w.t()
+    off = 2 * (2 * (columns + 4) * E * (ax @ aw.t()) + 3 * E * z.abs()).amax(1) + (80 + rows / 16) * E + 8 * E * (z.abs().amax(1) + np.log(rows) + 1)
+    total = torch.logsumexp(z, 1)
+    want = torch.zeros(n, dtype=torch.float64, device=DEVICE)
+    want[at] = total[at] - z[at, targets[at].long()]
+    assert torch.all((loss.detach().double() - want).abs() <= off * inside)
+    g = torch.exp(z - total[:, None])
+    del z
+    dg = up.abs() * (g * off[:, None] * 1.01 + 2 * E)
+    g[at, targets[at].long()] -= 1.0
+    g *= up
+    dg += (u * g.abs() * 1.02 + held * float(up.abs().max())) * inside[:, None]
+    dx, dw = g @ w, g.t().contiguous() @ x
+    ag = g.abs() + dg
+    bar_x = (dg @ aw + 2 * (rows + 4) * E * (ag @ aw)) * (1 + 4 * E)
+    bar_w = (dg.t().contiguous() @ ax + 2 * (n + 4) * E * (ag.t().contiguous() @ ax)) * (1 + 4 * E)
+    for name, got, value, bar in (('features', grad_x, dx, bar_x), ('table', grad_w, dw, bar_w)):
+        miss = (got.double() - value).abs() - (bar + u * (value.abs() + bar) + least)
+        assert bool((miss <= 0).all()), (name, float(miss.max()), int(miss.argmax()) // columns)
+
+
+@pytest.mark.parametrize('n,rows,columns,dtype', [
+    (20_001, 7_001, 72, 'bf16'), (20_001, 7_001, 72, 'f16'), (20_001, 2_600, 72, 'f32'),      # two pieces
+    (20_001, 13_001, 136, 'bf16'), (17_000, 17_009, 77, 'f16'), (20_001, 4_999, 65, 'f32'),   # three, tables that are copied
+])
+def test_several_pieces_of_the_table_the_last_one_shorter(n, rows, columns, dtype):
+    """A piece's logits' gradients take 256 MB at most: for 20,001 rows 6,400 table rows of a 16-bit type, 2,048 of float32; the pieces are alike but for the
+    last one."""
+    check_on_device(n, rows, columns, dtype, seed=rows)
+
+
+@pytest.mark.parametrize('columns', [32, 136])
+def test_rows_of_small_weights_beside_large_ones(columns):
+    """float16, weights from 1 down to 2^-20: every row's gradient as the formula has it, against bars that count each row's own weight but for the share of the
+    largest one that float16 holds g to (2^-38)."""
+    import efgs
+    features, table, targets, _ = inputs(210, 700, columns, 'f16', left_out=0.0)
+    features.requires_grad_()
+    weights = 2.0 ** -(torch.arange(210, device=DEVICE) % 21).float()
+    up = weights * 512.0
+    grad, = torch.autograd.grad(efgs.linear_cross_entropy(features, table, targets, reduction='none'), features, up)
+    _, _, dx, bar_x, _, _ = bounds(features, table, targets, up.double().cpu().numpy(), 1.0, 'f16')
+    within('features', grad, dx, bar_x)
