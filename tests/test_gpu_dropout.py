@@ -205,3 +205,17 @@ def test_threads_draw_different_masks():
     kept = (torch.stack([m for out in masks for m in out]) != 0).cpu().numpy()
     assert len({row.tobytes() for row in kept}) == threads * calls
     assert generator.get_offset() == before + 4 * threads * calls
+
+
+def test_where_a_launchs_threads_begin_again():
+    """A launch has 2^31 threads at most, eight elements each: both sides of element 2^34, and a tail of three."""
+    import efgs
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip('takes 70 GB of GPU memory')
+    n = (1 << 34) + 4099
+    x = torch.ones(n, dtype=torch.bfloat16, device=DEVICE)
+    out = efgs.dropout(x, 0.25, seed=33, offset=5)
+    for first, last in ((0, 4096), ((1 << 31) - 4096, (1 << 31) + 4096), ((1 << 34) - 4096, n)):
+        assert torch.equal(out[first:last], expected(x[first:last], R.philox_bits(last - first, 33, 5, first), 0.25))
+    del x, out
+    torch.cuda.empty_cache()
