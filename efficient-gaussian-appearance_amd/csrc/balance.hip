@@ -12,8 +12,8 @@
 // the block's end. The forward leaves a table of the blocks' sums, which a second kernel adds up in the blocks' order
 // (64 bits) and a third makes the loss of: no atomics on floats, the same bits from call to call.
 //
-// 1,000,000 x 64 float32, one choice each: forward 74 us (3.6 TB/s of logits and choices), sums 11, loss 4.3, backward 85 (6.1 TB/s of what it moves, the logits
-// partly from the memory-side cache). A pass took 213 us instead of 173 before the loads of several rows were under way together, choices came beside the logits
+// 1,000,000 x 64 float32, one choice each: forward 74 us (3.6 TB/s of logits and choices; a group of rows is loaded when the one before is summed), sums 11,
+// loss 4.3, backward 85 (6.1 TB/s of what it moves, the logits partly from the memory-side cache). A pass took 213 us instead of 173 before the loads of several rows were under way together, choices came beside the logits
 // and the lanes' exchanges went past LDS. 16,383 x 250 bfloat16, eight choices: 8.4, 7.1, 2.9 and 8.8, each at its latency.
 #include <algorithm>
 

@@ -9,8 +9,8 @@
 // second kernel joins them. The backward computes the logits again by pieces of the table, writes g of a piece, and multiplies
 // it by the piece and, transposed, by the rows: four products where three would do if g could be kept (N x V of it), and no more memory than a piece.
 // Statistics and sums are in 32 bits (logits in units of log 2), the sum over rows in 64. g is held in the inputs' type, as the matrix unit takes it (floats: three
-// bfloat16 parts): its rounding, 2^-9 of each, is as large as the gradients' own one only where one entry outweighs the others, which a row's target does; what
-// that one loses is added (cross_entropy_wide.hip).
+// bfloat16 parts): its rounding, bfloat16 2^-8 of each at most, is as large as the gradients' own one only where one entry outweighs the others, which a row's
+// target does; what that one loses is added (cross_entropy_wide.hip).
 //
 // This file: the packing, the joins and the launches, most of them at the latency of a launch, 4 to 9 us each. The products: cross_entropy_narrow.hip up to 64
 // columns, where its kernels are the faster ones (32,768 x 4,096 x 64: float32 0.66 ms and 1.07 by the wide one, bfloat16 0.24 and 0.34; float16 0.41 and 0.35, for
@@ -260,7 +260,8 @@ __global__ __launch_bounds__(256) void entropy_weights_kernel(WeightArgs a) {
 }
 
 // float16, a weight for each row: the weights over the power of two at or above the largest finite one, so that a product of weight and
-// probability keeps to the type's range (a row of an infinite one or NaN alone, as the plain product would have it). One block.
+// probability keeps to the type's range (a row of an infinite one or NaN alone, as the plain product would have it): held times 2^15, each to 2^-39 of the
+// largest weight, so that the entries of a row of a far smaller one have fewer bits than float16's eleven. One block.
 __global__ __launch_bounds__(1024) void entropy_half_weights_kernel(WeightArgs a) {
     __shared__ float lds[16];
     const uint32_t count = *a.count;

@@ -14,7 +14,8 @@ def linear_cross_entropy(features: torch.Tensor, table: torch.Tensor, targets: t
     without columns. A target outside [0, rows) (say -1 or -100) leaves its row out: its loss and gradient are zero, whatever its features hold.
     reduction: 'none' (a loss for each target), 'sum', or 'mean' over the rows that count (0 if none does). Logits, sums and statistics are in 32
     bits. Differentiable with respect to features and table, by pieces of the table whose logits are computed again; above 64 columns the logits'
-    gradients are held in the inputs' type between the two products, but for what a row's own target's loses as it is rounded, which is added. Every sum
+    gradients are held in the inputs' type between the two products, but for what a row's own target's loses as it is rounded, which is added;
+    of float16 with a loss for each target, to 2^-39 of the largest upstream gradient, so in fewer bits where a row's own is far smaller. Every sum
     has a fixed order, the same bits from call to call; second and forward-mode derivatives raise.
 
     Rows that count and the table should be finite: an infinity or NaN reaches the losses and gradients that its row has a part in, as NaN where

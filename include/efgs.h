@@ -375,7 +375,8 @@ int efgs_linear_cross_entropy_forward(const efgs_entropy* e, float* loss, void* 
 /* grad_features (n x columns) and grad_table (rows x columns), contiguous, in `type`, every row written; either may be NULL. upstream: one float, or n with
  * EFGS_EACH. `e` as in the forward (features and targets are not read: they are in `saved`). Up to 64 columns the logits' gradients stay in registers, as
  * parts of bfloat16 (three of a float, two otherwise); above, they are held by pieces of the table in `type` (floats in three parts), but for what a row's
- * own target's loses as it is rounded, which is added in 32 bits. Sums in 32 bits in a fixed order. Scratch from `alloc`. Stream-ordered, no host synchronisation. */
+ * own target's loses as it is rounded, which is added in 32 bits (float16 with EFGS_EACH: to 2^-39 of the largest finite
+ * upstream gradient, so in fewer bits where a row's own is far smaller). Sums in 32 bits in a fixed order. Scratch from `alloc`. Stream-ordered, no host synchronisation. */
 int efgs_linear_cross_entropy_backward(const efgs_entropy* e, const float* upstream, const void* saved, void* grad_features, void* grad_table,
                                        efgs_alloc_fn alloc, void* alloc_ctx, void* stream);
 
