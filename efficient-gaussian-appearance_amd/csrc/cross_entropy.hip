@@ -614,7 +614,8 @@ EntropyNarrowArgs narrow_args(const EntropyArgs& a, const Saved& s) {
 // Whether a row's own target's gradient goes apart, in the table's gradient: of 16-bit types what its rounding lost, always, as the roundings of many rows of one
 // target may be all alike (a table of zeros). With 64 and more rows of each target that takes 1 to 8 % of a pass, 13 where all are of one (200,000 x 300 x 200 bfloat16
 // 526 -> 554 us, error of the table's gradient 0.00187 -> 0.00169, of one rounding 0.00166), a fifth against a table of one tile (100,000 x 16 x 128 142 -> 172). Of
-// floats, which lose nothing, all of it, where no table row is the target of more than 64 on average: past that the rows to look up are as many as those of a product's steps.
+// floats, which lose nothing, all of it, where no table row is the target of more than 64 on average (rows left out
+// among them: how many count is known on the device alone): past that the rows to look up are as many as those of a product's steps.
 bool targets_apart(const EntropyArgs& a) { return !in_parts(a) || a.n / 64 <= a.rows; }
 
 // of a slab's first `rows` rows, as they lie
